@@ -377,6 +377,9 @@ __device__ __forceinline__ int build_tile_table(const GemmArgs& a, int valid_row
 }
 
 // ------------------------------------------------------------------------------ host
+// Tensor map over bytes with the 128-byte swizzle (dims and box of the innermost axis in bytes, out of bounds reads zero).
+int make_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+             const cuuint32_t* box);
 // Tensor maps of both operands: boxes of `a_box_rows` rows of A and of `b_box_rows` weight rows, 128 bytes of K wide.
 int make_gemm_maps(int stage, const GemmArgs& a, int a_box_rows, int b_box_rows, CUtensorMap* map_a, CUtensorMap* map_b);
 // Cluster sizes 1, 2, 4, 8: how many CTAs share a tile's K range, given how many clusters of each size run at once

@@ -1,0 +1,38 @@
+"""What the operator functions share: the device and stream of a call, and its argument checks."""
+
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from .. import _lib
+
+HALF = (torch.bfloat16, torch.float16)
+_HERE = contextlib.nullcontext()
+
+
+def on(device: torch.device, stream=None):
+    """Context in which a call allocates and launches: the device of its tensors, and ``stream`` (None: that device's
+    current one).  What is allocated inside belongs to that stream; the inputs have to be ready on it, as for every
+    launcher."""
+    if stream is not None:
+        if isinstance(stream, int) or not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(_lib.stream_handle(stream), device=device)
+        return torch.cuda.stream(stream)
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _HERE
+    return torch.cuda.device(device)
+
+
+def require_shape(name: str, t: torch.Tensor, shape: tuple) -> None:
+    """``None`` in ``shape`` stands for any size."""
+    if t.dim() != len(shape) or any(s is not None and s != d for s, d in zip(shape, t.shape)):
+        want = ", ".join("*" if s is None else str(s) for s in shape)
+        raise ValueError(f"{name} must have shape [{want}], got {list(t.shape)}")
+
+
+def require_same_device(first: str, device: torch.device, **others) -> None:
+    for name, t in others.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, {first} on {device}")

@@ -320,6 +320,20 @@ typedef struct flymoe_layer_args {
 } flymoe_layer_args;
 int flymoe_moe_layer(const flymoe_layer_args* args, void* stream);
 
+/* Matrix products grouped by expert over ragged rows, 16-bit operands (dtype F16 or BF16), and their gradients.  Expert e
+ * owns rows offsets[e] .. offsets[e+1]-1; offsets int32 [experts+1] on the device, ascending within [0, rows] (values that
+ * are not are taken into that range).  w [experts, n, k].  Sums in fp32, rounded once.
+ * flymoe_grouped_gemm: input_grad == 0: out [rows, n] = x [rows, k] . w[e]^T; else out [rows, k] = x [rows, n] . w[e] (the
+ * gradient of the first form with respect to its rows, x being the output's gradient).  Rows of no expert are zeroed if
+ * zero_uncovered, else left as they were.
+ * flymoe_grouped_gemm_wgrad: dw [experts, n, k], dw[e] = sum over the rows of e of dy[r]^T x[r]; zeros without rows.
+ * n and k multiples of 8, experts <= 1024, pointers 16-byte aligned.  No counterpart in the reference, whose grouped GEMMs
+ * (kernels/moe_gemm_2stage.py:90-108, :1780-1796) take padded row blocks and have no gradients. */
+int flymoe_grouped_gemm(void* out, const void* x, const void* w, const int32_t* offsets, int rows, int experts, int n,
+                        int k, int dtype, int input_grad, int zero_uncovered, void* stream);
+int flymoe_grouped_gemm_wgrad(void* dw, const void* dy, const void* x, const int32_t* offsets, int rows, int experts, int n,
+                              int k, int dtype, void* stream);
+
 /* Y[t,:] = sum_s w[t,s] * X[row(t,s),:] with fp32 accumulation; row(t,s) = t*k+s, or
  * row_index[t*k+s] when row_index is given (negative entries are skipped); optional u8
  * valid_mask [T,k] and optional f32 weights [T,k] (NULL = 1).
