@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "vec8.cuh"
 
 namespace flymoe {
 
@@ -88,47 +89,6 @@ dispatch_rows_kernel(const uint4* __restrict__ x, const float* __restrict__ x_sc
 }
 
 // ---------------------------------------------------------------------------- reduce
-template <typename T> struct Vec8;
-template <> struct Vec8<__half> {
-  static __device__ __forceinline__ void load(const __half* p, float* f) {
-    uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    const __half2* h = reinterpret_cast<const __half2*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { float2 x = __half22float2(h[i]); f[2 * i] = x.x; f[2 * i + 1] = x.y; }
-  }
-  static __device__ __forceinline__ void store(__half* p, const float* f) {
-    uint4 v;
-    v.x = pack_f16x2(f[0], f[1]); v.y = pack_f16x2(f[2], f[3]);
-    v.z = pack_f16x2(f[4], f[5]); v.w = pack_f16x2(f[6], f[7]);
-    *reinterpret_cast<uint4*>(p) = v;
-  }
-};
-template <> struct Vec8<__nv_bfloat16> {
-  static __device__ __forceinline__ void load(const __nv_bfloat16* p, float* f) {
-    uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { float2 x = __bfloat1622float2(h[i]); f[2 * i] = x.x; f[2 * i + 1] = x.y; }
-  }
-  static __device__ __forceinline__ void store(__nv_bfloat16* p, const float* f) {
-    uint4 v;
-    v.x = pack_bf16x2(f[0], f[1]); v.y = pack_bf16x2(f[2], f[3]);
-    v.z = pack_bf16x2(f[4], f[5]); v.w = pack_bf16x2(f[6], f[7]);
-    *reinterpret_cast<uint4*>(p) = v;
-  }
-};
-template <> struct Vec8<float> {
-  static __device__ __forceinline__ void load(const float* p, float* f) {
-    float4 a = __ldg(reinterpret_cast<const float4*>(p));
-    float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  }
-  static __device__ __forceinline__ void store(float* p, const float* f) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-  }
-};
-
 // grid (T, ceil(D / 2048)), 256 threads x 8 elements.
 template <typename T>
 __global__ void __launch_bounds__(256)

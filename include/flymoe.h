@@ -334,6 +334,34 @@ int flymoe_grouped_gemm(void* out, const void* x, const void* w, const int32_t* 
 int flymoe_grouped_gemm_wgrad(void* dw, const void* dy, const void* x, const int32_t* offsets, int rows, int experts, int n,
                               int k, int dtype, void* stream);
 
+/* Gradient of flymoe_topk_gating_softmax's weights with respect to the logits, dgating [T,E] of gating_dtype, from its
+ * outputs and dtopk_weights f32 [T,k].  gating may be NULL when renormalize (the gradient then only needs the weights).
+ * No counterpart in the reference. */
+int flymoe_topk_gating_softmax_backward(const void* gating, int gating_dtype, const float* topk_weights,
+                                        const int32_t* topk_indices, const float* dtopk_weights, void* dgating,
+                                        int num_tokens, int num_experts, int topk, int renormalize, void* stream);
+
+/* Rows in expert order without padding (a unit-1 sort).  flymoe_route_tables: from the sort's outputs, row_index i32 [T*k]
+ * (row of a pair, -1 without one) and offsets i32 [experts+1] (first row of each expert).  The calls below take these
+ * tables; a pair and a row belong together where sorted_ids and row_index name each other, other pairs have no row and
+ * other rows no pair.
+ * flymoe_permute_rows: rows_out[r] = x[token of r] (row_bytes each), zeros without a pair, for all `rows` rows.
+ * flymoe_combine_rows: out[t] = sum_s weights[t,s] * rows_in[row of (t,s)], fp32, weights NULL = 1 (the gradient of
+ * flymoe_permute_rows).  flymoe_combine_rows_backward: drows[row] = weights[t,s] * dout[t] (zeros without a pair) and
+ * dweights[t,s] = <rows_in[row], dout[t]> (0 without a row); either may be NULL.  dtype F16, BF16 or F32, dim a multiple of
+ * 8.  No counterpart in the reference beyond its inference-time reduce (kernels/moe_blockscale_2stage.py:2383-2589). */
+int flymoe_route_tables(const int32_t* sorted_ids, const int32_t* sorted_expert_ids, const int32_t* num_valid_ids,
+                        int32_t* row_index, int32_t* offsets, int num_tokens, int topk, int experts, int max_rows,
+                        void* stream);
+int flymoe_permute_rows(const void* x, void* rows_out, const int32_t* sorted_ids, const int32_t* num_valid_ids,
+                        const int32_t* row_index, int num_tokens, int topk, int rows, int row_bytes, void* stream);
+int flymoe_combine_rows(const void* rows_in, const float* weights, void* out, const int32_t* sorted_ids,
+                        const int32_t* num_valid_ids, const int32_t* row_index, int num_tokens, int topk, int rows, int dim,
+                        int dtype, void* stream);
+int flymoe_combine_rows_backward(const void* dout, const void* rows_in, const float* weights, void* drows, float* dweights,
+                                 const int32_t* sorted_ids, const int32_t* num_valid_ids, const int32_t* row_index,
+                                 int num_tokens, int topk, int rows, int dim, int dtype, void* stream);
+
 /* Y[t,:] = sum_s w[t,s] * X[row(t,s),:] with fp32 accumulation; row(t,s) = t*k+s, or
  * row_index[t*k+s] when row_index is given (negative entries are skipped); optional u8
  * valid_mask [T,k] and optional f32 weights [T,k] (NULL = 1).
