@@ -1,0 +1,134 @@
+"""Low-rank adapters of many requests at once, beside a shared projection (B200, bf16 / fp16).
+
+``lora_add(y, x, a, b, adapter_ids, scaling)`` adds every row's own adapter to the output of a projection that all rows
+share (``compile_blockscale_preshuffle_gemm`` or any other):
+
+    out[m] = y[m] + scaling[l] * b[l] (a[l] x[m]),   l = adapter_ids[m]
+
+    y [rows, n], x [rows, k], a [adapters, rank, k], b [adapters, n, rank]    bf16 or fp16, all of one type, contiguous
+    adapter_ids int32 [rows]   any order, one request a row or runs of rows; an id outside [0, adapters) means no adapter
+    scaling     f32 [adapters]
+
+The product with ``a`` is kept in fp32 between the two steps and the result is rounded once.  ``out=`` takes the caller's
+buffer and may be ``y`` itself (serving: in place).  Gradients reach y, x, a and b; adapters of smaller rank are padded with
+zeros by the caller.  rank is a multiple of 8 up to 128, k and n multiples of 8.  A row's result depends on its own inputs
+and adapter only; nothing is atomic.  The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from ._call import HALF, on, require_same_device, require_shape
+
+MAX_RANK = 128
+
+
+def _check(y, x, a, b, adapter_ids, scaling, out):
+    for name, t in (("y", y), ("x", x), ("a", a), ("b", b), ("adapter_ids", adapter_ids), ("scaling", scaling)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+    require_shape("x", x, (None, None))
+    rows, k = x.shape
+    require_shape("a", a, (None, None, k))
+    adapters, rank, _ = a.shape
+    require_shape("y", y, (rows, None))
+    n = y.shape[1]
+    require_shape("b", b, (adapters, n, rank))
+    require_shape("adapter_ids", adapter_ids, (rows,))
+    require_shape("scaling", scaling, (adapters,))
+    if rank < 8 or rank % 8 or rank > MAX_RANK:
+        raise ValueError(f"rank must be a multiple of 8 in [8, {MAX_RANK}], got {rank}")
+    if k < 8 or k % 8 or n < 8 or n % 8:
+        raise ValueError(f"k ({k}) and n ({n}) must be positive multiples of 8")
+    if not 1 <= adapters <= 65535:
+        raise ValueError(f"adapters must be in [1, 65535], got {adapters}")
+    _lib.require_cuda("x", x, HALF)
+    for name, t in (("y", y), ("a", a), ("b", b), ("out", out)):
+        if t is not None:
+            _lib.require_cuda(name, t, (x.dtype,))
+    if out is not None:
+        require_shape("out", out, (rows, n))
+        if x.data_ptr() == out.data_ptr() and rows:
+            raise ValueError("out must not be x")
+    _lib.require_cuda("adapter_ids", adapter_ids, (torch.int32,))
+    _lib.require_cuda("scaling", scaling, (torch.float32,))
+    require_same_device("x", x.device, y=y, a=a, b=b, adapter_ids=adapter_ids, scaling=scaling, out=out)
+
+
+def _shrink(x, a, ids, fold):
+    """x [rows, k], a [adapters, rank, k] -> f32 [splits, rows, rank], or with ``fold`` [1, rows, rank]."""
+    lib, (rows, k), (adapters, rank, _) = _lib.load(), x.shape, a.shape
+    splits = lib.flymoe_lora_shrink_splits(rows, k)
+    v = torch.empty((splits, rows, rank), dtype=torch.float32, device=x.device)
+    _lib.check(lib.flymoe_lora_shrink(v.data_ptr(), x.data_ptr(), a.data_ptr(), ids.data_ptr(), rows, k, rank, adapters,
+                                      splits, 1 if fold else 0, _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(None)),
+               "lora_shrink")
+    return v[:1] if fold else v
+
+
+def _expand(out, base, v, b, ids, scaling):
+    rows, n = out.shape
+    _lib.check(_lib.load().flymoe_lora_expand(out.data_ptr(), _lib.ptr(base), v.data_ptr(), b.data_ptr(), ids.data_ptr(),
+                                              scaling.data_ptr(), rows, n, b.shape[2], b.shape[0], v.shape[0],
+                                              _lib.DTYPE_CODE[out.dtype], _lib.stream_handle(None)), "lora_expand")
+    return out
+
+
+def _transposed(t):
+    mats, rows, cols = t.shape
+    res = torch.empty((mats, cols, rows), dtype=t.dtype, device=t.device)
+    _lib.check(_lib.load().flymoe_lora_transpose(t.data_ptr(), res.data_ptr(), mats, rows, cols, _lib.stream_handle(None)),
+               "lora_transpose")
+    return res
+
+
+class _LoraAdd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, x, a, b, ids, scaling):
+        with on(x.device):
+            v = _shrink(x, a, ids, fold=True)
+            ctx.save_for_backward(x, a, b, ids, scaling, v)
+            return _expand(torch.empty_like(y), y, v, b, ids, scaling)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, a, b, ids, scaling, v = ctx.saved_tensors
+        need_y, need_x, need_a, need_b = ctx.needs_input_grad[:4]
+        dx = da = db = None
+        with on(x.device):
+            dout = dout.contiguous()
+            dv = _shrink(dout, _transposed(b), ids, fold=True) if need_x or need_a else None
+            if need_x:
+                dx = _expand(torch.empty_like(x), None, dv, _transposed(a), ids, scaling)
+            if need_a or need_b:
+                lib, (rows, k), (adapters, n, rank) = _lib.load(), x.shape, b.shape
+                splits = lib.flymoe_lora_wgrad_splits(rows, k, n, adapters)
+                da = torch.empty_like(a) if need_a else None
+                db = torch.empty_like(b) if need_b else None
+                width = (k if need_a else 0) + (n if need_b else 0)
+                partial = (torch.empty(splits * adapters * rank * width, dtype=torch.float32, device=x.device)
+                           if splits > 1 else None)
+                _lib.check(lib.flymoe_lora_wgrad(
+                    _lib.ptr(da), _lib.ptr(db), x.data_ptr(), dout.data_ptr(), v.data_ptr(), _lib.ptr(dv), ids.data_ptr(),
+                    scaling.data_ptr(), _lib.ptr(partial), rows, k, n, rank, adapters, splits, _lib.DTYPE_CODE[x.dtype],
+                    _lib.stream_handle(None)), "lora_wgrad")
+        return dout if need_y else None, dx, da, db, None, None
+
+
+def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter_ids: torch.Tensor,
+             scaling: torch.Tensor, *, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """y + scaling[l] * (x a[l]^T) b[l]^T with l = adapter_ids of the row; see the module docstring.
+
+    With ``out`` or ``stream`` the call is for inference only (no input may require a gradient while gradients are on)."""
+    _check(y, x, a, b, adapter_ids, scaling, out)
+    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad):
+        if out is not None or stream is not None:
+            raise ValueError("out= and stream= are for inference: an input requires a gradient")
+        return _LoraAdd.apply(y, x, a, b, adapter_ids, scaling)
+    with on(x.device, stream):
+        return _expand(torch.empty_like(y) if out is None else out, y, _shrink(x, a, adapter_ids, fold=False), b, adapter_ids,
+                       scaling)
