@@ -87,6 +87,7 @@ _SIGNATURES = {
     "flymoe_permute_rows": (c_int, [_P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),
     "flymoe_combine_rows": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
     "flymoe_combine_rows_backward": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
+    "flymoe_lora_add": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
     "flymoe_lora_shrink_splits": (c_int, [c_int, c_int]),
     "flymoe_lora_shrink": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
     "flymoe_lora_expand": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
@@ -148,7 +149,8 @@ def ptr(t) -> int | None:
 def stream_handle(stream) -> int:
     """None -> current torch stream; int -> raw handle; else object with .cuda_stream."""
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+        # the handle of torch.cuda.current_stream() without building a stream object (0.1 us against 3 to 15)
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     if isinstance(stream, int):
         return stream
     return int(stream.cuda_stream)

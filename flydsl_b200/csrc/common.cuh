@@ -7,6 +7,8 @@
 #include <cuda_fp8.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/flymoe.h"
 
 namespace flymoe {
@@ -35,6 +37,20 @@ void set_last_error_msg(const char* msg);
 
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Raises a kernel's limit of dynamic shared memory, once per kernel (`seen` belongs to it) and device: the runtime call
+// costs a microsecond of every launch otherwise.
+struct SmemLimitSeen { std::atomic<bool> on[64]; };
+inline cudaError_t allow_smem(const void* kernel, int bytes, SmemLimitSeen& seen) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const bool known = dev >= 0 && dev < 64;
+  if (known && seen.on[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && known) seen.on[dev].store(true, std::memory_order_relaxed);
+  return e;
+}
 
 int* device_status_ptr();  // device address of the per-device status word (nullptr on failure)
 int sm_count();  // multiprocessor count of the current device (cached per device)

@@ -87,7 +87,7 @@ topk_gating_softmax_kernel(const T* __restrict__ gating, float* __restrict__ top
     const size_t o = size_t(token) * topk + lane;
     topk_weights[o] = p;
     topk_indices[o] = my_idx;
-    token_expert_indices[o] = lane * num_tokens + token;
+    if (token_expert_indices != nullptr) token_expert_indices[o] = lane * num_tokens + token;
   }
 }
 
@@ -121,7 +121,7 @@ extern "C" int flymoe_topk_gating_softmax(const void* gating, int gating_dtype, 
   FLYMOE_REQUIRE(num_experts >= 1 && num_experts <= 1024, "gating: num_experts must be in [1, 1024]");
   FLYMOE_REQUIRE(topk >= 1 && topk <= 32 && topk <= num_experts, "gating: topk must be in [1, min(32, E)]");
   if (num_tokens == 0) return FLYMOE_OK;
-  FLYMOE_REQUIRE(gating && topk_weights && topk_indices && token_expert_indices, "gating: null pointer");
+  FLYMOE_REQUIRE(gating && topk_weights && topk_indices, "gating: null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (gating_dtype) {
     case FLYMOE_F32:

@@ -324,7 +324,8 @@ template <int FORM>
 static int launch_ragged(const CUtensorMap& ma, const CUtensorMap& mb, const RaggedArgs& a, long long max_tiles,
                          cudaStream_t stream) {
   auto* kernel = grouped_gemm_kernel<FORM>;
-  FLYMOE_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kRagSmem)));
+  static SmemLimitSeen seen;
+  FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(kRagSmem), seen));
   const long long sms = sm_count();
   kernel<<<unsigned(max_tiles < sms ? max_tiles : sms), kRagThreads, kRagSmem, stream>>>(ma, mb, a);
   FLYMOE_CUDA_CHECK(cudaGetLastError());

@@ -600,7 +600,8 @@ template <typename T, int NT>
 static int launch_shrink(const ShrinkArgs& p, cudaStream_t stream) {
   auto* kernel = lora_shrink_kernel<T, NT>;
   constexpr int smem = kShrinkWarps * 16 * NT * 8 * 4;
-  FLYMOE_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static SmemLimitSeen seen;
+  FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), smem, seen));
   kernel<<<dim3(ceil_div(p.rows, 16), p.splits), kShrinkWarps * 32, smem, stream>>>(p);
   FLYMOE_CUDA_CHECK(cudaGetLastError());
   return FLYMOE_OK;
@@ -630,7 +631,8 @@ static int launch_expand_rank(const ExpandArgs& p, cudaStream_t s) {
 template <typename T, int NT>
 static int launch_wgrad(const AdapterGradArgs& p, cudaStream_t stream) {
   auto* kernel = lora_wgrad_kernel<T, NT>;
-  FLYMOE_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(wg_smem<NT>())));
+  static SmemLimitSeen seen;
+  FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(wg_smem<NT>()), seen));
   kernel<<<dim3(p.g[0].tiles + p.g[1].tiles, p.adapters, p.splits), 128, wg_smem<NT>(), stream>>>(p);
   FLYMOE_CUDA_CHECK(cudaGetLastError());
   if (p.splits > 1) {
@@ -683,6 +685,14 @@ extern "C" int flymoe_lora_expand(void* out, const void* base, const float* v, c
   const ExpandArgs p = {base, v, b, ids, scaling, out, rows, n, rank, adapters, splits, 0, 0};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == FLYMOE_BF16 ? launch_expand_rank<__nv_bfloat16>(p, s) : launch_expand_rank<__half>(p, s);
+}
+
+extern "C" int flymoe_lora_add(void* out, const void* base, const void* x, const void* a, const void* b, const int32_t* ids,
+                               const float* scaling, float* v, int rows, int k, int n, int rank, int adapters, int splits,
+                               int dtype, void* stream) {
+  const int rc = flymoe_lora_shrink(v, x, a, ids, rows, k, rank, adapters, splits, 0, dtype, stream);
+  return rc != FLYMOE_OK ? rc
+                         : flymoe_lora_expand(out, base, v, b, ids, scaling, rows, n, rank, adapters, splits, dtype, stream);
 }
 
 extern "C" int flymoe_lora_wgrad_splits(int rows, int k, int n, int adapters) {

@@ -44,7 +44,20 @@ def _check_sizes(experts, n, k):
         raise ValueError(f"n ({n}) and k ({k}) must be positive multiples of 8")
 
 
-def _rows_form(name, t, w, offsets, out, stream, input_grad):
+def _fits(t, w, offsets, out, input_grad):
+    """Whether the arguments are right, in as few steps as it takes; ``_check_rows_form`` says what is not."""
+    try:
+        experts, n, k = w.shape
+        dt, dev = t.dtype, t.device
+        return (t.is_cuda and dt in HALF and t.dim() == 2 and t.shape[1] == (n if input_grad else k)
+                and offsets.shape == (experts + 1,) and w.dtype is dt and offsets.dtype is torch.int32 and w.device == dev
+                and offsets.device == dev and t.is_contiguous() and w.is_contiguous() and offsets.is_contiguous()
+                and n >= 8 and not n % 8 and k >= 8 and not k % 8 and 1 <= experts <= 1024 and out is None)
+    except (AttributeError, ValueError):
+        return False
+
+
+def _check_rows_form(name, t, w, offsets, out, input_grad):
     if not (isinstance(t, torch.Tensor) and isinstance(w, torch.Tensor) and isinstance(offsets, torch.Tensor)):
         raise TypeError(f"{name}, w and offsets must be torch.Tensors")
     require_shape("w", w, (None, None, None))
@@ -52,12 +65,16 @@ def _rows_form(name, t, w, offsets, out, stream, input_grad):
     _check_sizes(experts, n, k)
     require_shape(name, t, (None, n if input_grad else k))
     require_shape("offsets", offsets, (experts + 1,))
-    rows = t.shape[0]
-    cols = k if input_grad else n
-    _check(name, t, "w", w, offsets, out, (rows, cols))
+    _check(name, t, "w", w, offsets, out, (t.shape[0], k if input_grad else n))
+
+
+def _rows_form(name, t, w, offsets, out, stream, input_grad):
+    if not _fits(t, w, offsets, out, input_grad):
+        _check_rows_form(name, t, w, offsets, out, input_grad)
+    (experts, n, k), rows = w.shape, t.shape[0]
     lib = _lib.load()
     with on(t.device, stream):
-        res = torch.empty((rows, cols), dtype=t.dtype, device=t.device) if out is None else out
+        res = t.new_empty((rows, k if input_grad else n)) if out is None else out
         _lib.check(lib.flymoe_grouped_gemm(res.data_ptr(), t.data_ptr(), w.data_ptr(), offsets.data_ptr(), rows, experts, n,
                                            k, _lib.DTYPE_CODE[t.dtype], 1 if input_grad else 0, 1 if out is None else 0,
                                            _lib.stream_handle(None)), "grouped_gemm")
@@ -90,7 +107,7 @@ def grouped_gemm_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor,
     _check("dy", dy, "x", x, offsets, out, (experts, n, k))
     lib = _lib.load()
     with on(dy.device, stream):
-        res = torch.empty((experts, n, k), dtype=dy.dtype, device=dy.device) if out is None else out
+        res = dy.new_empty((experts, n, k)) if out is None else out
         _lib.check(lib.flymoe_grouped_gemm_wgrad(res.data_ptr(), dy.data_ptr(), x.data_ptr(), offsets.data_ptr(), rows,
                                                  experts, n, k, _lib.DTYPE_CODE[dy.dtype], _lib.stream_handle(None)),
                    "grouped_gemm_wgrad")

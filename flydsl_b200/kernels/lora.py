@@ -26,6 +26,21 @@ from ._call import HALF, on, require_same_device, require_shape
 MAX_RANK = 128
 
 
+def _fits(y, x, a, b, ids, scaling, out):
+    """Whether the arguments are right, in as few steps as it takes; ``_check`` says what is not."""
+    try:
+        (rows, k), (adapters, rank, ka), n, dt, dev = x.shape, a.shape, y.shape[1], x.dtype, x.device
+        return (x.is_cuda and dt in HALF and ka == k and y.shape == (rows, n) and b.shape == (adapters, n, rank)
+                and ids.shape == (rows,) and scaling.shape == (adapters,) and y.dtype is dt and a.dtype is dt and b.dtype is dt
+                and ids.dtype is torch.int32 and scaling.dtype is torch.float32 and y.device == dev and a.device == dev
+                and b.device == dev and ids.device == dev and scaling.device == dev and x.is_contiguous()
+                and y.is_contiguous() and a.is_contiguous() and b.is_contiguous() and ids.is_contiguous()
+                and scaling.is_contiguous() and 8 <= rank <= MAX_RANK and not rank % 8 and k >= 8 and not k % 8 and n >= 8
+                and not n % 8 and 1 <= adapters <= 65535 and out is None)
+    except (AttributeError, ValueError, IndexError):
+        return False
+
+
 def _check(y, x, a, b, adapter_ids, scaling, out):
     for name, t in (("y", y), ("x", x), ("a", a), ("b", b), ("adapter_ids", adapter_ids), ("scaling", scaling)):
         if not isinstance(t, torch.Tensor):
@@ -62,7 +77,7 @@ def _shrink(x, a, ids, fold):
     """x [rows, k], a [adapters, rank, k] -> f32 [splits, rows, rank], or with ``fold`` [1, rows, rank]."""
     lib, (rows, k), (adapters, rank, _) = _lib.load(), x.shape, a.shape
     splits = lib.flymoe_lora_shrink_splits(rows, k)
-    v = torch.empty((splits, rows, rank), dtype=torch.float32, device=x.device)
+    v = x.new_empty((splits, rows, rank), dtype=torch.float32)
     _lib.check(lib.flymoe_lora_shrink(v.data_ptr(), x.data_ptr(), a.data_ptr(), ids.data_ptr(), rows, k, rank, adapters,
                                       splits, 1 if fold else 0, _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(None)),
                "lora_shrink")
@@ -79,7 +94,7 @@ def _expand(out, base, v, b, ids, scaling):
 
 def _transposed(t):
     mats, rows, cols = t.shape
-    res = torch.empty((mats, cols, rows), dtype=t.dtype, device=t.device)
+    res = t.new_empty((mats, cols, rows))
     _lib.check(_lib.load().flymoe_lora_transpose(t.data_ptr(), res.data_ptr(), mats, rows, cols, _lib.stream_handle(None)),
                "lora_transpose")
     return res
@@ -110,8 +125,7 @@ class _LoraAdd(torch.autograd.Function):
                 da = torch.empty_like(a) if need_a else None
                 db = torch.empty_like(b) if need_b else None
                 width = (k if need_a else 0) + (n if need_b else 0)
-                partial = (torch.empty(splits * adapters * rank * width, dtype=torch.float32, device=x.device)
-                           if splits > 1 else None)
+                partial = x.new_empty(splits * adapters * rank * width, dtype=torch.float32) if splits > 1 else None
                 _lib.check(lib.flymoe_lora_wgrad(
                     _lib.ptr(da), _lib.ptr(db), x.data_ptr(), dout.data_ptr(), v.data_ptr(), _lib.ptr(dv), ids.data_ptr(),
                     scaling.data_ptr(), _lib.ptr(partial), rows, k, n, rank, adapters, splits, _lib.DTYPE_CODE[x.dtype],
@@ -124,11 +138,19 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     """y + scaling[l] * (x a[l]^T) b[l]^T with l = adapter_ids of the row; see the module docstring.
 
     With ``out`` or ``stream`` the call is for inference only (no input may require a gradient while gradients are on)."""
-    _check(y, x, a, b, adapter_ids, scaling, out)
+    if not _fits(y, x, a, b, adapter_ids, scaling, out):
+        _check(y, x, a, b, adapter_ids, scaling, out)
     if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad):
         if out is not None or stream is not None:
             raise ValueError("out= and stream= are for inference: an input requires a gradient")
         return _LoraAdd.apply(y, x, a, b, adapter_ids, scaling)
     with on(x.device, stream):
-        return _expand(torch.empty_like(y) if out is None else out, y, _shrink(x, a, adapter_ids, fold=False), b, adapter_ids,
-                       scaling)
+        lib, (rows, k), (adapters, rank, _) = _lib.load(), x.shape, a.shape
+        splits = lib.flymoe_lora_shrink_splits(rows, k)
+        v = x.new_empty((splits, rows, rank), dtype=torch.float32)
+        if out is None:
+            out = torch.empty_like(y)
+        _lib.check(lib.flymoe_lora_add(out.data_ptr(), y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(),
+                                       adapter_ids.data_ptr(), scaling.data_ptr(), v.data_ptr(), rows, k, y.shape[1], rank,
+                                       adapters, splits, _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(None)), "lora_add")
+    return out

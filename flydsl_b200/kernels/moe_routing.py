@@ -37,6 +37,20 @@ class RoutedRows(NamedTuple):
     row_index: torch.Tensor
 
 
+def _combine_fits(rows, weights, plan):
+    """Whether the arguments are right, in as few steps as it takes; ``_check_plan`` and the rest say what is not."""
+    try:
+        (sorted_ids, nv, _, row_index), dev, i32 = plan, rows.device, torch.int32
+        return (rows.is_cuda and rows.dtype in _FLOATS and rows.dim() == 2 and rows.shape[1] >= 8 and not rows.shape[1] % 8
+                and weights.shape == row_index.shape and weights.dim() == 2 and weights.dtype is torch.float32
+                and sorted_ids.numel() >= rows.shape[0] and nv.numel() >= 1 and sorted_ids.dtype is i32 and nv.dtype is i32
+                and row_index.dtype is i32 and weights.device == dev and sorted_ids.device == dev and nv.device == dev
+                and row_index.device == dev and rows.is_contiguous() and weights.is_contiguous()
+                and sorted_ids.is_contiguous() and nv.is_contiguous() and row_index.is_contiguous())
+    except (AttributeError, TypeError, ValueError):
+        return False
+
+
 def _check_plan(plan: RoutedRows, name: str, t: torch.Tensor, rows: int) -> tuple[int, int]:
     if not isinstance(plan, tuple) or len(plan) != 4:
         raise TypeError("plan must be a RoutedRows (see route_rows)")
@@ -64,27 +78,31 @@ class _TopkGating(torch.autograd.Function):
     def forward(ctx, logits, topk, renormalize):
         tokens, experts = logits.shape
         with on(logits.device):
-            weights = torch.empty((tokens, topk), dtype=torch.float32, device=logits.device)
-            ids, pair_ids = torch.empty((2, tokens, topk), dtype=torch.int32, device=logits.device).unbind(0)
+            weights = logits.new_empty((tokens, topk), dtype=torch.float32)
+            ids = logits.new_empty((tokens, topk), dtype=torch.int32)
             _lib.check(_lib.load().flymoe_topk_gating_softmax(
-                logits.data_ptr(), _lib.DTYPE_CODE[logits.dtype], weights.data_ptr(), ids.data_ptr(), pair_ids.data_ptr(),
-                tokens, experts, topk, renormalize, _lib.stream_handle(None)), "topk_gating_softmax")
+                logits.data_ptr(), _lib.DTYPE_CODE[logits.dtype], weights.data_ptr(), ids.data_ptr(), None, tokens, experts,
+                topk, renormalize, _lib.stream_handle(None)), "topk_gating_softmax")
         ctx.mark_non_differentiable(ids)
-        ctx.save_for_backward(logits, weights, ids)
-        ctx.renormalize = renormalize
+        ctx.set_materialize_grads(False)         # no zeros are made for the ids
+        # weights that are a softmax over the picks are all that their gradient needs
+        ctx.save_for_backward(weights, ids, *(() if renormalize else (logits,)))
+        ctx.logits = logits.shape, logits.dtype, renormalize
         return weights, ids
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dweights, _):
-        logits, weights, ids = ctx.saved_tensors
-        tokens, experts = logits.shape
+        if dweights is None:
+            return None, None, None
+        weights, ids, *logits = ctx.saved_tensors
+        (tokens, experts), dtype, renormalize = ctx.logits
         dweights = dweights.contiguous()
-        with on(logits.device):
-            d = torch.empty_like(logits)
+        with on(weights.device):
+            d = weights.new_empty((tokens, experts), dtype=dtype)
             _lib.check(_lib.load().flymoe_topk_gating_softmax_backward(
-                logits.data_ptr(), _lib.DTYPE_CODE[logits.dtype], weights.data_ptr(), ids.data_ptr(), dweights.data_ptr(),
-                d.data_ptr(), tokens, experts, ids.shape[1], ctx.renormalize, _lib.stream_handle(None)),
+                _lib.ptr(logits[0]) if logits else None, _lib.DTYPE_CODE[dtype], weights.data_ptr(), ids.data_ptr(),
+                dweights.data_ptr(), d.data_ptr(), tokens, experts, ids.shape[1], renormalize, _lib.stream_handle(None)),
                 "topk_gating_softmax_backward")
         return d, None, None
 
@@ -131,7 +149,7 @@ def route_rows(topk_ids: torch.Tensor, num_experts: int) -> RoutedRows:
 
 # ------------------------------------------------------------------------- rows
 def _combine(rows, weights, plan, tokens, topk):
-    out = torch.empty((tokens, rows.shape[1]), dtype=rows.dtype, device=rows.device)
+    out = rows.new_empty((tokens, rows.shape[1]))
     _lib.check(_lib.load().flymoe_combine_rows(
         rows.data_ptr(), _lib.ptr(weights), out.data_ptr(), plan[0].data_ptr(), plan[1].data_ptr(), plan[3].data_ptr(),
         tokens, topk, rows.shape[0], rows.shape[1], _lib.DTYPE_CODE[rows.dtype], _lib.stream_handle(None)), "combine_rows")
@@ -145,7 +163,7 @@ class _Permute(torch.autograd.Function):
         tokens, topk = row_index.shape
         rows = tokens * topk
         with on(x.device):
-            xs = torch.empty((rows, x.shape[1]), dtype=x.dtype, device=x.device)
+            xs = x.new_empty((rows, x.shape[1]))
             _lib.check(_lib.load().flymoe_permute_rows(
                 x.data_ptr(), xs.data_ptr(), sorted_ids.data_ptr(), num_valid_ids.data_ptr(), row_index.data_ptr(), tokens,
                 topk, rows, x.shape[1] * x.element_size(), _lib.stream_handle(None)), "permute_rows")
@@ -195,9 +213,10 @@ class _Combine(torch.autograd.Function):
 
 def moe_combine(rows: torch.Tensor, weights: torch.Tensor, plan: RoutedRows) -> torch.Tensor:
     """rows [any, dim] in expert order, weights f32 [tokens, topk] -> [tokens, dim]; gradients reach rows and weights."""
-    _require_rows("rows", rows)
-    tokens, topk = _check_plan(plan, "rows", rows, rows.shape[0])
-    _lib.require_cuda("weights", weights, (torch.float32,))
-    require_shape("weights", weights, (tokens, topk))
-    require_same_device("rows", rows.device, weights=weights)
+    if not _combine_fits(rows, weights, plan):
+        _require_rows("rows", rows)
+        tokens, topk = _check_plan(plan, "rows", rows, rows.shape[0])
+        _lib.require_cuda("weights", weights, (torch.float32,))
+        require_shape("weights", weights, (tokens, topk))
+        require_same_device("rows", rows.device, weights=weights)
     return _Combine.apply(rows, weights, *plan)

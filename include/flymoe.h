@@ -71,7 +71,7 @@ int flymoe_device_status(int* status_out);
  * :336-344 (GatingOutput, TopkWeights, TopkIndices, TokenExpertIndices, num_tokens, stream).
  * gating [T,E] of gating_dtype (F32/F16/BF16), row-major.  topk_weights f32 [T,k],
  * topk_indices i32 [T,k] (descending by logit, ties to the lower expert id),
- * token_expert_indices i32 [T,k] = k_idx*T + t. */
+ * token_expert_indices i32 [T,k] = k_idx*T + t, or NULL. */
 int flymoe_topk_gating_softmax(const void* gating, int gating_dtype, float* topk_weights,
                                int32_t* topk_indices, int32_t* token_expert_indices,
                                int num_tokens, int num_experts, int topk, int renormalize,
@@ -366,6 +366,7 @@ int flymoe_combine_rows_backward(const void* dout, const void* rows_in, const fl
  * out[m] = base[m] + scaling[l] * B_l (A_l x[m]) with l = ids[m]; rows whose id is outside [0, adapters) pass through.
  * a [adapters, rank, k], b [adapters, n, rank], ids i32 [rows] in any order, scaling f32 [adapters].  rank a multiple of 8
  * up to 128, k and n multiples of 8, pointers 16-byte aligned.  Sums in fp32, the output rounded once.
+ * flymoe_lora_add: the two calls that follow in one (v f32 [splits, rows, rank] is scratch).
  * flymoe_lora_shrink: v f32 [splits, rows, rank] = partial sums of x A_l^T over `splits` pieces of k (zeros for a row without
  * an adapter); with `fold` they are added up into the first piece.  flymoe_lora_shrink_splits: the number that fills the
  * current device, 1..16.
@@ -375,6 +376,9 @@ int flymoe_combine_rows_backward(const void* dout, const void* rows_in, const fl
  * flymoe_lora_wgrad: da[l] = scaling[l] sum over l's rows of dv^T x, db[l] = scaling[l] sum of dout^T v (v, dv f32 [rows,
  * rank]); da or db may be NULL; an adapter without rows gets zeros.  splits > 1 cuts the rows, partial is then f32 scratch of
  * splits * adapters * rank * (k if da + n if db); flymoe_lora_wgrad_splits proposes a number.  No counterpart in the reference. */
+int flymoe_lora_add(void* out, const void* base, const void* x, const void* a, const void* b, const int32_t* ids,
+                    const float* scaling, float* v, int rows, int k, int n, int rank, int adapters, int splits, int dtype,
+                    void* stream);
 int flymoe_lora_shrink_splits(int rows, int k);
 int flymoe_lora_shrink(float* v, const void* x, const void* a, const int32_t* ids, int rows, int k, int rank, int adapters,
                        int splits, int fold, int dtype, void* stream);
