@@ -21,15 +21,14 @@
 // consecutive elements where the instruction's layout has pairs.
 #include <algorithm>
 #include <stdio.h>
+#include <stdlib.h>
 #include <type_traits>
 
 #include "common.cuh"
 #include "gemm_ptx.cuh"
+#include "lora_common.cuh"
 
 namespace flymoe {
-
-constexpr int kLoraMaxRank = 128;
-constexpr int kLoraMaxSplits = 16;
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
@@ -45,90 +44,145 @@ __device__ __forceinline__ void mma16816<__half>(float* c, const uint32_t* a, ui
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) { return pack_f16x2(a, b); }
-template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
-template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
-  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
-}
-template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&v));
-}
-// Two floats as high parts and remainders.  Where the high part is not finite there is no remainder.
-template <typename T>
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack2<T>(a, b);
-  const float2 h = unpack2<T>(hi);
-  lo = pack2<T>(isfinite(h.x) ? a - h.x : 0.f, isfinite(h.y) ? b - h.y : 0.f);
-}
-// 2^e and 2^-e with the largest of `amax`'s numbers at 2^13 .. 2^14 afterwards (fp16 overflows at 2^16).
-__device__ __forceinline__ int scale_exponent(float amax) {
-  if (!(amax > 0.f)) return 0;
-  const int e = int((__float_as_uint(amax) >> 23) & 0xff) - 127;     // 128: infinite, NaN
-  return e >= 128 ? 0 : max(-110, min(110, e - 13));
-}
-__device__ __forceinline__ float exp2i(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }
-__device__ __forceinline__ float finite_abs(float x) { return isfinite(x) ? fabsf(x) : 0.f; }
 __device__ __forceinline__ uint4 ldg16(const void* p) { return __ldg(static_cast<const uint4*>(p)); }
-__device__ __forceinline__ bool in_use(int id, int adapters) { return id >= 0 && id < adapters; }
 
-// ---------------------------------------------------------------------------- shrink
-struct ShrinkArgs {
-  const void* x;               // [rows, k]
-  const void* a;               // [adapters, rank, k]
-  const int* ids;              // [rows]
-  float* v;                    // [splits, rows, rank]
-  int rows, k, rank, adapters, splits;
+// ---------------------------------------------------------------------------- groups of rows
+// The rows of a window (512) in groups of up to 16 that share an adapter, whatever order they come in.  Every block builds
+// them for itself and all blocks alike: adapters in the order of their first rows, their rows in order.  A hash table finds
+// the rows of an adapter; what is kept of it, the smallest row, does not depend on the order of its atomics.
+constexpr int kWindow = 512, kTable = 1024;
+constexpr int kGroupThreads = 256;
+struct Groups {
+  int id[kWindow];             // adapter of a row; -1: none
+  uint16_t order[kWindow];     // rows of the window, an adapter's next to each other
+  uint16_t start[kWindow + 2]; // first entry of `order` of a group; an adapter's groups follow each other
+  uint16_t row_base[kWindow], group_base[kWindow];     // at an adapter's first row: entries and groups before it
+  uint8_t in_chunk[kWindow / 32][kWindow];             // rows among 32 of the adapter with that first row
+  int key[kTable], first[kTable];
+  int warp_sum[2][8], count, skip[kWindow / 128];
 };
-constexpr int kShrinkWarps = 8;
 
-// A block takes 16 rows and one split of K.  Its warps share out (adapter, part of the split): one adapter gets all eight
-// warps, eight or more one warp each; the parts meet in shared memory in a fixed order.
-template <typename T, int NT>
-__global__ void __launch_bounds__(kShrinkWarps * 32)
-lora_shrink_kernel(const ShrinkArgs p) {
-  constexpr int RP = NT * 8;
-  extern __shared__ float part[];                      // [parts][16][RP]
-  __shared__ int row_id[16], list[16], count;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int row0 = blockIdx.x * 16;
-  if (warp == 0) {
-    int id = -1;
-    if (lane < 16 && row0 + lane < p.rows) {
-      id = __ldg(p.ids + row0 + lane);
-      if (!in_use(id, p.adapters)) id = -1;
-    }
-    const uint32_t same = __match_any_sync(0xffffffffu, id);
-    const bool first = id >= 0 && (same & ((1u << lane) - 1)) == 0;
-    const uint32_t firsts = __ballot_sync(0xffffffffu, first);
-    if (first) list[__popc(firsts & ((1u << lane) - 1))] = id;
-    if (lane < 16) row_id[lane] = id;
-    if (lane == 0) count = __popc(firsts);
+// skip_tiles: rows of 128-row tiles with at most kTileAdapters distinct adapters belong to the tcgen05 kernels.  keep_none:
+// rows without an adapter form groups as well (adapter -1).
+__device__ __forceinline__ void build_groups(Groups* s, const int* ids, int row0, int rows, int adapters, bool skip_tiles,
+                                             bool keep_none) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n = min(kWindow, rows - row0), chunks = (n + 31) / 32;
+  const int mask = (n > 128 ? kTable : 256) - 1;               // at least twice as many entries as rows
+  for (int i = tid; i <= mask; i += kGroupThreads) { s->key[i] = -2; s->first[i] = kWindow; }
+  for (int i = tid; i < chunks * kWindow / 4; i += kGroupThreads) reinterpret_cast<int*>(s->in_chunk)[i] = 0;
+  if (skip_tiles && warp < kWindow / 128) {
+    int q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = row_adapter(ids, row0 + warp * 128 + i * 32 + lane, rows, adapters);
+    const int d = tile_adapters(q, lane, nullptr);
+    if (lane == 0) s->skip[warp] = d <= kTileAdapters;
   }
   __syncthreads();
-  const int d = count;
-  const int parts = d == 0 ? 1 : d >= kShrinkWarps ? 1 : kShrinkWarps / d;
+  int slot[2], lead[2], rank[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int i = u * kGroupThreads + tid;
+    slot[u] = -1;
+    if (i >= n) continue;
+    const int id = row_adapter(ids, row0 + i, rows, adapters);
+    s->id[i] = id;
+    if ((id < 0 && !keep_none) || (skip_tiles && s->skip[i / 128])) continue;
+    int h = int((uint32_t(id) * 0x9E3779B1u) >> 22) & mask;
+    for (;; h = (h + 1) & mask) {
+      const int old = atomicCAS(&s->key[h], -2, id);
+      if (old == -2 || old == id) break;
+    }
+    atomicMin(&s->first[h], i);
+    slot[u] = h;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    lead[u] = slot[u] >= 0 ? s->first[slot[u]] : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, lead[u]);
+    rank[u] = __popc(same & ((1u << lane) - 1));
+    if (lead[u] >= 0 && rank[u] == 0) s->in_chunk[u * 8 + warp][lead[u]] = uint8_t(__popc(same));
+  }
+  __syncthreads();
+  // totals at the first rows, two neighbouring rows a thread so that a scan over threads is one over rows
+  int total[2] = {0, 0};
+  for (int c = 0; c < chunks; ++c) {
+    const int v = *reinterpret_cast<const uint16_t*>(&s->in_chunk[c][2 * tid]);
+    total[0] += v & 0xff;
+    total[1] += v >> 8;
+  }
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (lead[u] >= 0)
+      for (int c = 0; c < u * 8 + warp; ++c) rank[u] += s->in_chunk[c][lead[u]];
+  const int rows_here = total[0] + total[1], groups_here = (total[0] + 15) / 16 + (total[1] + 15) / 16;
+  int rs = rows_here, gs = groups_here;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, rs, off), b = __shfl_up_sync(0xffffffffu, gs, off);
+    if (lane >= off) { rs += a; gs += b; }
+  }
+  if (lane == 31) { s->warp_sum[0][warp] = rs; s->warp_sum[1][warp] = gs; }
+  __syncthreads();
+  int rb = rs - rows_here, gb = gs - groups_here, all_groups = 0, all_rows = 0;
+#pragma unroll
+  for (int w = 0; w < kGroupThreads / 32; ++w) {
+    if (w < warp) { rb += s->warp_sum[0][w]; gb += s->warp_sum[1][w]; }
+    all_rows += s->warp_sum[0][w];
+    all_groups += s->warp_sum[1][w];
+  }
+  s->row_base[2 * tid] = uint16_t(rb);
+  s->row_base[2 * tid + 1] = uint16_t(rb + total[0]);
+  s->group_base[2 * tid] = uint16_t(gb);
+  s->group_base[2 * tid + 1] = uint16_t(gb + (total[0] + 15) / 16);
+  if (tid == 0) { s->count = all_groups; s->start[all_groups] = uint16_t(all_rows); }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    if (lead[u] >= 0) {
+      const int pos = s->row_base[lead[u]] + rank[u];
+      s->order[pos] = uint16_t(u * kGroupThreads + tid);
+      if ((rank[u] & 15) == 0) s->start[s->group_base[lead[u]] + rank[u] / 16] = uint16_t(pos);
+    }
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------- shrink
+constexpr int kShrinkWarps = kGroupThreads / 32;
+
+// Blocks share out the groups of a window (`slots` of them) and the splits of K; within a split each of the eight warps takes
+// a part of every group's product, and the parts meet in shared memory in a fixed order.
+template <typename T, int NT>
+__global__ void __launch_bounds__(kGroupThreads)
+lora_shrink_kernel(const ShrinkArgs p, const int slots, const bool skip_tiles) {
+  constexpr int RP = NT * 8;
+  extern __shared__ __align__(16) float part[];        // [warps][16][RP]
+  __shared__ __align__(16) Groups s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int row0 = int(blockIdx.x) / slots * kWindow;
+  build_groups(&s, p.ids, row0, p.rows, p.adapters, skip_tiles, false);
   const int steps = (p.k + 31) / 32;
   const int s0 = int((long long)steps * blockIdx.y / p.splits), s1 = int((long long)steps * (blockIdx.y + 1) / p.splits);
-  const T* xr0 = static_cast<const T*>(p.x) + (long long)min(row0 + g, p.rows - 1) * p.k;
-  const T* xr1 = static_cast<const T*>(p.x) + (long long)min(row0 + g + 8, p.rows - 1) * p.k;
-  const int id0 = row_id[g], id1 = row_id[g + 8];
+  const int from = s0 + (s1 - s0) * warp / kShrinkWarps, to = s0 + (s1 - s0) * (warp + 1) / kShrinkWarps;
   constexpr int U = NT <= 2 ? 4 : NT <= 4 ? 2 : 1;     // steps whose loads are in flight together
-  for (int item = warp; item < d * parts; item += kShrinkWarps) {
-    const int which = item / parts, part_i = item - which * parts;
-    const int l = list[which];
-    const int from = s0 + (s1 - s0) * part_i / parts, to = s0 + (s1 - s0) * (part_i + 1) / parts;
+  for (int grp = int(blockIdx.x) % slots; grp < s.count; grp += slots) {
+    const int at = s.start[grp];
+    const int l = s.id[s.order[at]];
+    // the group ends with the adapter's rows or after sixteen of them
+    const int n = min(16, s.start[grp + 1] - at);
+    const T* xr0 = static_cast<const T*>(p.x) + (long long)(row0 + s.order[at + min(g, n - 1)]) * p.k;
+    const T* xr1 = static_cast<const T*>(p.x) + (long long)(row0 + s.order[at + min(g + 8, n - 1)]) * p.k;
     const T* al = static_cast<const T*>(p.a) + (long long)l * p.rank * p.k;
     float c[NT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
-    for (int s = from; s < to; s += U) {
+    for (int st = from; st < to; st += U) {
       uint4 x0[U], x1[U], b[U][NT];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int k = (s + u) * 32 + t * 8;
-        const bool ok = s + u < to && k < p.k;
+        const int k = (st + u) * 32 + t * 8;
+        const bool ok = st + u < to && k < p.k;
         const uint4 zero = make_uint4(0, 0, 0, 0);
         x0[u] = ok ? ldg16(xr0 + k) : zero;
         x1[u] = ok ? ldg16(xr1 + k) : zero;
@@ -145,22 +199,22 @@ lora_shrink_kernel(const ShrinkArgs p) {
         }
       }
     }
-    float* slot = part + part_i * 16 * RP;
+    float* slot = part + warp * 16 * RP;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      if (id0 == l) *reinterpret_cast<float2*>(slot + g * RP + i * 8 + t * 2) = make_float2(c[i][0], c[i][1]);
-      if (id1 == l) *reinterpret_cast<float2*>(slot + (g + 8) * RP + i * 8 + t * 2) = make_float2(c[i][2], c[i][3]);
+      *reinterpret_cast<float2*>(slot + g * RP + i * 8 + t * 2) = make_float2(c[i][0], c[i][1]);
+      *reinterpret_cast<float2*>(slot + (g + 8) * RP + i * 8 + t * 2) = make_float2(c[i][2], c[i][3]);
     }
-  }
-  __syncthreads();
-  float* out = p.v + ((long long)blockIdx.y * p.rows + row0) * p.rank;
-  for (int i = threadIdx.x; i < 16 * p.rank; i += kShrinkWarps * 32) {
-    const int r = i / p.rank, j = i - r * p.rank;
-    if (row0 + r >= p.rows) break;
-    float sum = 0.f;
-    if (row_id[r] >= 0)
-      for (int q = 0; q < parts; ++q) sum += part[(q * 16 + r) * RP + j];
-    out[i] = sum;
+    __syncthreads();
+    float* out = p.v + (long long)blockIdx.y * p.rows * p.rank;
+    for (int i = threadIdx.x; i < n * p.rank; i += kGroupThreads) {
+      const int r = i / p.rank, j = i - r * p.rank;
+      float sum = 0.f;
+#pragma unroll
+      for (int q = 0; q < kShrinkWarps; ++q) sum += part[(q * 16 + r) * RP + j];
+      out[(long long)(row0 + s.order[at + r]) * p.rank + j] = sum;
+    }
+    __syncthreads();
   }
 }
 
@@ -178,137 +232,101 @@ lora_fold_kernel(float4* __restrict__ v, long long vecs, int splits) {
 }
 
 // ---------------------------------------------------------------------------- expand
-struct ExpandArgs {
-  const void* base;            // [rows, n] or null (zeros); may be `out`
-  const float* v;              // [splits, rows, rank]
-  const void* b;               // [adapters, n, rank]
-  const int* ids;
-  const float* scaling;        // [adapters]
-  void* out;                   // [rows, n]
-  int rows, n, rank, adapters, splits;
-  int row_groups, groups_per_warp;
-};
-
-// A warp takes 16 * MF rows and `groups_per_warp` groups of 32 columns.  The columns of a group are dealt to the four
-// 8-wide MMAs so that a lane ends up with eight consecutive ones: base and output move 16 bytes a lane.
-template <typename T, int KS, int MF>
-__global__ void __launch_bounds__(128)
-lora_expand_kernel(const ExpandArgs p) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int rg = int(w % p.row_groups);
-  const int c0 = int(w / p.row_groups) * p.groups_per_warp * 32;
+// Blocks share out the groups of a window (`slots`) and the columns: a warp walks through `per_warp` groups of 32 columns
+// with a row group's v in registers.  The columns are dealt to the four 8-wide MMAs so that a lane ends up with eight
+// consecutive ones: base and output move 16 bytes a lane.
+template <typename T, int KS>
+__global__ void __launch_bounds__(kGroupThreads)
+lora_expand_kernel(const ExpandArgs p, const int slots, const int per_warp, const bool skip_tiles) {
+  __shared__ __align__(16) Groups s;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int row0 = int(blockIdx.x) / slots * kWindow;
+  // rows without an adapter have to be written unless they are there already
+  build_groups(&s, p.ids, row0, p.rows, p.adapters, skip_tiles, p.out != p.base);
+  const int c0 = (int(blockIdx.y) * (kGroupThreads / 32) + warp) * per_warp * 32;
   if (c0 >= p.n) return;
-  const int row0 = rg * 16 * MF;
-  int my_id = -1;
-  if (lane < 16 * MF && row0 + lane < p.rows) {
-    my_id = __ldg(p.ids + row0 + lane);
-    if (!in_use(my_id, p.adapters)) my_id = -1;
-  }
-  const uint32_t used = __ballot_sync(0xffffffffu, my_id >= 0);
-  // the rows of this lane: g, g + 8 of every 16-row fragment
-  int id[2 * MF];
-  float scale[2 * MF];
-  uint32_t hi[MF][KS][4], lo[MF][KS][4];
-#pragma unroll
-  for (int f = 0; f < MF; ++f)
+  for (int grp = int(blockIdx.x) % slots; grp < s.count; grp += slots) {
+    const int at = s.start[grp], n = min(16, s.start[grp + 1] - at);
+    const int l = s.id[s.order[at]];
+    const long long row[2] = {row0 + s.order[at + min(g, n - 1)], row0 + s.order[at + min(g + 8, n - 1)]};
+    const bool live[2] = {g < n, g + 8 < n};
+    float scale[2];
+    uint32_t hi[KS][4], lo[KS][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = f * 16 + h * 8 + g, row = row0 + r;
-      id[f * 2 + h] = __shfl_sync(0xffffffffu, my_id, r);
-      const bool live = id[f * 2 + h] >= 0;
-      scale[f * 2 + h] = live ? __ldg(p.scaling + id[f * 2 + h]) : 0.f;
+      scale[h] = l >= 0 ? __ldg(p.scaling + l) : 0.f;
       float4 x[KS];
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         x[ks] = make_float4(0.f, 0.f, 0.f, 0.f);
         const int k = ks * 16 + t * 4;
-        if (live && k < p.rank)
-          for (int s = 0; s < p.splits; ++s) {
-            const float4 q = __ldg(reinterpret_cast<const float4*>(p.v + ((long long)s * p.rows + row) * p.rank + k));
-            x[ks].x += q.x; x[ks].y += q.y; x[ks].z += q.z; x[ks].w += q.w;
+        if (l >= 0 && live[h] && k < p.rank)
+          for (int q = 0; q < p.splits; ++q) {
+            const float4 v = __ldg(reinterpret_cast<const float4*>(p.v + ((long long)q * p.rows + row[h]) * p.rank + k));
+            x[ks].x += v.x; x[ks].y += v.y; x[ks].z += v.z; x[ks].w += v.w;
           }
       }
       if constexpr (std::is_same<T, __half>::value) {
         float amax = 0.f;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-          amax = fmaxf(amax, fmaxf(fmaxf(fabsf(x[ks].x), fabsf(x[ks].y)), fmaxf(fabsf(x[ks].z), fabsf(x[ks].w))));
+          amax = fmaxf(amax, fmaxf(fmaxf(finite_abs(x[ks].x), finite_abs(x[ks].y)), fmaxf(finite_abs(x[ks].z), finite_abs(x[ks].w))));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const int e = scale_exponent(amax);
         const float down = exp2i(-e);
-        scale[f * 2 + h] *= exp2i(e);
+        scale[h] *= exp2i(e);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) { x[ks].x *= down; x[ks].y *= down; x[ks].z *= down; x[ks].w *= down; }
       }
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        split2<T>(x[ks].x, x[ks].y, hi[f][ks][h], lo[f][ks][h]);
-        split2<T>(x[ks].z, x[ks].w, hi[f][ks][2 + h], lo[f][ks][2 + h]);
+        split2<T>(x[ks].x, x[ks].y, hi[ks][h], lo[ks][h]);
+        split2<T>(x[ks].z, x[ks].w, hi[ks][2 + h], lo[ks][2 + h]);
       }
     }
-  const bool copies = p.out != p.base;           // rows without an adapter have to be written too
-  for (int grp = 0; grp < p.groups_per_warp; ++grp) {
-    const int col = c0 + grp * 32 + t * 8;       // this lane's eight columns
-    if (c0 + grp * 32 >= p.n) break;
-    uint4 y[2 * MF];
+    const T* bl = static_cast<const T*>(p.b) + (long long)max(l, 0) * p.n * p.rank;
+    for (int cg = 0; cg < per_warp && c0 + cg * 32 < p.n; ++cg) {
+      const int col = c0 + cg * 32 + t * 8;      // this lane's eight columns
+      uint4 y[2];
 #pragma unroll
-    for (int i = 0; i < 2 * MF; ++i) {
-      const int row = row0 + i * 8 + g;
-      y[i] = p.base && row < p.rows && col < p.n
-                 ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + (long long)row * p.n + col)
-                 : make_uint4(0, 0, 0, 0);
-    }
-    if (copies) {
+      for (int h = 0; h < 2; ++h)
+        y[h] = p.base && live[h] && col < p.n ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + row[h] * p.n + col)
+                                              : make_uint4(0, 0, 0, 0);
+      float c[4][4];
 #pragma unroll
-      for (int i = 0; i < 2 * MF; ++i) {
-        const int row = row0 + i * 8 + g;
-        if (id[i] < 0 && row < p.rows && col < p.n)
-          *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (long long)row * p.n + col) = y[i];
-      }
-    }
-    for (uint32_t left = used; left;) {
-      const int l = __shfl_sync(0xffffffffu, my_id, __ffs(left) - 1);
-      left &= ~__ballot_sync(0xffffffffu, my_id == l);
-      const T* bl = static_cast<const T*>(p.b) + (long long)l * p.n * p.rank;
-      float c[MF][4][4];
+      for (int j = 0; j < 4; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+      if (l >= 0) {
+        uint2 b[KS][4];
 #pragma unroll
-      for (int f = 0; f < MF; ++f)
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) c[f][j][0] = c[f][j][1] = c[f][j][2] = c[f][j][3] = 0.f;
+          for (int j = 0; j < 4; ++j) {
+            const int k = ks * 16 + t * 4, bc = c0 + cg * 32 + 8 * (g >> 1) + 2 * j + (g & 1);
+            b[ks][j] = bc < p.n && k < p.rank ? __ldg(reinterpret_cast<const uint2*>(bl + (long long)bc * p.rank + k))
+                                              : make_uint2(0, 0);
+          }
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        uint2 b[4];
-        const int k = ks * 16 + t * 4;
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int bc = c0 + grp * 32 + 8 * (g >> 1) + 2 * j + (g & 1);
-          b[j] = bc < p.n && k < p.rank ? __ldg(reinterpret_cast<const uint2*>(bl + (long long)bc * p.rank + k))
-                                        : make_uint2(0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int f = 0; f < MF; ++f) {
-            mma16816<T>(c[f][j], hi[f][ks], b[j].x, b[j].y);
-            mma16816<T>(c[f][j], lo[f][ks], b[j].x, b[j].y);
+          for (int j = 0; j < 4; ++j) {
+            mma16816<T>(c[j], hi[ks], b[ks][j].x, b[ks][j].y);
+            mma16816<T>(c[j], lo[ks], b[ks][j].x, b[ks][j].y);
           }
       }
 #pragma unroll
-      for (int i = 0; i < 2 * MF; ++i) {
-        const int row = row0 + i * 8 + g;
-        if (id[i] != l || col >= p.n) continue;
-        const float s = scale[i];
-        uint4 o;
-        uint32_t* ow = reinterpret_cast<uint32_t*>(&o);
-        const uint32_t* yw = reinterpret_cast<const uint32_t*>(&y[i]);
+      for (int h = 0; h < 2; ++h) {
+        if (!live[h] || col >= p.n) continue;
+        uint4 o = y[h];
+        if (l >= 0) {
+          uint32_t* ow = reinterpret_cast<uint32_t*>(&o);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 q = unpack2<T>(yw[j]);
-          ow[j] = pack2<T>(fmaf(s, c[i >> 1][j][(i & 1) * 2], q.x), fmaf(s, c[i >> 1][j][(i & 1) * 2 + 1], q.y));
+          for (int j = 0; j < 4; ++j) {
+            const float2 q = unpack2<T>(ow[j]);
+            ow[j] = pack2<T>(fmaf(scale[h], c[j][h * 2], q.x), fmaf(scale[h], c[j][h * 2 + 1], q.y));
+          }
         }
-        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + (long long)row * p.n + col) = o;
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + row[h] * p.n + col) = o;
       }
     }
   }
@@ -581,6 +599,8 @@ lora_transpose_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ d
 }
 
 // ---------------------------------------------------------------------------- host
+static int envint(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
+static bool on_tiles(int rows) { return rows >= envint("TC", 1024); }
 static int lora_check(const char* what, int rows, int width, int rank, int adapters, int splits, int dtype) {
   char msg[160];
   const char* why = nullptr;
@@ -596,37 +616,47 @@ static int lora_check(const char* what, int rows, int width, int rank, int adapt
   return FLYMOE_ERR_INVALID_ARGUMENT;
 }
 
+// Groups that a window of up to 512 rows can hold: one for every sixteen rows and one for every adapter's last.
+static int window_groups(int rows, int adapters) {
+  const int n = std::min(rows, kWindow);
+  return std::min(n, n / 16 + std::min(adapters + 1, n));
+}
 template <typename T, int NT>
-static int launch_shrink(const ShrinkArgs& p, cudaStream_t stream) {
+static int launch_shrink(const ShrinkArgs& p, bool skip_tiles, cudaStream_t stream) {
   auto* kernel = lora_shrink_kernel<T, NT>;
   constexpr int smem = kShrinkWarps * 16 * NT * 8 * 4;
   static SmemLimitSeen seen;
   FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), smem, seen));
-  kernel<<<dim3(ceil_div(p.rows, 16), p.splits), kShrinkWarps * 32, smem, stream>>>(p);
+  // three blocks for every SM where there are that many groups
+  const int windows = ceil_div(p.rows, kWindow);
+  const int slots = std::max(1, std::min(window_groups(p.rows, p.adapters), 3 * sm_count() / (windows * p.splits)));
+  kernel<<<dim3(windows * slots, p.splits), kGroupThreads, smem, stream>>>(p, slots, skip_tiles);
   FLYMOE_CUDA_CHECK(cudaGetLastError());
   return FLYMOE_OK;
 }
 template <typename T>
-static int launch_shrink_rank(const ShrinkArgs& p, cudaStream_t s) {
-  return p.rank <= 16 ? launch_shrink<T, 2>(p, s) : p.rank <= 32 ? launch_shrink<T, 4>(p, s)
-       : p.rank <= 64 ? launch_shrink<T, 8>(p, s) : launch_shrink<T, 16>(p, s);
+static int launch_shrink_rank(const ShrinkArgs& p, bool skip, cudaStream_t s) {
+  return p.rank <= 16 ? launch_shrink<T, 2>(p, skip, s) : p.rank <= 32 ? launch_shrink<T, 4>(p, skip, s)
+       : p.rank <= 64 ? launch_shrink<T, 8>(p, skip, s) : launch_shrink<T, 16>(p, skip, s);
 }
-template <typename T, int KS, int MF>
-static int launch_expand(ExpandArgs p, cudaStream_t stream) {
-  p.row_groups = ceil_div(p.rows, 16 * MF);
-  const long long groups = ceil_div(p.n, 32);
-  // columns a warp walks through with its rows' v in registers: as many as leave every SM 16 warps
-  const long long per = groups * p.row_groups / (16LL * sm_count());
-  p.groups_per_warp = int(per < 1 ? 1 : per > 8 ? 8 : per);
-  const long long warps = (long long)p.row_groups * ceil_div(int(groups), p.groups_per_warp);
-  lora_expand_kernel<T, KS, MF><<<unsigned((warps + 3) / 4), 128, 0, stream>>>(p);
+template <typename T, int KS>
+static int launch_expand(const ExpandArgs& p, bool skip_tiles, cudaStream_t stream) {
+  const int windows = ceil_div(p.rows, kWindow), cols = ceil_div(p.n, 32), warps = kGroupThreads / 32;
+  // Three blocks for every SM: row groups first, then columns.  A warp walks through up to eight column groups.
+  const int want = 3 * sm_count();
+  const int groups = window_groups(p.rows, p.adapters);
+  const int spans = std::max(ceil_div(cols, 8 * warps), std::min(ceil_div(cols, warps), want / std::min(want, windows * groups)));
+  const int per_warp = ceil_div(cols, spans * warps);
+  const int slots = std::max(1, std::min(groups, want / (windows * spans)));
+  lora_expand_kernel<T, KS><<<dim3(windows * slots, ceil_div(cols, per_warp * warps)), kGroupThreads, 0, stream>>>(
+      p, slots, per_warp, skip_tiles);
   FLYMOE_CUDA_CHECK(cudaGetLastError());
   return FLYMOE_OK;
 }
 template <typename T>
-static int launch_expand_rank(const ExpandArgs& p, cudaStream_t s) {
-  return p.rank <= 16 ? launch_expand<T, 1, 2>(p, s) : p.rank <= 32 ? launch_expand<T, 2, 2>(p, s)
-       : p.rank <= 64 ? launch_expand<T, 4, 2>(p, s) : launch_expand<T, 8, 1>(p, s);
+static int launch_expand_rank(const ExpandArgs& p, bool skip, cudaStream_t s) {
+  return p.rank <= 16 ? launch_expand<T, 1>(p, skip, s) : p.rank <= 32 ? launch_expand<T, 2>(p, skip, s)
+       : p.rank <= 64 ? launch_expand<T, 4>(p, skip, s) : launch_expand<T, 8>(p, skip, s);
 }
 template <typename T, int NT>
 static int launch_wgrad(const AdapterGradArgs& p, cudaStream_t stream) {
@@ -651,9 +681,11 @@ static int launch_wgrad_rank(const AdapterGradArgs& p, cudaStream_t s) {
 
 extern "C" int flymoe_lora_shrink_splits(int rows, int k) {
   if (rows < 1 || k < 8) return 1;
-  // enough blocks of 16 rows for two on every SM, at least eight 32-wide steps (one a warp) in a split
+  if (flymoe::on_tiles(rows))                    // two tiles of 128 rows for every SM, at least four K blocks of 64 in a split
+    return std::max(1, std::min({flymoe::kLoraMaxSplits, 2 * flymoe::sm_count() / flymoe::ceil_div(rows, 128), k / 256}));
+  // blocks of 16 rows for three on every SM, at least sixteen 32-wide steps (two a warp) in a split
   const int groups = flymoe::ceil_div(rows, 16), steps = flymoe::ceil_div(k, 32);
-  return std::max(1, std::min({flymoe::kLoraMaxSplits, 2 * flymoe::sm_count() / groups, steps / 8}));
+  return std::max(1, std::min({flymoe::kLoraMaxSplits, 3 * flymoe::sm_count() / groups, steps / 16}));
 }
 
 extern "C" int flymoe_lora_shrink(float* v, const void* x, const void* a, const int32_t* ids, int rows, int k, int rank,
@@ -665,7 +697,10 @@ extern "C" int flymoe_lora_shrink(float* v, const void* x, const void* a, const 
   FLYMOE_REQUIRE(aligned16(x) && aligned16(a) && aligned16(v), "lora_shrink: pointers must be 16-byte aligned");
   const ShrinkArgs p = {x, a, ids, v, rows, k, rank, adapters, splits};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  rc = dtype == FLYMOE_BF16 ? launch_shrink_rank<__nv_bfloat16>(p, s) : launch_shrink_rank<__half>(p, s);
+  const bool skip = on_tiles(rows);
+  if (skip) rc = launch_shrink_sm100(p, dtype == FLYMOE_BF16, s);
+  if (rc == FLYMOE_OK && (!skip || adapters > kTileAdapters))
+    rc = dtype == FLYMOE_BF16 ? launch_shrink_rank<__nv_bfloat16>(p, skip, s) : launch_shrink_rank<__half>(p, skip, s);
   if (rc != FLYMOE_OK || !fold || splits == 1) return rc;
   const long long vecs = (long long)rows * rank / 4;
   lora_fold_kernel<<<unsigned(std::min<long long>((vecs + 255) / 256, 4LL * sm_count())), 256, 0, s>>>(
@@ -682,17 +717,25 @@ extern "C" int flymoe_lora_expand(void* out, const void* base, const float* v, c
   if (rc != FLYMOE_OK || rows == 0) return rc;
   FLYMOE_REQUIRE(out && v && b && ids && scaling, "lora_expand: null pointer");
   FLYMOE_REQUIRE(aligned16(out) && aligned16(base) && aligned16(v) && aligned16(b), "lora_expand: pointers must be 16-byte aligned");
-  const ExpandArgs p = {base, v, b, ids, scaling, out, rows, n, rank, adapters, splits, 0, 0};
+  FLYMOE_REQUIRE(splits == 1 || !on_tiles(rows), "lora_expand: this many rows take folded sums (splits = 1)");
+  const ExpandArgs p = {base, v, b, ids, scaling, out, rows, n, rank, adapters, splits};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == FLYMOE_BF16 ? launch_expand_rank<__nv_bfloat16>(p, s) : launch_expand_rank<__half>(p, s);
+  const bool skip = on_tiles(rows);
+  if (skip) {
+    const int tc = launch_expand_sm100(p, dtype == FLYMOE_BF16, s);
+    if (tc != FLYMOE_OK || adapters <= kTileAdapters) return tc;
+  }
+  return dtype == FLYMOE_BF16 ? launch_expand_rank<__nv_bfloat16>(p, skip, s) : launch_expand_rank<__half>(p, skip, s);
 }
 
 extern "C" int flymoe_lora_add(void* out, const void* base, const void* x, const void* a, const void* b, const int32_t* ids,
                                const float* scaling, float* v, int rows, int k, int n, int rank, int adapters, int splits,
                                int dtype, void* stream) {
-  const int rc = flymoe_lora_shrink(v, x, a, ids, rows, k, rank, adapters, splits, 0, dtype, stream);
+  const int fold = flymoe::on_tiles(rows);       // whose expand reads a row's v once for every column tile
+  const int rc = flymoe_lora_shrink(v, x, a, ids, rows, k, rank, adapters, splits, fold, dtype, stream);
   return rc != FLYMOE_OK ? rc
-                         : flymoe_lora_expand(out, base, v, b, ids, scaling, rows, n, rank, adapters, splits, dtype, stream);
+                         : flymoe_lora_expand(out, base, v, b, ids, scaling, rows, n, rank, adapters, fold ? 1 : splits, dtype,
+                                              stream);
 }
 
 extern "C" int flymoe_lora_wgrad_splits(int rows, int k, int n, int adapters) {

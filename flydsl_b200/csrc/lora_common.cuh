@@ -1,0 +1,88 @@
+// What the adapter kernels share: 16-bit packing, the two-part form of the middle factor, argument blocks.
+#pragma once
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace flymoe {
+
+constexpr int kLoraMaxRank = 128;
+constexpr int kLoraMaxSplits = 16;
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) { return pack_f16x2(a, b); }
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+// Two floats as high parts and remainders.  Where the high part is not finite there is no remainder.
+template <typename T>
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<T>(a, b);
+  const float2 h = unpack2<T>(hi);
+  lo = pack2<T>(isfinite(h.x) ? a - h.x : 0.f, isfinite(h.y) ? b - h.y : 0.f);
+}
+// 2^e and 2^-e with the largest of `amax`'s numbers at 2^13 .. 2^14 afterwards (fp16 overflows at 2^16).
+__device__ __forceinline__ int scale_exponent(float amax) {
+  if (!(amax > 0.f)) return 0;
+  const int e = int((__float_as_uint(amax) >> 23) & 0xff) - 127;     // 128: infinite, NaN
+  return e >= 128 ? 0 : max(-110, min(110, e - 13));
+}
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float(uint32_t(127 + e) << 23); }
+__device__ __forceinline__ float finite_abs(float x) { return isfinite(x) ? fabsf(x) : 0.f; }
+__device__ __forceinline__ bool in_use(int id, int adapters) { return id >= 0 && id < adapters; }
+
+struct ShrinkArgs {
+  const void* x;               // [rows, k]
+  const void* a;               // [adapters, rank, k]
+  const int* ids;              // [rows]
+  float* v;                    // [splits, rows, rank]
+  int rows, k, rank, adapters, splits;
+};
+struct ExpandArgs {
+  const void* base;            // [rows, n] or null (zeros); may be `out`
+  const float* v;              // [splits, rows, rank]; splits is 1 on tiles
+  const void* b;               // [adapters, n, rank]
+  const int* ids;
+  const float* scaling;        // [adapters]
+  void* out;                   // [rows, n]
+  int rows, n, rank, adapters, splits;
+};
+
+// Tiles of 128 rows on tcgen05 (lora_sm100.cu), of which these launches take those with at most kTileAdapters distinct
+// adapters among their rows; the kernels of lora.cu take the others, and batches of too few tiles.
+constexpr int kTileAdapters = 4;
+int launch_shrink_sm100(const ShrinkArgs& p, int bf16, cudaStream_t stream);
+int launch_expand_sm100(const ExpandArgs& p, int bf16, cudaStream_t stream);
+
+// Distinct adapters among the 128 ids that a warp holds, four a lane (negative: none): their number, kTileAdapters + 1 if
+// there are more, and the first kTileAdapters of them in `list` (written by lane 0).
+__device__ __forceinline__ int tile_adapters(const int* id, int lane, int* list) {
+  bool left[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) left[i] = id[i] >= 0;
+  int count = 0;
+  while (true) {
+    const bool any = left[0] || left[1] || left[2] || left[3];
+    const uint32_t who = __ballot_sync(0xffffffffu, any);
+    if (who == 0 || count == kTileAdapters) return count + (who != 0);
+    const int mine = left[0] ? id[0] : left[1] ? id[1] : left[2] ? id[2] : id[3];
+    const int l = __shfl_sync(0xffffffffu, mine, __ffs(who) - 1);
+    if (lane == 0 && list) list[count] = l;
+    ++count;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) left[i] = left[i] && id[i] != l;
+  }
+}
+// A row's adapter, -1 for none and for rows behind the last.
+__device__ __forceinline__ int row_adapter(const int* ids, int row, int rows, int adapters) {
+  if (row >= rows) return -1;
+  const int id = __ldg(ids + row);
+  return in_use(id, adapters) ? id : -1;
+}
+
+}  // namespace flymoe

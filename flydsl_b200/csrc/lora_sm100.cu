@@ -1,0 +1,527 @@
+// Adapters on tcgen05: shrink and expand for batches that fill tiles of 128 rows (see lora.cu for the operator).
+//
+// Both kernels stream their large operand through TMA and leave the thin products to the tensor cores, so what is left is
+// the traffic: x once for the shrink, base and output once each for the expand.  A tile goes through the distinct adapters
+// among its rows; of each product only that adapter's rows are kept.
+//
+// Shrink: 128 rows x one split of K.  Every adapter of the tile has its own columns of TMEM (rank each); a K block of x is
+// loaded once and multiplied with each adapter's block.  The splits' sums are folded by a launch of their own (a cluster
+// over K would save it, but CTAs that wait for one another must not wait for TMEM as well).
+//
+// Expand: the base tile (128 x 128) is loaded into shared memory, gets the adapters' products added row by row where it
+// lies, and is stored from there; rows without an adapter are simply not touched.  The rows' v stands in shared memory as
+// high parts and remainders, [128, rank] each, for all column tiles of the row tile.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "gemm_ptx.cuh"
+#include "lora_common.cuh"
+
+namespace flymoe {
+
+constexpr int kTileRows = 128;
+constexpr int kChunkBytes = kTileRows * 128;     // 128 rows x 64 16-bit columns, 128-byte swizzle
+
+__device__ __forceinline__ uint32_t instr_desc(int bf16, int n) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
+}
+// ---------------------------------------------------------------------------- shrink
+constexpr int kShX = 4;                          // K blocks of x in flight
+constexpr int kShABytes = 32768;                 // ring of adapter blocks, rank rows x 128 bytes each
+struct __align__(16) ShrinkCtrl {
+  unsigned long long x_full[kShX], x_empty[kShX], a_full[16], a_empty[16], acc_full;
+  uint32_t tmem_base;
+  int abort_flag, count, list[kTileAdapters];
+};
+constexpr size_t kShSmem = size_t(kShX) * kChunkBytes + kShABytes + sizeof(ShrinkCtrl) + 1024;
+
+struct ShrinkTcArgs {
+  ShrinkArgs p;
+  int bf16, rank_pad, slots, tmem_cols;
+  int* status;
+};
+
+__global__ void __launch_bounds__(256, 2)
+lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_a,
+                      const ShrinkTcArgs q) {
+  extern __shared__ uint8_t smem_dyn[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  uint8_t* aring = smem + kShX * kChunkBytes;
+  ShrinkCtrl* c = reinterpret_cast<ShrinkCtrl*>(aring + kShABytes);
+  volatile int* abort_flag = &c->abort_flag;
+  const ShrinkArgs& p = q.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row0 = blockIdx.x * kTileRows;
+  const int a_bytes = q.rank_pad * 128;
+
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&c->tmem_base)), "r"(uint32_t(q.tmem_cols)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (threadIdx.x == 0) {
+    for (int i = 0; i < kShX; ++i) { mbar_init(smem_u32(&c->x_full[i]), 1); mbar_init(smem_u32(&c->x_empty[i]), 1); }
+    for (int i = 0; i < 16; ++i) { mbar_init(smem_u32(&c->a_full[i]), 1); mbar_init(smem_u32(&c->a_empty[i]), 1); }
+    mbar_init(smem_u32(&c->acc_full), 1);
+    c->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  } else if (warp == 2) {
+    int id[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, row0 + i * 32 + lane, p.rows, p.adapters);
+    const int n = tile_adapters(id, lane, c->list);
+    if (lane == 0) c->count = n <= kTileAdapters ? n : 0;        // the other tiles are not this kernel's
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = c->tmem_base;
+  const int d = c->count;
+  const int blocks = (p.k + 63) / 64;
+  const int kb0 = int((long long)blocks * blockIdx.y / p.splits), kb1 = int((long long)blocks * (blockIdx.y + 1) / p.splits);
+
+  if (warp == 0 && d > 0) {
+    // ------------------------------------------------------------------ TMA producer
+    int xs = 0, as = 0;
+    uint32_t xp = 0, ap = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1 && ok; ++kb) {
+      ok = warp_wait(smem_u32(&c->x_empty[xs]), xp ^ 1, abort_flag, q.status, 1, 32);
+      if (!ok) break;
+      if (elect_one()) {
+        mbar_expect_tx(smem_u32(&c->x_full[xs]), kChunkBytes);
+        tma_load_2d(smem_u32(smem + xs * kChunkBytes), &tmap_x, smem_u32(&c->x_full[xs]), kb * 128, row0);
+      }
+      __syncwarp();
+      if (++xs == kShX) { xs = 0; xp ^= 1; }
+      for (int i = 0; i < d; ++i) {
+        ok = warp_wait(smem_u32(&c->a_empty[as]), ap ^ 1, abort_flag, q.status, 1, 32);
+        if (!ok) break;
+        if (elect_one()) {
+          mbar_expect_tx(smem_u32(&c->a_full[as]), a_bytes);
+          tma_load_3d(smem_u32(aring + as * a_bytes), &tmap_a, smem_u32(&c->a_full[as]), kb * 128, 0, c->list[i]);
+        }
+        __syncwarp();
+        if (++as == q.slots) { as = 0; ap ^= 1; }
+      }
+    }
+  } else if (warp == 1 && d > 0) {
+    // ------------------------------------------------------------------ MMA issuer
+    const uint32_t idesc = instr_desc(q.bf16, q.rank_pad);
+    int xs = 0, as = 0;
+    uint32_t xp = 0, ap = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1 && ok; ++kb) {
+      ok = warp_wait(smem_u32(&c->x_full[xs]), xp, abort_flag, q.status, 3);
+      const uint64_t adesc = make_smem_desc(smem_u32(smem + xs * kChunkBytes));
+      for (int i = 0; i < d && ok; ++i) {
+        ok = warp_wait(smem_u32(&c->a_full[as]), ap, abort_flag, q.status, 3);
+        if (!ok) break;
+        const uint64_t bdesc = make_smem_desc(smem_u32(aring + as * a_bytes));
+        tcgen05_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(tmem + i * q.rank_pad, adesc + k * 2, bdesc + k * 2, idesc, (k > 0 || kb > kb0) ? 1u : 0u);
+          umma_commit(smem_u32(&c->a_empty[as]));
+          if (i + 1 == d) {
+            umma_commit(smem_u32(&c->x_empty[xs]));
+            if (kb + 1 == kb1) umma_commit(smem_u32(&c->acc_full));
+          }
+        }
+        __syncwarp();
+        if (++as == q.slots) { as = 0; ap ^= 1; }
+      }
+      if (++xs == kShX) { xs = 0; xp ^= 1; }
+    }
+  } else if (warp >= 4 && d > 0) {
+    // ------------------------------------------------------------------ epilogue: a thread per row
+    const int i = threadIdx.x - 128, mine = row_adapter(p.ids, row0 + i, p.rows, p.adapters);
+    float* out = p.v + ((long long)blockIdx.y * p.rows + row0 + i) * p.rank;
+    const bool summed = kb1 > kb0;               // more splits than K blocks: some have nothing to add
+    if (!summed || warp_wait(smem_u32(&c->acc_full), 0, abort_flag, q.status, 4)) {
+      tcgen05_fence_after();
+      for (int a = 0; a < d; ++a) {
+        const bool hit = mine == c->list[a];
+        if (!__any_sync(0xffffffffu, hit)) continue;
+        for (int j = 0; j < p.rank; j += 32) {
+          float v[32];
+          if (summed) {
+            tmem_ld_x32(tmem + (uint32_t((warp & 3) * 32) << 16) + a * q.rank_pad + j, reinterpret_cast<uint32_t*>(v));
+            tmem_ld_wait();
+          }
+          if (hit) {
+#pragma unroll
+            for (int u = 0; u < 32; u += 4)
+              if (j + u < p.rank)
+                *reinterpret_cast<float4*>(out + j + u) = summed ? make_float4(v[u], v[u + 1], v[u + 2], v[u + 3])
+                                                                 : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        }
+      }
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(q.tmem_cols)) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------- expand
+constexpr int kExCols = 128;                     // columns of a tile: two chunks of 64
+constexpr int kExThreads = 384;
+constexpr int kExEpi = 256;
+struct __align__(16) ExpandCtrl {
+  unsigned long long y_full[4], y_empty[4], b_full[2], b_empty[2], acc_full[2], acc_empty[2];
+  unsigned long long row_ready, row_taken;       // a row tile's list and v are set up; producer and issuer know its count
+  unsigned long long together, tile_done;        // epilogue warps: barrier; their part of the output tile is written
+  uint32_t tmem_base;
+  int abort_flag, count, list[kTileAdapters];
+  int id[kTileRows], row_max[kTileRows];
+};
+constexpr int kExB = 2;                          // adapter tiles in flight
+template <int KC> constexpr int ex_y_stages() { return KC == 1 ? 4 : 3; }      // base / output tiles in shared memory
+template <int KC> constexpr size_t ex_smem() {
+  return size_t(ex_y_stages<KC>()) * 2 * kChunkBytes + size_t(kExB) * KC * kChunkBytes + 2 * KC * kChunkBytes + sizeof(ExpandCtrl) + 1024;
+}
+static_assert(ex_smem<2>() <= 232448, "shared memory budget of one SM exceeded");
+
+struct ExpandTcArgs {
+  ExpandArgs p;
+  int col_tiles, units;
+  int* status;
+};
+
+// KC: chunks of 64 in the rank.
+template <typename T, int KC>
+__global__ void __launch_bounds__(kExThreads, 1)
+lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_constant__ CUtensorMap tmap_out,
+                      const __grid_constant__ CUtensorMap tmap_b, const ExpandTcArgs q) {
+  constexpr int kExY = ex_y_stages<KC>();
+  extern __shared__ uint8_t smem_dyn[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  uint8_t* bring = smem + kExY * 2 * kChunkBytes;
+  uint8_t* vtile = bring + kExB * KC * kChunkBytes;              // [hi, lo][KC] chunks
+  ExpandCtrl* c = reinterpret_cast<ExpandCtrl*>(vtile + 2 * KC * kChunkBytes);
+  volatile int* abort_flag = &c->abort_flag;
+  const ExpandArgs& p = q.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&c->tmem_base)), "r"(uint32_t(2 * kExCols)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  } else if (threadIdx.x == 0) {
+    for (int i = 0; i < kExY; ++i) { mbar_init(smem_u32(&c->y_full[i]), 1); mbar_init(smem_u32(&c->y_empty[i]), 1); }
+    for (int i = 0; i < kExB; ++i) { mbar_init(smem_u32(&c->b_full[i]), 1); mbar_init(smem_u32(&c->b_empty[i]), 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&c->acc_full[i]), 1); mbar_init(smem_u32(&c->acc_empty[i]), kExEpi / 32); }
+    mbar_init(smem_u32(&c->row_ready), kExEpi);
+    mbar_init(smem_u32(&c->row_taken), 2);
+    mbar_init(smem_u32(&c->together), kExEpi / 32);
+    mbar_init(smem_u32(&c->tile_done), kExEpi / 32);
+    c->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = c->tmem_base;
+  // consecutive column tiles of a row tile, so that the rows' v is set up once or twice per block
+  const int u0 = int((long long)q.units * blockIdx.x / gridDim.x), u1 = int((long long)q.units * (blockIdx.x + 1) / gridDim.x);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    int ys = 0, bs = 0, row_tile = -1, d = 0;
+    uint32_t yp = 0, bp = 0, rp = 0;
+    bool ok = true;
+    for (int u = u0; u < u1 && ok; ++u) {
+      const int rt = u / q.col_tiles, col = (u - rt * q.col_tiles) * kExCols;
+      if (rt != row_tile) {
+        ok = warp_wait(smem_u32(&c->row_ready), rp, abort_flag, q.status, 5, 32);
+        if (!ok) break;
+        rp ^= 1;
+        row_tile = rt;
+        d = c->count;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&c->row_taken));
+      }
+      if (d > kTileAdapters) continue;
+      ok = warp_wait(smem_u32(&c->y_empty[ys]), yp ^ 1, abort_flag, q.status, 1, 32);
+      if (!ok) break;
+      const uint32_t full = smem_u32(&c->y_full[ys]), dst = smem_u32(smem + ys * 2 * kChunkBytes);
+      if (elect_one()) {
+        if (p.base) {
+          mbar_expect_tx(full, 2 * kChunkBytes);
+          tma_load_2d(dst, &tmap_y, full, col * 2, rt * kTileRows);
+          tma_load_2d(dst + kChunkBytes, &tmap_y, full, col * 2 + 128, rt * kTileRows);
+        } else {
+          mbar_arrive(full);
+        }
+      }
+      __syncwarp();
+      if (++ys == kExY) { ys = 0; yp ^= 1; }
+      for (int i = 0; i < d && ok; ++i) {
+        ok = warp_wait(smem_u32(&c->b_empty[bs]), bp ^ 1, abort_flag, q.status, 1, 32);
+        if (!ok) break;
+        const uint32_t bfull = smem_u32(&c->b_full[bs]), bdst = smem_u32(bring + bs * KC * kChunkBytes);
+        if (elect_one()) {
+          mbar_expect_tx(bfull, KC * kChunkBytes);
+#pragma unroll
+          for (int k = 0; k < KC; ++k) tma_load_3d(bdst + k * kChunkBytes, &tmap_b, bfull, k * 128, col, c->list[i]);
+        }
+        __syncwarp();
+        if (++bs == kExB) { bs = 0; bp ^= 1; }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer
+    const uint32_t idesc = instr_desc(std::is_same<T, __nv_bfloat16>::value, kExCols);
+    const int steps = (p.rank + 15) / 16;
+    int bs = 0, acc = 0, row_tile = -1, d = 0;
+    uint32_t bp = 0, rp = 0, accp = 0;
+    bool ok = true;
+    for (int u = u0; u < u1 && ok; ++u) {
+      const int rt = u / q.col_tiles;
+      if (rt != row_tile) {
+        ok = warp_wait(smem_u32(&c->row_ready), rp, abort_flag, q.status, 5);
+        if (!ok) break;
+        rp ^= 1;
+        row_tile = rt;
+        d = c->count;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&c->row_taken));
+      }
+      if (d > kTileAdapters) continue;
+      for (int i = 0; i < d && ok; ++i) {
+        ok = warp_wait(smem_u32(&c->acc_empty[acc]), accp ^ 1, abort_flag, q.status, 2) &&
+             warp_wait(smem_u32(&c->b_full[bs]), bp, abort_flag, q.status, 3);
+        if (!ok) break;
+        tcgen05_fence_after();
+        if (elect_one()) {
+          for (int part = 0; part < 2; ++part)
+            for (int k = 0; k < steps; ++k) {
+              const uint64_t ad = make_smem_desc(smem_u32(vtile + (part * KC + (k >> 2)) * kChunkBytes)) + (k & 3) * 2;
+              const uint64_t bd = make_smem_desc(smem_u32(bring + (bs * KC + (k >> 2)) * kChunkBytes)) + (k & 3) * 2;
+              umma_f16(tmem + acc * kExCols, ad, bd, idesc, (part > 0 || k > 0) ? 1u : 0u);
+            }
+          umma_commit(smem_u32(&c->b_empty[bs]));
+          umma_commit(smem_u32(&c->acc_full[acc]));
+        }
+        __syncwarp();
+        if (++bs == kExB) { bs = 0; bp ^= 1; }
+        if (++acc == 2) { acc = 0; accp ^= 1; }
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ epilogue: a thread per row and half tile
+    const int et = threadIdx.x - 128, wg = et >> 7, row = et & 127;
+    const int sw = row & 7;
+    int ys = 0, acc = 0, row_tile = -1, d = 0, mine = -1, stored = 0;
+    uint32_t yp = 0, accp = 0, tp = 0;
+    float scale = 0.f;
+    bool ok = true;
+    uint32_t together = 0, done = 0;
+    auto sync = [&]() -> bool {                  // bounded: a warp that gave up elsewhere does not leave the others waiting
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&c->together));
+      const bool met = warp_wait(smem_u32(&c->together), together, abort_flag, q.status, 7);
+      together ^= 1;
+      return met;
+    };
+    for (int u = u0; u < u1 && ok; ++u) {
+      const int rt = u / q.col_tiles, col = (u - rt * q.col_tiles) * kExCols;
+      if (rt != row_tile) {
+        // The MMAs of the previous row tile are done (their last sums have been read here), and with them all loads by
+        // its list; its count may still be unread where it was zero.
+        if (row_tile >= 0) {
+          ok = warp_wait(smem_u32(&c->row_taken), tp, abort_flag, q.status, 7);
+          if (!ok) break;
+          tp ^= 1;
+        }
+        row_tile = rt;
+        mine = row_adapter(p.ids, rt * kTileRows + row, p.rows, p.adapters);
+        ok = sync();                             // all have left the previous list
+        if (!ok) break;
+        if (et < 32) {
+          int id[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, rt * kTileRows + i * 32 + lane, p.rows, p.adapters);
+          const int n = tile_adapters(id, lane, c->list);
+          if (lane == 0) c->count = n;
+        }
+        if (wg == 0) c->id[row] = mine;
+        ok = sync();
+        if (!ok) break;
+        d = c->count;
+        scale = mine >= 0 ? __ldg(p.scaling + mine) : 0.f;
+        // v as high parts and remainders: four numbers a thread and step, consecutive threads along a row
+        const int vecs = (p.rank + 15) / 16 * 4;
+        auto load = [&](int i, int& r, int& k4) {
+          r = i / vecs;
+          k4 = i - r * vecs;
+          return d <= kTileAdapters && c->id[r] >= 0 && k4 * 4 < p.rank
+                     ? __ldg(reinterpret_cast<const float4*>(p.v + (long long)(rt * kTileRows + r) * p.rank + k4 * 4))
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        if constexpr (std::is_same<T, __half>::value) {
+          if (wg == 0) c->row_max[row] = 0;
+          ok = sync();
+          if (!ok) break;
+          for (int i = et; i < kTileRows * vecs; i += kExEpi) {
+            int r, k4;
+            const float4 x = load(i, r, k4);
+            const float m = fmaxf(fmaxf(finite_abs(x.x), finite_abs(x.y)), fmaxf(finite_abs(x.z), finite_abs(x.w)));
+            atomicMax(&c->row_max[r], __float_as_int(m));          // not negative: ordered like the numbers
+          }
+          ok = sync();
+          if (!ok) break;
+          scale *= exp2i(scale_exponent(__int_as_float(c->row_max[row])));
+        }
+#pragma unroll 4
+        for (int i = et; i < kTileRows * vecs; i += kExEpi) {
+          int r, k4;
+          const float4 x = load(i, r, k4);
+          float down = 1.f;
+          if constexpr (std::is_same<T, __half>::value) down = exp2i(-scale_exponent(__int_as_float(c->row_max[r])));
+          uint2 hi, lo;
+          split2<T>(x.x * down, x.y * down, hi.x, lo.x);
+          split2<T>(x.z * down, x.w * down, hi.y, lo.y);
+          uint8_t* at = vtile + (k4 >> 4) * kChunkBytes + r * 128 + ((((k4 >> 1) & 7) ^ (r & 7)) * 16) + (k4 & 1) * 8;
+          *reinterpret_cast<uint2*>(at) = hi;
+          *reinterpret_cast<uint2*>(at + KC * kChunkBytes) = lo;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(smem_u32(&c->row_ready));
+      }
+      if (d > kTileAdapters) continue;           // its rows are the other kernel's
+      ok = warp_wait(smem_u32(&c->y_full[ys]), yp, abort_flag, q.status, 6);
+      if (!ok) break;
+      uint8_t* line = smem + (ys * 2 + wg) * kChunkBytes + row * 128;
+      if (p.base == nullptr) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(line + j * 16) = make_uint4(0, 0, 0, 0);
+      }
+      for (int i = 0; i < d && ok; ++i) {
+        ok = warp_wait(smem_u32(&c->acc_full[acc]), accp, abort_flag, q.status, 4);
+        if (!ok) break;
+        tcgen05_fence_after();
+        const bool hit = mine == c->list[i];
+        if (__any_sync(0xffffffffu, hit)) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float v[32];
+            tmem_ld_x32(tmem + (uint32_t((warp & 3) * 32) << 16) + acc * kExCols + wg * 64 + h * 32,
+                        reinterpret_cast<uint32_t*>(v));
+            tmem_ld_wait();
+            if (hit) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                uint4* at = reinterpret_cast<uint4*>(line + (((h * 4 + j) ^ sw) * 16));
+                uint4 y = *at;
+                uint32_t* w = reinterpret_cast<uint32_t*>(&y);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const float2 f = unpack2<T>(w[k]);
+                  w[k] = pack2<T>(fmaf(scale, v[j * 8 + k * 2], f.x), fmaf(scale, v[j * 8 + k * 2 + 1], f.y));
+                }
+                *at = y;
+              }
+            }
+          }
+        }
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&c->acc_empty[acc]));
+        if (++acc == 2) { acc = 0; accp ^= 1; }
+      }
+      if (!ok) break;
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&c->tile_done));
+      if (et < 32) {
+        ok = warp_wait(smem_u32(&c->tile_done), done, abort_flag, q.status, 7);
+        if (!ok) break;
+      }
+      done ^= 1;
+      if (et == 0) {
+        const uint32_t src = smem_u32(smem + ys * 2 * kChunkBytes);
+        tma_store_2d(&tmap_out, src, col * 2, rt * kTileRows);
+        if (col + 64 < p.n) tma_store_2d(&tmap_out, src + kChunkBytes, col * 2 + 128, rt * kTileRows);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        // the store before this one has been read out of its tile: that tile is free
+        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        if (stored++ > 0) mbar_arrive(smem_u32(&c->y_empty[ys == 0 ? kExY - 1 : ys - 1]));
+      }
+      if (++ys == kExY) { ys = 0; yp ^= 1; }
+    }
+    if (et == 0) bulk_wait_all();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(2 * kExCols)) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------- host
+static int matrix_map(CUtensorMap* map, const void* base, long long cols, long long rows, int mats, int box_rows) {
+  cuuint64_t dims[3] = {cuuint64_t(cols) * 2, cuuint64_t(rows), cuuint64_t(mats)};
+  cuuint64_t strides[2] = {cuuint64_t(cols) * 2, cuuint64_t(cols) * 2 * cuuint64_t(rows)};
+  cuuint32_t box[3] = {128, cuuint32_t(box_rows), 1};
+  return make_map(map, base, mats > 0 ? 3 : 2, dims, strides, box);
+}
+
+int launch_shrink_sm100(const ShrinkArgs& p, int bf16, cudaStream_t stream) {
+  ShrinkTcArgs q = {p, bf16, (p.rank + 15) / 16 * 16, 0, 0, device_status_ptr()};
+  if (q.status == nullptr) return FLYMOE_ERR_CUDA;
+  q.slots = std::min(16, kShABytes / (q.rank_pad * 128));
+  // columns for kTileAdapters adapters; sums are read 32 columns at a time, so also for what the last read reaches
+  static_assert(kTileAdapters == 4, "TMEM columns below");
+  q.tmem_cols = q.rank_pad <= 64 ? 256 : 512;
+  CUtensorMap mx, ma;
+  int rc = matrix_map(&mx, p.x, p.k, p.rows, 0, kTileRows);
+  if (rc == FLYMOE_OK) rc = matrix_map(&ma, p.a, p.k, p.rank, p.adapters, q.rank_pad);
+  if (rc != FLYMOE_OK) return rc;
+  static SmemLimitSeen seen;
+  FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(lora_shrink_tc_kernel), int(kShSmem), seen));
+  lora_shrink_tc_kernel<<<dim3(ceil_div(p.rows, kTileRows), p.splits), 256, kShSmem, stream>>>(mx, ma, q);
+  FLYMOE_CUDA_CHECK(cudaGetLastError());
+  return FLYMOE_OK;
+}
+
+template <typename T, int KC>
+static int launch_expand_tc(const CUtensorMap& my, const CUtensorMap& mo, const CUtensorMap& mb, const ExpandTcArgs& q,
+                            cudaStream_t stream) {
+  auto* kernel = lora_expand_tc_kernel<T, KC>;
+  static SmemLimitSeen seen;
+  FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(ex_smem<KC>()), seen));
+  kernel<<<std::min(q.units, sm_count()), kExThreads, ex_smem<KC>(), stream>>>(my, mo, mb, q);
+  FLYMOE_CUDA_CHECK(cudaGetLastError());
+  return FLYMOE_OK;
+}
+
+int launch_expand_sm100(const ExpandArgs& p, int bf16, cudaStream_t stream) {
+  ExpandTcArgs q = {p, ceil_div(p.n, kExCols), 0, device_status_ptr()};
+  if (q.status == nullptr) return FLYMOE_ERR_CUDA;
+  const long long units = (long long)ceil_div(p.rows, kTileRows) * q.col_tiles;
+  FLYMOE_REQUIRE(units < (1LL << 31), "lora_expand: too many tiles");
+  q.units = int(units);
+  CUtensorMap my, mo, mb;
+  int rc = matrix_map(&my, p.base ? p.base : p.out, p.n, p.rows, 0, kTileRows);
+  if (rc == FLYMOE_OK) rc = matrix_map(&mo, p.out, p.n, p.rows, 0, kTileRows);
+  if (rc == FLYMOE_OK) rc = matrix_map(&mb, p.b, p.rank, p.n, p.adapters, kExCols);
+  if (rc != FLYMOE_OK) return rc;
+  if (p.rank <= 64)
+    return bf16 ? launch_expand_tc<__nv_bfloat16, 1>(my, mo, mb, q, stream) : launch_expand_tc<__half, 1>(my, mo, mb, q, stream);
+  return bf16 ? launch_expand_tc<__nv_bfloat16, 2>(my, mo, mb, q, stream) : launch_expand_tc<__half, 2>(my, mo, mb, q, stream);
+}
+
+}  // namespace flymoe

@@ -62,7 +62,7 @@ def check(got, want, terms, what):
 SIZES = [
     (1, 8, 8, 8, 1, "requests"), (1, 7168, 2112, 16, 4, "tokens"), (17, 264, 136, 24, 40, "tokens"),
     (64, 1024, 520, 16, 32, "tokens"), (33, 40, 1032, 128, 5, "tokens"), (130, 512, 256, 64, 3, "requests"),
-    (1000, 328, 200, 32, 6, "requests"), (1500, 256, 264, 72, 2, "tokens"), (2100, 136, 72, 8, 1, "requests"),
+    (1000, 328, 200, 32, 6, "requests"), (1500, 256, 264, 72, 2, "tokens"), (2100, 136, 72, 8, 1, "requests"), (700, 1096, 392, 48, 150, "tokens"), (512, 64, 72, 16, 1, "none"),
     (50, 64, 64, 40, 3, "none"), (600, 2048, 136, 104, 9, "tokens"),
 ]
 
