@@ -91,7 +91,7 @@ _SIGNATURES = {
     "flymoe_lora_shrink_splits": (c_int, [c_int, c_int]),
     "flymoe_lora_shrink": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
     "flymoe_lora_expand": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
-    "flymoe_lora_wgrad_splits": (c_int, [c_int, c_int, c_int, c_int]),
+    "flymoe_lora_wgrad_splits": (c_int, [c_int, c_int, c_int, c_int, c_int]),
     "flymoe_lora_wgrad": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
     "flymoe_lora_transpose": (c_int, [_P, _P, c_int, c_int, c_int, _P]),
     "flymoe_moe_reduce": (c_int, [_P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),

@@ -79,6 +79,11 @@ __device__ __forceinline__ void build_groups(Groups* s, const int* ids, int row0
     if (lane == 0) s->skip[warp] = d <= kTileAdapters;
   }
   __syncthreads();
+  if (skip_tiles && s->skip[0] && s->skip[1] && s->skip[2] && s->skip[3]) {      // nothing here (no rows: no adapters)
+    if (tid == 0) s->count = 0;
+    __syncthreads();
+    return;
+  }
   int slot[2], lead[2], rank[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -345,10 +350,12 @@ struct AdapterGradArgs {
   AdapterGrad g[2];
   const int* ids;
   const float* scaling;
+  int* present;                // [splits, adapters]: whether the split has rows of the adapter, when splits > 1
   int rows, rank, adapters, splits;
 };
 constexpr int kWgCols = 128, kWgRows = 32, kWgStages = 4, kWgList = 1024;
-constexpr int kWgXStride = kWgCols * 2 + 16;     // 16 bytes of skew: eight rows of a matrix in eight different banks groups
+constexpr int kWgRank = 64;                      // ranks a block sums up; more are shared out
+constexpr int kWgXStride = kWgCols * 2 + 16;     // 16 bytes of skew: a matrix's eight rows lie in different banks
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
@@ -362,10 +369,11 @@ template <int NT> constexpr size_t wg_smem() {
   return size_t(kWgStages) * kWgRows * (kWgXStride + NT * 32) + 2 * 2 * kWgRows * size_t(wg_v_stride<NT>());
 }
 
-// A block takes 128 columns of one adapter's gradient and one split of the rows: it scans the ids, gathers the adapter's
-// rows 32 at a time (cp.async, four chunks in flight) and contracts over them; both operands are read across their rows
-// with transposing ldmatrix.  fp16: chunks of v share a running power of two; when a chunk needs a larger one the sums are
-// brought to it.
+// A block takes 128 columns (and up to 64 ranks) of a gradient and one split of the rows, and goes through the adapters with
+// rows in it: it lists an adapter's rows by scanning the ids, gathers them 32 at a time (cp.async, four chunks in flight)
+// and contracts over them; both operands are read across their rows with transposing ldmatrix.  Splits are pieces of the
+// batch, so blocks have like amounts of rows however the adapters share them.  fp16: chunks of v share a running power of
+// two; when a chunk needs a larger one the sums are brought to it.
 template <typename T, int NT>
 __global__ void __launch_bounds__(128)
 lora_wgrad_kernel(const AdapterGradArgs p) {
@@ -375,194 +383,233 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
   uint8_t* xs = sm;                                                     // [stages][32][kWgXStride]
   float* vf = reinterpret_cast<float*>(sm + kWgStages * kWgRows * kWgXStride);      // [stages][32][RP]
   uint8_t* vh = sm + kWgStages * kWgRows * (kWgXStride + RP * 4);       // [2][hi, lo][32][VS]
-  __shared__ int list[kWgList + kWgRows], warp_n[4], list_n;
+  __shared__ int list[kWgList + kWgRows], warp_n[4], next_adapter;
   __shared__ float warp_max[4];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const bool second = int(blockIdx.x) >= p.g[0].tiles;
   const AdapterGrad q = second ? p.g[1] : p.g[0];
   const int col0 = (second ? int(blockIdx.x) - p.g[0].tiles : int(blockIdx.x)) * kWgCols;
-  const int l = blockIdx.y;
-  int next = int((long long)p.rows * blockIdx.z / p.splits);
-  const int end = int((long long)p.rows * (blockIdx.z + 1) / p.splits);
+  const int j0 = int(blockIdx.z) * kWgRank;      // first of this block's ranks
+  const int begin = int((long long)p.rows * blockIdx.y / p.splits), end = int((long long)p.rows * (blockIdx.y + 1) / p.splits);
   const T* X = static_cast<const T*>(q.x);
-
-  if (tid == 0) list_n = 0;
-  int taken = 0, have = 0;                       // entries of the list already used, entries in it (same in all threads)
-  __syncthreads();
-  // appends rows of this adapter until the list holds a chunk or the rows are through
-  auto refill = [&]() {
-    if (have - taken >= kWgRows || next >= end) return;
-    __syncthreads();                             // nobody reads the part that moves
-    const int rest = have - taken;
-    const int keep = tid < rest ? list[taken + tid] : 0;
-    __syncthreads();
-    if (tid < rest) list[tid] = keep;
-    have = rest;
-    taken = 0;
-    while (have < kWgRows && next < end) {
-      // 1024 ids: eight a thread, in order
-      const int at = next + tid * 8;
-      uint32_t mine = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (at + i < end && __ldg(p.ids + at + i) == l) mine |= 1u << i;
-      int before = __popc(mine);
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, before, off);
-        if (lane >= off) before += o;
-      }
-      if (lane == 31) warp_n[warp] = before;
-      __syncthreads();
-      int base = have, all = 0;
-      for (int i = 0; i < 4; ++i) {
-        if (i < warp) base += warp_n[i];
-        all += warp_n[i];
-      }
-      int pos = base + before - __popc(mine);
-      for (; mine; mine &= mine - 1) list[pos++] = at + __ffs(mine) - 1;
-      have += all;
-      next += kWgList;
-      __syncthreads();
-    }
-  };
-  // one chunk of up to 32 rows into a stage; returns its rows
-  auto load = [&](int stage) -> int {
-    refill();
-    const int n = min(kWgRows, have - taken);
-    if (n > 0) {
-      for (int i = tid; i < kWgRows * (kWgCols / 8); i += 128) {
-        const int r = i / (kWgCols / 8), c = i - r * (kWgCols / 8);
-        const bool ok = r < n && col0 + c * 8 < q.cols;
-        const T* src = X + (long long)(r < n ? list[taken + r] : 0) * q.cols + (ok ? col0 + c * 8 : 0);
-        cp_async16(smem_u32(xs + (stage * kWgRows + r) * kWgXStride + c * 16), src, ok);
-      }
-      for (int i = tid; i < kWgRows * (RP / 4); i += 128) {
-        const int r = i / (RP / 4), c = i - r * (RP / 4);
-        const bool ok = r < n && c * 4 < p.rank;
-        const float* src = q.v + (long long)(r < n ? list[taken + r] : 0) * p.rank + (ok ? c * 4 : 0);
-        cp_async16(smem_u32(vf + (stage * kWgRows + r) * RP + c * 4), src, ok);
-      }
-      taken += n;
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    return n;
-  };
-
-  float c[2][NT][4];
-#pragma unroll
-  for (int f = 0; f < 2; ++f)
-#pragma unroll
-    for (int i = 0; i < NT; ++i) c[f][i][0] = c[f][i][1] = c[f][i][2] = c[f][i][3] = 0.f;
-  int exponent = -200;
-  int chunk_n[kWgStages];
-#pragma unroll
-  for (int s = 0; s < kWgStages - 1; ++s) chunk_n[s] = load(s);
-  for (int i = 0;; ++i) {
-    const int stage = i % kWgStages;
-    int n = 0;
-#pragma unroll
-    for (int s = 0; s < kWgStages; ++s)
-      if (s == stage) n = chunk_n[s];
-    if (n == 0) break;
-    asm volatile("cp.async.wait_group %0;" ::"n"(kWgStages - 2) : "memory");
-    __syncthreads();
-    // the chunk's v as high parts and remainders
-    uint8_t* vb = vh + (i & 1) * 2 * kWgRows * VS;
-    const float* vc = vf + stage * kWgRows * RP;
-    float down = 1.f;
-    if constexpr (kHalf) {
-      float amax = 0.f;
-      for (int e = tid; e < kWgRows * RP / 4; e += 128) {
-        const float4 x = reinterpret_cast<const float4*>(vc)[e];
-        amax = fmaxf(amax, fmaxf(fmaxf(finite_abs(x.x), finite_abs(x.y)), fmaxf(finite_abs(x.z), finite_abs(x.w))));
-      }
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
-      if (lane == 0) warp_max[warp] = amax;
-      __syncthreads();
-      amax = fmaxf(fmaxf(warp_max[0], warp_max[1]), fmaxf(warp_max[2], warp_max[3]));
-      const int e = scale_exponent(amax);
-      if (amax > 0.f && e > exponent) {
-        const float f = exponent < -110 ? 0.f : exp2i(max(-126, exponent - e));
-        if (exponent >= -110) {
-#pragma unroll
-          for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int b = 0; b < NT; ++b) { c[a][b][0] *= f; c[a][b][1] *= f; c[a][b][2] *= f; c[a][b][3] *= f; }
-        }
-        exponent = e;
-      }
-      down = exponent < -110 ? 1.f : exp2i(-exponent);
-    }
-    for (int e = tid; e < kWgRows * RP / 4; e += 128) {
-      const int r = e / (RP / 4), j = e - r * (RP / 4);
-      const float4 x = reinterpret_cast<const float4*>(vc)[e];
-      uint2 h, w;
-      split2<T>(x.x * down, x.y * down, h.x, w.x);
-      split2<T>(x.z * down, x.w * down, h.y, w.y);
-      *reinterpret_cast<uint2*>(vb + r * VS + j * 8) = h;
-      *reinterpret_cast<uint2*>(vb + (kWgRows + r) * VS + j * 8) = w;
-    }
-    const int into = (i + kWgStages - 1) % kWgStages;
-    const int got = load(into);                  // the stage that chunk i - 1 used: all have passed the barrier above
-#pragma unroll
-    for (int s = 0; s < kWgStages; ++s)
-      if (s == into) chunk_n[s] = got;
-    __syncthreads();
-    const uint32_t xa = smem_u32(xs + stage * kWgRows * kWgXStride) +
-                        ((lane >> 4) * 8 + (lane & 7)) * kWgXStride + (warp * 32 + ((lane >> 3) & 1) * 8) * 2;
-    const uint32_t va = smem_u32(vb) + (((lane >> 3) & 1) * 8 + (lane & 7)) * VS + (lane >> 4) * 16;
-#pragma unroll
-    for (int k = 0; k < kWgRows / 16; ++k) {
-      uint32_t a[2][4];
-      ldmatrix_x4_trans(a[0], xa + k * 16 * kWgXStride);
-      ldmatrix_x4_trans(a[1], xa + k * 16 * kWgXStride + 32);
-#pragma unroll
-      for (int j = 0; j < NT / 2; ++j) {
-        uint32_t h[4], w[4];
-        ldmatrix_x4_trans(h, va + k * 16 * VS + j * 32);
-        ldmatrix_x4_trans(w, va + (kWgRows + k * 16) * VS + j * 32);
-#pragma unroll
-        for (int f = 0; f < 2; ++f) {
-          mma16816<T>(c[f][2 * j], a[f], h[0], h[1]);
-          mma16816<T>(c[f][2 * j], a[f], w[0], w[1]);
-          mma16816<T>(c[f][2 * j + 1], a[f], h[2], h[3]);
-          mma16816<T>(c[f][2 * j + 1], a[f], w[2], w[3]);
-        }
-      }
-    }
-  }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-
-  const float s = (p.splits == 1 ? __ldg(p.scaling + l) : 1.f);
-  const float up = kHalf && exponent >= -110 ? exp2i(exponent) : 1.f;
   const long long mat = (long long)q.cols * p.rank;
+
+  // the smallest adapter above `l` with rows here, or p.adapters
+  auto find_next = [&](int l) -> int {
+    if (tid == 0) next_adapter = p.adapters;
+    __syncthreads();
+    int best = p.adapters;
+    for (int i = begin + tid; i < end; i += 128) {
+      const int id = __ldg(p.ids + i);
+      if (id > l && id < best) best = id;
+    }
 #pragma unroll
-  for (int f = 0; f < 2; ++f)
+    for (int off = 16; off > 0; off >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, off));
+    if (lane == 0) atomicMin(&next_adapter, best);
+    __syncthreads();
+    return next_adapter;
+  };
+  // adapters without rows here: zeros, or (several splits) the finishing launch is told
+  auto skip_adapters = [&](int from, int to) {
+    if (p.splits > 1) {
+      if (blockIdx.x == 0 && blockIdx.z == 0)
+        for (int l = from + tid; l < to; l += 128) p.present[(long long)blockIdx.y * p.adapters + l] = 0;
+      return;
+    }
+    const int jn = min(kWgRank, p.rank - j0), cn = min(kWgCols, q.cols - col0);
+    for (int l = from; l < to; ++l)
+      for (int i = tid; i < jn * cn; i += 128) {
+        const long long at = q.rank_major ? (long long)(j0 + i / cn) * q.cols + col0 + i % cn
+                                          : (long long)(col0 + i / jn) * p.rank + j0 + i % jn;
+        static_cast<T*>(q.out)[(long long)l * mat + at] = T(0.f);
+      }
+  };
+
+  int done = 0;                                  // adapters below this one are dealt with
+  for (int l = find_next(-1); l < p.adapters; l = find_next(l)) {
+    skip_adapters(done, l);
+    done = l + 1;
+    if (p.splits > 1 && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) p.present[(long long)blockIdx.y * p.adapters + l] = 1;
+
+    int next = begin, taken = 0, have = 0;       // ids scanned, entries of the list used and in it (same in all threads)
+    // appends rows of this adapter until the list holds a chunk or the rows are through
+    auto refill = [&]() {
+      if (have - taken >= kWgRows || next >= end) return;
+      __syncthreads();                           // nobody reads the part that moves
+      const int rest = have - taken;
+      const int keep = tid < rest ? list[taken + tid] : 0;
+      __syncthreads();
+      if (tid < rest) list[tid] = keep;
+      have = rest;
+      taken = 0;
+      while (have < kWgRows && next < end) {
+        // 1024 ids, warp by warp 32 in a row
+        uint32_t mine[8];
+        int n = 0;
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
+        for (int i = 0; i < 8; ++i) {
+          const int at = next + (warp * 8 + i) * 32 + lane;
+          mine[i] = __ballot_sync(0xffffffffu, at < end && __ldg(p.ids + at) == l);
+          n += __popc(mine[i]);
+        }
+        if (lane == 0) warp_n[warp] = n;
+        __syncthreads();
+        int pos = have, all = 0;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int col = col0 + warp * 32 + f * 16 + h * 8 + g, j = i * 8 + t * 2;
-        if (col >= q.cols || j >= p.rank) continue;
-        const float v0 = c[f][i][h * 2] * up * s, v1 = c[f][i][h * 2 + 1] * up * s;
-        const long long at = q.rank_major ? (long long)j * q.cols + col : (long long)col * p.rank + j;
-        const long long step = q.rank_major ? q.cols : 1;
-        if (p.splits > 1) {
-          float* o = q.partial + ((long long)blockIdx.z * p.adapters + l) * mat + at;
-          o[0] = v0;
-          o[step] = v1;
-        } else {
-          const uint32_t pk = pack2<T>(v0, v1);
-          T* o = static_cast<T*>(q.out) + (long long)l * mat + at;
-          o[0] = reinterpret_cast<const T*>(&pk)[0];
-          o[step] = reinterpret_cast<const T*>(&pk)[1];
+        for (int i = 0; i < 4; ++i) {
+          if (i < warp) pos += warp_n[i];
+          all += warp_n[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if ((mine[i] >> lane) & 1) list[pos + __popc(mine[i] & ((1u << lane) - 1))] = next + (warp * 8 + i) * 32 + lane;
+          pos += __popc(mine[i]);
+        }
+        have += all;
+        next += kWgList;
+        __syncthreads();
+      }
+    };
+    // one chunk of up to 32 rows into a stage; returns its rows
+    auto load = [&](int stage) -> int {
+      refill();
+      const int n = min(kWgRows, have - taken);
+      if (n > 0) {
+#pragma unroll
+        for (int i0 = 0; i0 < kWgRows * (kWgCols / 8); i0 += 128) {
+          const int i = i0 + tid, r = i / (kWgCols / 8), c = i - r * (kWgCols / 8);
+          const bool ok = r < n && col0 + c * 8 < q.cols;
+          const T* src = X + (long long)list[taken + (r < n ? r : 0)] * q.cols + (ok ? col0 + c * 8 : 0);
+          cp_async16(smem_u32(xs + (stage * kWgRows + r) * kWgXStride + c * 16), src, ok);
+        }
+#pragma unroll
+        for (int i0 = 0; i0 < kWgRows * (RP / 4); i0 += 128) {
+          const int i = i0 + tid, r = i / (RP / 4), c = i - r * (RP / 4);
+          const bool ok = r < n && j0 + c * 4 < p.rank;
+          const float* src = q.v + (long long)list[taken + (r < n ? r : 0)] * p.rank + (ok ? j0 + c * 4 : 0);
+          cp_async16(smem_u32(vf + (stage * kWgRows + r) * RP + c * 4), src, ok);
+        }
+        taken += n;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      return n;
+    };
+
+    float c[2][NT][4];
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) c[f][i][0] = c[f][i][1] = c[f][i][2] = c[f][i][3] = 0.f;
+    int exponent = -200;
+    uint32_t filled = 0;                         // stages that hold rows
+#pragma unroll
+    for (int s = 0; s < kWgStages - 1; ++s) filled |= load(s) > 0 ? 1u << s : 0u;
+    for (int i = 0;; ++i) {
+      const int stage = i % kWgStages;
+      if (((filled >> stage) & 1) == 0) break;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kWgStages - 2) : "memory");
+      __syncthreads();
+      // the chunk's v as high parts and remainders
+      uint8_t* vb = vh + (i & 1) * 2 * kWgRows * VS;
+      const float* vc = vf + stage * kWgRows * RP;
+      float down = 1.f;
+      if constexpr (kHalf) {
+        float amax = 0.f;
+#pragma unroll
+        for (int e = tid; e < kWgRows * RP / 4; e += 128) {
+          const float4 x = reinterpret_cast<const float4*>(vc)[e];
+          amax = fmaxf(amax, fmaxf(fmaxf(finite_abs(x.x), finite_abs(x.y)), fmaxf(finite_abs(x.z), finite_abs(x.w))));
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+        if (lane == 0) warp_max[warp] = amax;
+        __syncthreads();
+        amax = fmaxf(fmaxf(warp_max[0], warp_max[1]), fmaxf(warp_max[2], warp_max[3]));
+        const int e = scale_exponent(amax);
+        if (amax > 0.f && e > exponent) {
+          if (exponent >= -110) {
+            const float f = exp2i(max(-126, exponent - e));
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+              for (int b = 0; b < NT; ++b) { c[a][b][0] *= f; c[a][b][1] *= f; c[a][b][2] *= f; c[a][b][3] *= f; }
+          }
+          exponent = e;
+        }
+        down = exponent < -110 ? 1.f : exp2i(-exponent);
+      }
+#pragma unroll
+      for (int e = tid; e < kWgRows * RP / 4; e += 128) {
+        const int r = e / (RP / 4), j = e - r * (RP / 4);
+        const float4 x = reinterpret_cast<const float4*>(vc)[e];
+        uint2 h, w;
+        split2<T>(x.x * down, x.y * down, h.x, w.x);
+        split2<T>(x.z * down, x.w * down, h.y, w.y);
+        *reinterpret_cast<uint2*>(vb + r * VS + j * 8) = h;
+        *reinterpret_cast<uint2*>(vb + (kWgRows + r) * VS + j * 8) = w;
+      }
+      const int into = (i + kWgStages - 1) % kWgStages;
+      const bool got = load(into) > 0;           // the stage of chunk i - 1: all have passed the barrier above
+      filled = (filled & ~(1u << into)) | (got ? 1u << into : 0u);
+      __syncthreads();
+      const uint32_t xa = smem_u32(xs + stage * kWgRows * kWgXStride) +
+                          ((lane >> 4) * 8 + (lane & 7)) * kWgXStride + (warp * 32 + ((lane >> 3) & 1) * 8) * 2;
+      const uint32_t va = smem_u32(vb) + (((lane >> 3) & 1) * 8 + (lane & 7)) * VS + (lane >> 4) * 16;
+#pragma unroll
+      for (int k = 0; k < kWgRows / 16; ++k) {
+        uint32_t a[2][4];
+        ldmatrix_x4_trans(a[0], xa + k * 16 * kWgXStride);
+        ldmatrix_x4_trans(a[1], xa + k * 16 * kWgXStride + 32);
+#pragma unroll
+        for (int j = 0; j < NT / 2; ++j) {
+          uint32_t h[4], w[4];
+          ldmatrix_x4_trans(h, va + k * 16 * VS + j * 32);
+          ldmatrix_x4_trans(w, va + (kWgRows + k * 16) * VS + j * 32);
+#pragma unroll
+          for (int f = 0; f < 2; ++f) {
+            mma16816<T>(c[f][2 * j], a[f], h[0], h[1]);
+            mma16816<T>(c[f][2 * j + 1], a[f], h[2], h[3]);
+          }
+#pragma unroll
+          for (int f = 0; f < 2; ++f) {
+            mma16816<T>(c[f][2 * j], a[f], w[0], w[1]);
+            mma16816<T>(c[f][2 * j + 1], a[f], w[2], w[3]);
+          }
         }
       }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+    const float s = (p.splits == 1 ? __ldg(p.scaling + l) : 1.f);
+    const float up = kHalf && exponent >= -110 ? exp2i(exponent) : 1.f;
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int col = col0 + warp * 32 + f * 16 + h * 8 + g, j = j0 + i * 8 + t * 2;
+          if (col >= q.cols || j >= p.rank) continue;
+          const float v0 = c[f][i][h * 2] * up * s, v1 = c[f][i][h * 2 + 1] * up * s;
+          const long long at = q.rank_major ? (long long)j * q.cols + col : (long long)col * p.rank + j;
+          const long long step = q.rank_major ? q.cols : 1;
+          if (p.splits > 1) {
+            float* o = q.partial + ((long long)blockIdx.y * p.adapters + l) * mat + at;
+            o[0] = v0;
+            o[step] = v1;
+          } else {
+            const uint32_t pk = pack2<T>(v0, v1);
+            T* o = static_cast<T*>(q.out) + (long long)l * mat + at;
+            o[0] = reinterpret_cast<const T*>(&pk)[0];
+            o[step] = reinterpret_cast<const T*>(&pk)[1];
+          }
+        }
+    __syncthreads();                             // the list and the stages are free for the next adapter
+  }
+  skip_adapters(done, p.adapters);
 }
 
-// out = s_l * sum of the splits' partials, in split order.
+// out = s_l * sum of the splits' partials that hold rows of the adapter, in split order.
 template <typename T>
 __global__ void __launch_bounds__(256)
 lora_wgrad_finish_kernel(const AdapterGradArgs p) {
@@ -571,12 +618,16 @@ lora_wgrad_finish_kernel(const AdapterGradArgs p) {
     if (q.out == nullptr) continue;
     const long long mat = (long long)q.cols * p.rank, all = mat * p.adapters;
     for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < all; i += (long long)gridDim.x * 1024) {
+      const int l = int(i / mat);
       float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      bool any = false;
       for (int s = 0; s < p.splits; ++s) {
+        if (__ldg(p.present + (long long)s * p.adapters + l) == 0) continue;
         const float4 v = __ldg(reinterpret_cast<const float4*>(q.partial + s * all + i));
         sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+        any = true;
       }
-      const float f = __ldg(p.scaling + i / mat);
+      const float f = any ? __ldg(p.scaling + l) : 0.f;
       uint2 o;
       o.x = pack2<T>(sum.x * f, sum.y * f);
       o.y = pack2<T>(sum.z * f, sum.w * f);
@@ -663,7 +714,7 @@ static int launch_wgrad(const AdapterGradArgs& p, cudaStream_t stream) {
   auto* kernel = lora_wgrad_kernel<T, NT>;
   static SmemLimitSeen seen;
   FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(wg_smem<NT>()), seen));
-  kernel<<<dim3(p.g[0].tiles + p.g[1].tiles, p.adapters, p.splits), 128, wg_smem<NT>(), stream>>>(p);
+  kernel<<<dim3(p.g[0].tiles + p.g[1].tiles, p.splits, ceil_div(p.rank, kWgRank)), 128, wg_smem<NT>(), stream>>>(p);
   FLYMOE_CUDA_CHECK(cudaGetLastError());
   if (p.splits > 1) {
     lora_wgrad_finish_kernel<T><<<sm_count() * 2, 256, 0, stream>>>(p);
@@ -673,8 +724,7 @@ static int launch_wgrad(const AdapterGradArgs& p, cudaStream_t stream) {
 }
 template <typename T>
 static int launch_wgrad_rank(const AdapterGradArgs& p, cudaStream_t s) {
-  return p.rank <= 16 ? launch_wgrad<T, 2>(p, s) : p.rank <= 32 ? launch_wgrad<T, 4>(p, s)
-       : p.rank <= 64 ? launch_wgrad<T, 8>(p, s) : launch_wgrad<T, 16>(p, s);
+  return p.rank <= 16 ? launch_wgrad<T, 2>(p, s) : p.rank <= 32 ? launch_wgrad<T, 4>(p, s) : launch_wgrad<T, 8>(p, s);
 }
 
 }  // namespace flymoe
@@ -738,12 +788,15 @@ extern "C" int flymoe_lora_add(void* out, const void* base, const void* x, const
                                               stream);
 }
 
-extern "C" int flymoe_lora_wgrad_splits(int rows, int k, int n, int adapters) {
-  if (rows < 1 || k < 8 || n < 8 || adapters < 1) return 1;
-  // four blocks for every SM, at least 512 rows in a split (its partial sums cost as much as they save below that)
-  const long long blocks = (long long)adapters * (flymoe::ceil_div(k, flymoe::kWgCols) + flymoe::ceil_div(n, flymoe::kWgCols));
-  const long long want = 4LL * flymoe::sm_count() / blocks;
-  return int(std::max(1LL, std::min({(long long)flymoe::kLoraMaxSplits, want, (long long)rows / 512})));
+extern "C" int flymoe_lora_wgrad_splits(int rows, int k, int n, int rank, int adapters) {
+  using namespace flymoe;
+  if (rows < 1 || k < 8 || n < 8 || rank < 8 || adapters < 1) return 1;
+  // blocks for every place on the device (three an SM, two from rank 33 on), at least 256 rows in a split, and partial sums
+  // of 256 MB at most
+  const long long blocks = (long long)(ceil_div(k, kWgCols) + ceil_div(n, kWgCols)) * ceil_div(rank, kWgRank);
+  const long long want = (rank <= 32 ? 3LL : 2LL) * sm_count() / blocks;
+  const long long fit = (256LL << 20) / ((long long)adapters * rank * (k + n) * 4);
+  return int(std::max(1LL, std::min({(long long)kLoraMaxSplits, want, fit, (long long)rows / 256})));
 }
 
 extern "C" int flymoe_lora_wgrad(void* da, void* db, const void* x, const void* dout, const float* v, const float* dv,
@@ -760,6 +813,7 @@ extern "C" int flymoe_lora_wgrad(void* da, void* db, const void* x, const void* 
                      aligned16(partial), "lora_wgrad: pointers must be 16-byte aligned");
   AdapterGradArgs p = {};
   float* partial_b = da && partial ? partial + (long long)splits * adapters * k * rank : partial;
+  p.present = partial_b ? reinterpret_cast<int*>(partial_b + (db ? (long long)splits * adapters * n * rank : 0)) : nullptr;
   if (da) p.g[0] = {x, dv, da, partial, k, ceil_div(k, kWgCols), 1};
   if (db) p.g[1] = {dout, v, db, partial_b, n, ceil_div(n, kWgCols), 0};
   p.ids = ids;

@@ -180,10 +180,10 @@ constexpr int kExThreads = 384;
 constexpr int kExEpi = 256;
 struct __align__(16) ExpandCtrl {
   unsigned long long y_full[4], y_empty[4], b_full[2], b_empty[2], acc_full[2], acc_empty[2];
-  unsigned long long row_ready, row_taken;       // a row tile's list and v are set up; producer and issuer know its count
+  unsigned long long row_ready;                  // a row tile's v is set up
   unsigned long long together, tile_done;        // epilogue warps: barrier; their part of the output tile is written
   uint32_t tmem_base;
-  int abort_flag, count, list[kTileAdapters];
+  int abort_flag, count, list[2][kTileAdapters];   // the producer's and the epilogue's
   int id[kTileRows], row_max[kTileRows];
 };
 constexpr int kExB = 2;                          // adapter tiles in flight
@@ -223,7 +223,6 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     for (int i = 0; i < kExB; ++i) { mbar_init(smem_u32(&c->b_full[i]), 1); mbar_init(smem_u32(&c->b_empty[i]), 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&c->acc_full[i]), 1); mbar_init(smem_u32(&c->acc_empty[i]), kExEpi / 32); }
     mbar_init(smem_u32(&c->row_ready), kExEpi);
-    mbar_init(smem_u32(&c->row_taken), 2);
     mbar_init(smem_u32(&c->together), kExEpi / 32);
     mbar_init(smem_u32(&c->tile_done), kExEpi / 32);
     c->abort_flag = 0;
@@ -234,23 +233,28 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   tcgen05_fence_after();
   const uint32_t tmem = c->tmem_base;
   // consecutive column tiles of a row tile, so that the rows' v is set up once or twice per block
+  // adapters of a row tile: every role looks for itself, ahead of the others where it can
+  auto find_adapters = [&](int rt, int* list) {
+    int id[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, rt * kTileRows + i * 32 + lane, p.rows, p.adapters);
+    const int n = tile_adapters(id, lane, list);
+    __syncwarp();
+    return n;
+  };
   const int u0 = int((long long)q.units * blockIdx.x / gridDim.x), u1 = int((long long)q.units * (blockIdx.x + 1) / gridDim.x);
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     int ys = 0, bs = 0, row_tile = -1, d = 0;
-    uint32_t yp = 0, bp = 0, rp = 0;
+    int* list = c->list[0];
+    uint32_t yp = 0, bp = 0;
     bool ok = true;
     for (int u = u0; u < u1 && ok; ++u) {
       const int rt = u / q.col_tiles, col = (u - rt * q.col_tiles) * kExCols;
       if (rt != row_tile) {
-        ok = warp_wait(smem_u32(&c->row_ready), rp, abort_flag, q.status, 5, 32);
-        if (!ok) break;
-        rp ^= 1;
         row_tile = rt;
-        d = c->count;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&c->row_taken));
+        d = find_adapters(rt, list);
       }
       if (d > kTileAdapters) continue;
       ok = warp_wait(smem_u32(&c->y_empty[ys]), yp ^ 1, abort_flag, q.status, 1, 32);
@@ -274,7 +278,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
         if (elect_one()) {
           mbar_expect_tx(bfull, KC * kChunkBytes);
 #pragma unroll
-          for (int k = 0; k < KC; ++k) tma_load_3d(bdst + k * kChunkBytes, &tmap_b, bfull, k * 128, col, c->list[i]);
+          for (int k = 0; k < KC; ++k) tma_load_3d(bdst + k * kChunkBytes, &tmap_b, bfull, k * 128, col, list[i]);
         }
         __syncwarp();
         if (++bs == kExB) { bs = 0; bp ^= 1; }
@@ -290,13 +294,13 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     for (int u = u0; u < u1 && ok; ++u) {
       const int rt = u / q.col_tiles;
       if (rt != row_tile) {
-        ok = warp_wait(smem_u32(&c->row_ready), rp, abort_flag, q.status, 5);
-        if (!ok) break;
-        rp ^= 1;
         row_tile = rt;
-        d = c->count;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&c->row_taken));
+        d = find_adapters(rt, nullptr);
+        if (d >= 1 && d <= kTileAdapters) {      // otherwise nobody multiplies, and nobody signals
+          ok = warp_wait(smem_u32(&c->row_ready), rp, abort_flag, q.status, 5);
+          if (!ok) break;
+          rp ^= 1;
+        }
       }
       if (d > kTileAdapters) continue;
       for (int i = 0; i < d && ok; ++i) {
@@ -324,7 +328,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     const int et = threadIdx.x - 128, wg = et >> 7, row = et & 127;
     const int sw = row & 7;
     int ys = 0, acc = 0, row_tile = -1, d = 0, mine = -1, stored = 0;
-    uint32_t yp = 0, accp = 0, tp = 0;
+    uint32_t yp = 0, accp = 0;
     float scale = 0.f;
     bool ok = true;
     uint32_t together = 0, done = 0;
@@ -338,67 +342,60 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     for (int u = u0; u < u1 && ok; ++u) {
       const int rt = u / q.col_tiles, col = (u - rt * q.col_tiles) * kExCols;
       if (rt != row_tile) {
-        // The MMAs of the previous row tile are done (their last sums have been read here), and with them all loads by
-        // its list; its count may still be unread where it was zero.
-        if (row_tile >= 0) {
-          ok = warp_wait(smem_u32(&c->row_taken), tp, abort_flag, q.status, 7);
-          if (!ok) break;
-          tp ^= 1;
-        }
+        // the MMAs of the previous row tile are done (their last sums have been read here): its v may go
         row_tile = rt;
         mine = row_adapter(p.ids, rt * kTileRows + row, p.rows, p.adapters);
-        ok = sync();                             // all have left the previous list
+        ok = sync();                             // and all have left its list
         if (!ok) break;
         if (et < 32) {
-          int id[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, rt * kTileRows + i * 32 + lane, p.rows, p.adapters);
-          const int n = tile_adapters(id, lane, c->list);
-          if (lane == 0) c->count = n;
+          d = find_adapters(rt, c->list[1]);
+          if (lane == 0) c->count = d;
         }
         if (wg == 0) c->id[row] = mine;
         ok = sync();
         if (!ok) break;
         d = c->count;
-        scale = mine >= 0 ? __ldg(p.scaling + mine) : 0.f;
-        // v as high parts and remainders: four numbers a thread and step, consecutive threads along a row
-        const int vecs = (p.rank + 15) / 16 * 4;
-        auto load = [&](int i, int& r, int& k4) {
-          r = i / vecs;
-          k4 = i - r * vecs;
-          return d <= kTileAdapters && c->id[r] >= 0 && k4 * 4 < p.rank
-                     ? __ldg(reinterpret_cast<const float4*>(p.v + (long long)(rt * kTileRows + r) * p.rank + k4 * 4))
-                     : make_float4(0.f, 0.f, 0.f, 0.f);
-        };
-        if constexpr (std::is_same<T, __half>::value) {
-          if (wg == 0) c->row_max[row] = 0;
-          ok = sync();
-          if (!ok) break;
+        if (d >= 1 && d <= kTileAdapters) {
+          scale = mine >= 0 ? __ldg(p.scaling + mine) : 0.f;
+          // v as high parts and remainders: four numbers a thread and step, consecutive threads along a row
+          const int vecs = (p.rank + 15) / 16 * 4;
+          auto load = [&](int i, int& r, int& k4) {
+            r = i / vecs;
+            k4 = i - r * vecs;
+            return c->id[r] >= 0 && k4 * 4 < p.rank
+                       ? __ldg(reinterpret_cast<const float4*>(p.v + (long long)(rt * kTileRows + r) * p.rank + k4 * 4))
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+          };
+          if constexpr (std::is_same<T, __half>::value) {
+            if (wg == 0) c->row_max[row] = 0;
+            ok = sync();
+            if (!ok) break;
+            for (int i = et; i < kTileRows * vecs; i += kExEpi) {
+              int r, k4;
+              const float4 x = load(i, r, k4);
+              const float m = fmaxf(fmaxf(finite_abs(x.x), finite_abs(x.y)), fmaxf(finite_abs(x.z), finite_abs(x.w)));
+              atomicMax(&c->row_max[r], __float_as_int(m));          // not negative: ordered like the numbers
+            }
+            ok = sync();
+            if (!ok) break;
+            scale *= exp2i(scale_exponent(__int_as_float(c->row_max[row])));
+          }
+#pragma unroll 4
           for (int i = et; i < kTileRows * vecs; i += kExEpi) {
             int r, k4;
             const float4 x = load(i, r, k4);
-            const float m = fmaxf(fmaxf(finite_abs(x.x), finite_abs(x.y)), fmaxf(finite_abs(x.z), finite_abs(x.w)));
-            atomicMax(&c->row_max[r], __float_as_int(m));          // not negative: ordered like the numbers
+            float down = 1.f;
+            if constexpr (std::is_same<T, __half>::value) down = exp2i(-scale_exponent(__int_as_float(c->row_max[r])));
+            uint2 hi, lo;
+            split2<T>(x.x * down, x.y * down, hi.x, lo.x);
+            split2<T>(x.z * down, x.w * down, hi.y, lo.y);
+            uint8_t* at = vtile + (k4 >> 4) * kChunkBytes + r * 128 + ((((k4 >> 1) & 7) ^ (r & 7)) * 16) + (k4 & 1) * 8;
+            *reinterpret_cast<uint2*>(at) = hi;
+            *reinterpret_cast<uint2*>(at + KC * kChunkBytes) = lo;
           }
-          ok = sync();
-          if (!ok) break;
-          scale *= exp2i(scale_exponent(__int_as_float(c->row_max[row])));
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          mbar_arrive(smem_u32(&c->row_ready));
         }
-#pragma unroll 4
-        for (int i = et; i < kTileRows * vecs; i += kExEpi) {
-          int r, k4;
-          const float4 x = load(i, r, k4);
-          float down = 1.f;
-          if constexpr (std::is_same<T, __half>::value) down = exp2i(-scale_exponent(__int_as_float(c->row_max[r])));
-          uint2 hi, lo;
-          split2<T>(x.x * down, x.y * down, hi.x, lo.x);
-          split2<T>(x.z * down, x.w * down, hi.y, lo.y);
-          uint8_t* at = vtile + (k4 >> 4) * kChunkBytes + r * 128 + ((((k4 >> 1) & 7) ^ (r & 7)) * 16) + (k4 & 1) * 8;
-          *reinterpret_cast<uint2*>(at) = hi;
-          *reinterpret_cast<uint2*>(at + KC * kChunkBytes) = lo;
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(smem_u32(&c->row_ready));
       }
       if (d > kTileAdapters) continue;           // its rows are the other kernel's
       ok = warp_wait(smem_u32(&c->y_full[ys]), yp, abort_flag, q.status, 6);
@@ -412,7 +409,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
         ok = warp_wait(smem_u32(&c->acc_full[acc]), accp, abort_flag, q.status, 4);
         if (!ok) break;
         tcgen05_fence_after();
-        const bool hit = mine == c->list[i];
+        const bool hit = mine == c->list[1][i];
         if (__any_sync(0xffffffffu, hit)) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {

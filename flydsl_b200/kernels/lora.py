@@ -121,11 +121,11 @@ class _LoraAdd(torch.autograd.Function):
                 dx = _expand(torch.empty_like(x), None, dv, _transposed(a), ids, scaling)
             if need_a or need_b:
                 lib, (rows, k), (adapters, n, rank) = _lib.load(), x.shape, b.shape
-                splits = lib.flymoe_lora_wgrad_splits(rows, k, n, adapters)
+                splits = lib.flymoe_lora_wgrad_splits(rows, k, n, rank, adapters)
                 da = torch.empty_like(a) if need_a else None
                 db = torch.empty_like(b) if need_b else None
                 width = (k if need_a else 0) + (n if need_b else 0)
-                partial = x.new_empty(splits * adapters * rank * width, dtype=torch.float32) if splits > 1 else None
+                partial = x.new_empty(splits * adapters * (rank * width + 1), dtype=torch.float32) if splits > 1 else None
                 _lib.check(lib.flymoe_lora_wgrad(
                     _lib.ptr(da), _lib.ptr(db), x.data_ptr(), dout.data_ptr(), v.data_ptr(), _lib.ptr(dv), ids.data_ptr(),
                     scaling.data_ptr(), _lib.ptr(partial), rows, k, n, rank, adapters, splits, _lib.DTYPE_CODE[x.dtype],

@@ -375,7 +375,7 @@ int flymoe_combine_rows_backward(const void* dout, const void* rows_in, const fl
  * [adapters, k, rank] (flymoe_lora_transpose: `mats` matrices [rows, cols] of 16-bit values).
  * flymoe_lora_wgrad: da[l] = scaling[l] sum over l's rows of dv^T x, db[l] = scaling[l] sum of dout^T v (v, dv f32 [rows,
  * rank]); da or db may be NULL; an adapter without rows gets zeros.  splits > 1 cuts the rows, partial is then f32 scratch of
- * splits * adapters * rank * (k if da + n if db); flymoe_lora_wgrad_splits proposes a number.  No counterpart in the reference. */
+ * splits * adapters * (rank * (k if da + n if db) + 1); flymoe_lora_wgrad_splits proposes a number.  No counterpart in the reference. */
 int flymoe_lora_add(void* out, const void* base, const void* x, const void* a, const void* b, const int32_t* ids,
                     const float* scaling, float* v, int rows, int k, int n, int rank, int adapters, int splits, int dtype,
                     void* stream);
@@ -384,7 +384,7 @@ int flymoe_lora_shrink(float* v, const void* x, const void* a, const int32_t* id
                        int splits, int fold, int dtype, void* stream);
 int flymoe_lora_expand(void* out, const void* base, const float* v, const void* b, const int32_t* ids, const float* scaling,
                        int rows, int n, int rank, int adapters, int splits, int dtype, void* stream);
-int flymoe_lora_wgrad_splits(int rows, int k, int n, int adapters);
+int flymoe_lora_wgrad_splits(int rows, int k, int n, int rank, int adapters);
 int flymoe_lora_wgrad(void* da, void* db, const void* x, const void* dout, const float* v, const float* dv,
                       const int32_t* ids, const float* scaling, float* partial, int rows, int k, int n, int rank,
                       int adapters, int splits, int dtype, void* stream);
