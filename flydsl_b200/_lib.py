@@ -87,13 +87,11 @@ _SIGNATURES = {
     "flymoe_permute_rows": (c_int, [_P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),
     "flymoe_combine_rows": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
     "flymoe_combine_rows_backward": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
-    "flymoe_lora_add": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
-    "flymoe_lora_shrink_splits": (c_int, [c_int, c_int]),
-    "flymoe_lora_shrink": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
-    "flymoe_lora_expand": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
-    "flymoe_lora_wgrad_splits": (c_int, [c_int, c_int, c_int, c_int, c_int]),
-    "flymoe_lora_wgrad": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
-    "flymoe_lora_transpose": (c_int, [_P, _P, c_int, c_int, c_int, _P]),
+    "flymoe_lora_v_elems": (c_int64, [c_int, c_int, c_int]),
+    "flymoe_lora_add": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
+    "flymoe_lora_backward_workspace_elems": (c_int64, [c_int, c_int, c_int, c_int, c_int]),
+    "flymoe_lora_backward": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64,
+                                     c_int, c_int, c_int, c_int, c_int, c_int, _P]),
     "flymoe_moe_reduce": (c_int, [_P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),
     "flymoe_sorted_inverse": (c_int, [_P, _P, _P, c_int, c_int, c_int, _P]),
     "flymoe_quant_act_1x128": (c_int, [_P, c_int, _P, _P, c_int64, c_int, c_int, _P]),

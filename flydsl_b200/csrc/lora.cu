@@ -21,7 +21,6 @@
 // consecutive elements where the instruction's layout has pairs.
 #include <algorithm>
 #include <stdio.h>
-#include <stdlib.h>
 #include <type_traits>
 
 #include "common.cuh"
@@ -166,6 +165,7 @@ lora_shrink_kernel(const ShrinkArgs p, const int slots, const bool skip_tiles) {
   __shared__ __align__(16) Groups s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int row0 = int(blockIdx.x) / slots * kWindow;
+  after_previous_launch();
   build_groups(&s, p.ids, row0, p.rows, p.adapters, skip_tiles, false);
   const int steps = (p.k + 31) / 32;
   const int s0 = int((long long)steps * blockIdx.y / p.splits), s1 = int((long long)steps * (blockIdx.y + 1) / p.splits);
@@ -226,6 +226,7 @@ lora_shrink_kernel(const ShrinkArgs p, const int slots, const bool skip_tiles) {
 // The splits' sums added up into the first, in their order.
 __global__ void __launch_bounds__(256)
 lora_fold_kernel(float4* __restrict__ v, long long vecs, int splits) {
+  after_previous_launch();
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < vecs; i += (long long)gridDim.x * 256) {
     float4 sum = v[i];
     for (int s = 1; s < splits; ++s) {
@@ -246,6 +247,7 @@ lora_expand_kernel(const ExpandArgs p, const int slots, const int per_warp, cons
   __shared__ __align__(16) Groups s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int row0 = int(blockIdx.x) / slots * kWindow;
+  after_previous_launch();
   // rows without an adapter have to be written unless they are there already
   build_groups(&s, p.ids, row0, p.rows, p.adapters, skip_tiles, p.out != p.base);
   const int c0 = (int(blockIdx.y) * (kGroupThreads / 32) + warp) * per_warp * 32;
@@ -393,6 +395,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
   const int begin = int((long long)p.rows * blockIdx.y / p.splits), end = int((long long)p.rows * (blockIdx.y + 1) / p.splits);
   const T* X = static_cast<const T*>(q.x);
   const long long mat = (long long)q.cols * p.rank;
+  after_previous_launch();
 
   // the smallest adapter above `l` with rows here, or p.adapters
   auto find_next = [&](int l) -> int {
@@ -500,18 +503,12 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
     for (int f = 0; f < 2; ++f)
 #pragma unroll
       for (int i = 0; i < NT; ++i) c[f][i][0] = c[f][i][1] = c[f][i][2] = c[f][i][3] = 0.f;
-    int exponent = -200;
+    int exponent = -200, next_exponent = -200;   // of the sums, of the chunk converted last
     uint32_t filled = 0;                         // stages that hold rows
-#pragma unroll
-    for (int s = 0; s < kWgStages - 1; ++s) filled |= load(s) > 0 ? 1u << s : 0u;
-    for (int i = 0;; ++i) {
-      const int stage = i % kWgStages;
-      if (((filled >> stage) & 1) == 0) break;
-      asm volatile("cp.async.wait_group %0;" ::"n"(kWgStages - 2) : "memory");
-      __syncthreads();
-      // the chunk's v as high parts and remainders
+    // a chunk's v as high parts and remainders, into one of two buffers
+    auto convert = [&](int i) {
       uint8_t* vb = vh + (i & 1) * 2 * kWgRows * VS;
-      const float* vc = vf + stage * kWgRows * RP;
+      const float* vc = vf + (i % kWgStages) * kWgRows * RP;
       float down = 1.f;
       if constexpr (kHalf) {
         float amax = 0.f;
@@ -526,17 +523,8 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
         __syncthreads();
         amax = fmaxf(fmaxf(warp_max[0], warp_max[1]), fmaxf(warp_max[2], warp_max[3]));
         const int e = scale_exponent(amax);
-        if (amax > 0.f && e > exponent) {
-          if (exponent >= -110) {
-            const float f = exp2i(max(-126, exponent - e));
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-              for (int b = 0; b < NT; ++b) { c[a][b][0] *= f; c[a][b][1] *= f; c[a][b][2] *= f; c[a][b][3] *= f; }
-          }
-          exponent = e;
-        }
-        down = exponent < -110 ? 1.f : exp2i(-exponent);
+        if (amax > 0.f && e > next_exponent) next_exponent = e;
+        down = next_exponent < -110 ? 1.f : exp2i(-next_exponent);
       }
 #pragma unroll
       for (int e = tid; e < kWgRows * RP / 4; e += 128) {
@@ -548,10 +536,34 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
         *reinterpret_cast<uint2*>(vb + r * VS + j * 8) = h;
         *reinterpret_cast<uint2*>(vb + (kWgRows + r) * VS + j * 8) = w;
       }
+    };
+#pragma unroll
+    for (int s = 0; s < kWgStages - 1; ++s) filled |= load(s) > 0 ? 1u << s : 0u;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kWgStages - 2) : "memory");
+    __syncthreads();
+    convert(0);                                  // an adapter in the list has a row
+    // one barrier a chunk: chunk i is multiplied while chunk i + 1 is converted and chunk i + 3 asked for
+    for (int i = 0; (filled >> (i % kWgStages)) & 1; ++i) {
+      const int stage = i % kWgStages;
+      if constexpr (kHalf) {
+        if (next_exponent > exponent) {          // the scale that chunk i was converted with
+          if (exponent >= -110) {
+            const float f = exp2i(max(-126, exponent - next_exponent));
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+              for (int b = 0; b < NT; ++b) { c[a][b][0] *= f; c[a][b][1] *= f; c[a][b][2] *= f; c[a][b][3] *= f; }
+          }
+          exponent = next_exponent;
+        }
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(kWgStages - 3) : "memory");
+      __syncthreads();                           // chunk i + 1 is here, chunk i converted, chunk i - 1 multiplied
       const int into = (i + kWgStages - 1) % kWgStages;
-      const bool got = load(into) > 0;           // the stage of chunk i - 1: all have passed the barrier above
+      const bool got = load(into) > 0;
       filled = (filled & ~(1u << into)) | (got ? 1u << into : 0u);
-      __syncthreads();
+      if ((filled >> ((i + 1) % kWgStages)) & 1) convert(i + 1);
+      uint8_t* vb = vh + (i & 1) * 2 * kWgRows * VS;
       const uint32_t xa = smem_u32(xs + stage * kWgRows * kWgXStride) +
                           ((lane >> 4) * 8 + (lane & 7)) * kWgXStride + (warp * 32 + ((lane >> 3) & 1) * 8) * 2;
       const uint32_t va = smem_u32(vb) + (((lane >> 3) & 1) * 8 + (lane & 7)) * VS + (lane >> 4) * 16;
@@ -613,53 +625,69 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
 template <typename T>
 __global__ void __launch_bounds__(256)
 lora_wgrad_finish_kernel(const AdapterGradArgs p) {
-  for (int which = 0; which < 2; ++which) {
-    const AdapterGrad q = p.g[which];
-    if (q.out == nullptr) continue;
-    const long long mat = (long long)q.cols * p.rank, all = mat * p.adapters;
-    for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < all; i += (long long)gridDim.x * 1024) {
-      const int l = int(i / mat);
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      bool any = false;
-      for (int s = 0; s < p.splits; ++s) {
-        if (__ldg(p.present + (long long)s * p.adapters + l) == 0) continue;
-        const float4 v = __ldg(reinterpret_cast<const float4*>(q.partial + s * all + i));
-        sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
-        any = true;
-      }
-      const float f = any ? __ldg(p.scaling + l) : 0.f;
-      uint2 o;
-      o.x = pack2<T>(sum.x * f, sum.y * f);
-      o.y = pack2<T>(sum.z * f, sum.w * f);
-      *reinterpret_cast<uint2*>(static_cast<T*>(q.out) + i) = o;
+  const AdapterGrad q = p.g[blockIdx.y];
+  if (q.out == nullptr) return;
+  const long long mat = (long long)q.cols * p.rank, all = mat * p.adapters;
+  after_previous_launch();
+  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < all; i += (long long)gridDim.x * 1024) {
+    const int l = int(i / mat);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    bool any = false;
+    for (int s = 0; s < p.splits; ++s) {
+      if (__ldg(p.present + (long long)s * p.adapters + l) == 0) continue;
+      const float4 v = __ldg(reinterpret_cast<const float4*>(q.partial + s * all + i));
+      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+      any = true;
     }
+    const float f = any ? __ldg(p.scaling + l) : 0.f;
+    uint2 o;
+    o.x = pack2<T>(sum.x * f, sum.y * f);
+    o.y = pack2<T>(sum.z * f, sum.w * f);
+    *reinterpret_cast<uint2*>(static_cast<T*>(q.out) + i) = o;
   }
 }
 
-// dst[m][c][r] = src[m][r][c], 32 x 32 tiles.
+// dst[m][c][r] = src[m][r][c] for two sets of matrices (blockIdx.z: of the first, then of the second), 32 x 32 tiles.
+struct TransposeArgs {
+  const uint16_t* src[2];
+  uint16_t* dst[2];
+  int rows[2], cols[2], mats;
+};
 __global__ void __launch_bounds__(256)
-lora_transpose_kernel(const uint16_t* __restrict__ src, uint16_t* __restrict__ dst, int rows, int cols) {
+lora_transpose_kernel(const TransposeArgs p) {
   __shared__ uint16_t tile[32][34];
-  const long long mat = (long long)blockIdx.z * rows * cols;
-  const int c0 = blockIdx.x * 32, r0 = blockIdx.y * 32, x = threadIdx.x & 31, y = threadIdx.x >> 5;
-  for (int i = y; i < 32; i += 8)
-    if (r0 + i < rows && c0 + x < cols) tile[i][x] = src[mat + (long long)(r0 + i) * cols + c0 + x];
-  __syncthreads();
-  for (int i = y; i < 32; i += 8)
-    if (c0 + i < cols && r0 + x < rows) dst[mat + (long long)(c0 + i) * rows + r0 + x] = tile[x][i];
+  const int which = int(blockIdx.y) >= p.mats;
+  const int rows = p.rows[which], cols = p.cols[which], across = (cols + 31) / 32;
+  const long long mat = (long long)(int(blockIdx.y) - which * p.mats) * rows * cols;
+  const uint16_t* src = p.src[which] + mat;
+  uint16_t* dst = p.dst[which] + mat;
+  after_previous_launch();
+  for (int t = blockIdx.x; t < across * ((rows + 31) / 32); t += gridDim.x) {
+    const int c0 = t % across * 32, r0 = t / across * 32, x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    for (int i = y; i < 32; i += 8)
+      if (r0 + i < rows && c0 + x < cols) tile[i][x] = src[(long long)(r0 + i) * cols + c0 + x];
+    __syncthreads();
+    for (int i = y; i < 32; i += 8)
+      if (c0 + i < cols && r0 + x < rows) dst[(long long)(c0 + i) * rows + r0 + x] = tile[x][i];
+    __syncthreads();
+  }
 }
 
 // ---------------------------------------------------------------------------- host
-static int envint(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
-static bool on_tiles(int rows) { return rows >= envint("TC", 1024); }
-static int lora_check(const char* what, int rows, int width, int rank, int adapters, int splits, int dtype) {
+// Tiles of 128 rows from 512 rows on.  Both ways, whole calls, 4096 -> 4096, bf16, us on one B200 (tiles / groups of 16 rows):
+// 4 adapters in runs: 256 rows, rank 16 13.8 / 13.4, rank 128 20.8 / 43.5; 512 rows 13.6 / 16.8 and 24.5 / 50.6; 1024 rows
+// 15.9 / 26.2 and 27.0 / 95.3.  16 adapters in any order (tiles then only add launches that find nothing to do): 256 rows,
+// rank 16 21.2 / 12.7; 512 rows 29.1 / 20.5, rank 128 88.6 / 74.6; 8192 rows 134 / 82 and 484 / 388.
+static bool on_tiles(int rows) { return rows >= 512; }
+
+static int lora_check(const char* what, int rows, int k, int n, int rank, int adapters, int dtype) {
   char msg[160];
   const char* why = nullptr;
   if (rows < 0) why = "rows < 0";
-  else if (width < 8 || width % 8) why = "k and n must be positive multiples of 8";
+  else if (k < 8 || k % 8 || n < 8 || n % 8) why = "k and n must be positive multiples of 8";
+  else if (k > (1 << 29) || n > (1 << 29)) why = "k and n must not exceed 2^29";       // the tiles count bytes in 32 bits
   else if (rank < 8 || rank % 8 || rank > kLoraMaxRank) why = "rank must be a multiple of 8 in [8, 128]";
-  else if (adapters < 1 || adapters > 65535) why = "adapters must be in [1, 65535]";
-  else if (splits < 1 || splits > kLoraMaxSplits) why = "splits must be in [1, 16]";
+  else if (adapters < 1 || adapters > 32767) why = "adapters must be in [1, 32767]";
   else if (dtype != FLYMOE_BF16 && dtype != FLYMOE_F16) why = "dtype must be F16 or BF16";
   if (why == nullptr) return FLYMOE_OK;
   snprintf(msg, sizeof(msg), "%s: %s", what, why);
@@ -667,6 +695,14 @@ static int lora_check(const char* what, int rows, int width, int rank, int adapt
   return FLYMOE_ERR_INVALID_ARGUMENT;
 }
 
+// Pieces of k that a shrink's sums are cut into.
+static int shrink_splits(int rows, int k) {
+  if (rows < 1) return 1;
+  if (on_tiles(rows))                            // two tiles of 128 rows for every SM, at least four K blocks of 64 in a piece
+    return std::max(1, std::min({kLoraMaxSplits, 2 * sm_count() / ceil_div(rows, 128), k / 256}));
+  // blocks of 16 rows for three on every SM, at least sixteen 32-wide steps (two a warp) in a piece
+  return std::max(1, std::min({kLoraMaxSplits, 3 * sm_count() / ceil_div(rows, 16), ceil_div(k, 32) / 16}));
+}
 // Groups that a window of up to 512 rows can hold: one for every sixteen rows and one for every adapter's last.
 static int window_groups(int rows, int adapters) {
   const int n = std::min(rows, kWindow);
@@ -681,8 +717,7 @@ static int launch_shrink(const ShrinkArgs& p, bool skip_tiles, cudaStream_t stre
   // three blocks for every SM where there are that many groups
   const int windows = ceil_div(p.rows, kWindow);
   const int slots = std::max(1, std::min(window_groups(p.rows, p.adapters), 3 * sm_count() / (windows * p.splits)));
-  kernel<<<dim3(windows * slots, p.splits), kGroupThreads, smem, stream>>>(p, slots, skip_tiles);
-  FLYMOE_CUDA_CHECK(cudaGetLastError());
+  FLYMOE_CUDA_CHECK(launch_closely(kernel, dim3(windows * slots, p.splits), kGroupThreads, smem, stream, p, slots, skip_tiles));
   return FLYMOE_OK;
 }
 template <typename T>
@@ -696,12 +731,12 @@ static int launch_expand(const ExpandArgs& p, bool skip_tiles, cudaStream_t stre
   // Three blocks for every SM: row groups first, then columns.  A warp walks through up to eight column groups.
   const int want = 3 * sm_count();
   const int groups = window_groups(p.rows, p.adapters);
-  const int spans = std::max(ceil_div(cols, 8 * warps), std::min(ceil_div(cols, warps), want / std::min(want, windows * groups)));
+  const int spans = std::max(ceil_div(cols, 8 * warps),
+                             std::min(ceil_div(cols, warps), want / int(std::min<long long>(want, (long long)windows * groups))));
   const int per_warp = ceil_div(cols, spans * warps);
-  const int slots = std::max(1, std::min(groups, want / (windows * spans)));
-  lora_expand_kernel<T, KS><<<dim3(windows * slots, ceil_div(cols, per_warp * warps)), kGroupThreads, 0, stream>>>(
-      p, slots, per_warp, skip_tiles);
-  FLYMOE_CUDA_CHECK(cudaGetLastError());
+  const int slots = int(std::max(1LL, std::min((long long)groups, want / ((long long)windows * spans))));
+  FLYMOE_CUDA_CHECK(launch_closely(lora_expand_kernel<T, KS>, dim3(windows * slots, ceil_div(cols, per_warp * warps)), kGroupThreads,
+                                   0, stream, p, slots, per_warp, skip_tiles));
   return FLYMOE_OK;
 }
 template <typename T>
@@ -714,12 +749,12 @@ static int launch_wgrad(const AdapterGradArgs& p, cudaStream_t stream) {
   auto* kernel = lora_wgrad_kernel<T, NT>;
   static SmemLimitSeen seen;
   FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(wg_smem<NT>()), seen));
-  kernel<<<dim3(p.g[0].tiles + p.g[1].tiles, p.splits, ceil_div(p.rank, kWgRank)), 128, wg_smem<NT>(), stream>>>(p);
-  FLYMOE_CUDA_CHECK(cudaGetLastError());
-  if (p.splits > 1) {
-    lora_wgrad_finish_kernel<T><<<sm_count() * 2, 256, 0, stream>>>(p);
-    FLYMOE_CUDA_CHECK(cudaGetLastError());
-  }
+  FLYMOE_CUDA_CHECK(launch_closely(kernel, dim3(p.g[0].tiles + p.g[1].tiles, p.splits, ceil_div(p.rank, kWgRank)), 128,
+                                   wg_smem<NT>(), stream, p));
+  if (p.splits == 1) return FLYMOE_OK;
+  const long long most = (long long)std::max(p.g[0].cols, p.g[1].cols) * p.rank * p.adapters / 4;
+  FLYMOE_CUDA_CHECK(launch_closely(lora_wgrad_finish_kernel<T>, dim3(unsigned(std::min<long long>((most + 255) / 256, 8LL * sm_count())), 2),
+                                   256, 0, stream, p));
   return FLYMOE_OK;
 }
 template <typename T>
@@ -727,113 +762,155 @@ static int launch_wgrad_rank(const AdapterGradArgs& p, cudaStream_t s) {
   return p.rank <= 16 ? launch_wgrad<T, 2>(p, s) : p.rank <= 32 ? launch_wgrad<T, 4>(p, s) : launch_wgrad<T, 8>(p, s);
 }
 
-}  // namespace flymoe
-
-extern "C" int flymoe_lora_shrink_splits(int rows, int k) {
-  if (rows < 1 || k < 8) return 1;
-  if (flymoe::on_tiles(rows))                    // two tiles of 128 rows for every SM, at least four K blocks of 64 in a split
-    return std::max(1, std::min({flymoe::kLoraMaxSplits, 2 * flymoe::sm_count() / flymoe::ceil_div(rows, 128), k / 256}));
-  // blocks of 16 rows for three on every SM, at least sixteen 32-wide steps (two a warp) in a split
-  const int groups = flymoe::ceil_div(rows, 16), steps = flymoe::ceil_div(k, 32);
-  return std::max(1, std::min({flymoe::kLoraMaxSplits, 3 * flymoe::sm_count() / groups, steps / 16}));
-}
-
-extern "C" int flymoe_lora_shrink(float* v, const void* x, const void* a, const int32_t* ids, int rows, int k, int rank,
-                                  int adapters, int splits, int fold, int dtype, void* stream) {
-  using namespace flymoe;
-  int rc = lora_check("lora_shrink", rows, k, rank, adapters, splits, dtype);
-  if (rc != FLYMOE_OK || rows == 0) return rc;
-  FLYMOE_REQUIRE(v && x && a && ids, "lora_shrink: null pointer");
-  FLYMOE_REQUIRE(aligned16(x) && aligned16(a) && aligned16(v), "lora_shrink: pointers must be 16-byte aligned");
-  const ShrinkArgs p = {x, a, ids, v, rows, k, rank, adapters, splits};
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool skip = on_tiles(rows);
-  if (skip) rc = launch_shrink_sm100(p, dtype == FLYMOE_BF16, s);
-  if (rc == FLYMOE_OK && (!skip || adapters > kTileAdapters))
-    rc = dtype == FLYMOE_BF16 ? launch_shrink_rank<__nv_bfloat16>(p, skip, s) : launch_shrink_rank<__half>(p, skip, s);
-  if (rc != FLYMOE_OK || !fold || splits == 1) return rc;
-  const long long vecs = (long long)rows * rank / 4;
-  lora_fold_kernel<<<unsigned(std::min<long long>((vecs + 255) / 256, 4LL * sm_count())), 256, 0, s>>>(
-      reinterpret_cast<float4*>(v), vecs, splits);
-  FLYMOE_CUDA_CHECK(cudaGetLastError());
+// v = x A^T for all rows.  a_t: A transposed ([adapters, k, rank]), if that is what there is; then `a` is its other form
+// where the rows may need the kernels of this file (needs_both), else null.
+static int shrink(ShrinkArgs p, const void* a_t, bool fold, int dtype, cudaStream_t s) {
+  const bool bf = dtype == FLYMOE_BF16, tiles = on_tiles(p.rows);
+  int rc = FLYMOE_OK;
+  if (tiles) {
+    ShrinkArgs q = p;
+    if (a_t) { q.a = a_t; q.transposed = 1; }
+    rc = launch_shrink_sm100(q, bf, s);
+  }
+  if (rc == FLYMOE_OK && (!tiles || p.adapters > kTileAdapters))
+    rc = bf ? launch_shrink_rank<__nv_bfloat16>(p, tiles, s) : launch_shrink_rank<__half>(p, tiles, s);
+  if (rc != FLYMOE_OK || !fold || p.splits == 1) return rc;
+  const long long vecs = (long long)p.rows * p.rank / 4;
+  FLYMOE_CUDA_CHECK(launch_closely(lora_fold_kernel, unsigned(std::min<long long>((vecs + 255) / 256, 4LL * sm_count())), 256, 0, s,
+                                   reinterpret_cast<float4*>(p.v), vecs, p.splits));
   return FLYMOE_OK;
 }
-
-extern "C" int flymoe_lora_expand(void* out, const void* base, const float* v, const void* b, const int32_t* ids,
-                                  const float* scaling, int rows, int n, int rank, int adapters, int splits, int dtype,
-                                  void* stream) {
-  using namespace flymoe;
-  const int rc = lora_check("lora_expand", rows, n, rank, adapters, splits, dtype);
-  if (rc != FLYMOE_OK || rows == 0) return rc;
-  FLYMOE_REQUIRE(out && v && b && ids && scaling, "lora_expand: null pointer");
-  FLYMOE_REQUIRE(aligned16(out) && aligned16(base) && aligned16(v) && aligned16(b), "lora_expand: pointers must be 16-byte aligned");
-  FLYMOE_REQUIRE(splits == 1 || !on_tiles(rows), "lora_expand: this many rows take folded sums (splits = 1)");
-  const ExpandArgs p = {base, v, b, ids, scaling, out, rows, n, rank, adapters, splits};
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool skip = on_tiles(rows);
-  if (skip) {
-    const int tc = launch_expand_sm100(p, dtype == FLYMOE_BF16, s);
-    if (tc != FLYMOE_OK || adapters <= kTileAdapters) return tc;
+static int expand(ExpandArgs p, const void* b_t, int dtype, cudaStream_t s) {
+  const bool bf = dtype == FLYMOE_BF16, tiles = on_tiles(p.rows);
+  if (tiles) {
+    ExpandArgs q = p;
+    if (b_t) { q.b = b_t; q.transposed = 1; }
+    const int rc = launch_expand_sm100(q, bf, s);
+    if (rc != FLYMOE_OK || p.adapters <= kTileAdapters) return rc;
   }
-  return dtype == FLYMOE_BF16 ? launch_expand_rank<__nv_bfloat16>(p, skip, s) : launch_expand_rank<__half>(p, skip, s);
+  return bf ? launch_expand_rank<__nv_bfloat16>(p, tiles, s) : launch_expand_rank<__half>(p, tiles, s);
+}
+// Whether a backward pass reads A and B through the kernels of this file, which want the contraction along a row.
+static bool needs_transposed(int rows, int adapters) { return !on_tiles(rows) || adapters > kTileAdapters; }
+
+// Pieces of the batch that the adapters' gradients are summed over: blocks for every place on the device (three an SM, two
+// from rank 33 on), at least 256 rows in a piece, and partial sums of 256 MB at most.
+static int wgrad_splits(int rows, int k, int n, int rank, int adapters) {
+  const long long blocks = (long long)(ceil_div(k, kWgCols) + ceil_div(n, kWgCols)) * ceil_div(rank, kWgRank);
+  const long long want = (rank <= 32 ? 3LL : 2LL) * sm_count() / blocks;
+  const long long fit = (256LL << 20) / ((long long)adapters * rank * ((long long)k + n) * 4);
+  return int(std::max(1LL, std::min({(long long)kLoraMaxSplits, want, fit, (long long)rows / 256})));
+}
+// The backward pass's scratch, in floats: dv | A transposed | B transposed | partial sums, 16-byte aligned each.
+struct BackwardScratch {
+  long long dv, a_t, b_t, partial, total;
+  int dv_splits, splits;
+};
+static BackwardScratch backward_scratch(int rows, int k, int n, int rank, int adapters) {
+  BackwardScratch w;
+  auto up4 = [](long long x) { return (x + 3) / 4 * 4; };
+  w.dv_splits = shrink_splits(rows, n);
+  w.splits = wgrad_splits(rows, k, n, rank, adapters);
+  const bool both = needs_transposed(rows, adapters);
+  const long long weights = (long long)adapters * rank;
+  w.dv = 0;
+  w.a_t = up4((long long)w.dv_splits * rows * rank);
+  w.b_t = w.a_t + (both ? up4(weights * k / 2) : 0);
+  w.partial = w.b_t + (both ? up4(weights * n / 2) : 0);
+  w.total = w.partial + (w.splits > 1 ? up4((long long)w.splits * adapters * ((long long)rank * ((long long)k + n) + 1)) : 0);
+  return w;
+}
+
+}  // namespace flymoe
+
+extern "C" int64_t flymoe_lora_v_elems(int rows, int k, int rank) {
+  if (rows < 1 || k < 8 || rank < 8) return 0;
+  return (int64_t)flymoe::shrink_splits(rows, k) * rows * rank;
 }
 
 extern "C" int flymoe_lora_add(void* out, const void* base, const void* x, const void* a, const void* b, const int32_t* ids,
-                               const float* scaling, float* v, int rows, int k, int n, int rank, int adapters, int splits,
-                               int dtype, void* stream) {
-  const int fold = flymoe::on_tiles(rows);       // whose expand reads a row's v once for every column tile
-  const int rc = flymoe_lora_shrink(v, x, a, ids, rows, k, rank, adapters, splits, fold, dtype, stream);
-  return rc != FLYMOE_OK ? rc
-                         : flymoe_lora_expand(out, base, v, b, ids, scaling, rows, n, rank, adapters, fold ? 1 : splits, dtype,
-                                              stream);
+                               const float* scaling, float* v, int64_t v_elems, int rows, int k, int n, int rank, int adapters,
+                               int keep_v, int dtype, void* stream) {
+  using namespace flymoe;
+  int rc = lora_check("lora_add", rows, k, n, rank, adapters, dtype);
+  if (rc != FLYMOE_OK || rows == 0) return rc;
+  FLYMOE_REQUIRE(out && base && x && a && b && ids && scaling && v, "lora_add: null pointer");
+  FLYMOE_REQUIRE(aligned16(out) && aligned16(base) && aligned16(x) && aligned16(a) && aligned16(b) && aligned16(v),
+                 "lora_add: pointers must be 16-byte aligned");
+  const int splits = shrink_splits(rows, k);
+  if (v_elems < (int64_t)splits * rows * rank) {
+    set_last_error_msg("lora_add: v is smaller than flymoe_lora_v_elems()");
+    return FLYMOE_ERR_WORKSPACE;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // tiles read a row's v once for every block that works on it: one sum, not several
+  const bool fold = keep_v || on_tiles(rows);
+  rc = shrink({x, a, ids, v, rows, k, rank, adapters, splits, 0}, nullptr, fold, dtype, s);
+  if (rc != FLYMOE_OK) return rc;
+  return expand({base, v, b, ids, scaling, out, rows, n, rank, adapters, fold ? 1 : splits, 0}, nullptr, dtype, s);
 }
 
-extern "C" int flymoe_lora_wgrad_splits(int rows, int k, int n, int rank, int adapters) {
-  using namespace flymoe;
-  if (rows < 1 || k < 8 || n < 8 || rank < 8 || adapters < 1) return 1;
-  // blocks for every place on the device (three an SM, two from rank 33 on), at least 256 rows in a split, and partial sums
-  // of 256 MB at most
-  const long long blocks = (long long)(ceil_div(k, kWgCols) + ceil_div(n, kWgCols)) * ceil_div(rank, kWgRank);
-  const long long want = (rank <= 32 ? 3LL : 2LL) * sm_count() / blocks;
-  const long long fit = (256LL << 20) / ((long long)adapters * rank * (k + n) * 4);
-  return int(std::max(1LL, std::min({(long long)kLoraMaxSplits, want, fit, (long long)rows / 256})));
+extern "C" int64_t flymoe_lora_backward_workspace_elems(int rows, int k, int n, int rank, int adapters) {
+  if (rows < 1 || k < 8 || n < 8 || rank < 8 || adapters < 1) return 4;
+  return flymoe::backward_scratch(rows, k, n, rank, adapters).total;
 }
 
-extern "C" int flymoe_lora_wgrad(void* da, void* db, const void* x, const void* dout, const float* v, const float* dv,
-                                 const int32_t* ids, const float* scaling, float* partial, int rows, int k, int n, int rank,
-                                 int adapters, int splits, int dtype, void* stream) {
+extern "C" int flymoe_lora_backward(void* dx, void* da, void* db, const void* dout, const void* x, const void* a, const void* b,
+                                    const int32_t* ids, const float* scaling, const float* v, float* workspace,
+                                    int64_t workspace_elems, int rows, int k, int n, int rank, int adapters, int dtype,
+                                    void* stream) {
   using namespace flymoe;
-  int rc = lora_check("lora_wgrad", rows, k, rank, adapters, splits, dtype);
-  if (rc == FLYMOE_OK) rc = lora_check("lora_wgrad", rows, n, rank, adapters, splits, dtype);
-  if (rc != FLYMOE_OK || (!da && !db)) return rc;
-  FLYMOE_REQUIRE(scaling && (rows == 0 || ids), "lora_wgrad: null pointer");
-  FLYMOE_REQUIRE(rows == 0 || ((!da || (x && dv)) && (!db || (dout && v))), "lora_wgrad: null pointer");
-  FLYMOE_REQUIRE(splits == 1 || partial, "lora_wgrad: partial is needed for more than one split");
-  FLYMOE_REQUIRE(aligned16(da) && aligned16(db) && aligned16(x) && aligned16(dout) && aligned16(v) && aligned16(dv) &&
-                     aligned16(partial), "lora_wgrad: pointers must be 16-byte aligned");
+  int rc = lora_check("lora_backward", rows, k, n, rank, adapters, dtype);
+  if (rc != FLYMOE_OK || (!dx && !da && !db)) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const size_t a_bytes = size_t(adapters) * rank * k * 2, b_bytes = size_t(adapters) * rank * n * 2;
+  if (rows == 0) {
+    if (da) FLYMOE_CUDA_CHECK(cudaMemsetAsync(da, 0, a_bytes, s));
+    if (db) FLYMOE_CUDA_CHECK(cudaMemsetAsync(db, 0, b_bytes, s));
+    return FLYMOE_OK;
+  }
+  FLYMOE_REQUIRE(dout && x && a && b && ids && scaling && v && workspace, "lora_backward: null pointer");
+  FLYMOE_REQUIRE(aligned16(dx) && aligned16(da) && aligned16(db) && aligned16(dout) && aligned16(x) && aligned16(a) &&
+                     aligned16(b) && aligned16(v) && aligned16(workspace), "lora_backward: pointers must be 16-byte aligned");
+  const BackwardScratch w = backward_scratch(rows, k, n, rank, adapters);
+  if (workspace_elems < w.total) {
+    set_last_error_msg("lora_backward: the workspace is smaller than flymoe_lora_backward_workspace_elems()");
+    return FLYMOE_ERR_WORKSPACE;
+  }
+  float* dv = workspace + w.dv;
+  if (dx || da) {
+    const void *a_t = a, *b_t = b;               // dx contracts over the rank, dv over the columns: B and A the other way round
+    if (needs_transposed(rows, adapters)) {
+      TransposeArgs t = {};
+      uint16_t* at = reinterpret_cast<uint16_t*>(workspace + w.a_t);
+      uint16_t* bt = reinterpret_cast<uint16_t*>(workspace + w.b_t);
+      t.src[0] = static_cast<const uint16_t*>(b); t.dst[0] = bt; t.rows[0] = n; t.cols[0] = rank;
+      t.src[1] = static_cast<const uint16_t*>(a); t.dst[1] = at; t.rows[1] = rank; t.cols[1] = k;
+      t.mats = adapters;
+      const int tiles = ceil_div(std::max(k, n), 32) * ceil_div(rank, 32);
+      FLYMOE_CUDA_CHECK(launch_closely(lora_transpose_kernel,
+                                       dim3(std::max(1, std::min(tiles, 16 * sm_count() / adapters)), dx ? 2 * adapters : adapters),
+                                       256, 0, s, t));
+      a_t = at;
+      b_t = bt;
+    }
+    rc = shrink({dout, b_t, ids, dv, rows, n, rank, adapters, w.dv_splits, 0}, b, true, dtype, s);
+    if (rc != FLYMOE_OK) return rc;
+    if (dx) rc = expand({nullptr, dv, a_t, ids, scaling, dx, rows, k, rank, adapters, 1, 0}, a, dtype, s);
+    if (rc != FLYMOE_OK) return rc;
+  }
+  if (!da && !db) return FLYMOE_OK;
   AdapterGradArgs p = {};
-  float* partial_b = da && partial ? partial + (long long)splits * adapters * k * rank : partial;
-  p.present = partial_b ? reinterpret_cast<int*>(partial_b + (db ? (long long)splits * adapters * n * rank : 0)) : nullptr;
+  const long long piece = (long long)w.splits * adapters * rank;
+  float* partial = workspace + w.partial;
   if (da) p.g[0] = {x, dv, da, partial, k, ceil_div(k, kWgCols), 1};
-  if (db) p.g[1] = {dout, v, db, partial_b, n, ceil_div(n, kWgCols), 0};
+  if (db) p.g[1] = {dout, v, db, partial + piece * k, n, ceil_div(n, kWgCols), 0};
+  p.present = reinterpret_cast<int*>(partial + piece * ((long long)k + n));
   p.ids = ids;
   p.scaling = scaling;
   p.rows = rows;
   p.rank = rank;
   p.adapters = adapters;
-  p.splits = splits;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  p.splits = w.splits;
   return dtype == FLYMOE_BF16 ? launch_wgrad_rank<__nv_bfloat16>(p, s) : launch_wgrad_rank<__half>(p, s);
-}
-
-extern "C" int flymoe_lora_transpose(const void* src, void* dst, int mats, int rows, int cols, void* stream) {
-  using namespace flymoe;
-  FLYMOE_REQUIRE(mats >= 0 && mats <= 65535 && rows >= 1 && cols >= 1, "lora_transpose: bad sizes");
-  FLYMOE_REQUIRE(ceil_div(rows, 32) <= 65535, "lora_transpose: too many rows");
-  if (mats == 0) return FLYMOE_OK;
-  FLYMOE_REQUIRE(src && dst, "lora_transpose: null pointer");
-  lora_transpose_kernel<<<dim3(ceil_div(cols, 32), ceil_div(rows, 32), mats), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      static_cast<const uint16_t*>(src), static_cast<uint16_t*>(dst), rows, cols);
-  FLYMOE_CUDA_CHECK(cudaGetLastError());
-  return FLYMOE_OK;
 }

@@ -38,20 +38,42 @@ __device__ __forceinline__ bool in_use(int id, int adapters) { return id >= 0 &&
 
 struct ShrinkArgs {
   const void* x;               // [rows, k]
-  const void* a;               // [adapters, rank, k]
+  const void* a;               // [adapters, rank, k], or transposed [adapters, k, rank] (on tiles only)
   const int* ids;              // [rows]
   float* v;                    // [splits, rows, rank]
-  int rows, k, rank, adapters, splits;
+  int rows, k, rank, adapters, splits, transposed;
 };
 struct ExpandArgs {
   const void* base;            // [rows, n] or null (zeros); may be `out`
   const float* v;              // [splits, rows, rank]; splits is 1 on tiles
-  const void* b;               // [adapters, n, rank]
+  const void* b;               // [adapters, n, rank], or transposed [adapters, rank, n] (on tiles only)
   const int* ids;
   const float* scaling;        // [adapters]
   void* out;                   // [rows, n]
-  int rows, n, rank, adapters, splits;
+  int rows, n, rank, adapters, splits, transposed;
 };
+
+// The launches of one operator follow each other closely (programmatic stream serialisation): the next one's blocks start,
+// and set up what touches no global memory, while the last blocks of this one run.  Every kernel launched this way waits
+// here before its first access to global memory; the wait ends when all launches before it are done.
+__device__ __forceinline__ void after_previous_launch() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <typename... Params, typename... Args>
+inline cudaError_t launch_closely(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
 
 // Tiles of 128 rows on tcgen05 (lora_sm100.cu), of which these launches take those with at most kTileAdapters distinct
 // adapters among their rows; the kernels of lora.cu take the others, and batches of too few tiles.

@@ -27,6 +27,10 @@ constexpr int kChunkBytes = kTileRows * 128;     // 128 rows x 64 16-bit columns
 __device__ __forceinline__ uint32_t instr_desc(int bf16, int n) {
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
 }
+// Operand tile whose contraction runs over its rows (MN-major): chunks of 64 columns (128 bytes a row) `chunk` bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, uint32_t chunk) {
+  return uint64_t((addr >> 4) & 0x3FFF) | uint64_t(chunk >> 4) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
+}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
                ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
@@ -44,6 +48,7 @@ constexpr size_t kShSmem = size_t(kShX) * kChunkBytes + kShABytes + sizeof(Shrin
 struct ShrinkTcArgs {
   ShrinkArgs p;
   int bf16, rank_pad, slots, tmem_cols;
+  int a_bytes;                 // an adapter's block in shared memory
   int* status;
 };
 
@@ -58,7 +63,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
   const ShrinkArgs& p = q.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row0 = blockIdx.x * kTileRows;
-  const int a_bytes = q.rank_pad * 128;
+  const int a_bytes = q.a_bytes;
 
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
@@ -71,6 +76,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     c->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   } else if (warp == 2) {
+    after_previous_launch();
     int id[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, row0 + i * 32 + lane, p.rows, p.adapters);
@@ -80,6 +86,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
+  after_previous_launch();
   const uint32_t tmem = c->tmem_base;
   const int d = c->count;
   const int blocks = (p.k + 63) / 64;
@@ -104,7 +111,10 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
         if (!ok) break;
         if (elect_one()) {
           mbar_expect_tx(smem_u32(&c->a_full[as]), a_bytes);
-          tma_load_3d(smem_u32(aring + as * a_bytes), &tmap_a, smem_u32(&c->a_full[as]), kb * 128, 0, c->list[i]);
+          const uint32_t dst = smem_u32(aring + as * a_bytes), full = smem_u32(&c->a_full[as]);
+          if (!p.transposed) tma_load_3d(dst, &tmap_a, full, kb * 128, 0, c->list[i]);
+          else
+            for (int j = 0; j < a_bytes; j += 8192) tma_load_3d(dst + j, &tmap_a, full, j / 64, kb * 64, c->list[i]);
         }
         __syncwarp();
         if (++as == q.slots) { as = 0; ap ^= 1; }
@@ -112,7 +122,8 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     }
   } else if (warp == 1 && d > 0) {
     // ------------------------------------------------------------------ MMA issuer
-    const uint32_t idesc = instr_desc(q.bf16, q.rank_pad);
+    const uint32_t idesc = instr_desc(q.bf16, q.rank_pad) | (p.transposed ? 1u << 16 : 0u);
+    const uint64_t b_step = p.transposed ? 16 * 128 / 16 : 2;
     int xs = 0, as = 0;
     uint32_t xp = 0, ap = 0;
     bool ok = true;
@@ -122,12 +133,13 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
       for (int i = 0; i < d && ok; ++i) {
         ok = warp_wait(smem_u32(&c->a_full[as]), ap, abort_flag, q.status, 3);
         if (!ok) break;
-        const uint64_t bdesc = make_smem_desc(smem_u32(aring + as * a_bytes));
+        const uint32_t at = smem_u32(aring + as * a_bytes);
+        const uint64_t bdesc = p.transposed ? smem_desc_mn(at, 8192) : make_smem_desc(at);
         tcgen05_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            umma_f16(tmem + i * q.rank_pad, adesc + k * 2, bdesc + k * 2, idesc, (k > 0 || kb > kb0) ? 1u : 0u);
+            umma_f16(tmem + i * q.rank_pad, adesc + k * 2, bdesc + k * b_step, idesc, (k > 0 || kb > kb0) ? 1u : 0u);
           umma_commit(smem_u32(&c->a_empty[as]));
           if (i + 1 == d) {
             umma_commit(smem_u32(&c->x_empty[xs]));
@@ -231,7 +243,11 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
+  after_previous_launch();
   const uint32_t tmem = c->tmem_base;
+  const int steps = (p.rank + 15) / 16;          // of the contraction
+  // an adapter's tile: 128 columns along the rank, or (transposed) two chunks of 64 columns with a row per rank
+  const uint32_t b_bytes = p.transposed ? steps * 16 * 256 : KC * kChunkBytes;
   // consecutive column tiles of a row tile, so that the rows' v is set up once or twice per block
   // adapters of a row tile: every role looks for itself, ahead of the others where it can
   auto find_adapters = [&](int rt, int* list) {
@@ -276,7 +292,11 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
         if (!ok) break;
         const uint32_t bfull = smem_u32(&c->b_full[bs]), bdst = smem_u32(bring + bs * KC * kChunkBytes);
         if (elect_one()) {
-          mbar_expect_tx(bfull, KC * kChunkBytes);
+          mbar_expect_tx(bfull, b_bytes);
+          if (p.transposed) {
+            tma_load_3d(bdst, &tmap_b, bfull, col * 2, 0, list[i]);
+            tma_load_3d(bdst + b_bytes / 2, &tmap_b, bfull, col * 2 + 128, 0, list[i]);
+          } else
 #pragma unroll
           for (int k = 0; k < KC; ++k) tma_load_3d(bdst + k * kChunkBytes, &tmap_b, bfull, k * 128, col, list[i]);
         }
@@ -286,8 +306,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    const uint32_t idesc = instr_desc(std::is_same<T, __nv_bfloat16>::value, kExCols);
-    const int steps = (p.rank + 15) / 16;
+    const uint32_t idesc = instr_desc(std::is_same<T, __nv_bfloat16>::value, kExCols) | (p.transposed ? 1u << 16 : 0u);
     int bs = 0, acc = 0, row_tile = -1, d = 0;
     uint32_t bp = 0, rp = 0, accp = 0;
     bool ok = true;
@@ -312,7 +331,8 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
           for (int part = 0; part < 2; ++part)
             for (int k = 0; k < steps; ++k) {
               const uint64_t ad = make_smem_desc(smem_u32(vtile + (part * KC + (k >> 2)) * kChunkBytes)) + (k & 3) * 2;
-              const uint64_t bd = make_smem_desc(smem_u32(bring + (bs * KC + (k >> 2)) * kChunkBytes)) + (k & 3) * 2;
+              const uint64_t bd = p.transposed ? smem_desc_mn(smem_u32(bring + bs * KC * kChunkBytes) + k * 2048, b_bytes / 2)
+                                               : make_smem_desc(smem_u32(bring + (bs * KC + (k >> 2)) * kChunkBytes)) + (k & 3) * 2;
               umma_f16(tmem + acc * kExCols, ad, bd, idesc, (part > 0 || k > 0) ? 1u : 0u);
             }
           umma_commit(smem_u32(&c->b_empty[bs]));
@@ -342,53 +362,52 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     for (int u = u0; u < u1 && ok; ++u) {
       const int rt = u / q.col_tiles, col = (u - rt * q.col_tiles) * kExCols;
       if (rt != row_tile) {
-        // the MMAs of the previous row tile are done (their last sums have been read here): its v may go
+        // The MMAs of the previous row tile are done (their last sums have been read here): its v may go.  Everything of
+        // the new one is asked for at once: v, four numbers a thread and step with consecutive threads along a row, and ids.
         row_tile = rt;
+        const int vecs = (p.rank + 15) / 16 * 4;
+        float4 x[KC * 8];
+#pragma unroll
+        for (int s = 0; s < KC * 8; ++s) {
+          const int i = s * kExEpi + et, r = i / vecs, k4 = i - r * vecs;
+          x[s] = r < kTileRows && rt * kTileRows + r < p.rows && k4 * 4 < p.rank
+                     ? __ldg(reinterpret_cast<const float4*>(p.v + (long long)(rt * kTileRows + r) * p.rank + k4 * 4))
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
         mine = row_adapter(p.ids, rt * kTileRows + row, p.rows, p.adapters);
-        ok = sync();                             // and all have left its list
+        ok = sync();                             // all have left the previous list
         if (!ok) break;
         if (et < 32) {
           d = find_adapters(rt, c->list[1]);
           if (lane == 0) c->count = d;
         }
-        if (wg == 0) c->id[row] = mine;
+        if (wg == 0) { c->id[row] = mine; c->row_max[row] = 0; }
         ok = sync();
         if (!ok) break;
         d = c->count;
         if (d >= 1 && d <= kTileAdapters) {
           scale = mine >= 0 ? __ldg(p.scaling + mine) : 0.f;
-          // v as high parts and remainders: four numbers a thread and step, consecutive threads along a row
-          const int vecs = (p.rank + 15) / 16 * 4;
-          auto load = [&](int i, int& r, int& k4) {
-            r = i / vecs;
-            k4 = i - r * vecs;
-            return c->id[r] >= 0 && k4 * 4 < p.rank
-                       ? __ldg(reinterpret_cast<const float4*>(p.v + (long long)(rt * kTileRows + r) * p.rank + k4 * 4))
-                       : make_float4(0.f, 0.f, 0.f, 0.f);
-          };
           if constexpr (std::is_same<T, __half>::value) {
-            if (wg == 0) c->row_max[row] = 0;
-            ok = sync();
-            if (!ok) break;
-            for (int i = et; i < kTileRows * vecs; i += kExEpi) {
-              int r, k4;
-              const float4 x = load(i, r, k4);
-              const float m = fmaxf(fmaxf(finite_abs(x.x), finite_abs(x.y)), fmaxf(finite_abs(x.z), finite_abs(x.w)));
-              atomicMax(&c->row_max[r], __float_as_int(m));          // not negative: ordered like the numbers
+#pragma unroll
+            for (int s = 0; s < KC * 8; ++s) {
+              const int r = (s * kExEpi + et) / vecs;
+              const float m = fmaxf(fmaxf(finite_abs(x[s].x), finite_abs(x[s].y)), fmaxf(finite_abs(x[s].z), finite_abs(x[s].w)));
+              if (r < kTileRows) atomicMax(&c->row_max[r], __float_as_int(m));     // not negative: ordered like the numbers
             }
             ok = sync();
             if (!ok) break;
             scale *= exp2i(scale_exponent(__int_as_float(c->row_max[row])));
           }
-#pragma unroll 4
-          for (int i = et; i < kTileRows * vecs; i += kExEpi) {
-            int r, k4;
-            const float4 x = load(i, r, k4);
+#pragma unroll
+          for (int s = 0; s < KC * 8; ++s) {
+            const int i = s * kExEpi + et, r = i / vecs, k4 = i - r * vecs;
+            if (r >= kTileRows) continue;
+            if (c->id[r] < 0) x[s] = make_float4(0.f, 0.f, 0.f, 0.f);      // nothing has been summed up for it
             float down = 1.f;
             if constexpr (std::is_same<T, __half>::value) down = exp2i(-scale_exponent(__int_as_float(c->row_max[r])));
             uint2 hi, lo;
-            split2<T>(x.x * down, x.y * down, hi.x, lo.x);
-            split2<T>(x.z * down, x.w * down, hi.y, lo.y);
+            split2<T>(x[s].x * down, x[s].y * down, hi.x, lo.x);
+            split2<T>(x[s].z * down, x[s].w * down, hi.y, lo.y);
             uint8_t* at = vtile + (k4 >> 4) * kChunkBytes + r * 128 + ((((k4 >> 1) & 7) ^ (r & 7)) * 16) + (k4 & 1) * 8;
             *reinterpret_cast<uint2*>(at) = hi;
             *reinterpret_cast<uint2*>(at + KC * kChunkBytes) = lo;
@@ -403,7 +422,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
       uint8_t* line = smem + (ys * 2 + wg) * kChunkBytes + row * 128;
       if (p.base == nullptr) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(line + j * 16) = make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(line + ((j ^ sw) * 16)) = make_uint4(0, 0, 0, 0);
       }
       for (int i = 0; i < d && ok; ++i) {
         ok = warp_wait(smem_u32(&c->acc_full[acc]), accp, abort_flag, q.status, 4);
@@ -477,20 +496,21 @@ static int matrix_map(CUtensorMap* map, const void* base, long long cols, long l
 }
 
 int launch_shrink_sm100(const ShrinkArgs& p, int bf16, cudaStream_t stream) {
-  ShrinkTcArgs q = {p, bf16, (p.rank + 15) / 16 * 16, 0, 0, device_status_ptr()};
+  ShrinkTcArgs q = {p, bf16, (p.rank + 15) / 16 * 16, 0, 0, 0, device_status_ptr()};
   if (q.status == nullptr) return FLYMOE_ERR_CUDA;
-  q.slots = std::min(16, kShABytes / (q.rank_pad * 128));
+  q.a_bytes = p.transposed ? ceil_div(p.rank, 64) * 8192 : q.rank_pad * 128;
+  q.slots = std::min(16, kShABytes / q.a_bytes);
   // columns for kTileAdapters adapters; sums are read 32 columns at a time, so also for what the last read reaches
   static_assert(kTileAdapters == 4, "TMEM columns below");
   q.tmem_cols = q.rank_pad <= 64 ? 256 : 512;
   CUtensorMap mx, ma;
   int rc = matrix_map(&mx, p.x, p.k, p.rows, 0, kTileRows);
-  if (rc == FLYMOE_OK) rc = matrix_map(&ma, p.a, p.k, p.rank, p.adapters, q.rank_pad);
+  if (rc == FLYMOE_OK)
+    rc = p.transposed ? matrix_map(&ma, p.a, p.rank, p.k, p.adapters, 64) : matrix_map(&ma, p.a, p.k, p.rank, p.adapters, q.rank_pad);
   if (rc != FLYMOE_OK) return rc;
   static SmemLimitSeen seen;
   FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(lora_shrink_tc_kernel), int(kShSmem), seen));
-  lora_shrink_tc_kernel<<<dim3(ceil_div(p.rows, kTileRows), p.splits), 256, kShSmem, stream>>>(mx, ma, q);
-  FLYMOE_CUDA_CHECK(cudaGetLastError());
+  FLYMOE_CUDA_CHECK(launch_closely(lora_shrink_tc_kernel, dim3(ceil_div(p.rows, kTileRows), p.splits), 256, kShSmem, stream, mx, ma, q));
   return FLYMOE_OK;
 }
 
@@ -500,8 +520,7 @@ static int launch_expand_tc(const CUtensorMap& my, const CUtensorMap& mo, const 
   auto* kernel = lora_expand_tc_kernel<T, KC>;
   static SmemLimitSeen seen;
   FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(ex_smem<KC>()), seen));
-  kernel<<<std::min(q.units, sm_count()), kExThreads, ex_smem<KC>(), stream>>>(my, mo, mb, q);
-  FLYMOE_CUDA_CHECK(cudaGetLastError());
+  FLYMOE_CUDA_CHECK(launch_closely(kernel, std::min(q.units, sm_count()), kExThreads, ex_smem<KC>(), stream, my, mo, mb, q));
   return FLYMOE_OK;
 }
 
@@ -514,7 +533,9 @@ int launch_expand_sm100(const ExpandArgs& p, int bf16, cudaStream_t stream) {
   CUtensorMap my, mo, mb;
   int rc = matrix_map(&my, p.base ? p.base : p.out, p.n, p.rows, 0, kTileRows);
   if (rc == FLYMOE_OK) rc = matrix_map(&mo, p.out, p.n, p.rows, 0, kTileRows);
-  if (rc == FLYMOE_OK) rc = matrix_map(&mb, p.b, p.rank, p.n, p.adapters, kExCols);
+  if (rc == FLYMOE_OK)
+    rc = p.transposed ? matrix_map(&mb, p.b, p.n, p.rank, p.adapters, (p.rank + 15) / 16 * 16)
+                      : matrix_map(&mb, p.b, p.rank, p.n, p.adapters, kExCols);
   if (rc != FLYMOE_OK) return rc;
   if (p.rank <= 64)
     return bf16 ? launch_expand_tc<__nv_bfloat16, 1>(my, mo, mb, q, stream) : launch_expand_tc<__half, 1>(my, mo, mb, q, stream);

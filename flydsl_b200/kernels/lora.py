@@ -36,7 +36,7 @@ def _fits(y, x, a, b, ids, scaling, out):
                 and b.device == dev and ids.device == dev and scaling.device == dev and x.is_contiguous()
                 and y.is_contiguous() and a.is_contiguous() and b.is_contiguous() and ids.is_contiguous()
                 and scaling.is_contiguous() and 8 <= rank <= MAX_RANK and not rank % 8 and k >= 8 and not k % 8 and n >= 8
-                and not n % 8 and 1 <= adapters <= 65535 and out is None)
+                and not n % 8 and 1 <= adapters <= 32767 and out is None)
     except (AttributeError, ValueError, IndexError):
         return False
 
@@ -58,8 +58,8 @@ def _check(y, x, a, b, adapter_ids, scaling, out):
         raise ValueError(f"rank must be a multiple of 8 in [8, {MAX_RANK}], got {rank}")
     if k < 8 or k % 8 or n < 8 or n % 8:
         raise ValueError(f"k ({k}) and n ({n}) must be positive multiples of 8")
-    if not 1 <= adapters <= 65535:
-        raise ValueError(f"adapters must be in [1, 65535], got {adapters}")
+    if not 1 <= adapters <= 32767:
+        raise ValueError(f"adapters must be in [1, 32767], got {adapters}")
     _lib.require_cuda("x", x, HALF)
     for name, t in (("y", y), ("a", a), ("b", b), ("out", out)):
         if t is not None:
@@ -73,40 +73,25 @@ def _check(y, x, a, b, adapter_ids, scaling, out):
     require_same_device("x", x.device, y=y, a=a, b=b, adapter_ids=adapter_ids, scaling=scaling, out=out)
 
 
-def _shrink(x, a, ids, fold):
-    """x [rows, k], a [adapters, rank, k] -> f32 [splits, rows, rank], or with ``fold`` [1, rows, rank]."""
+def _add(out, y, x, a, b, ids, scaling, keep_v):
+    """Enqueues the forward pass; returns its scratch, which begins with v if ``keep_v``."""
     lib, (rows, k), (adapters, rank, _) = _lib.load(), x.shape, a.shape
-    splits = lib.flymoe_lora_shrink_splits(rows, k)
-    v = x.new_empty((splits, rows, rank), dtype=torch.float32)
-    _lib.check(lib.flymoe_lora_shrink(v.data_ptr(), x.data_ptr(), a.data_ptr(), ids.data_ptr(), rows, k, rank, adapters,
-                                      splits, 1 if fold else 0, _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(None)),
-               "lora_shrink")
-    return v[:1] if fold else v
-
-
-def _expand(out, base, v, b, ids, scaling):
-    rows, n = out.shape
-    _lib.check(_lib.load().flymoe_lora_expand(out.data_ptr(), _lib.ptr(base), v.data_ptr(), b.data_ptr(), ids.data_ptr(),
-                                              scaling.data_ptr(), rows, n, b.shape[2], b.shape[0], v.shape[0],
-                                              _lib.DTYPE_CODE[out.dtype], _lib.stream_handle(None)), "lora_expand")
-    return out
-
-
-def _transposed(t):
-    mats, rows, cols = t.shape
-    res = t.new_empty((mats, cols, rows))
-    _lib.check(_lib.load().flymoe_lora_transpose(t.data_ptr(), res.data_ptr(), mats, rows, cols, _lib.stream_handle(None)),
-               "lora_transpose")
-    return res
+    elems = lib.flymoe_lora_v_elems(rows, k, rank)
+    v = x.new_empty(elems, dtype=torch.float32)
+    _lib.check(lib.flymoe_lora_add(out.data_ptr(), y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(),
+                                   scaling.data_ptr(), v.data_ptr(), elems, rows, k, y.shape[1], rank, adapters, keep_v,
+                                   _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(None)), "lora_add")
+    return v
 
 
 class _LoraAdd(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, x, a, b, ids, scaling):
         with on(x.device):
-            v = _shrink(x, a, ids, fold=True)
-            ctx.save_for_backward(x, a, b, ids, scaling, v)
-            return _expand(torch.empty_like(y), y, v, b, ids, scaling)
+            out = torch.empty_like(y)
+            v = _add(out, y, x, a, b, ids, scaling, 1)
+        ctx.save_for_backward(x, a, b, ids, scaling, v)
+        return out
 
     @staticmethod
     @once_differentiable
@@ -114,22 +99,22 @@ class _LoraAdd(torch.autograd.Function):
         x, a, b, ids, scaling, v = ctx.saved_tensors
         need_y, need_x, need_a, need_b = ctx.needs_input_grad[:4]
         dx = da = db = None
-        with on(x.device):
-            dout = dout.contiguous()
-            dv = _shrink(dout, _transposed(b), ids, fold=True) if need_x or need_a else None
-            if need_x:
-                dx = _expand(torch.empty_like(x), None, dv, _transposed(a), ids, scaling)
-            if need_a or need_b:
-                lib, (rows, k), (adapters, n, rank) = _lib.load(), x.shape, b.shape
-                splits = lib.flymoe_lora_wgrad_splits(rows, k, n, rank, adapters)
-                da = torch.empty_like(a) if need_a else None
-                db = torch.empty_like(b) if need_b else None
-                width = (k if need_a else 0) + (n if need_b else 0)
-                partial = x.new_empty(splits * adapters * (rank * width + 1), dtype=torch.float32) if splits > 1 else None
-                _lib.check(lib.flymoe_lora_wgrad(
-                    _lib.ptr(da), _lib.ptr(db), x.data_ptr(), dout.data_ptr(), v.data_ptr(), _lib.ptr(dv), ids.data_ptr(),
-                    scaling.data_ptr(), _lib.ptr(partial), rows, k, n, rank, adapters, splits, _lib.DTYPE_CODE[x.dtype],
-                    _lib.stream_handle(None)), "lora_wgrad")
+        if need_x or need_a or need_b:
+            lib, (rows, k), (adapters, n, rank) = _lib.load(), x.shape, b.shape
+            with on(x.device):
+                dout = dout.contiguous()
+                elems = lib.flymoe_lora_backward_workspace_elems(rows, k, n, rank, adapters)
+                work = x.new_empty(elems, dtype=torch.float32)
+                if need_x:
+                    dx = torch.empty_like(x)
+                if need_a:
+                    da = torch.empty_like(a)
+                if need_b:
+                    db = torch.empty_like(b)
+                _lib.check(lib.flymoe_lora_backward(
+                    _lib.ptr(dx), _lib.ptr(da), _lib.ptr(db), dout.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(),
+                    ids.data_ptr(), scaling.data_ptr(), v.data_ptr(), work.data_ptr(), elems, rows, k, n, rank, adapters,
+                    _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(None)), "lora_backward")
         return dout if need_y else None, dx, da, db, None, None
 
 
@@ -145,12 +130,7 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
             raise ValueError("out= and stream= are for inference: an input requires a gradient")
         return _LoraAdd.apply(y, x, a, b, adapter_ids, scaling)
     with on(x.device, stream):
-        lib, (rows, k), (adapters, rank, _) = _lib.load(), x.shape, a.shape
-        splits = lib.flymoe_lora_shrink_splits(rows, k)
-        v = x.new_empty((splits, rows, rank), dtype=torch.float32)
         if out is None:
             out = torch.empty_like(y)
-        _lib.check(lib.flymoe_lora_add(out.data_ptr(), y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(),
-                                       adapter_ids.data_ptr(), scaling.data_ptr(), v.data_ptr(), rows, k, y.shape[1], rank,
-                                       adapters, splits, _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(None)), "lora_add")
+        _add(out, y, x, a, b, adapter_ids, scaling, 0)
     return out

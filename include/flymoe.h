@@ -364,31 +364,23 @@ int flymoe_combine_rows_backward(const void* dout, const void* rows_in, const fl
 
 /* Low-rank adapters of many requests beside a shared projection, 16-bit operands (dtype F16 or BF16):
  * out[m] = base[m] + scaling[l] * B_l (A_l x[m]) with l = ids[m]; rows whose id is outside [0, adapters) pass through.
- * a [adapters, rank, k], b [adapters, n, rank], ids i32 [rows] in any order, scaling f32 [adapters].  rank a multiple of 8
- * up to 128, k and n multiples of 8, pointers 16-byte aligned.  Sums in fp32, the output rounded once.
- * flymoe_lora_add: the two calls that follow in one (v f32 [splits, rows, rank] is scratch).
- * flymoe_lora_shrink: v f32 [splits, rows, rank] = partial sums of x A_l^T over `splits` pieces of k (zeros for a row without
- * an adapter); with `fold` they are added up into the first piece.  flymoe_lora_shrink_splits: the number that fills the
- * current device, 1..16.
- * flymoe_lora_expand: out = base + scaling * (sum over splits of v) B_l^T; base may be NULL (zeros) or out itself.
- * Gradients: dv is a shrink of dout with B transposed to [adapters, rank, n], dx an expand of dv with A transposed to
- * [adapters, k, rank] (flymoe_lora_transpose: `mats` matrices [rows, cols] of 16-bit values).
- * flymoe_lora_wgrad: da[l] = scaling[l] sum over l's rows of dv^T x, db[l] = scaling[l] sum of dout^T v (v, dv f32 [rows,
- * rank]); da or db may be NULL; an adapter without rows gets zeros.  splits > 1 cuts the rows, partial is then f32 scratch of
- * splits * adapters * (rank * (k if da + n if db) + 1); flymoe_lora_wgrad_splits proposes a number.  No counterpart in the reference. */
+ * x [rows, k], base and out [rows, n] (out may be base), a [adapters, rank, k], b [adapters, n, rank], ids i32 [rows] in any
+ * order, scaling f32 [adapters].  rank a multiple of 8 up to 128, k and n multiples of 8, at most 32767 adapters, pointers
+ * 16-byte aligned.  Sums in fp32, the output rounded once; no atomics decide a result.
+ * v: f32 scratch of flymoe_lora_v_elems(); with keep_v its first rows * rank floats hold A_l x[m] afterwards, as the gradient
+ * wants it (rows without an adapter: unspecified).
+ * flymoe_lora_backward: from dout [rows, n], dx [rows, k] = scaling (dout B_l) A_l (zeros without an adapter), da[l] =
+ * scaling[l] sum over l's rows of (dout B_l)^T x, db[l] = scaling[l] sum of dout^T v (zeros for an adapter without rows);
+ * each of the three may be NULL.  workspace: f32 of flymoe_lora_backward_workspace_elems().  No counterpart in the
+ * reference. */
+int64_t flymoe_lora_v_elems(int rows, int k, int rank);
 int flymoe_lora_add(void* out, const void* base, const void* x, const void* a, const void* b, const int32_t* ids,
-                    const float* scaling, float* v, int rows, int k, int n, int rank, int adapters, int splits, int dtype,
-                    void* stream);
-int flymoe_lora_shrink_splits(int rows, int k);
-int flymoe_lora_shrink(float* v, const void* x, const void* a, const int32_t* ids, int rows, int k, int rank, int adapters,
-                       int splits, int fold, int dtype, void* stream);
-int flymoe_lora_expand(void* out, const void* base, const float* v, const void* b, const int32_t* ids, const float* scaling,
-                       int rows, int n, int rank, int adapters, int splits, int dtype, void* stream);
-int flymoe_lora_wgrad_splits(int rows, int k, int n, int rank, int adapters);
-int flymoe_lora_wgrad(void* da, void* db, const void* x, const void* dout, const float* v, const float* dv,
-                      const int32_t* ids, const float* scaling, float* partial, int rows, int k, int n, int rank,
-                      int adapters, int splits, int dtype, void* stream);
-int flymoe_lora_transpose(const void* src, void* dst, int mats, int rows, int cols, void* stream);
+                    const float* scaling, float* v, int64_t v_elems, int rows, int k, int n, int rank, int adapters,
+                    int keep_v, int dtype, void* stream);
+int64_t flymoe_lora_backward_workspace_elems(int rows, int k, int n, int rank, int adapters);
+int flymoe_lora_backward(void* dx, void* da, void* db, const void* dout, const void* x, const void* a, const void* b,
+                         const int32_t* ids, const float* scaling, const float* v, float* workspace, int64_t workspace_elems,
+                         int rows, int k, int n, int rank, int adapters, int dtype, void* stream);
 
 /* Y[t,:] = sum_s w[t,s] * X[row(t,s),:] with fp32 accumulation; row(t,s) = t*k+s, or
  * row_index[t*k+s] when row_index is given (negative entries are skipped); optional u8

@@ -33,20 +33,19 @@ def test_shapes(name):
 
 def test_c_entries_refuse_bad_arguments(lib):
     err = lib.flymoe_last_error
-    for rows, k, rank, adapters, splits, dtype, word in (
-            (-1, 16, 8, 1, 1, 2, b"rows"), (4, 12, 8, 1, 1, 2, b"multiples of 8"), (4, 16, 4, 1, 1, 2, b"rank"),
-            (4, 16, 136, 1, 1, 2, b"rank"), (4, 16, 8, 0, 1, 2, b"adapters"), (4, 16, 8, 1, 17, 2, b"splits"),
-            (4, 16, 8, 1, 1, 0, b"dtype"), (4, 16, 8, 1, 1, 2, b"null")):
-        assert lib.flymoe_lora_shrink(None, None, None, None, rows, k, rank, adapters, splits, 0, dtype, None) == -1
+    for rows, k, rank, adapters, dtype, word in (
+            (-1, 16, 8, 1, 2, b"rows"), (4, 12, 8, 1, 2, b"multiples of 8"), (4, 16, 4, 1, 2, b"rank"),
+            (4, 16, 136, 1, 2, b"rank"), (4, 16, 8, 0, 2, b"adapters"), (4, 16, 8, 32768, 2, b"adapters"),
+            (4, 16, 8, 1, 0, b"dtype"), (4, 16, 8, 1, 2, b"null")):
+        assert lib.flymoe_lora_add(None, None, None, None, None, None, None, None, 0, rows, k, 16, rank, adapters, 0, dtype,
+                                   None) == -1
         assert word in err()
-        assert lib.flymoe_lora_expand(None, None, None, None, None, None, rows, k, rank, adapters, splits, dtype, None) == -1
+        assert lib.flymoe_lora_backward(64, None, None, None, None, None, None, None, None, None, None, 0, rows, 16, k, rank,
+                                        adapters, dtype, None) == -1
         assert word in err()
-        assert lib.flymoe_lora_wgrad(64, 64, None, None, None, None, None, None, None, rows, k, 16, rank, adapters, splits,
-                                     dtype, None) == -1
-        assert word in err()
-    assert lib.flymoe_lora_shrink(64, 72, 64, 64, 4, 16, 8, 1, 1, 0, 2, None) == -1 and b"aligned" in err()
-    assert lib.flymoe_lora_wgrad(64, None, 64, 64, 64, 64, 64, 64, None, 4, 16, 16, 8, 1, 2, 2, None) == -1
-    assert b"partial" in err()
-    assert lib.flymoe_lora_transpose(None, None, 1, 0, 8, None) == -1
-    assert 1 <= lib.flymoe_lora_shrink_splits(1, 7168) <= 16 and 1 <= lib.flymoe_lora_shrink_splits(8192, 64) <= 16
-    assert lib.flymoe_lora_wgrad_splits(64, 4096, 4096, 16, 1) == 1
+    assert lib.flymoe_lora_add(64, 64, 72, 64, 64, 64, 64, 64, 1 << 20, 4, 16, 16, 8, 1, 0, 2, None) == -1 and b"aligned" in err()
+    assert lib.flymoe_lora_add(64, 64, 64, 64, 64, 64, 64, 64, 8, 4, 16, 16, 8, 1, 0, 2, None) == -4 and b"v_elems" in err()
+    assert lib.flymoe_lora_backward(64, 64, 64, 64, 64, 64, 64, 64, 64, 64, 64, 8, 4, 16, 16, 8, 1, 2, None) == -4
+    assert b"workspace" in err()
+    assert lib.flymoe_lora_v_elems(0, 64, 8) == 0 and lib.flymoe_lora_v_elems(5, 64, 8) >= 40
+    assert lib.flymoe_lora_backward_workspace_elems(5, 64, 64, 8, 2) >= 40
