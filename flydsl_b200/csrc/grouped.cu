@@ -15,30 +15,18 @@
 // there may be infinite).
 #include <cuda.h>
 #include <stdio.h>
+#include <stdlib.h>
 
 #include "common.cuh"
 #include "gemm_ptx.cuh"
+#include "grouped.cuh"
 
 namespace flymoe {
 
-constexpr int kRagM = 128, kRagN = 256, kRagK = 64;
+constexpr int kRagM = 128, kRagN = 256;
 constexpr int kRagStages = 4;
 constexpr int kRagStageBytes = (kRagM + kRagN) * kRagK * 2;      // 48 KB
-constexpr int kRagMaxExperts = 1024;
 constexpr int kRagThreads = 384;
-
-struct RaggedArgs {
-  const int* offsets;          // [experts + 1]
-  void* out;
-  int rows, experts;
-  int m_dim;                   // form 2: rows of an expert's output matrix
-  int n_dim;                   // columns of the output
-  int k_dim;                   // forms 0 and 1: length of the contraction
-  int n_tiles, m_tiles;        // m_tiles: form 2 only
-  int group_m;
-  int bf16, zero_uncovered;
-  int* status;
-};
 
 struct __align__(16) RaggedCtrl {
   unsigned long long full[kRagStages];
@@ -47,70 +35,10 @@ struct __align__(16) RaggedCtrl {
   unsigned long long acc_empty[2];
   uint32_t tmem_base;
   int abort_flag;
-  int start[kRagMaxExperts + 1];                 // first row of an expert
-  int tile0[kRagMaxExperts + 1];                 // first tile of an expert
+  RaggedTables tab;
 };
 constexpr size_t kRagSmem = size_t(kRagStages) * kRagStageBytes + sizeof(RaggedCtrl) + 1024;
 static_assert(kRagSmem <= 232448, "shared memory budget of one SM exceeded");
-
-// Segment bounds and tile counts.  Offsets come from the device, so they are taken into [0, rows] and made ascending
-// here: whatever they hold, no access leaves the tensors.
-template <int FORM>
-__device__ __forceinline__ void ragged_tables(const RaggedArgs& a, RaggedCtrl* c, int lane) {
-  int run = 0, tiles = 0;
-  for (int e0 = 0; e0 <= a.experts; e0 += 32) {
-    const int e = e0 + lane;
-    int v = e <= a.experts ? min(max(__ldg(a.offsets + e), 0), a.rows) : 0;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, v, off);
-      if (lane >= off) v = max(v, o);
-    }
-    v = max(v, run);
-    // tiles of expert e - 1 are known once its end is
-    int before = __shfl_up_sync(0xffffffffu, v, 1);
-    if (lane == 0) before = run;
-    int t = 0;
-    if (e >= 1 && e <= a.experts)
-      t = FORM == 2 ? a.m_tiles * a.n_tiles : (v - before + kRagM - 1) / kRagM * a.n_tiles;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int o = __shfl_up_sync(0xffffffffu, t, off);
-      if (lane >= off) t += o;
-    }
-    t += tiles;
-    if (e <= a.experts) { c->start[e] = v; c->tile0[e] = t; }
-    run = __shfl_sync(0xffffffffu, v, 31);
-    tiles = __shfl_sync(0xffffffffu, t, 31);
-  }
-}
-
-struct RaggedTile {
-  int e = 0;                   // expert; only moves forward
-  int m, n;                    // row and column tile inside the expert
-  __device__ __forceinline__ void at(const RaggedArgs& a, const RaggedCtrl* c, int t, int form) {
-    while (t >= c->tile0[e + 1]) ++e;
-    const int local = t - c->tile0[e];
-    const int mt = form == 2 ? a.m_tiles : (c->tile0[e + 1] - c->tile0[e]) / a.n_tiles;
-    const int per_group = a.group_m * a.n_tiles;
-    const int bg = local / per_group;
-    const int rem = local - bg * per_group;
-    const int gs = min(a.group_m, mt - bg * a.group_m);
-    n = rem / gs;
-    m = bg * a.group_m + (rem - n * gs);
-  }
-};
-
-// MN-major, 128-byte-swizzled operand tile: chunks of 64 columns x 64 contraction rows (8 KB), 8-row groups 1024 B apart.
-__device__ __forceinline__ uint64_t make_smem_desc_mn(uint32_t smem_addr) {
-  uint64_t d = 0;
-  d |= uint64_t((smem_addr >> 4) & 0x3FFF);
-  d |= uint64_t((kRagK * 128) >> 4) << 16;           // leading byte offset: next 64 columns
-  d |= uint64_t(1024 >> 4) << 32;                    // stride byte offset: next 8 contraction rows
-  d |= uint64_t(1) << 46;
-  d |= uint64_t(2) << 61;                            // SWIZZLE_128B
-  return d;
-}
 
 template <int FORM>
 __global__ void __launch_bounds__(kRagThreads, 1)
@@ -125,7 +53,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   constexpr int kABytes = kRagM * kRagK * 2;
 
   if (warp == 2) {
-    ragged_tables<FORM>(a, ctrl, lane);
+    ragged_tables<FORM, kRagM>(a, &ctrl->tab, lane);
   } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(&ctrl->tmem_base)), "r"(uint32_t(kTmemCols)) : "memory");
@@ -146,9 +74,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem_base = ctrl->tmem_base;
-  const int total = ctrl->tile0[a.experts];
+  const int total = ctrl->tab.tile0[a.experts];
   auto k_blocks = [&](int e) {
-    return FORM == 2 ? (ctrl->start[e + 1] - ctrl->start[e] + kRagK - 1) / kRagK : (a.k_dim + kRagK - 1) / kRagK;
+    return FORM == 2 ? (ctrl->tab.start[e + 1] - ctrl->tab.start[e] + kRagK - 1) / kRagK : (a.k_dim + kRagK - 1) / kRagK;
   };
 
   if (warp == 0) {
@@ -158,8 +86,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     bool ok = true;
     RaggedTile tile;
     for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      tile.at(a, ctrl, t, FORM);
-      const int KB = k_blocks(tile.e), row0 = ctrl->start[tile.e];
+      tile.at(a, &ctrl->tab, t, FORM);
+      const int KB = k_blocks(tile.e), row0 = ctrl->tab.start[tile.e];
       for (int kb = 0; kb < KB; ++kb) {
         ok = warp_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag, a.status, 1, 32);
         if (!ok) break;
@@ -200,9 +128,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
       int KB = (a.k_dim + kRagK - 1) / kRagK, seg = 0;
       if (FORM == 2) {
-        tile.at(a, ctrl, t, FORM);
+        tile.at(a, &ctrl->tab, t, FORM);
         KB = k_blocks(tile.e);
-        seg = ctrl->start[tile.e + 1] - ctrl->start[tile.e];
+        seg = ctrl->tab.start[tile.e + 1] - ctrl->tab.start[tile.e];
         if (KB == 0) continue;                   // the epilogue writes zeros on its own
       }
       ok = warp_wait(smem_u32(&ctrl->acc_empty[acc]), acc_phase ^ 1, abort_flag, a.status, 2);
@@ -215,19 +143,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         if (FORM == 2 && kb + 1 == KB && (seg & (kRagK - 1)) != 0) {
           const int have = seg & (kRagK - 1);    // rows of this expert in the block
           steps = (have + 15) / 16;
-          const int zero = steps * 16 - have;
-          // (64-column chunks of A and B) x zero rows x 8 vectors of 16 bytes; the swizzle stays inside a row
-          for (int i = lane; i < zero * (kRagM + kRagN) / 8; i += 32) {
-            const int chunk = i / (zero * 8), rem = i - chunk * zero * 8;
-            *reinterpret_cast<uint4*>(sp + chunk * kRagK * 128 + (have + rem / 8) * 128 + (rem & 7) * 16) =
-                make_uint4(0, 0, 0, 0);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
+          zero_block_rows(sp, (kRagM + kRagN) / 64, have, steps * 16 - have, lane);
         }
         const uint32_t sa = smem_u32(sp);
-        const uint64_t adesc = kAMn ? make_smem_desc_mn(sa) : make_smem_desc(sa);
-        const uint64_t bdesc = kBMn ? make_smem_desc_mn(sa + kABytes) : make_smem_desc(sa + kABytes);
+        const uint64_t adesc = kAMn ? make_smem_desc_mn(sa, kRagK * 128) : make_smem_desc(sa);
+        const uint64_t bdesc = kBMn ? make_smem_desc_mn(sa + kABytes, kRagK * 128) : make_smem_desc(sa + kABytes);
         tcgen05_fence_after();
         if (elect_one()) {
           for (int k = 0; k < steps; ++k)
@@ -250,8 +170,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     bool ok = true;
     RaggedTile tile;
     for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      tile.at(a, ctrl, t, FORM);
-      const int e = tile.e, start = ctrl->start[e], seg = ctrl->start[e + 1] - start;
+      tile.at(a, &ctrl->tab, t, FORM);
+      const int e = tile.e, start = ctrl->tab.start[e], seg = ctrl->tab.start[e + 1] - start;
       const bool none = FORM == 2 && seg == 0;
       const int local = tile.m * kRagM + row;
       const bool valid = FORM == 2 ? local < a.m_dim : local < seg;
@@ -279,27 +199,12 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
         }
 #pragma unroll
         for (int j = 0; j < 32; j += 8) {
-          uint4 pk;
-          if (a.bf16) {
-            pk.x = pack_bf16x2(v[j], v[j + 1]); pk.y = pack_bf16x2(v[j + 2], v[j + 3]);
-            pk.z = pack_bf16x2(v[j + 4], v[j + 5]); pk.w = pack_bf16x2(v[j + 6], v[j + 7]);
-          } else {
-            pk.x = pack_f16x2(v[j], v[j + 1]); pk.y = pack_f16x2(v[j + 2], v[j + 3]);
-            pk.z = pack_f16x2(v[j + 4], v[j + 5]); pk.w = pack_f16x2(v[j + 6], v[j + 7]);
-          }
-          if (q * 32 + j < cols) *reinterpret_cast<uint4*>(op + (q * 32 + j) * 2) = pk;
+          if (q * 32 + j < cols) *reinterpret_cast<uint4*>(op + (q * 32 + j) * 2) = pack8(v + j, a.bf16);
         }
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
-    if (FORM != 2 && a.zero_uncovered) {
-      // rows that belong to no expert: in front of the first segment and behind the last
-      const int lo = ctrl->start[0], hi = ctrl->start[a.experts];
-      const long long vec = a.n_dim / 8, head = lo * vec, all = head + (a.rows - hi) * vec;
-      uint4* out = static_cast<uint4*>(a.out);
-      for (long long i = (long long)blockIdx.x * 256 + threadIdx.x - 128; i < all; i += (long long)gridDim.x * 256)
-        out[i < head ? i : (long long)hi * vec + i - head] = make_uint4(0, 0, 0, 0);
-    }
+    if (FORM != 2 && a.zero_uncovered) zero_uncovered_rows(a, &ctrl->tab, threadIdx.x - 128, 256);
   }
 
   tcgen05_fence_before();
@@ -312,8 +217,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
 }
 
 // ------------------------------------------------------------------------------ host
-// Row-major 16-bit matrix [rows, cols] (or `mats` of them), boxes of 64 columns x box_rows rows.
-static int ragged_map(CUtensorMap* map, const void* base, long long cols, long long rows, int mats, int box_rows) {
+int ragged_map(CUtensorMap* map, const void* base, long long cols, long long rows, int mats, int box_rows) {
   cuuint64_t dims[3] = {cuuint64_t(cols) * 2, cuuint64_t(rows), cuuint64_t(mats)};
   cuuint64_t strides[2] = {cuuint64_t(cols) * 2, cuuint64_t(cols) * 2 * cuuint64_t(rows)};
   cuuint32_t box[3] = {128, cuuint32_t(box_rows), 1};
@@ -331,6 +235,9 @@ static int launch_ragged(const CUtensorMap& ma, const CUtensorMap& mb, const Rag
   FLYMOE_CUDA_CHECK(cudaGetLastError());
   return FLYMOE_OK;
 }
+
+static int envint(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
+static bool use_pairs(int rows, int experts) { return rows >= envint("PAIR", 128) * experts; }
 
 static int ragged_common(RaggedArgs* a, const char* what, const void* out, const void* p, const void* q,
                          const int32_t* offsets, int rows, int experts, int n, int k, int dtype) {
@@ -374,6 +281,7 @@ extern "C" int flymoe_grouped_gemm(void* out, const void* x, const void* w, cons
   a.group_m = 8;
   const long long max_tiles = ((long long)rows / kRagM + experts) * a.n_tiles;
   FLYMOE_REQUIRE(max_tiles < (1LL << 31), "grouped_gemm: too many tiles");
+  if (use_pairs(rows, experts)) return launch_ragged_pair(input_grad ? 1 : 0, x, w, a, n, k, static_cast<cudaStream_t>(stream));
   CUtensorMap ma, mb;
   if ((rc = ragged_map(&ma, x, a.k_dim, rows, 0, kRagM)) != FLYMOE_OK) return rc;
   if ((rc = ragged_map(&mb, w, k, n, experts, input_grad ? kRagK : kRagN)) != FLYMOE_OK) return rc;
@@ -400,6 +308,7 @@ extern "C" int flymoe_grouped_gemm_wgrad(void* dw, const void* dy, const void* x
   a.group_m = 8;
   const long long max_tiles = (long long)experts * a.m_tiles * a.n_tiles;
   FLYMOE_REQUIRE(max_tiles < (1LL << 31), "grouped_gemm_wgrad: too many tiles");
+  if (use_pairs(rows, experts)) return launch_ragged_pair(2, dy, x, a, n, k, s);
   CUtensorMap ma, mb;
   if ((rc = ragged_map(&ma, dy, n, rows, 0, kRagK)) != FLYMOE_OK) return rc;
   if ((rc = ragged_map(&mb, x, k, rows, 0, kRagK)) != FLYMOE_OK) return rc;

@@ -1,0 +1,322 @@
+// Ragged grouped products on CTA pairs (tcgen05 cta_group::2): tiles of 256 x 256 for experts with many rows.
+//
+// Each CTA of a pair brings 128 rows of A and 128 rows (or columns) of B into shared memory, 32 KB per K block of 64, and the
+// leader's MMAs read both halves.  The one-CTA kernel (grouped.cu) needs 48 KB for half the work: at the 64 bytes a cycle
+// that an SM takes from L2 those are 768 cycles per K block against 512 of MMA, and that is what it measures.
+//   warp 0      TMA producer; both CTAs' operands complete on the leader's barrier
+//   warp 1      (leader) MMA issuer, two accumulators of 256 columns
+//   warp 2      segment tables
+//   warp 3      weight gradient: the last K block of an expert completes on each CTA's own barrier; this warp zeroes the rows
+//               behind the expert's end and then tells the leader
+//   warps 4-11  epilogue, two warpgroups with 128 columns each: 64 columns at a time to shared memory and out by one tiled
+//               store (rows of another expert in the tile: by plain stores of the valid rows)
+//
+// Every wait is bounded as in the other kernels.  Epilogue warps keep step with one another on hardware barriers, so after a
+// wait that ran out they walk on through their tiles without storing instead of leaving.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "gemm_ptx.cuh"
+#include "grouped.cuh"
+
+namespace flymoe {
+
+constexpr int kRpTile = 256;
+constexpr int kRpStages = 5;
+constexpr int kRpHalf = 128 * kRagK * 2;                         // 16 KB: one operand of one CTA and K block
+constexpr int kRpStageBytes = 2 * kRpHalf;
+constexpr int kRpThreads = 384;
+constexpr int kRpStaging = 128 * 128;                            // 128 rows x 64 columns of output per warpgroup
+
+struct __align__(16) RagPairCtrl {
+  unsigned long long full[kRpStages], empty[kRpStages], tail[kRpStages];
+  unsigned long long acc_full[2], acc_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+  RaggedTables tab;
+};
+constexpr size_t kRpSmem = size_t(kRpStages) * kRpStageBytes + 2 * kRpStaging + sizeof(RagPairCtrl) + 1024;
+static_assert(kRpSmem <= 232448, "shared memory budget of one SM exceeded");
+
+__device__ __forceinline__ void mbar_arrive_release_cluster(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+template <int FORM>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRpThreads, 1)
+grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                    const __grid_constant__ CUtensorMap tmap_out, const RaggedArgs a) {
+  extern __shared__ uint8_t smem_dyn[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  uint8_t* staging = smem + size_t(kRpStages) * kRpStageBytes;
+  RagPairCtrl* ctrl = reinterpret_cast<RagPairCtrl*>(staging + 2 * kRpStaging);
+  volatile int* abort_flag = &ctrl->abort_flag;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = int(cluster_rank());
+  constexpr bool kAMn = FORM == 2, kBMn = FORM != 0;
+
+  if (warp == 2) {
+    ragged_tables<FORM, kRpTile>(a, &ctrl->tab, lane);
+  } else if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(smem_u32(&ctrl->tmem_base)), "r"(uint32_t(kTmemCols)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else if (threadIdx.x == 0) {
+    for (int i = 0; i < kRpStages; ++i) {
+      // weight gradient: two arrivals, the producer's or, for an expert's last block, one from either CTA's warp 3
+      mbar_init(smem_u32(&ctrl->full[i]), FORM == 2 ? 2 : 1);
+      mbar_init(smem_u32(&ctrl->empty[i]), 1);
+      mbar_init(smem_u32(&ctrl->tail[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&ctrl->acc_full[i]), 1);
+      mbar_init(smem_u32(&ctrl->acc_empty[i]), 2 * kEpilogueWarps);
+    }
+    ctrl->abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();                            // both CTAs' barriers and TMEM exist
+  tcgen05_fence_after();
+  const uint32_t tmem_base = ctrl->tmem_base;
+  const RaggedTables* tab = &ctrl->tab;
+  const int total = tab->tile0[a.experts];
+  const int first = int(blockIdx.x) >> 1, step = int(gridDim.x) >> 1;
+  const int k_blocks = (a.k_dim + kRagK - 1) / kRagK;
+  auto rows_of = [&](int e) { return tab->start[e + 1] - tab->start[e]; };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    RaggedTile tile;
+    for (int t = first; t < total && ok; t += step) {
+      tile.at(a, tab, t, FORM);
+      const int seg = rows_of(tile.e), row0 = tab->start[tile.e];
+      const int KB = FORM == 2 ? (seg + kRagK - 1) / kRagK : k_blocks;
+      for (int kb = 0; kb < KB; ++kb) {
+        ok = warp_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag, a.status, 1, 32);
+        if (!ok) break;
+        const uint32_t sa = smem_u32(smem + size_t(stage) * kRpStageBytes), sb = sa + kRpHalf;
+        const bool tail = FORM == 2 && kb + 1 == KB && (seg & (kRagK - 1)) != 0;
+        if (elect_one()) {
+          if (tail) {
+            const uint32_t bar = smem_u32(&ctrl->tail[stage]);
+            mbar_expect_tx(bar, kRpStageBytes);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              tma_load_2d(sa + j * kRagK * 128, &tmap_a, bar, (tile.m * kRpTile + rank * 128 + j * 64) * 2, row0 + kb * kRagK);
+              tma_load_2d(sb + j * kRagK * 128, &tmap_b, bar, (tile.n * kRpTile + rank * 128 + j * 64) * 2, row0 + kb * kRagK);
+            }
+          } else {
+            // the leader announces the bytes of both CTAs; the other's may land before that
+            const uint32_t bar = map_to_rank(smem_u32(&ctrl->full[stage]), 0);
+            if (rank == 0) {
+              mbar_expect_tx(smem_u32(&ctrl->full[stage]), 2 * kRpStageBytes);
+              if (FORM == 2) mbar_arrive(smem_u32(&ctrl->full[stage]));
+            }
+            if (FORM == 2) {
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                tma_load_2d_pair(sa + j * kRagK * 128, &tmap_a, bar, (tile.m * kRpTile + rank * 128 + j * 64) * 2, row0 + kb * kRagK);
+            } else {
+              tma_load_2d_pair(sa, &tmap_a, bar, kb * kRagK * 2, row0 + tile.m * kRpTile + rank * 128);
+            }
+            if (FORM == 0) {
+              tma_load_3d_pair(sb, &tmap_b, bar, kb * kRagK * 2, tile.n * kRpTile + rank * 128, tile.e);
+            } else {
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const int col = (tile.n * kRpTile + rank * 128 + j * 64) * 2;
+                if (FORM == 1) tma_load_3d_pair(sb + j * kRagK * 128, &tmap_b, bar, col, kb * kRagK, tile.e);
+                else tma_load_2d_pair(sb + j * kRagK * 128, &tmap_b, bar, col, row0 + kb * kRagK);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (++stage == kRpStages) { stage = 0; phase ^= 1; }
+      }
+    }
+    // the last releases of the ring are the leader's MMAs arriving in both CTAs: they have to land before this CTA's shared
+    // memory goes away
+    for (int i = 0; i < kRpStages && ok; ++i) {
+      ok = warp_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag, a.status, 1, 32);
+      if (++stage == kRpStages) { stage = 0; phase ^= 1; }
+    }
+  } else if (warp == 1 && rank == 0) {
+    // ------------------------------------------------------------------ MMA issuer
+    const uint32_t idesc = ((a.bf16 ? kInstrDescBF16 : kInstrDescF16) - kInstrDescShape) | uint32_t(kRpTile >> 3) << 17 |
+                           uint32_t(kRpTile >> 4) << 24 | (kAMn ? 1u << 15 : 0u) | (kBMn ? 1u << 16 : 0u);
+    constexpr uint64_t a_step = kAMn ? (16 * 128) >> 4 : 2, b_step = kBMn ? (16 * 128) >> 4 : 2;
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    RaggedTile tile;
+    for (int t = first; t < total && ok; t += step) {
+      int KB = k_blocks, seg = 0;
+      if (FORM == 2) {
+        tile.at(a, tab, t, FORM);
+        seg = rows_of(tile.e);
+        KB = (seg + kRagK - 1) / kRagK;
+        if (KB == 0) continue;                   // the epilogue writes zeros on its own
+      }
+      ok = warp_wait(smem_u32(&ctrl->acc_empty[acc]), acc_phase ^ 1, abort_flag, a.status, 2);
+      const uint32_t d_tmem = tmem_base + uint32_t(acc) * kRpTile;
+      for (int kb = 0; kb < KB && ok; ++kb) {
+        ok = __all_sync(0xffffffffu, mbar_wait_cluster(smem_u32(&ctrl->full[stage]), phase, abort_flag, a.status, 3));
+        if (!ok) break;
+        const uint32_t sa = smem_u32(smem + size_t(stage) * kRpStageBytes);
+        const uint64_t adesc = kAMn ? make_smem_desc_mn(sa, kRagK * 128) : make_smem_desc(sa);
+        const uint64_t bdesc = kBMn ? make_smem_desc_mn(sa + kRpHalf, kRagK * 128) : make_smem_desc(sa + kRpHalf);
+        const int rest = seg & (kRagK - 1);
+        const int steps = FORM == 2 && kb + 1 == KB && rest != 0 ? (rest + 15) / 16 : kRagK / 16;
+        tcgen05_fence_after();
+        if (elect_one()) {
+          for (int k = 0; k < steps; ++k)
+            umma_pair<2>(d_tmem, adesc + a_step * k, bdesc + b_step * k, idesc, (k > 0 || kb > 0) ? 1u : 0u);
+          umma_commit_pair(smem_u32(&ctrl->empty[stage]));
+          if (kb + 1 == KB) umma_commit_pair(smem_u32(&ctrl->acc_full[acc]));
+        }
+        __syncwarp();
+        if (++stage == kRpStages) { stage = 0; phase ^= 1; }
+      }
+      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+  } else if (warp == 3 && FORM == 2) {
+    // ------------------------------------------------------------------ last blocks: rows behind the end become zeros
+    uint32_t parity = 0;                         // a bit per stage
+    long long blocks = 0;
+    bool ok = true;
+    RaggedTile tile;
+    for (int t = first; t < total && ok; t += step) {
+      tile.at(a, tab, t, FORM);
+      const int seg = rows_of(tile.e), rest = seg & (kRagK - 1);
+      blocks += (seg + kRagK - 1) / kRagK;
+      if (rest == 0) continue;
+      const int stage = int((blocks - 1) % kRpStages);
+      ok = warp_wait(smem_u32(&ctrl->tail[stage]), (parity >> stage) & 1, abort_flag, a.status, 5, 32);
+      if (!ok) break;
+      parity ^= 1u << stage;
+      zero_block_rows(smem + size_t(stage) * kRpStageBytes, 4, rest, (16 - rest % 16) % 16, lane);
+      if (lane == 0) mbar_arrive_release_cluster(map_to_rank(smem_u32(&ctrl->full[stage]), 0));
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ epilogue
+    const int wg = (warp - 4) >> 2, tid = threadIdx.x - 128 - wg * 128;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t tcol = tmem_base + (uint32_t((warp & 3) * 32) << 16) + uint32_t(wg * 128);
+    const uint32_t empty_bar = map_to_rank(smem_u32(&ctrl->acc_empty[0]), 0);
+    uint8_t* stg = staging + wg * kRpStaging;
+    uint8_t* line = stg + row * 128;
+    const int sw = row & 7;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    bool ok = true;
+    RaggedTile tile;
+    for (int t = first; t < total; t += step) {
+      tile.at(a, tab, t, FORM);
+      const int e = tile.e, seg = rows_of(e);
+      const int m0 = tile.m * kRpTile + rank * 128;              // first row of this CTA inside the expert's output
+      const int rows = max(0, min(128, (FORM == 2 ? a.m_dim : seg) - m0));
+      const long long row0 = FORM == 2 ? (long long)e * a.m_dim + m0 : (long long)tab->start[e] + m0;
+      const bool none = FORM == 2 && seg == 0;
+      if (!none) {
+        ok = ok && warp_wait(smem_u32(&ctrl->acc_full[acc]), acc_phase, abort_flag, a.status, 4);
+        tcgen05_fence_after();
+      }
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int col = tile.n * kRpTile + wg * 128 + q * 64;
+        const bool wanted = rows > 0 && col < a.n_dim;           // the same in the whole warpgroup
+        float v[64];
+        if (wanted && !none) {
+          tmem_ld_x32(tcol + uint32_t(acc) * kRpTile + q * 64, reinterpret_cast<uint32_t*>(v));
+          tmem_ld_x32(tcol + uint32_t(acc) * kRpTile + q * 64 + 32, reinterpret_cast<uint32_t*>(v + 32));
+          tmem_ld_wait();
+        }
+        if (q == 1 && !none) {
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_relaxed_cluster(empty_bar + uint32_t(acc) * 8u);
+        }
+        if (!wanted) continue;
+        if (tid == 0) bulk_wait_read_all();      // the staging area's last store has been read out
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<uint4*>(line + ((j ^ sw) * 16)) = none ? make_uint4(0, 0, 0, 0) : pack8(v + j * 8, a.bf16);
+        const bool tiled = FORM == 2 || rows == 128;             // form 2: the map ends with the expert's matrix
+        if (tiled) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
+        if (tiled) {
+          if (tid == 0 && ok) {
+            if (FORM == 2) tma_store_3d(&tmap_out, smem_u32(stg), col * 2, m0, e);
+            else tma_store_2d(&tmap_out, smem_u32(stg), col * 2, int(row0));
+            bulk_commit();
+          }
+        } else if (ok) {
+          for (int i = tid; i < rows * 8; i += 128) {
+            const int r = i >> 3, c = i & 7;
+            if (col + c * 8 < a.n_dim)
+              *reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.out) + ((row0 + r) * a.n_dim + col + c * 8) * 2) =
+                  *reinterpret_cast<const uint4*>(stg + r * 128 + ((c ^ (r & 7)) * 16));
+          }
+        }
+      }
+      if (!none && ++acc == 2) { acc = 0; acc_phase ^= 1; }
+    }
+    if (tid == 0) bulk_wait_all();
+    if (FORM != 2 && a.zero_uncovered) zero_uncovered_rows(a, tab, threadIdx.x - 128, 256);
+  }
+
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync_all();                            // no remote arrival or MMA is outstanding when a CTA leaves
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(uint32_t(kTmemCols))
+                 : "memory");
+  }
+}
+
+// ------------------------------------------------------------------------------ host
+template <int FORM>
+static int launch_pair_form(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const RaggedArgs& a,
+                            long long max_tiles, cudaStream_t stream) {
+  auto* kernel = grouped_pair_kernel<FORM>;
+  static SmemLimitSeen seen;
+  FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(kRpSmem), seen));
+  const unsigned pairs = unsigned(std::min<long long>(max_tiles, sm_count() / 2));
+  kernel<<<2 * pairs, kRpThreads, kRpSmem, stream>>>(ma, mb, mo, a);
+  FLYMOE_CUDA_CHECK(cudaGetLastError());
+  return FLYMOE_OK;
+}
+
+int launch_ragged_pair(int form, const void* p, const void* q, const RaggedArgs& args, int n, int k, cudaStream_t stream) {
+  RaggedArgs a = args;
+  a.n_tiles = ceil_div(a.n_dim, kRpTile);
+  if (form == 2) a.m_tiles = ceil_div(a.m_dim, kRpTile);
+  CUtensorMap ma, mb, mo;
+  int rc;
+  if (form == 2) {
+    rc = ragged_map(&ma, p, n, a.rows, 0, kRagK);
+    if (rc == FLYMOE_OK) rc = ragged_map(&mb, q, k, a.rows, 0, kRagK);
+    if (rc == FLYMOE_OK) rc = ragged_map(&mo, a.out, a.n_dim, a.m_dim, a.experts, 128);
+    const long long tiles = (long long)a.experts * a.m_tiles * a.n_tiles;
+    return rc != FLYMOE_OK ? rc : launch_pair_form<2>(ma, mb, mo, a, tiles, stream);
+  }
+  rc = ragged_map(&ma, p, a.k_dim, a.rows, 0, 128);
+  if (rc == FLYMOE_OK) rc = ragged_map(&mb, q, k, n, a.experts, form == 1 ? kRagK : 128);
+  if (rc == FLYMOE_OK) rc = ragged_map(&mo, a.out, a.n_dim, a.rows, 0, 128);
+  if (rc != FLYMOE_OK) return rc;
+  const long long tiles = ((long long)a.rows / kRpTile + a.experts) * a.n_tiles;
+  return form == 1 ? launch_pair_form<1>(ma, mb, mo, a, tiles, stream) : launch_pair_form<0>(ma, mb, mo, a, tiles, stream);
+}
+
+}  // namespace flymoe

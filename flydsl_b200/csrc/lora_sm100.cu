@@ -27,14 +27,7 @@ constexpr int kChunkBytes = kTileRows * 128;     // 128 rows x 64 16-bit columns
 __device__ __forceinline__ uint32_t instr_desc(int bf16, int n) {
   return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(n >> 3) << 17) | (uint32_t(kTileRows >> 4) << 24);
 }
-// Operand tile whose contraction runs over its rows (MN-major): chunks of 64 columns (128 bytes a row) `chunk` bytes apart.
-__device__ __forceinline__ uint64_t smem_desc_mn(uint32_t addr, uint32_t chunk) {
-  return uint64_t((addr >> 4) & 0x3FFF) | uint64_t(chunk >> 4) << 16 | uint64_t(1024 >> 4) << 32 | uint64_t(1) << 46 | uint64_t(2) << 61;
-}
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];"
-               ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
-}
+
 // ---------------------------------------------------------------------------- shrink
 constexpr int kShX = 4;                          // K blocks of x in flight
 constexpr int kShABytes = 32768;                 // ring of adapter blocks, rank rows x 128 bytes each
@@ -134,7 +127,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
         ok = warp_wait(smem_u32(&c->a_full[as]), ap, abort_flag, q.status, 3);
         if (!ok) break;
         const uint32_t at = smem_u32(aring + as * a_bytes);
-        const uint64_t bdesc = p.transposed ? smem_desc_mn(at, 8192) : make_smem_desc(at);
+        const uint64_t bdesc = p.transposed ? make_smem_desc_mn(at, 8192) : make_smem_desc(at);
         tcgen05_fence_after();
         if (elect_one()) {
 #pragma unroll
@@ -331,7 +324,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
           for (int part = 0; part < 2; ++part)
             for (int k = 0; k < steps; ++k) {
               const uint64_t ad = make_smem_desc(smem_u32(vtile + (part * KC + (k >> 2)) * kChunkBytes)) + (k & 3) * 2;
-              const uint64_t bd = p.transposed ? smem_desc_mn(smem_u32(bring + bs * KC * kChunkBytes) + k * 2048, b_bytes / 2)
+              const uint64_t bd = p.transposed ? make_smem_desc_mn(smem_u32(bring + bs * KC * kChunkBytes) + k * 2048, b_bytes / 2)
                                                : make_smem_desc(smem_u32(bring + (bs * KC + (k >> 2)) * kChunkBytes)) + (k & 3) * 2;
               umma_f16(tmem + acc * kExCols, ad, bd, idesc, (part > 0 || k > 0) ? 1u : 0u);
             }

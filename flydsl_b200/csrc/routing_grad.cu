@@ -33,6 +33,11 @@ route_tables_kernel(const int* __restrict__ sorted_ids, const int* __restrict__ 
 }
 
 // ---------------------------------------------------------------------------- rows <-> pairs
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
 struct Routed {
   const int* sorted_ids;       // [rows] (slot << 24) | token
   const int* num_valid_ids;    // rows of them in use
@@ -81,34 +86,48 @@ permute_rows_kernel(const uint4* __restrict__ src, uint4* __restrict__ dst, cons
 }
 
 // out[t] = sum_s weights[t, s] * rows[row of (t, s)], fp32 in slot order, rounded once; weights null: ones.
-// grid (columns / 2048, tokens), 8 columns a thread, four rows in flight.
+// A block per token: its rows are looked up once, then every thread has eight of their 16-byte pieces in flight.  4096
+// tokens x 8 rows of 7168, bf16 (one B200): with the look-up in every thread 159 us.
+constexpr int kCombineSlots = 256;
 template <typename T>
 __global__ void __launch_bounds__(256)
 combine_rows_kernel(const T* __restrict__ rows, const float* __restrict__ weights, T* __restrict__ out, const Routed p,
                     int dim) {
-  const int col = (blockIdx.x * 256 + threadIdx.x) * 8;
-  for (int t = blockIdx.y; t < p.tokens; t += gridDim.y) {
-    if (col >= dim) return;
-    float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (int s0 = 0; s0 < p.topk; s0 += 4) {
-      float f[4][8], w[4];
-      int r[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        r[j] = s0 + j < p.topk ? p.row_of(t, s0 + j) : -1;
-        w[j] = r[j] >= 0 && weights ? __ldg(weights + (long long)t * p.topk + s0 + j) : 1.f;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (r[j] >= 0) Vec8<T>::load(rows + (long long)r[j] * dim + col, f[j]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (r[j] >= 0) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) acc[i] = fmaf(f[j][i], w[j], acc[i]);
-        }
+  __shared__ int row[kCombineSlots];
+  __shared__ float weight[kCombineSlots];
+  constexpr int kVec = 16 / sizeof(T);           // elements of a 16-byte piece
+  for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+    if (int(threadIdx.x) < p.topk) {
+      const int r = p.row_of(t, threadIdx.x);
+      row[threadIdx.x] = r;
+      weight[threadIdx.x] = r >= 0 && weights ? __ldg(weights + (long long)t * p.topk + threadIdx.x) : 1.f;
     }
-    Vec8<T>::store(out + (long long)t * dim + col, acc);
+    __syncthreads();
+    for (int col = threadIdx.x * kVec; col < dim; col += 256 * kVec) {
+      float acc[kVec];
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) acc[i] = 0.f;
+      for (int s0 = 0; s0 < p.topk; s0 += 8) {
+        uint4 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (s0 + j < p.topk && row[s0 + j] >= 0)
+            v[j] = __ldg(reinterpret_cast<const uint4*>(rows + (long long)row[s0 + j] * dim + col));
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (s0 + j < p.topk && row[s0 + j] >= 0) {
+            const T* x = reinterpret_cast<const T*>(&v[j]);
+#pragma unroll
+            for (int i = 0; i < kVec; ++i) acc[i] = fmaf(float(x[i]), weight[s0 + j], acc[i]);
+          }
+      }
+      uint4 o;
+      T* y = reinterpret_cast<T*>(&o);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) y[i] = from_float<T>(acc[i]);
+      *reinterpret_cast<uint4*>(out + (long long)t * dim + col) = o;
+    }
+    __syncthreads();
   }
 }
 
@@ -119,6 +138,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 combine_backward_kernel(const T* __restrict__ dout, const T* __restrict__ rows, const float* __restrict__ weights,
                         T* __restrict__ drows, float* __restrict__ dweights, const Routed p, int dim) {
+  constexpr int kVec = 16 / sizeof(T);           // elements of a 16-byte piece
   const int lane = threadIdx.x & 31;
   const long long warp = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), warps = (long long)gridDim.x * 8;
   const long long pairs = (long long)p.tokens * p.topk;
@@ -130,26 +150,26 @@ combine_backward_kernel(const T* __restrict__ dout, const T* __restrict__ rows, 
       const T* g = dout + (long long)t * dim;
       const T* z = rows + (long long)r * dim;
       T* d = drows + (long long)r * dim;
-      for (int c = lane * 8; c < dim; c += 512) {
-        float a[2][8], b[2][8];
+      for (int c = lane * kVec; c < dim; c += 128 * kVec) {
+        uint4 a[4], b[4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (c + 256 * j < dim) {
-            Vec8<T>::load(g + c + 256 * j, a[j]);
-            if (dweights) Vec8<T>::load(z + c + 256 * j, b[j]);
+        for (int j = 0; j < 4; ++j)
+          if (c + 32 * kVec * j < dim) {
+            a[j] = __ldg(reinterpret_cast<const uint4*>(g + c + 32 * kVec * j));
+            if (dweights) b[j] = __ldg(reinterpret_cast<const uint4*>(z + c + 32 * kVec * j));
           }
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          if (c + 256 * j < dim) {
-            if (dweights) {
+        for (int j = 0; j < 4; ++j)
+          if (c + 32 * kVec * j < dim) {
+            T* x = reinterpret_cast<T*>(&a[j]);
+            const T* y = reinterpret_cast<const T*>(&b[j]);
 #pragma unroll
-              for (int q = 0; q < 8; ++q) dot = fmaf(a[j][q], b[j][q], dot);
+            for (int q = 0; q < kVec; ++q) {
+              const float f = float(x[q]);
+              if (dweights) dot = fmaf(f, float(y[q]), dot);
+              x[q] = from_float<T>(f * w);
             }
-            if (drows) {
-#pragma unroll
-              for (int q = 0; q < 8; ++q) a[j][q] *= w;
-              Vec8<T>::store(d + c + 256 * j, a[j]);
-            }
+            if (drows) *reinterpret_cast<uint4*>(d + c + 32 * kVec * j) = a[j];
           }
       }
     }
@@ -172,11 +192,6 @@ combine_backward_kernel(const T* __restrict__ dout, const T* __restrict__ rows, 
 }
 
 // ---------------------------------------------------------------------------- gate
-template <typename T> __device__ __forceinline__ T from_float(float x);
-template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
-template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-
 // One warp per token; expert e lives in lane e % 32, register e / 32; lane j holds pick j.
 //   renormalised: w = softmax over the picks      dlogit_i = w_i (g_i - sum_j w_j g_j) on the picks, 0 elsewhere
 //   else:         w = softmax over all, p         dlogit_e = [picked] p_e g_e - p_e sum_j p_j g_j
@@ -310,7 +325,7 @@ extern "C" int flymoe_combine_rows(const void* rows_in, const float* weights, vo
   FLYMOE_REQUIRE((rows_in || rows == 0) && out, "combine_rows: null pointer");
   FLYMOE_REQUIRE(aligned16(rows_in) && aligned16(out), "combine_rows: pointers must be 16-byte aligned");
   const Routed p = {sorted_ids, num_valid_ids, row_index, num_tokens, topk, rows};
-  const dim3 grid(ceil_div(dim, 2048), std::min(num_tokens, 65535));
+  const int grid = num_tokens;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == FLYMOE_BF16)
     combine_rows_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(rows_in), weights,
