@@ -4,18 +4,23 @@
 //   form 0   y[r, n]     = sum_k x[r, k]  w[e, n, k]        forward
 //   form 1   dx[r, k]    = sum_n dy[r, n] w[e, n, k]        input gradient
 //   form 2   dw[e, n, k] = sum_{r in e} dy[r, n] x[r, k]    weight gradient (an expert without rows gets zeros)
-// One kernel: 128 x 256 output tiles, K blocks of 64, fp32 accumulation in TMEM, one rounding at the end.  What changes is
-// which axis of an operand is contiguous: form 0 reads both along the contraction (K-major tiles), form 1 the weights
-// across it, form 2 both operands across it (MN-major tiles: 64-column chunks of 64 contraction rows, 128 bytes a row).
-// No operand is transposed in memory.
+// 16-bit operands through TMA, fp32 accumulation in TMEM, one rounding at the end.  What changes between the forms is which
+// axis of an operand is contiguous: form 0 reads both along the contraction (K-major tiles), form 1 the weights across it,
+// form 2 both operands across it (MN-major tiles: 64-column chunks of 64 contraction rows, 128 bytes a row).  No operand is
+// transposed in memory.
 //
-// Ragged ends.  Forms 0 and 1: a tile may read rows of the next expert; they only reach accumulator rows that are not
-// stored.  Form 2 contracts over the rows, so the last K block of an expert issues only the 16-row steps that hold rows of
-// it, and of the last step the rows behind the end are overwritten with zeros in shared memory (both operands: what stands
-// there may be infinite).
+// This file: forms 0 and 1 on one CTA per tile, of 128 rows x 256 or 128 columns or, where most experts have few rows, of 32
+// rows x 128 or 32 (form 1: 64) columns; all of form 2 and experts with many rows run on CTA pairs (grouped_pair.cu).  A tile may read rows
+// of the next expert; they only reach accumulator rows that are not stored.  A 32-row tile loads 32 rows per K block; the MMAs
+// have 128 and read on into whatever follows in shared memory, which reaches no stored row either.  What small launches need
+// is bytes in flight (a K block takes about 2 us from its request to its release when the weights come from HBM), so their
+// tiles are narrow and the ring is deep: one expert of 4096 x 4096 with one row takes 33 us on 128-row tiles.
 #include <cuda.h>
 #include <stdio.h>
 #include <stdlib.h>
+
+#include <algorithm>
+#include <cmath>
 
 #include "common.cuh"
 #include "gemm_ptx.cuh"
@@ -23,49 +28,56 @@
 
 namespace flymoe {
 
-constexpr int kRagM = 128, kRagN = 256;
-constexpr int kRagStages = 4;
-constexpr int kRagStageBytes = (kRagM + kRagN) * kRagK * 2;      // 48 KB
 constexpr int kRagThreads = 384;
+constexpr int kRagMaxStages = 24;
+template <int TM, int BN> constexpr int rag_stage_bytes() { return (TM + BN) * kRagK * 2; }
+// As many K blocks as fit beside the tables; behind the last one, what a 128-row read of a 32-row block reaches.
+template <int TM, int BN> constexpr int rag_stages() {
+  const int n = (232448 - 1024 - 9216 - (128 - TM) * kRagK * 2) / rag_stage_bytes<TM, BN>();
+  return n > kRagMaxStages ? kRagMaxStages : n;
+}
 
 struct __align__(16) RaggedCtrl {
-  unsigned long long full[kRagStages];
-  unsigned long long empty[kRagStages];
+  unsigned long long full[kRagMaxStages], empty[kRagMaxStages];
   unsigned long long acc_full[2];
   unsigned long long acc_empty[2];
   uint32_t tmem_base;
   int abort_flag;
   RaggedTables tab;
 };
-constexpr size_t kRagSmem = size_t(kRagStages) * kRagStageBytes + sizeof(RaggedCtrl) + 1024;
-static_assert(kRagSmem <= 232448, "shared memory budget of one SM exceeded");
+template <int TM, int BN> constexpr size_t rag_ring() {
+  return size_t(rag_stages<TM, BN>()) * rag_stage_bytes<TM, BN>() + (128 - TM) * kRagK * 2;
+}
+static_assert(sizeof(RaggedCtrl) <= 9216, "shared memory budget of one SM exceeded");
 
-template <int FORM>
+template <int FORM, int TM, int BN>
 __global__ void __launch_bounds__(kRagThreads, 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                     const RaggedArgs a) {
+  constexpr int kStages = rag_stages<TM, BN>(), kStageBytes = rag_stage_bytes<TM, BN>(), kABytes = TM * kRagK * 2;
+  constexpr int kTmem = 2 * BN < 32 ? 32 : 2 * BN;             // two accumulators
+  constexpr int kWgs = BN >= 64 ? 2 : 1;                         // warpgroups of the epilogue that have columns
+  static_assert(FORM == 0 || BN % 64 == 0, "columns across the contraction come 64 at a time");
   extern __shared__ uint8_t smem_dyn[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
-  RaggedCtrl* ctrl = reinterpret_cast<RaggedCtrl*>(smem + size_t(kRagStages) * kRagStageBytes);
+  RaggedCtrl* ctrl = reinterpret_cast<RaggedCtrl*>(smem + rag_ring<TM, BN>());
   volatile int* abort_flag = &ctrl->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr bool kAMn = FORM == 2, kBMn = FORM != 0;
-  constexpr int kABytes = kRagM * kRagK * 2;
 
   if (warp == 2) {
-    ragged_tables<FORM, kRagM>(a, &ctrl->tab, lane);
+    ragged_tables<FORM, TM>(a, &ctrl->tab, lane);
   } else if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                 ::"r"(smem_u32(&ctrl->tmem_base)), "r"(uint32_t(kTmemCols)) : "memory");
+                 ::"r"(smem_u32(&ctrl->tmem_base)), "r"(uint32_t(kTmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   } else if (threadIdx.x == 0) {
-    for (int i = 0; i < kRagStages; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(smem_u32(&ctrl->full[i]), 1);
       mbar_init(smem_u32(&ctrl->empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&ctrl->acc_full[i]), 1);
-      mbar_init(smem_u32(&ctrl->acc_empty[i]), kEpilogueWarps);
+      mbar_init(smem_u32(&ctrl->acc_empty[i]), 4 * kWgs);
     }
     ctrl->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -74,10 +86,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem_base = ctrl->tmem_base;
-  const int total = ctrl->tab.tile0[a.experts];
-  auto k_blocks = [&](int e) {
-    return FORM == 2 ? (ctrl->tab.start[e + 1] - ctrl->tab.start[e] + kRagK - 1) / kRagK : (a.k_dim + kRagK - 1) / kRagK;
-  };
+  const RaggedTables* tab = &ctrl->tab;
+  const int total = tab->tile0[a.experts];
+  const int KB = (a.k_dim + kRagK - 1) / kRagK;
 
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
@@ -86,133 +97,105 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     bool ok = true;
     RaggedTile tile;
     for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      tile.at(a, &ctrl->tab, t, FORM);
-      const int KB = k_blocks(tile.e), row0 = ctrl->tab.start[tile.e];
+      tile.at(a, tab, t, FORM);
+      const int row0 = tab->start[tile.e] + tile.m * TM;
       for (int kb = 0; kb < KB; ++kb) {
         ok = warp_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag, a.status, 1, 32);
         if (!ok) break;
         const uint32_t full = smem_u32(&ctrl->full[stage]);
-        const uint32_t sa = smem_u32(smem + size_t(stage) * kRagStageBytes), sb = sa + kABytes;
+        const uint32_t sa = smem_u32(smem + size_t(stage) * kStageBytes), sb = sa + kABytes;
         if (elect_one()) {
-          mbar_expect_tx(full, kRagStageBytes);
-          if (kAMn) {
-#pragma unroll
-            for (int j = 0; j < kRagM / 64; ++j)
-              tma_load_2d(sa + j * kRagK * 128, &tmap_a, full, (tile.m * kRagM + j * 64) * 2, row0 + kb * kRagK);
-          } else {
-            tma_load_2d(sa, &tmap_a, full, kb * kRagK * 2, row0 + tile.m * kRagM);
-          }
+          mbar_expect_tx(full, kStageBytes);
+          tma_load_2d(sa, &tmap_a, full, kb * kRagK * 2, row0);
           if (FORM == 0) {
-            tma_load_3d(sb, &tmap_b, full, kb * kRagK * 2, tile.n * kRagN, tile.e);
+            tma_load_3d(sb, &tmap_b, full, kb * kRagK * 2, tile.n * BN, tile.e);
           } else {
 #pragma unroll
-            for (int j = 0; j < kRagN / 64; ++j) {
-              const int col = (tile.n * kRagN + j * 64) * 2;
-              if (FORM == 1) tma_load_3d(sb + j * kRagK * 128, &tmap_b, full, col, kb * kRagK, tile.e);
-              else tma_load_2d(sb + j * kRagK * 128, &tmap_b, full, col, row0 + kb * kRagK);
-            }
+            for (int j = 0; j < BN / 64; ++j)
+              tma_load_3d(sb + j * kRagK * 128, &tmap_b, full, (tile.n * BN + j * 64) * 2, kb * kRagK, tile.e);
           }
         }
         __syncwarp();
-        if (++stage == kRagStages) { stage = 0; phase ^= 1; }
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    const uint32_t idesc = (a.bf16 ? kInstrDescBF16 : kInstrDescF16) | (kAMn ? 1u << 15 : 0u) | (kBMn ? 1u << 16 : 0u);
-    constexpr uint64_t a_step = kAMn ? (16 * 128) >> 4 : 2, b_step = kBMn ? (16 * 128) >> 4 : 2;
+    const uint32_t idesc = ((a.bf16 ? kInstrDescBF16 : kInstrDescF16) - kInstrDescShape) | uint32_t(BN >> 3) << 17 |
+                           uint32_t(128 >> 4) << 24 | (FORM != 0 ? 1u << 16 : 0u);
+    constexpr uint64_t b_step = FORM != 0 ? (16 * 128) >> 4 : 2;
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
-    RaggedTile tile;
     for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      int KB = (a.k_dim + kRagK - 1) / kRagK, seg = 0;
-      if (FORM == 2) {
-        tile.at(a, &ctrl->tab, t, FORM);
-        KB = k_blocks(tile.e);
-        seg = ctrl->tab.start[tile.e + 1] - ctrl->tab.start[tile.e];
-        if (KB == 0) continue;                   // the epilogue writes zeros on its own
-      }
       ok = warp_wait(smem_u32(&ctrl->acc_empty[acc]), acc_phase ^ 1, abort_flag, a.status, 2);
-      const uint32_t d_tmem = tmem_base + uint32_t(acc) * kRagN;
+      const uint32_t d_tmem = tmem_base + uint32_t(acc) * BN;
       for (int kb = 0; kb < KB && ok; ++kb) {
         ok = warp_wait(smem_u32(&ctrl->full[stage]), phase, abort_flag, a.status, 3);
         if (!ok) break;
-        uint8_t* sp = smem + size_t(stage) * kRagStageBytes;
-        int steps = kRagK / 16;
-        if (FORM == 2 && kb + 1 == KB && (seg & (kRagK - 1)) != 0) {
-          const int have = seg & (kRagK - 1);    // rows of this expert in the block
-          steps = (have + 15) / 16;
-          zero_block_rows(sp, (kRagM + kRagN) / 64, have, steps * 16 - have, lane);
-        }
-        const uint32_t sa = smem_u32(sp);
-        const uint64_t adesc = kAMn ? make_smem_desc_mn(sa, kRagK * 128) : make_smem_desc(sa);
-        const uint64_t bdesc = kBMn ? make_smem_desc_mn(sa + kABytes, kRagK * 128) : make_smem_desc(sa + kABytes);
+        const uint32_t sa = smem_u32(smem + size_t(stage) * kStageBytes);
+        const uint64_t adesc = make_smem_desc(sa);
+        const uint64_t bdesc = FORM != 0 ? make_smem_desc_mn(sa + kABytes, kRagK * 128) : make_smem_desc(sa + kABytes);
         tcgen05_fence_after();
         if (elect_one()) {
-          for (int k = 0; k < steps; ++k)
-            umma_f16(d_tmem, adesc + a_step * k, bdesc + b_step * k, idesc, (k > 0 || kb > 0) ? 1u : 0u);
+#pragma unroll
+          for (int k = 0; k < kRagK / 16; ++k)
+            umma_f16(d_tmem, adesc + uint64_t(2) * k, bdesc + b_step * k, idesc, (k > 0 || kb > 0) ? 1u : 0u);
           umma_commit(smem_u32(&ctrl->empty[stage]));
           if (kb + 1 == KB) umma_commit(smem_u32(&ctrl->acc_full[acc]));
         }
         __syncwarp();
-        if (++stage == kRagStages) { stage = 0; phase ^= 1; }
+        if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
-  } else if (warp >= 4) {
-    // ------------------------------------------------------------------ epilogue
+  } else if (warp >= 4 && warp < 4 + 4 * kWgs) {
+    // ------------------------------------------------------------------ epilogue: a thread per row and half of the columns
+    constexpr int kCols = BN / kWgs;
     const int wg = (warp - 4) >> 2;
     const int row = (warp & 3) * 32 + lane;
-    const uint32_t tcol = tmem_base + (uint32_t((warp & 3) * 32) << 16) + uint32_t(wg * 128);
+    const uint32_t tcol = tmem_base + (uint32_t((warp & 3) * 32) << 16) + uint32_t(wg * kCols);
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
     RaggedTile tile;
     for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      tile.at(a, &ctrl->tab, t, FORM);
-      const int e = tile.e, start = ctrl->tab.start[e], seg = ctrl->tab.start[e + 1] - start;
-      const bool none = FORM == 2 && seg == 0;
-      const int local = tile.m * kRagM + row;
-      const bool valid = FORM == 2 ? local < a.m_dim : local < seg;
-      const long long orow = FORM == 2 ? (long long)e * a.m_dim + local : (long long)start + local;
-      const int col0 = tile.n * kRagN + wg * 128;
-      uint8_t* op = static_cast<uint8_t*>(a.out) + (orow * a.n_dim + col0) * 2;
-      const int cols = valid ? a.n_dim - col0 : 0;             // a multiple of 8
-      if (none) {
-        for (int j = 0; j < min(cols, 128); j += 8) *reinterpret_cast<uint4*>(op + j * 2) = make_uint4(0, 0, 0, 0);
-        continue;
-      }
+      tile.at(a, tab, t, FORM);
+      const int r = tab->start[tile.e] + tile.m * TM + row;
+      const int col0 = tile.n * BN + wg * kCols;
+      uint8_t* op = static_cast<uint8_t*>(a.out) + ((long long)r * a.n_dim + col0) * 2;
+      const int cols = row < TM && r < tab->start[tile.e + 1] ? a.n_dim - col0 : 0;      // a multiple of 8
+      const bool any = __any_sync(0xffffffffu, cols > 0);
       ok = warp_wait(smem_u32(&ctrl->acc_full[acc]), acc_phase, abort_flag, a.status, 4);
       if (!ok) break;
       tcgen05_fence_after();
-      const uint32_t tc = tcol + uint32_t(acc) * kRagN;
+      const uint32_t tc = tcol + uint32_t(acc) * BN;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < kCols / 32; ++q) {
         float v[32];
-        tmem_ld_x32(tc + q * 32, reinterpret_cast<uint32_t*>(v));
-        tmem_ld_wait();
-        if (q == 3) {
+        if (any) {
+          tmem_ld_x32(tc + q * 32, reinterpret_cast<uint32_t*>(v));
+          tmem_ld_wait();
+        }
+        if (q + 1 == kCols / 32) {
           tcgen05_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&ctrl->acc_empty[acc]));
         }
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
+        for (int j = 0; j < 32; j += 8)
           if (q * 32 + j < cols) *reinterpret_cast<uint4*>(op + (q * 32 + j) * 2) = pack8(v + j, a.bf16);
-        }
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
-    if (FORM != 2 && a.zero_uncovered) zero_uncovered_rows(a, &ctrl->tab, threadIdx.x - 128, 256);
+    if (a.zero_uncovered) zero_uncovered_rows(a, tab, threadIdx.x - 128, 128 * kWgs);
   }
 
   tcgen05_fence_before();
   __syncthreads();
   if (warp == 1) {
     tcgen05_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(uint32_t(kTmemCols))
-                 : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(uint32_t(kTmem)) : "memory");
   }
 }
 
@@ -224,20 +207,50 @@ int ragged_map(CUtensorMap* map, const void* base, long long cols, long long row
   return make_map(map, base, mats > 0 ? 3 : 2, dims, strides, box);
 }
 
-template <int FORM>
-static int launch_ragged(const CUtensorMap& ma, const CUtensorMap& mb, const RaggedArgs& a, long long max_tiles,
-                         cudaStream_t stream) {
-  auto* kernel = grouped_gemm_kernel<FORM>;
+template <int FORM, int TM, int BN>
+static int launch_ragged(const void* x, const void* w, RaggedArgs a, int n, int k, cudaStream_t stream) {
+  a.n_tiles = ceil_div(a.n_dim, BN);
+  CUtensorMap ma, mb;
+  int rc = ragged_map(&ma, x, a.k_dim, a.rows, 0, TM);
+  if (rc == FLYMOE_OK) rc = ragged_map(&mb, w, k, n, a.experts, FORM == 1 ? kRagK : BN);
+  if (rc != FLYMOE_OK) return rc;
+  auto* kernel = grouped_gemm_kernel<FORM, TM, BN>;
+  constexpr size_t smem = rag_ring<TM, BN>() + sizeof(RaggedCtrl) + 1024;
   static SmemLimitSeen seen;
-  FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(kRagSmem), seen));
-  const long long sms = sm_count();
-  kernel<<<unsigned(max_tiles < sms ? max_tiles : sms), kRagThreads, kRagSmem, stream>>>(ma, mb, a);
+  FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(smem), seen));
+  const long long tiles = ((long long)a.rows / TM + std::min(a.rows, a.experts)) * a.n_tiles, sms = sm_count();
+  kernel<<<unsigned(std::min(tiles, sms)), kRagThreads, smem, stream>>>(ma, mb, a);
   FLYMOE_CUDA_CHECK(cudaGetLastError());
   return FLYMOE_OK;
 }
 
 static int envint(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
-static bool use_pairs(int rows, int experts) { return rows >= envint("PAIR", 128) * experts; }
+enum RaggedTileKind { kPairTile, kTile256, kTile128, kFew128, kFewNarrow };
+// Tile of forms 0 and 1, by estimated time.  Tiles: the rows an expert adds to the last one are half a tile on average.  A
+// CTA (or pair) spends on a K block what is longest of its MMAs, its bytes at 80 a cycle, and the latency of a request
+// (about 2600 cycles) shared by the ring; all CTAs together cannot be faster than HBM.
+static RaggedTileKind choose_tile(bool input_grad, int rows, int experts, int n_dim, int k_dim) {
+  int force = envint("TILE", -1);
+  if (force >= 0) return RaggedTileKind(force);
+  struct Kind { int tm, tn; double share, mma, bytes, stages, fixed, hbm; };
+  const double narrow = input_grad ? 64 : 32;    // columns across the contraction come 64 at a time
+  const Kind kinds[5] = {
+      {256, 256, 0.5, 512, 32768, 5, 3500, 1.15}, {128, 256, 1, 512, 49152, rag_stages<128, 256>(), 3000, 1.0},
+      {128, 128, 1, 256, 32768, rag_stages<128, 128>(), 2500, 1.02}, {32, 128, 1, 256, 20480, rag_stages<32, 128>(), 2500, 1.0},
+      {32, int(narrow), 1, 2.5 * narrow, (32 + narrow) * 128, input_grad ? rag_stages<32, 64>() : rag_stages<32, 32>(), 2500, 1.05}};
+  const double blocks = ceil_div(k_dim, kRagK), used = std::min(rows, experts), sms = sm_count();
+  const double hbm_cycles = 2.0 * (used * n_dim * k_dim + double(rows) * (double(n_dim) + k_dim)) * 2.9e-4;
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < 5; ++i) {
+    const Kind& q = kinds[i];
+    const double tiles = (double(rows) / q.tm + 0.5 * used) * ceil_div(n_dim, q.tn);
+    const double block = std::max({q.mma, q.bytes / 80, 2600 / q.stages});
+    const double cost = std::max(std::ceil(tiles / (sms * q.share)) * (blocks * block + q.fixed), hbm_cycles * q.hbm);
+    if (i == 0 || cost < least) { best = i; least = cost; }
+  }
+  return RaggedTileKind(best);
+}
 
 static int ragged_common(RaggedArgs* a, const char* what, const void* out, const void* p, const void* q,
                          const int32_t* offsets, int rows, int experts, int n, int k, int dtype) {
@@ -275,18 +288,19 @@ extern "C" int flymoe_grouped_gemm(void* out, const void* x, const void* w, cons
   if (rc != FLYMOE_OK || rows == 0) return rc;
   a.n_dim = input_grad ? k : n;
   a.k_dim = input_grad ? n : k;
-  a.n_tiles = ceil_div(a.n_dim, kRagN);
-  a.m_tiles = 0;
   a.zero_uncovered = zero_uncovered;
   a.group_m = 8;
-  const long long max_tiles = ((long long)rows / kRagM + experts) * a.n_tiles;
-  FLYMOE_REQUIRE(max_tiles < (1LL << 31), "grouped_gemm: too many tiles");
-  if (use_pairs(rows, experts)) return launch_ragged_pair(input_grad ? 1 : 0, x, w, a, n, k, static_cast<cudaStream_t>(stream));
-  CUtensorMap ma, mb;
-  if ((rc = ragged_map(&ma, x, a.k_dim, rows, 0, kRagM)) != FLYMOE_OK) return rc;
-  if ((rc = ragged_map(&mb, w, k, n, experts, input_grad ? kRagK : kRagN)) != FLYMOE_OK) return rc;
+  FLYMOE_REQUIRE(((long long)rows / 32 + experts) * ceil_div(a.n_dim, 32) < (1LL << 31), "grouped_gemm: too many tiles");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return input_grad ? launch_ragged<1>(ma, mb, a, max_tiles, s) : launch_ragged<0>(ma, mb, a, max_tiles, s);
+#define FLYMOE_RAGGED_CASE(TM, BN) input_grad ? launch_ragged<1, TM, BN>(x, w, a, n, k, s) : launch_ragged<0, TM, BN>(x, w, a, n, k, s)
+  switch (choose_tile(input_grad, rows, experts, a.n_dim, a.k_dim)) {
+    case kTile256: return FLYMOE_RAGGED_CASE(128, 256);
+    case kTile128: return FLYMOE_RAGGED_CASE(128, 128);
+    case kFew128: return FLYMOE_RAGGED_CASE(32, 128);
+    case kFewNarrow: return input_grad ? launch_ragged<1, 32, 64>(x, w, a, n, k, s) : launch_ragged<0, 32, 32>(x, w, a, n, k, s);
+    default: return launch_ragged_pair(input_grad ? 1 : 0, x, w, a, n, k, s);
+  }
+#undef FLYMOE_RAGGED_CASE
 }
 
 extern "C" int flymoe_grouped_gemm_wgrad(void* dw, const void* dy, const void* x, const int32_t* offsets, int rows,
@@ -303,14 +317,7 @@ extern "C" int flymoe_grouped_gemm_wgrad(void* dw, const void* dy, const void* x
   }
   a.m_dim = n;
   a.n_dim = k;
-  a.m_tiles = ceil_div(n, kRagM);
-  a.n_tiles = ceil_div(k, kRagN);
-  a.group_m = 8;
-  const long long max_tiles = (long long)experts * a.m_tiles * a.n_tiles;
-  FLYMOE_REQUIRE(max_tiles < (1LL << 31), "grouped_gemm_wgrad: too many tiles");
-  if (use_pairs(rows, experts)) return launch_ragged_pair(2, dy, x, a, n, k, s);
-  CUtensorMap ma, mb;
-  if ((rc = ragged_map(&ma, dy, n, rows, 0, kRagK)) != FLYMOE_OK) return rc;
-  if ((rc = ragged_map(&mb, x, k, rows, 0, kRagK)) != FLYMOE_OK) return rc;
-  return launch_ragged<2>(ma, mb, a, max_tiles, s);
+  a.group_m = envint("GM", 8);
+  FLYMOE_REQUIRE((long long)experts * ceil_div(n, 128) * ceil_div(k, 128) < (1LL << 31), "grouped_gemm_wgrad: too many tiles");
+  return launch_ragged_pair(2, dy, x, a, n, k, s);
 }
