@@ -81,6 +81,7 @@ _SIGNATURES = {
     "flymoe_blockscale_gemm": (c_int, [_P, _P, _P, c_int64, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int, _P]),
     "flymoe_set_gemm_cta_limit": (c_int, [c_int]),
     "flymoe_grouped_gemm": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
+    "flymoe_grouped_gemm_tile": (c_int, [c_int] * 5),
     "flymoe_grouped_gemm_wgrad": (c_int, [_P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
     "flymoe_topk_gating_softmax_backward": (c_int, [_P, c_int, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),
     "flymoe_route_tables": (c_int, [_P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),

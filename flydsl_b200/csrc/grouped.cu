@@ -17,7 +17,6 @@
 // tiles are narrow and the ring is deep: one expert of 4096 x 4096 with one row takes 33 us on 128-row tiles.
 #include <cuda.h>
 #include <stdio.h>
-#include <stdlib.h>
 
 #include <algorithm>
 #include <cmath>
@@ -30,10 +29,13 @@ namespace flymoe {
 
 constexpr int kRagThreads = 384;
 constexpr int kRagMaxStages = 24;
-template <int TM, int BN> constexpr int rag_stage_bytes() { return (TM + BN) * kRagK * 2; }
+constexpr int kRagStaging = 8 * 32 * 64;         // epilogue: 32 rows x 32 columns a warp
+// K blocks of 64 that share a stage: handing a stage over costs the issuing thread about as much as five MMAs.
+template <int TM> constexpr int rag_sub() { return TM == 128 ? 1 : 2; }
+template <int TM, int BN> constexpr int rag_stage_bytes() { return (TM + BN) * kRagK * 2 * rag_sub<TM>(); }
 // As many K blocks as fit beside the tables; behind the last one, what a 128-row read of a 32-row block reaches.
 template <int TM, int BN> constexpr int rag_stages() {
-  const int n = (232448 - 1024 - 9216 - (128 - TM) * kRagK * 2) / rag_stage_bytes<TM, BN>();
+  const int n = (232448 - 1024 - 9216 - kRagStaging - (128 - TM) * kRagK * 2) / rag_stage_bytes<TM, BN>();
   return n > kRagMaxStages ? kRagMaxStages : n;
 }
 
@@ -46,7 +48,7 @@ struct __align__(16) RaggedCtrl {
   RaggedTables tab;
 };
 template <int TM, int BN> constexpr size_t rag_ring() {
-  return size_t(rag_stages<TM, BN>()) * rag_stage_bytes<TM, BN>() + (128 - TM) * kRagK * 2;
+  return size_t(rag_stages<TM, BN>()) * rag_stage_bytes<TM, BN>() + (128 - TM) * kRagK * 2 + kRagStaging;
 }
 static_assert(sizeof(RaggedCtrl) <= 9216, "shared memory budget of one SM exceeded");
 
@@ -54,7 +56,8 @@ template <int FORM, int TM, int BN>
 __global__ void __launch_bounds__(kRagThreads, 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                     const RaggedArgs a) {
-  constexpr int kStages = rag_stages<TM, BN>(), kStageBytes = rag_stage_bytes<TM, BN>(), kABytes = TM * kRagK * 2;
+  constexpr int kStages = rag_stages<TM, BN>(), kStageBytes = rag_stage_bytes<TM, BN>();
+  constexpr int kSub = rag_sub<TM>(), kStageK = kRagK * kSub, kABytes = TM * kStageK * 2;
   constexpr int kTmem = 2 * BN < 32 ? 32 : 2 * BN;             // two accumulators
   constexpr int kWgs = BN >= 64 ? 2 : 1;                         // warpgroups of the epilogue that have columns
   static_assert(FORM == 0 || BN % 64 == 0, "columns across the contraction come 64 at a time");
@@ -88,92 +91,101 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   const uint32_t tmem_base = ctrl->tmem_base;
   const RaggedTables* tab = &ctrl->tab;
   const int total = tab->tile0[a.experts];
-  const int KB = (a.k_dim + kRagK - 1) / kRagK;
+  const int KB = (a.k_dim + kStageK - 1) / kStageK;
 
+  // Producer and issuer are one thread each, waits included: with a warp that waits together and elects a thread for every K
+  // block the issuer took 490 cycles a block, whatever the tile.
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    RaggedTile tile;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      tile.at(a, tab, t, FORM);
-      const int row0 = tab->start[tile.e] + tile.m * TM;
-      for (int kb = 0; kb < KB; ++kb) {
-        ok = warp_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag, a.status, 1, 32);
-        if (!ok) break;
-        const uint32_t full = smem_u32(&ctrl->full[stage]);
-        const uint32_t sa = smem_u32(smem + size_t(stage) * kStageBytes), sb = sa + kABytes;
-        if (elect_one()) {
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      RaggedTile tile;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        tile.at(a, tab, t, FORM);
+        const int row0 = tab->start[tile.e] + tile.m * TM;
+        for (int kb = 0; kb < KB; ++kb) {
+          ok = mbar_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag, a.status, 1, 32);
+          if (!ok) break;
+          const uint32_t full = smem_u32(&ctrl->full[stage]);
+          const uint32_t sa = smem_u32(smem + size_t(stage) * kStageBytes), sb = sa + kABytes;
           mbar_expect_tx(full, kStageBytes);
-          tma_load_2d(sa, &tmap_a, full, kb * kRagK * 2, row0);
-          if (FORM == 0) {
-            tma_load_3d(sb, &tmap_b, full, kb * kRagK * 2, tile.n * BN, tile.e);
-          } else {
+#pragma unroll
+          for (int h = 0; h < kSub; ++h) {
+            const int k = kb * kStageK + h * kRagK;
+            tma_load_2d(sa + h * TM * 128, &tmap_a, full, k * 2, row0);
+            if (FORM == 0) tma_load_3d(sb + h * BN * 128, &tmap_b, full, k * 2, tile.n * BN, tile.e);
+          }
+          if (FORM == 1) {
 #pragma unroll
             for (int j = 0; j < BN / 64; ++j)
-              tma_load_3d(sb + j * kRagK * 128, &tmap_b, full, (tile.n * BN + j * 64) * 2, kb * kRagK, tile.e);
+              tma_load_3d(sb + j * kStageK * 128, &tmap_b, full, (tile.n * BN + j * 64) * 2, kb * kStageK, tile.e);
           }
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
-        __syncwarp();
-        if (++stage == kStages) { stage = 0; phase ^= 1; }
       }
     }
+    __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
-    const uint32_t idesc = ((a.bf16 ? kInstrDescBF16 : kInstrDescF16) - kInstrDescShape) | uint32_t(BN >> 3) << 17 |
-                           uint32_t(128 >> 4) << 24 | (FORM != 0 ? 1u << 16 : 0u);
-    constexpr uint64_t b_step = FORM != 0 ? (16 * 128) >> 4 : 2;
-    int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-      ok = warp_wait(smem_u32(&ctrl->acc_empty[acc]), acc_phase ^ 1, abort_flag, a.status, 2);
-      const uint32_t d_tmem = tmem_base + uint32_t(acc) * BN;
-      for (int kb = 0; kb < KB && ok; ++kb) {
-        ok = warp_wait(smem_u32(&ctrl->full[stage]), phase, abort_flag, a.status, 3);
-        if (!ok) break;
-        const uint32_t sa = smem_u32(smem + size_t(stage) * kStageBytes);
-        const uint64_t adesc = make_smem_desc(sa);
-        const uint64_t bdesc = FORM != 0 ? make_smem_desc_mn(sa + kABytes, kRagK * 128) : make_smem_desc(sa + kABytes);
-        tcgen05_fence_after();
-        if (elect_one()) {
+    if (elect_one()) {
+      const uint32_t idesc = ((a.bf16 ? kInstrDescBF16 : kInstrDescF16) - kInstrDescShape) | uint32_t(BN >> 3) << 17 |
+                             uint32_t(128 >> 4) << 24 | (FORM != 0 ? 1u << 16 : 0u);
+      const uint32_t base = smem_u32(smem);
+      const uint64_t adesc0 = make_smem_desc(base);
+      const uint64_t bdesc0 = FORM != 0 ? make_smem_desc_mn(base + kABytes, kStageK * 128) : make_smem_desc(base + kABytes);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        ok = mbar_wait(smem_u32(&ctrl->acc_empty[acc]), acc_phase ^ 1, abort_flag, a.status, 2);
+        const uint32_t d_tmem = tmem_base + uint32_t(acc) * BN;
+        for (int kb = 0; kb < KB && ok; ++kb) {
+          ok = mbar_wait(smem_u32(&ctrl->full[stage]), phase, abort_flag, a.status, 3);
+          if (!ok) break;
+          const uint64_t at = uint64_t(stage * (kStageBytes >> 4));
+          tcgen05_fence_after();
 #pragma unroll
-          for (int k = 0; k < kRagK / 16; ++k)
-            umma_f16(d_tmem, adesc + uint64_t(2) * k, bdesc + b_step * k, idesc, (k > 0 || kb > 0) ? 1u : 0u);
+          for (int k = 0; k < kStageK / 16; ++k) {
+            const uint64_t ak = (k / 4) * (TM * 128 >> 4) + (k % 4) * 2;
+            const uint64_t bk = FORM != 0 ? k * (16 * 128 >> 4) : (k / 4) * (BN * 128 >> 4) + (k % 4) * 2;
+            umma_f16(d_tmem, adesc0 + at + ak, bdesc0 + at + bk, idesc, (k > 0 || kb > 0) ? 1u : 0u);
+          }
           umma_commit(smem_u32(&ctrl->empty[stage]));
           if (kb + 1 == KB) umma_commit(smem_u32(&ctrl->acc_full[acc]));
+          if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
-        __syncwarp();
-        if (++stage == kStages) { stage = 0; phase ^= 1; }
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
-      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
+    __syncwarp();
   } else if (warp >= 4 && warp < 4 + 4 * kWgs) {
-    // ------------------------------------------------------------------ epilogue: a thread per row and half of the columns
+    // ------------------------------------------------------------------ epilogue
+    // A thread has a row of the tile; 32 columns at a time go through the warp's staging area and leave four lanes a row, 64
+    // contiguous bytes.  Stored straight from the registers (16 bytes a row) a full 128 x 256 tile took as long as 30 K blocks.
     constexpr int kCols = BN / kWgs;
     const int wg = (warp - 4) >> 2;
-    const int row = (warp & 3) * 32 + lane;
     const uint32_t tcol = tmem_base + (uint32_t((warp & 3) * 32) << 16) + uint32_t(wg * kCols);
+    uint8_t* stg = smem + rag_ring<TM, BN>() - kRagStaging + (warp - 4) * 32 * 64;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
     RaggedTile tile;
     for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
       tile.at(a, tab, t, FORM);
-      const int r = tab->start[tile.e] + tile.m * TM + row;
-      const int col0 = tile.n * BN + wg * kCols;
-      uint8_t* op = static_cast<uint8_t*>(a.out) + ((long long)r * a.n_dim + col0) * 2;
-      const int cols = row < TM && r < tab->start[tile.e + 1] ? a.n_dim - col0 : 0;      // a multiple of 8
-      const bool any = __any_sync(0xffffffffu, cols > 0);
+      const int row0 = tab->start[tile.e] + tile.m * TM + (warp & 3) * 32;
+      const int rows = min(min(32, TM - (warp & 3) * 32), tab->start[tile.e + 1] - row0);      // this warp's, if positive
       ok = warp_wait(smem_u32(&ctrl->acc_full[acc]), acc_phase, abort_flag, a.status, 4);
       if (!ok) break;
       tcgen05_fence_after();
       const uint32_t tc = tcol + uint32_t(acc) * BN;
 #pragma unroll
       for (int q = 0; q < kCols / 32; ++q) {
+        const int col = tile.n * BN + wg * kCols + q * 32;
+        const bool wanted = rows > 0 && col < a.n_dim;
         float v[32];
-        if (any) {
+        if (wanted) {
           tmem_ld_x32(tc + q * 32, reinterpret_cast<uint32_t*>(v));
           tmem_ld_wait();
         }
@@ -182,9 +194,19 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&ctrl->acc_empty[acc]));
         }
+        if (!wanted) continue;
 #pragma unroll
-        for (int j = 0; j < 32; j += 8)
-          if (q * 32 + j < cols) *reinterpret_cast<uint4*>(op + (q * 32 + j) * 2) = pack8(v + j, a.bf16);
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<uint4*>(stg + lane * 64 + ((j ^ ((lane >> 1) & 3)) * 16)) = pack8(v + j * 8, a.bf16);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 8 + (lane >> 2), c = lane & 3;
+          if (r < rows && col + c * 8 < a.n_dim)
+            *reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.out) + ((long long)(row0 + r) * a.n_dim + col + c * 8) * 2) =
+                *reinterpret_cast<const uint4*>(stg + r * 64 + ((c ^ ((r >> 1) & 3)) * 16));
+        }
+        __syncwarp();
       }
       if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
@@ -212,7 +234,7 @@ static int launch_ragged(const void* x, const void* w, RaggedArgs a, int n, int 
   a.n_tiles = ceil_div(a.n_dim, BN);
   CUtensorMap ma, mb;
   int rc = ragged_map(&ma, x, a.k_dim, a.rows, 0, TM);
-  if (rc == FLYMOE_OK) rc = ragged_map(&mb, w, k, n, a.experts, FORM == 1 ? kRagK : BN);
+  if (rc == FLYMOE_OK) rc = ragged_map(&mb, w, k, n, a.experts, FORM == 1 ? kRagK * rag_sub<TM>() : BN);
   if (rc != FLYMOE_OK) return rc;
   auto* kernel = grouped_gemm_kernel<FORM, TM, BN>;
   constexpr size_t smem = rag_ring<TM, BN>() + sizeof(RaggedCtrl) + 1024;
@@ -224,29 +246,40 @@ static int launch_ragged(const void* x, const void* w, RaggedArgs a, int n, int 
   return FLYMOE_OK;
 }
 
-static int envint(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
 enum RaggedTileKind { kPairTile, kTile256, kTile128, kFew128, kFewNarrow };
-// Tile of forms 0 and 1, by estimated time.  Tiles: the rows an expert adds to the last one are half a tile on average.  A
-// CTA (or pair) spends on a K block what is longest of its MMAs, its bytes at 80 a cycle, and the latency of a request
-// (about 2600 cycles) shared by the ring; all CTAs together cannot be faster than HBM.
+// Row tiles that an expert with `mean` rows on average can be expected to have: the sum over j of the chance of more than
+// j * tm rows, spread as by even routing with experts that differ by a quarter of the mean besides.
+static double expected_tiles(double mean, int tm) {
+  const double sd = std::sqrt(mean + 0.0625 * mean * mean);
+  double sum = 1.0 - std::exp(-mean);
+  for (int j = 1; j < 64; ++j) {
+    const double p = 0.5 * std::erfc((j * double(tm) + 0.5 - mean) / (sd * 1.4142135623730951));
+    if (p < 1e-4) return sum;
+    sum += p;
+  }
+  return mean / tm + 0.5;
+}
+// Tile of forms 0 and 1, by estimated cycles.  A K block costs what is longest of its MMAs (with the issuing thread's work)
+// and its bytes at 70 to 77 a cycle; that and the time on HBM hide each other only in part (root of the sum of squares).
+// Over 154 sizes (1 to 64 experts, 1 to 700 rows each, even and skewed) both forms took 1.014 of the time of the best kind
+// on geometric mean, 1.35 at worst (16 experts of 1048 x 2104, whose rows are not aligned to 128 bytes).  A fixed kind costs
+// more: pairs for one row on one expert of 4096 x 4096 23 us against 13, 128 x 256 tiles for 8 experts of 2048 x 2048 with 40
+// rows 16 against 11, 32-row tiles for 32 experts of 4096 x 7168 with 160 rows 1343 against 382.
 static RaggedTileKind choose_tile(bool input_grad, int rows, int experts, int n_dim, int k_dim) {
-  int force = envint("TILE", -1);
-  if (force >= 0) return RaggedTileKind(force);
-  struct Kind { int tm, tn; double share, mma, bytes, stages, fixed, hbm; };
-  const double narrow = input_grad ? 64 : 32;    // columns across the contraction come 64 at a time
-  const Kind kinds[5] = {
-      {256, 256, 0.5, 512, 32768, 5, 3500, 1.15}, {128, 256, 1, 512, 49152, rag_stages<128, 256>(), 3000, 1.0},
-      {128, 128, 1, 256, 32768, rag_stages<128, 128>(), 2500, 1.02}, {32, 128, 1, 256, 20480, rag_stages<32, 128>(), 2500, 1.0},
-      {32, int(narrow), 1, 2.5 * narrow, (32 + narrow) * 128, input_grad ? rag_stages<32, 64>() : rag_stages<32, 32>(), 2500, 1.05}};
-  const double blocks = ceil_div(k_dim, kRagK), used = std::min(rows, experts), sms = sm_count();
+  const int narrow = input_grad ? 64 : 32;       // columns across the contraction come 64 at a time
+  struct Kind { int tm, tn, per_sm_x2, block, launch; double hbm; };
+  const Kind kinds[5] = {{256, 256, 1, 540, 9700, 1.15}, {128, 256, 2, 720, 8100, 1.0}, {128, 128, 2, 425, 7400, 1.03},
+                         {32, 128, 2, 310, 7400, 1.0}, {32, narrow, 2, 250, 6400, 1.1}};
+  const double blocks = ceil_div(k_dim, kRagK), used = std::min(rows, experts);
   const double hbm_cycles = 2.0 * (used * n_dim * k_dim + double(rows) * (double(n_dim) + k_dim)) * 2.9e-4;
   int best = 0;
   double least = 0;
   for (int i = 0; i < 5; ++i) {
     const Kind& q = kinds[i];
-    const double tiles = (double(rows) / q.tm + 0.5 * used) * ceil_div(n_dim, q.tn);
-    const double block = std::max({q.mma, q.bytes / 80, 2600 / q.stages});
-    const double cost = std::max(std::ceil(tiles / (sms * q.share)) * (blocks * block + q.fixed), hbm_cycles * q.hbm);
+    const double tiles = std::max(1.0, experts * expected_tiles(double(rows) / experts, q.tm)) * ceil_div(n_dim, q.tn);
+    const double waves = std::ceil(tiles / (0.5 * sm_count() * q.per_sm_x2));
+    const double work = waves * (blocks * q.block + 400), wire = hbm_cycles * q.hbm;
+    const double cost = q.launch + std::sqrt(work * work + wire * wire);
     if (i == 0 || cost < least) { best = i; least = cost; }
   }
   return RaggedTileKind(best);
@@ -303,6 +336,12 @@ extern "C" int flymoe_grouped_gemm(void* out, const void* x, const void* w, cons
 #undef FLYMOE_RAGGED_CASE
 }
 
+extern "C" int flymoe_grouped_gemm_tile(int rows, int experts, int n, int k, int input_grad) {
+  using namespace flymoe;
+  if (rows < 1 || experts < 1 || n < 8 || k < 8) return -1;
+  return choose_tile(input_grad != 0, rows, experts, input_grad ? k : n, input_grad ? n : k);
+}
+
 extern "C" int flymoe_grouped_gemm_wgrad(void* dw, const void* dy, const void* x, const int32_t* offsets, int rows,
                                          int experts, int n, int k, int dtype, void* stream) {
   using namespace flymoe;
@@ -317,7 +356,7 @@ extern "C" int flymoe_grouped_gemm_wgrad(void* dw, const void* dy, const void* x
   }
   a.m_dim = n;
   a.n_dim = k;
-  a.group_m = envint("GM", 8);
+  a.group_m = 8;
   FLYMOE_REQUIRE((long long)experts * ceil_div(n, 128) * ceil_div(k, 128) < (1LL << 31), "grouped_gemm_wgrad: too many tiles");
   return launch_ragged_pair(2, dy, x, a, n, k, s);
 }

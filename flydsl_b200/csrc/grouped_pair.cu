@@ -101,101 +101,101 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
   const int k_blocks = (a.k_dim + kRagK - 1) / kRagK;
   auto rows_of = [&](int e) { return tab->start[e + 1] - tab->start[e]; };
 
+  // Producer and issuer are one thread each, waits included (see grouped.cu).
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
-    int stage = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    RaggedTile tile;
-    for (int t = first; t < total && ok; t += step) {
-      tile.at(a, tab, t, FORM);
-      const int seg = rows_of(tile.e), row0 = tab->start[tile.e];
-      const int KB = FORM == 2 ? (seg + kRagK - 1) / kRagK : k_blocks;
-      for (int kb = 0; kb < KB; ++kb) {
-        ok = warp_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag, a.status, 1, 32);
-        if (!ok) break;
-        const uint32_t sa = smem_u32(smem + size_t(stage) * kRpStageBytes), sb = sa + kRpHalf;
-        const int rest = seg & (kRagK - 1);
-        const bool tail = FORM == 2 && kb + 1 == KB && rest != 0;
-        if (elect_one()) {
+    if (elect_one()) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      RaggedTile tile;
+      for (int t = first; t < total && ok; t += step) {
+        tile.at(a, tab, t, FORM);
+        const int seg = rows_of(tile.e), row0 = tab->start[tile.e], rest = seg & (kRagK - 1);
+        const int KB = FORM == 2 ? (seg + kRagK - 1) / kRagK : k_blocks;
+        for (int kb = 0; kb < KB; ++kb) {
+          ok = mbar_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag, a.status, 1, 32);
+          if (!ok) break;
+          const uint32_t sa = smem_u32(smem + size_t(stage) * kRpStageBytes), sb = sa + kRpHalf;
+          const bool tail = FORM == 2 && kb + 1 == KB && rest != 0;
           // the leader announces the bytes of both CTAs; the other's may land before that
           const uint32_t bar = map_to_rank(smem_u32(&ctrl->full[stage]), 0);
           if (rank == 0)
             mbar_expect_tx(smem_u32(&ctrl->full[stage]), 2 * (tail ? (rest + 15) / 16 * 16 * 4 * 128 : kRpStageBytes));
+          const int acol = (tile.m * kRpTile + rank * 128) * 2, bcol = (tile.n * kRpTile + rank * 128) * 2;
           if (tail) {
             for (int j = 0; j < 2; ++j) {
-              load_tail(sa + j * kRagK * 128, tails.a, bar, (tile.m * kRpTile + rank * 128 + j * 64) * 2, row0 + kb * kRagK, rest, a.rows);
-              load_tail(sb + j * kRagK * 128, tails.b, bar, (tile.n * kRpTile + rank * 128 + j * 64) * 2, row0 + kb * kRagK, rest, a.rows);
+              load_tail(sa + j * kRagK * 128, tails.a, bar, acol + j * 128, row0 + kb * kRagK, rest, a.rows);
+              load_tail(sb + j * kRagK * 128, tails.b, bar, bcol + j * 128, row0 + kb * kRagK, rest, a.rows);
+            }
+          } else if (FORM == 2) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              tma_load_2d_pair(sa + j * kRagK * 128, &tmap_a, bar, acol + j * 128, row0 + kb * kRagK);
+              tma_load_2d_pair(sb + j * kRagK * 128, &tmap_b, bar, bcol + j * 128, row0 + kb * kRagK);
             }
           } else {
-            if (FORM == 2) {
-#pragma unroll
-              for (int j = 0; j < 2; ++j)
-                tma_load_2d_pair(sa + j * kRagK * 128, &tmap_a, bar, (tile.m * kRpTile + rank * 128 + j * 64) * 2, row0 + kb * kRagK);
-            } else {
-              tma_load_2d_pair(sa, &tmap_a, bar, kb * kRagK * 2, row0 + tile.m * kRpTile + rank * 128);
-            }
+            tma_load_2d_pair(sa, &tmap_a, bar, kb * kRagK * 2, row0 + tile.m * kRpTile + rank * 128);
             if (FORM == 0) {
               tma_load_3d_pair(sb, &tmap_b, bar, kb * kRagK * 2, tile.n * kRpTile + rank * 128, tile.e);
             } else {
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                const int col = (tile.n * kRpTile + rank * 128 + j * 64) * 2;
-                if (FORM == 1) tma_load_3d_pair(sb + j * kRagK * 128, &tmap_b, bar, col, kb * kRagK, tile.e);
-                else tma_load_2d_pair(sb + j * kRagK * 128, &tmap_b, bar, col, row0 + kb * kRagK);
-              }
+              for (int j = 0; j < 2; ++j) tma_load_3d_pair(sb + j * kRagK * 128, &tmap_b, bar, bcol + j * 128, kb * kRagK, tile.e);
             }
           }
+          if (++stage == kRpStages) { stage = 0; phase ^= 1; }
         }
-        __syncwarp();
+      }
+      // the last releases of the ring are the leader's MMAs arriving in both CTAs: they have to land before this CTA's shared
+      // memory goes away
+      for (int i = 0; i < kRpStages && ok; ++i) {
+        ok = mbar_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag, a.status, 1, 32);
         if (++stage == kRpStages) { stage = 0; phase ^= 1; }
       }
     }
-    // the last releases of the ring are the leader's MMAs arriving in both CTAs: they have to land before this CTA's shared
-    // memory goes away
-    for (int i = 0; i < kRpStages && ok; ++i) {
-      ok = warp_wait(smem_u32(&ctrl->empty[stage]), phase ^ 1, abort_flag, a.status, 1, 32);
-      if (++stage == kRpStages) { stage = 0; phase ^= 1; }
-    }
+    __syncwarp();
   } else if (warp == 1 && rank == 0) {
     // ------------------------------------------------------------------ MMA issuer
-    const uint32_t idesc = ((a.bf16 ? kInstrDescBF16 : kInstrDescF16) - kInstrDescShape) | uint32_t(kRpTile >> 3) << 17 |
-                           uint32_t(kRpTile >> 4) << 24 | (kAMn ? 1u << 15 : 0u) | (kBMn ? 1u << 16 : 0u);
-    constexpr uint64_t a_step = kAMn ? (16 * 128) >> 4 : 2, b_step = kBMn ? (16 * 128) >> 4 : 2;
-    int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    bool ok = true;
-    RaggedTile tile;
-    for (int t = first; t < total && ok; t += step) {
-      int KB = k_blocks, seg = 0;
-      if (FORM == 2) {
-        tile.at(a, tab, t, FORM);
-        seg = rows_of(tile.e);
-        KB = (seg + kRagK - 1) / kRagK;
-        if (KB == 0) continue;                   // the epilogue writes zeros on its own
-      }
-      ok = warp_wait(smem_u32(&ctrl->acc_empty[acc]), acc_phase ^ 1, abort_flag, a.status, 2);
-      const uint32_t d_tmem = tmem_base + uint32_t(acc) * kRpTile;
-      for (int kb = 0; kb < KB && ok; ++kb) {
-        ok = __all_sync(0xffffffffu, mbar_wait_cluster(smem_u32(&ctrl->full[stage]), phase, abort_flag, a.status, 3));
-        if (!ok) break;
-        const uint32_t sa = smem_u32(smem + size_t(stage) * kRpStageBytes);
-        const uint64_t adesc = kAMn ? make_smem_desc_mn(sa, kRagK * 128) : make_smem_desc(sa);
-        const uint64_t bdesc = kBMn ? make_smem_desc_mn(sa + kRpHalf, kRagK * 128) : make_smem_desc(sa + kRpHalf);
-        const int rest = seg & (kRagK - 1);
-        const int steps = FORM == 2 && kb + 1 == KB && rest != 0 ? (rest + 15) / 16 : kRagK / 16;
-        tcgen05_fence_after();
-        if (elect_one()) {
-          for (int k = 0; k < steps; ++k)
-            umma_pair<2>(d_tmem, adesc + a_step * k, bdesc + b_step * k, idesc, (k > 0 || kb > 0) ? 1u : 0u);
+    if (elect_one()) {
+      const uint32_t idesc = ((a.bf16 ? kInstrDescBF16 : kInstrDescF16) - kInstrDescShape) | uint32_t(kRpTile >> 3) << 17 |
+                             uint32_t(kRpTile >> 4) << 24 | (kAMn ? 1u << 15 : 0u) | (kBMn ? 1u << 16 : 0u);
+      constexpr uint64_t a_step = kAMn ? (16 * 128) >> 4 : 2, b_step = kBMn ? (16 * 128) >> 4 : 2;
+      const uint32_t base = smem_u32(smem);
+      const uint64_t adesc0 = kAMn ? make_smem_desc_mn(base, kRagK * 128) : make_smem_desc(base);
+      const uint64_t bdesc0 = kBMn ? make_smem_desc_mn(base + kRpHalf, kRagK * 128) : make_smem_desc(base + kRpHalf);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      RaggedTile tile;
+      for (int t = first; t < total && ok; t += step) {
+        int KB = k_blocks, rest = 0;
+        if (FORM == 2) {
+          tile.at(a, tab, t, FORM);
+          const int seg = rows_of(tile.e);
+          KB = (seg + kRagK - 1) / kRagK;
+          rest = seg & (kRagK - 1);
+          if (KB == 0) continue;                 // the epilogue writes zeros on its own
+        }
+        ok = mbar_wait(smem_u32(&ctrl->acc_empty[acc]), acc_phase ^ 1, abort_flag, a.status, 2);
+        const uint32_t d_tmem = tmem_base + uint32_t(acc) * kRpTile;
+        for (int kb = 0; kb < KB && ok; ++kb) {
+          ok = mbar_wait_cluster(smem_u32(&ctrl->full[stage]), phase, abort_flag, a.status, 3);
+          if (!ok) break;
+          const uint64_t at = uint64_t(stage * (kRpStageBytes >> 4));
+          const int steps = FORM == 2 && kb + 1 == KB && rest != 0 ? (rest + 15) / 16 : kRagK / 16;
+          tcgen05_fence_after();
+#pragma unroll
+          for (int k = 0; k < kRagK / 16; ++k)
+            if (FORM != 2 || k < steps)
+              umma_pair<2>(d_tmem, adesc0 + at + a_step * k, bdesc0 + at + b_step * k, idesc, (k > 0 || kb > 0) ? 1u : 0u);
           umma_commit_pair(smem_u32(&ctrl->empty[stage]));
           if (kb + 1 == KB) umma_commit_pair(smem_u32(&ctrl->acc_full[acc]));
+          if (++stage == kRpStages) { stage = 0; phase ^= 1; }
         }
-        __syncwarp();
-        if (++stage == kRpStages) { stage = 0; phase ^= 1; }
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
-      if (++acc == 2) { acc = 0; acc_phase ^= 1; }
     }
+    __syncwarp();
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ epilogue
     const int wg = (warp - 4) >> 2, tid = threadIdx.x - 128 - wg * 128;

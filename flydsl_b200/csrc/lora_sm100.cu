@@ -85,51 +85,50 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
   const int blocks = (p.k + 63) / 64;
   const int kb0 = int((long long)blocks * blockIdx.y / p.splits), kb1 = int((long long)blocks * (blockIdx.y + 1) / p.splits);
 
+  // Producer and issuer are one thread each, waits included: a warp that waits together and elects a thread for every block
+  // takes twice as long per block.
   if (warp == 0 && d > 0) {
     // ------------------------------------------------------------------ TMA producer
-    int xs = 0, as = 0;
-    uint32_t xp = 0, ap = 0;
-    bool ok = true;
-    for (int kb = kb0; kb < kb1 && ok; ++kb) {
-      ok = warp_wait(smem_u32(&c->x_empty[xs]), xp ^ 1, abort_flag, q.status, 1, 32);
-      if (!ok) break;
-      if (elect_one()) {
+    if (elect_one()) {
+      int xs = 0, as = 0;
+      uint32_t xp = 0, ap = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+        ok = mbar_wait(smem_u32(&c->x_empty[xs]), xp ^ 1, abort_flag, q.status, 1, 32);
+        if (!ok) break;
         mbar_expect_tx(smem_u32(&c->x_full[xs]), kChunkBytes);
         tma_load_2d(smem_u32(smem + xs * kChunkBytes), &tmap_x, smem_u32(&c->x_full[xs]), kb * 128, row0);
-      }
-      __syncwarp();
-      if (++xs == kShX) { xs = 0; xp ^= 1; }
-      for (int i = 0; i < d; ++i) {
-        ok = warp_wait(smem_u32(&c->a_empty[as]), ap ^ 1, abort_flag, q.status, 1, 32);
-        if (!ok) break;
-        if (elect_one()) {
-          mbar_expect_tx(smem_u32(&c->a_full[as]), a_bytes);
+        if (++xs == kShX) { xs = 0; xp ^= 1; }
+        for (int i = 0; i < d; ++i) {
+          ok = mbar_wait(smem_u32(&c->a_empty[as]), ap ^ 1, abort_flag, q.status, 1, 32);
+          if (!ok) break;
           const uint32_t dst = smem_u32(aring + as * a_bytes), full = smem_u32(&c->a_full[as]);
+          mbar_expect_tx(full, a_bytes);
           if (!p.transposed) tma_load_3d(dst, &tmap_a, full, kb * 128, 0, c->list[i]);
           else
             for (int j = 0; j < a_bytes; j += 8192) tma_load_3d(dst + j, &tmap_a, full, j / 64, kb * 64, c->list[i]);
+          if (++as == q.slots) { as = 0; ap ^= 1; }
         }
-        __syncwarp();
-        if (++as == q.slots) { as = 0; ap ^= 1; }
       }
     }
+    __syncwarp();
   } else if (warp == 1 && d > 0) {
     // ------------------------------------------------------------------ MMA issuer
-    const uint32_t idesc = instr_desc(q.bf16, q.rank_pad) | (p.transposed ? 1u << 16 : 0u);
-    const uint64_t b_step = p.transposed ? 16 * 128 / 16 : 2;
-    int xs = 0, as = 0;
-    uint32_t xp = 0, ap = 0;
-    bool ok = true;
-    for (int kb = kb0; kb < kb1 && ok; ++kb) {
-      ok = warp_wait(smem_u32(&c->x_full[xs]), xp, abort_flag, q.status, 3);
-      const uint64_t adesc = make_smem_desc(smem_u32(smem + xs * kChunkBytes));
-      for (int i = 0; i < d && ok; ++i) {
-        ok = warp_wait(smem_u32(&c->a_full[as]), ap, abort_flag, q.status, 3);
-        if (!ok) break;
-        const uint32_t at = smem_u32(aring + as * a_bytes);
-        const uint64_t bdesc = p.transposed ? make_smem_desc_mn(at, 8192) : make_smem_desc(at);
-        tcgen05_fence_after();
-        if (elect_one()) {
+    if (elect_one()) {
+      const uint32_t idesc = instr_desc(q.bf16, q.rank_pad) | (p.transposed ? 1u << 16 : 0u);
+      const uint64_t b_step = p.transposed ? 16 * 128 / 16 : 2;
+      int xs = 0, as = 0;
+      uint32_t xp = 0, ap = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1 && ok; ++kb) {
+        ok = mbar_wait(smem_u32(&c->x_full[xs]), xp, abort_flag, q.status, 3);
+        const uint64_t adesc = make_smem_desc(smem_u32(smem + xs * kChunkBytes));
+        for (int i = 0; i < d && ok; ++i) {
+          ok = mbar_wait(smem_u32(&c->a_full[as]), ap, abort_flag, q.status, 3);
+          if (!ok) break;
+          const uint32_t at = smem_u32(aring + as * a_bytes);
+          const uint64_t bdesc = p.transposed ? make_smem_desc_mn(at, 8192) : make_smem_desc(at);
+          tcgen05_fence_after();
 #pragma unroll
           for (int k = 0; k < 4; ++k)
             umma_f16(tmem + i * q.rank_pad, adesc + k * 2, bdesc + k * b_step, idesc, (k > 0 || kb > kb0) ? 1u : 0u);
@@ -138,12 +137,12 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
             umma_commit(smem_u32(&c->x_empty[xs]));
             if (kb + 1 == kb1) umma_commit(smem_u32(&c->acc_full));
           }
+          if (++as == q.slots) { as = 0; ap ^= 1; }
         }
-        __syncwarp();
-        if (++as == q.slots) { as = 0; ap ^= 1; }
+        if (++xs == kShX) { xs = 0; xp ^= 1; }
       }
-      if (++xs == kShX) { xs = 0; xp ^= 1; }
     }
+    __syncwarp();
   } else if (warp >= 4 && d > 0) {
     // ------------------------------------------------------------------ epilogue: a thread per row
     const int i = threadIdx.x - 128, mine = row_adapter(p.ids, row0 + i, p.rows, p.adapters);

@@ -331,6 +331,9 @@ int flymoe_moe_layer(const flymoe_layer_args* args, void* stream);
  * (kernels/moe_gemm_2stage.py:90-108, :1780-1796) take padded row blocks and have no gradients. */
 int flymoe_grouped_gemm(void* out, const void* x, const void* w, const int32_t* offsets, int rows, int experts, int n,
                         int k, int dtype, int input_grad, int zero_uncovered, void* stream);
+/* Which kernel flymoe_grouped_gemm takes for these sizes: 0 CTA pairs with 256 x 256 tiles, 1 tiles of 128 x 256, 2 of 128 x
+ * 128, 3 of 32 x 128, 4 of 32 rows x 32 (input_grad: 64) columns.  A host-only query, for tests. */
+int flymoe_grouped_gemm_tile(int rows, int experts, int n, int k, int input_grad);
 int flymoe_grouped_gemm_wgrad(void* dw, const void* dy, const void* x, const int32_t* offsets, int rows, int experts, int n,
                               int k, int dtype, void* stream);
 

@@ -64,6 +64,26 @@ def test_forms_against_64_bits(counts, k, n, front, behind, dtype):
     check(grouped_gemm_wgrad(dy, x, off), (dw, dws), max(counts), "dw")
 
 
+# (rows per expert, k, n) and the kernels that they take, forward and for the input gradient
+KINDS = [
+    ([1024, 700, 1300, 1100], 2048, 2048, 0, 0), ([130, 100, 150, 90, 0] * 5, 1000, 1032, 1, 1),
+    ([80, 100, 129, 90, 0] * 5, 1544, 1032, 1, 2), ([100, 120] * 10, 264, 1800, 2, 2),
+    ([5, 33, 0, 64, 31, 32] * 2, 520, 1544, 3, 4), ([1, 2], 2048, 1048, 4, 4),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("counts,k,n,forward,backward", KINDS)
+def test_every_kernel(lib, counts, k, n, forward, backward, dtype):
+    rows, e = sum(counts), len(counts)
+    kinds = tuple(lib.flymoe_grouped_gemm_tile(rows, e, n, k, g) for g in (0, 1))
+    assert kinds == (forward, backward)
+    x, w, dy, off = make(counts, k, n, dtype, 0, 40)
+    (y, ys), (dx, dxs), _ = exact(x, w, dy, off)
+    check(grouped_gemm(x, w, off), (y, ys), k, "y")
+    check(grouped_gemm_dgrad(dy, w, off), (dx, dxs), n, "dx")
+
+
 @pytest.mark.parametrize("experts", [1, 1024])
 def test_no_rows(experts):
     w = torch.randn((experts, 64, 72), device="cuda").to(BF)
