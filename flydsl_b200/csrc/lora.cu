@@ -223,14 +223,14 @@ lora_shrink_kernel(const ShrinkArgs p, const int slots, const bool skip_tiles) {
   }
 }
 
-// The splits' sums added up into the first, in their order.
+// The splits' sums added up, in their order.
 __global__ void __launch_bounds__(256)
-lora_fold_kernel(float4* __restrict__ v, long long vecs, int splits) {
+lora_fold_kernel(const float4* __restrict__ planes, float4* __restrict__ v, long long vecs, int splits) {
   after_previous_launch();
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < vecs; i += (long long)gridDim.x * 256) {
-    float4 sum = v[i];
+    float4 sum = __ldg(planes + i);
     for (int s = 1; s < splits; ++s) {
-      const float4 x = v[s * vecs + i];
+      const float4 x = __ldg(planes + s * vecs + i);
       sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
     }
     v[i] = sum;
@@ -762,33 +762,49 @@ static int launch_wgrad_rank(const AdapterGradArgs& p, cudaStream_t s) {
   return p.rank <= 16 ? launch_wgrad<T, 2>(p, s) : p.rank <= 32 ? launch_wgrad<T, 4>(p, s) : launch_wgrad<T, 8>(p, s);
 }
 
-// v = x A^T for all rows.  a_t: A transposed ([adapters, k, rank]), if that is what there is; then `a` is its other form
-// where the rows may need the kernels of this file (needs_both), else null.
-static int shrink(ShrinkArgs p, const void* a_t, bool fold, int dtype, cudaStream_t s) {
-  const bool bf = dtype == FLYMOE_BF16, tiles = on_tiles(p.rows);
+// Floats of v: the sum and, where there are several, the splits behind it.
+static long long v_elems(int rows, int splits, int rank) { return (splits > 1 ? splits + 1LL : 1LL) * rows * rank; }
+
+// One product with the adapters and back: out = base + scaling * (x A^T) B^T, or with a_t / b_t (then `a` and `b` are only
+// read where needs_transposed) for A and B given the other way round.  v: v_elems() floats; `keep`: its first rows * rank
+// hold x A^T afterwards.
+struct Chain {
+  const void *x, *a, *a_t, *base, *b, *b_t;
+  void* out;                   // null: only x A^T
+  float* v;
+  const int* ids;
+  const float* scaling;
+  int rows, k, n, rank, adapters, dtype;
+  bool keep;
+};
+static int run_chain(const Chain& c, cudaStream_t s) {
+  const bool bf = c.dtype == FLYMOE_BF16, tiles = on_tiles(c.rows), others = !tiles || c.adapters > kTileAdapters;
+  const int splits = shrink_splits(c.rows, c.k);
+  float* planes = splits > 1 ? c.v + (long long)c.rows * c.rank : c.v;
+  ShrinkArgs sh = {c.x, c.a, c.ids, planes, c.rows, c.k, c.rank, c.adapters, splits, 0};
   int rc = FLYMOE_OK;
-  if (tiles) {
-    ShrinkArgs q = p;
-    if (a_t) { q.a = a_t; q.transposed = 1; }
-    rc = launch_shrink_sm100(q, bf, s);
+  if (others) rc = bf ? launch_shrink_rank<__nv_bfloat16>(sh, tiles, s) : launch_shrink_rank<__half>(sh, tiles, s);
+  if (rc == FLYMOE_OK && tiles) {
+    if (c.a_t) { sh.a = c.a_t; sh.transposed = 1; }
+    rc = launch_shrink_sm100(sh, bf, s);
   }
-  if (rc == FLYMOE_OK && (!tiles || p.adapters > kTileAdapters))
-    rc = bf ? launch_shrink_rank<__nv_bfloat16>(p, tiles, s) : launch_shrink_rank<__half>(p, tiles, s);
-  if (rc != FLYMOE_OK || !fold || p.splits == 1) return rc;
-  const long long vecs = (long long)p.rows * p.rank / 4;
-  FLYMOE_CUDA_CHECK(launch_closely(lora_fold_kernel, unsigned(std::min<long long>((vecs + 255) / 256, 4LL * sm_count())), 256, 0, s,
-                                   reinterpret_cast<float4*>(p.v), vecs, p.splits));
-  return FLYMOE_OK;
-}
-static int expand(ExpandArgs p, const void* b_t, int dtype, cudaStream_t s) {
-  const bool bf = dtype == FLYMOE_BF16, tiles = on_tiles(p.rows);
-  if (tiles) {
-    ExpandArgs q = p;
-    if (b_t) { q.b = b_t; q.transposed = 1; }
-    const int rc = launch_expand_sm100(q, bf, s);
-    if (rc != FLYMOE_OK || p.adapters <= kTileAdapters) return rc;
+  if (rc != FLYMOE_OK) return rc;
+  // tiles read a row's v once for every block that works on it, and the gradient wants it whole: one sum, not several
+  const bool fold = splits > 1 && (tiles || c.keep);
+  if (fold) {
+    const long long vecs = (long long)c.rows * c.rank / 4;
+    FLYMOE_CUDA_CHECK(launch_closely(lora_fold_kernel, unsigned(std::min<long long>((vecs + 255) / 256, 4LL * sm_count())), 256, 0, s,
+                                     reinterpret_cast<const float4*>(planes), reinterpret_cast<float4*>(c.v), vecs, splits));
   }
-  return bf ? launch_expand_rank<__nv_bfloat16>(p, tiles, s) : launch_expand_rank<__half>(p, tiles, s);
+  if (!c.out) return FLYMOE_OK;
+  ExpandArgs ex = {c.base, fold ? c.v : planes, c.b, c.ids, c.scaling, c.out, c.rows, c.n, c.rank, c.adapters,
+                   fold ? 1 : splits, 0};
+  if (others) rc = bf ? launch_expand_rank<__nv_bfloat16>(ex, tiles, s) : launch_expand_rank<__half>(ex, tiles, s);
+  if (rc == FLYMOE_OK && tiles) {
+    if (c.b_t) { ex.b = c.b_t; ex.transposed = 1; }
+    rc = launch_expand_sm100(ex, bf, s);
+  }
+  return rc;
 }
 // Whether a backward pass reads A and B through the kernels of this file, which want the contraction along a row.
 static bool needs_transposed(int rows, int adapters) { return !on_tiles(rows) || adapters > kTileAdapters; }
@@ -814,7 +830,7 @@ static BackwardScratch backward_scratch(int rows, int k, int n, int rank, int ad
   const bool both = needs_transposed(rows, adapters);
   const long long weights = (long long)adapters * rank;
   w.dv = 0;
-  w.a_t = up4((long long)w.dv_splits * rows * rank);
+  w.a_t = up4(v_elems(rows, w.dv_splits, rank));
   w.b_t = w.a_t + (both ? up4(weights * k / 2) : 0);
   w.partial = w.b_t + (both ? up4(weights * n / 2) : 0);
   w.total = w.partial + (w.splits > 1 ? up4((long long)w.splits * adapters * ((long long)rank * ((long long)k + n) + 1)) : 0);
@@ -825,11 +841,11 @@ static BackwardScratch backward_scratch(int rows, int k, int n, int rank, int ad
 
 extern "C" int64_t flymoe_lora_v_elems(int rows, int k, int rank) {
   if (rows < 1 || k < 8 || rank < 8) return 0;
-  return (int64_t)flymoe::shrink_splits(rows, k) * rows * rank;
+  return flymoe::v_elems(rows, flymoe::shrink_splits(rows, k), rank);
 }
 
 extern "C" int flymoe_lora_add(void* out, const void* base, const void* x, const void* a, const void* b, const int32_t* ids,
-                               const float* scaling, float* v, int64_t v_elems, int rows, int k, int n, int rank, int adapters,
+                               const float* scaling, float* v, int64_t v_floats, int rows, int k, int n, int rank, int adapters,
                                int keep_v, int dtype, void* stream) {
   using namespace flymoe;
   int rc = lora_check("lora_add", rows, k, n, rank, adapters, dtype);
@@ -837,17 +853,12 @@ extern "C" int flymoe_lora_add(void* out, const void* base, const void* x, const
   FLYMOE_REQUIRE(out && base && x && a && b && ids && scaling && v, "lora_add: null pointer");
   FLYMOE_REQUIRE(aligned16(out) && aligned16(base) && aligned16(x) && aligned16(a) && aligned16(b) && aligned16(v),
                  "lora_add: pointers must be 16-byte aligned");
-  const int splits = shrink_splits(rows, k);
-  if (v_elems < (int64_t)splits * rows * rank) {
+  if (v_floats < v_elems(rows, shrink_splits(rows, k), rank)) {
     set_last_error_msg("lora_add: v is smaller than flymoe_lora_v_elems()");
     return FLYMOE_ERR_WORKSPACE;
   }
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // tiles read a row's v once for every block that works on it: one sum, not several
-  const bool fold = keep_v || on_tiles(rows);
-  rc = shrink({x, a, ids, v, rows, k, rank, adapters, splits, 0}, nullptr, fold, dtype, s);
-  if (rc != FLYMOE_OK) return rc;
-  return expand({base, v, b, ids, scaling, out, rows, n, rank, adapters, fold ? 1 : splits, 0}, nullptr, dtype, s);
+  return run_chain({x, a, nullptr, base, b, nullptr, out, v, ids, scaling, rows, k, n, rank, adapters, dtype, keep_v != 0},
+                   static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int64_t flymoe_lora_backward_workspace_elems(int rows, int k, int n, int rank, int adapters) {
@@ -879,7 +890,7 @@ extern "C" int flymoe_lora_backward(void* dx, void* da, void* db, const void* do
   }
   float* dv = workspace + w.dv;
   if (dx || da) {
-    const void *a_t = a, *b_t = b;               // dx contracts over the rank, dv over the columns: B and A the other way round
+    const void *a_t = nullptr, *b_t = nullptr;   // dv contracts over B's columns, dx over A's rows: both the other way round
     if (needs_transposed(rows, adapters)) {
       TransposeArgs t = {};
       uint16_t* at = reinterpret_cast<uint16_t*>(workspace + w.a_t);
@@ -894,9 +905,7 @@ extern "C" int flymoe_lora_backward(void* dx, void* da, void* db, const void* do
       a_t = at;
       b_t = bt;
     }
-    rc = shrink({dout, b_t, ids, dv, rows, n, rank, adapters, w.dv_splits, 0}, b, true, dtype, s);
-    if (rc != FLYMOE_OK) return rc;
-    if (dx) rc = expand({nullptr, dv, a_t, ids, scaling, dx, rows, k, rank, adapters, 1, 0}, a, dtype, s);
+    rc = run_chain({dout, b_t, b, nullptr, a_t, a, dx, dv, ids, scaling, rows, n, k, rank, adapters, dtype, da != nullptr}, s);
     if (rc != FLYMOE_OK) return rc;
   }
   if (!da && !db) return FLYMOE_OK;

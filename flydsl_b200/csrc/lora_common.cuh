@@ -45,7 +45,7 @@ struct ShrinkArgs {
 };
 struct ExpandArgs {
   const void* base;            // [rows, n] or null (zeros); may be `out`
-  const float* v;              // [splits, rows, rank]; splits is 1 on tiles
+  const float* v;              // [splits, rows, rank]; on tiles one split
   const void* b;               // [adapters, n, rank], or transposed [adapters, rank, n] (on tiles only)
   const int* ids;
   const float* scaling;        // [adapters]

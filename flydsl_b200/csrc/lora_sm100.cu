@@ -5,8 +5,9 @@
 // among its rows; of each product only that adapter's rows are kept.
 //
 // Shrink: 128 rows x one split of K.  Every adapter of the tile has its own columns of TMEM (rank each); a K block of x is
-// loaded once and multiplied with each adapter's block.  The splits' sums are folded by a launch of their own (a cluster
-// over K would save it, but CTAs that wait for one another must not wait for TMEM as well).
+// loaded once and multiplied with each adapter's block.  The splits' sums are folded by a launch of their own: a cluster over
+// K would save it, but CTAs that wait for one another must not wait for TMEM as well, and the expand, whose blocks each
+// read a row tile's v, took 15000 cycles to add up nine splits where one takes 2000.
 //
 // Expand: the base tile (128 x 128) is loaded into shared memory, gets the adapters' products added row by row where it
 // lies, and is stored from there; rows without an adapter are simply not touched.  The rows' v stands in shared memory as
@@ -183,19 +184,23 @@ constexpr int kExCols = 128;                     // columns of a tile: two chunk
 constexpr int kExThreads = 384;
 constexpr int kExEpi = 256;
 struct __align__(16) ExpandCtrl {
-  unsigned long long y_full[4], y_empty[4], b_full[2], b_empty[2], acc_full[2], acc_empty[2];
+  unsigned long long y_full[4], y_empty[4], b_full[3], b_empty[3], acc_full[4], acc_empty[4];
   unsigned long long row_ready;                  // a row tile's v is set up
-  unsigned long long together, tile_done;        // epilogue warps: barrier; their part of the output tile is written
+  unsigned long long together;                   // barrier of the epilogue warps
+  // Their part of the output tile is written.  One for each tile in shared memory: a warp without rows of an adapter is
+  // through with a tile early, and may be with the next one before another warp is with this.
+  unsigned long long tile_done[4];
   uint32_t tmem_base;
-  int abort_flag, count, list[2][kTileAdapters];   // the producer's and the epilogue's
-  int id[kTileRows], row_max[kTileRows];
+  int abort_flag, count[2], list[3][kTileAdapters];            // the producer's, and the epilogue's for two row tiles
+  float up[2][kTileRows];
 };
-constexpr int kExB = 2;                          // adapter tiles in flight
+constexpr int kExAcc = 4;                        // accumulators
+template <int KC> constexpr int ex_b_stages() { return KC == 1 ? 3 : 2; }      // adapter tiles in flight
 template <int KC> constexpr int ex_y_stages() { return KC == 1 ? 4 : 3; }      // base / output tiles in shared memory
 template <int KC> constexpr size_t ex_smem() {
-  return size_t(ex_y_stages<KC>()) * 2 * kChunkBytes + size_t(kExB) * KC * kChunkBytes + 2 * KC * kChunkBytes + sizeof(ExpandCtrl) + 1024;
+  return size_t(ex_y_stages<KC>()) * 2 * kChunkBytes + size_t(ex_b_stages<KC>()) * KC * kChunkBytes + 2 * KC * kChunkBytes + sizeof(ExpandCtrl) + 1024;
 }
-static_assert(ex_smem<2>() <= 232448, "shared memory budget of one SM exceeded");
+static_assert(ex_smem<1>() <= 232448 && ex_smem<2>() <= 232448, "shared memory budget of one SM exceeded");
 
 struct ExpandTcArgs {
   ExpandArgs p;
@@ -208,7 +213,7 @@ template <typename T, int KC>
 __global__ void __launch_bounds__(kExThreads, 1)
 lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_constant__ CUtensorMap tmap_out,
                       const __grid_constant__ CUtensorMap tmap_b, const ExpandTcArgs q) {
-  constexpr int kExY = ex_y_stages<KC>();
+  constexpr int kExY = ex_y_stages<KC>(), kExB = ex_b_stages<KC>();
   extern __shared__ uint8_t smem_dyn[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
   uint8_t* bring = smem + kExY * 2 * kChunkBytes;
@@ -220,15 +225,14 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
 
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                 ::"r"(smem_u32(&c->tmem_base)), "r"(uint32_t(2 * kExCols)) : "memory");
+                 ::"r"(smem_u32(&c->tmem_base)), "r"(uint32_t(kExAcc * kExCols)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   } else if (threadIdx.x == 0) {
-    for (int i = 0; i < kExY; ++i) { mbar_init(smem_u32(&c->y_full[i]), 1); mbar_init(smem_u32(&c->y_empty[i]), 1); }
+    for (int i = 0; i < kExY; ++i) { mbar_init(smem_u32(&c->y_full[i]), 1); mbar_init(smem_u32(&c->y_empty[i]), 1); mbar_init(smem_u32(&c->tile_done[i]), kExEpi / 32); }
     for (int i = 0; i < kExB; ++i) { mbar_init(smem_u32(&c->b_full[i]), 1); mbar_init(smem_u32(&c->b_empty[i]), 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&c->acc_full[i]), 1); mbar_init(smem_u32(&c->acc_empty[i]), kExEpi / 32); }
+    for (int i = 0; i < kExAcc; ++i) { mbar_init(smem_u32(&c->acc_full[i]), 1); mbar_init(smem_u32(&c->acc_empty[i]), kExEpi / 32); }
     mbar_init(smem_u32(&c->row_ready), kExEpi);
     mbar_init(smem_u32(&c->together), kExEpi / 32);
-    mbar_init(smem_u32(&c->tile_done), kExEpi / 32);
     c->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -240,7 +244,6 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   const int steps = (p.rank + 15) / 16;          // of the contraction
   // an adapter's tile: 128 columns along the rank, or (transposed) two chunks of 64 columns with a row per rank
   const uint32_t b_bytes = p.transposed ? steps * 16 * 256 : KC * kChunkBytes;
-  // consecutive column tiles of a row tile, so that the rows' v is set up once or twice per block
   // adapters of a row tile: every role looks for itself, ahead of the others where it can
   auto find_adapters = [&](int rt, int* list) {
     int id[4];
@@ -250,100 +253,113 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     __syncwarp();
     return n;
   };
+  // consecutive column tiles of a row tile, so that the rows' v is set up once or twice per block
   const int u0 = int((long long)q.units * blockIdx.x / gridDim.x), u1 = int((long long)q.units * (blockIdx.x + 1) / gridDim.x);
 
+  // Producers and issuer: a warp looks at the ids, one thread (the same every time) does the rest, waits included.
   if (warp == 0) {
-    // ------------------------------------------------------------------ TMA producer
-    int ys = 0, bs = 0, row_tile = -1, d = 0;
-    int* list = c->list[0];
-    uint32_t yp = 0, bp = 0;
+    // ------------------------------------------------------------------ base tiles
+    const bool all_ours = p.adapters <= kTileAdapters;
+    int ys = 0;
+    uint32_t yp = 0;
     bool ok = true;
-    for (int u = u0; u < u1 && ok; ++u) {
-      const int rt = u / q.col_tiles, col = (u - rt * q.col_tiles) * kExCols;
-      if (rt != row_tile) {
-        row_tile = rt;
-        d = find_adapters(rt, list);
-      }
-      if (d > kTileAdapters) continue;
-      ok = warp_wait(smem_u32(&c->y_empty[ys]), yp ^ 1, abort_flag, q.status, 1, 32);
-      if (!ok) break;
-      const uint32_t full = smem_u32(&c->y_full[ys]), dst = smem_u32(smem + ys * 2 * kChunkBytes);
-      if (elect_one()) {
-        if (p.base) {
-          mbar_expect_tx(full, 2 * kChunkBytes);
-          tma_load_2d(dst, &tmap_y, full, col * 2, rt * kTileRows);
-          tma_load_2d(dst + kChunkBytes, &tmap_y, full, col * 2 + 128, rt * kTileRows);
-        } else {
-          mbar_arrive(full);
+    for (int u = u0; u < u1;) {
+      const int rt = u / q.col_tiles, end = min(u1, (rt + 1) * q.col_tiles);
+      const bool ours = all_ours || find_adapters(rt, nullptr) <= kTileAdapters;
+      if (ours && elect_one()) {
+        for (int t = u; t < end && ok; ++t) {
+          const int col = (t - rt * q.col_tiles) * kExCols;
+          ok = mbar_wait(smem_u32(&c->y_empty[ys]), yp ^ 1, abort_flag, q.status, 1, 32);
+          if (!ok) break;
+          const uint32_t full = smem_u32(&c->y_full[ys]), dst = smem_u32(smem + ys * 2 * kChunkBytes);
+          if (p.base) {
+            mbar_expect_tx(full, 2 * kChunkBytes);
+            tma_load_2d(dst, &tmap_y, full, col * 2, rt * kTileRows);
+            tma_load_2d(dst + kChunkBytes, &tmap_y, full, col * 2 + 128, rt * kTileRows);
+          } else {
+            mbar_arrive(full);
+          }
+          if (++ys == kExY) { ys = 0; yp ^= 1; }
         }
       }
       __syncwarp();
-      if (++ys == kExY) { ys = 0; yp ^= 1; }
-      for (int i = 0; i < d && ok; ++i) {
-        ok = warp_wait(smem_u32(&c->b_empty[bs]), bp ^ 1, abort_flag, q.status, 1, 32);
-        if (!ok) break;
-        const uint32_t bfull = smem_u32(&c->b_full[bs]), bdst = smem_u32(bring + bs * KC * kChunkBytes);
-        if (elect_one()) {
-          mbar_expect_tx(bfull, b_bytes);
-          if (p.transposed) {
-            tma_load_3d(bdst, &tmap_b, bfull, col * 2, 0, list[i]);
-            tma_load_3d(bdst + b_bytes / 2, &tmap_b, bfull, col * 2 + 128, 0, list[i]);
-          } else
+      u = end;
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ adapter tiles
+    int bs = 0;
+    int* list = c->list[0];
+    uint32_t bp = 0;
+    bool ok = true;
+    for (int u = u0; u < u1;) {
+      const int rt = u / q.col_tiles, end = min(u1, (rt + 1) * q.col_tiles);
+      const int d = find_adapters(rt, list);
+      if (d <= kTileAdapters && elect_one()) {
+        for (int t = u; t < end && ok; ++t) {
+          const int col = (t - rt * q.col_tiles) * kExCols;
+          for (int i = 0; i < d && ok; ++i) {
+            ok = mbar_wait(smem_u32(&c->b_empty[bs]), bp ^ 1, abort_flag, q.status, 1, 32);
+            if (!ok) break;
+            const uint32_t bfull = smem_u32(&c->b_full[bs]), bdst = smem_u32(bring + bs * KC * kChunkBytes);
+            mbar_expect_tx(bfull, b_bytes);
+            if (p.transposed) {
+              tma_load_3d(bdst, &tmap_b, bfull, col * 2, 0, list[i]);
+              tma_load_3d(bdst + b_bytes / 2, &tmap_b, bfull, col * 2 + 128, 0, list[i]);
+            } else {
 #pragma unroll
-          for (int k = 0; k < KC; ++k) tma_load_3d(bdst + k * kChunkBytes, &tmap_b, bfull, k * 128, col, list[i]);
+              for (int k = 0; k < KC; ++k) tma_load_3d(bdst + k * kChunkBytes, &tmap_b, bfull, k * 128, col, list[i]);
+            }
+            if (++bs == kExB) { bs = 0; bp ^= 1; }
+          }
         }
-        __syncwarp();
-        if (++bs == kExB) { bs = 0; bp ^= 1; }
       }
+      __syncwarp();
+      u = end;
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA issuer
     const uint32_t idesc = instr_desc(std::is_same<T, __nv_bfloat16>::value, kExCols) | (p.transposed ? 1u << 16 : 0u);
-    int bs = 0, acc = 0, row_tile = -1, d = 0;
+    const uint32_t b_step = p.transposed ? 2048 >> 4 : 2, b_chunk = p.transposed ? 4 * (2048 >> 4) : kChunkBytes >> 4;
+    int bs = 0, acc = 0;
     uint32_t bp = 0, rp = 0, accp = 0;
     bool ok = true;
-    for (int u = u0; u < u1 && ok; ++u) {
-      const int rt = u / q.col_tiles;
-      if (rt != row_tile) {
-        row_tile = rt;
-        d = find_adapters(rt, nullptr);
-        if (d >= 1 && d <= kTileAdapters) {      // otherwise nobody multiplies, and nobody signals
-          ok = warp_wait(smem_u32(&c->row_ready), rp, abort_flag, q.status, 5);
+    for (int u = u0; u < u1;) {
+      const int rt = u / q.col_tiles, end = min(u1, (rt + 1) * q.col_tiles);
+      const int d = find_adapters(rt, nullptr);
+      if (d >= 1 && d <= kTileAdapters && elect_one()) {         // otherwise nobody multiplies, and nobody signals
+        ok = ok && mbar_wait(smem_u32(&c->row_ready), rp, abort_flag, q.status, 5);
+        rp ^= 1;
+        for (int t = (end - u) * d; t > 0 && ok; --t) {
+          ok = mbar_wait(smem_u32(&c->acc_empty[acc]), accp ^ 1, abort_flag, q.status, 2) &&
+               mbar_wait(smem_u32(&c->b_full[bs]), bp, abort_flag, q.status, 3);
           if (!ok) break;
-          rp ^= 1;
-        }
-      }
-      if (d > kTileAdapters) continue;
-      for (int i = 0; i < d && ok; ++i) {
-        ok = warp_wait(smem_u32(&c->acc_empty[acc]), accp ^ 1, abort_flag, q.status, 2) &&
-             warp_wait(smem_u32(&c->b_full[bs]), bp, abort_flag, q.status, 3);
-        if (!ok) break;
-        tcgen05_fence_after();
-        if (elect_one()) {
-          for (int part = 0; part < 2; ++part)
-            for (int k = 0; k < steps; ++k) {
-              const uint64_t ad = make_smem_desc(smem_u32(vtile + (part * KC + (k >> 2)) * kChunkBytes)) + (k & 3) * 2;
-              const uint64_t bd = p.transposed ? make_smem_desc_mn(smem_u32(bring + bs * KC * kChunkBytes) + k * 2048, b_bytes / 2)
-                                               : make_smem_desc(smem_u32(bring + (bs * KC + (k >> 2)) * kChunkBytes)) + (k & 3) * 2;
-              umma_f16(tmem + acc * kExCols, ad, bd, idesc, (part > 0 || k > 0) ? 1u : 0u);
-            }
+          const uint32_t at = smem_u32(bring + bs * KC * kChunkBytes);
+          const uint64_t bd = p.transposed ? make_smem_desc_mn(at, b_bytes / 2) : make_smem_desc(at);
+          tcgen05_fence_after();
+          for (int part = 0; part < 2; ++part) {
+            const uint64_t ad = make_smem_desc(smem_u32(vtile + part * KC * kChunkBytes));
+            for (int k = 0; k < steps; ++k)
+              umma_f16(tmem + acc * kExCols, ad + uint64_t((k >> 2) * (kChunkBytes >> 4) + (k & 3) * 2),
+                       bd + uint64_t((k >> 2) * b_chunk + (k & 3) * b_step), idesc, (part > 0 || k > 0) ? 1u : 0u);
+          }
           umma_commit(smem_u32(&c->b_empty[bs]));
           umma_commit(smem_u32(&c->acc_full[acc]));
+          if (++bs == kExB) { bs = 0; bp ^= 1; }
+          if (++acc == kExAcc) { acc = 0; accp ^= 1; }
         }
-        __syncwarp();
-        if (++bs == kExB) { bs = 0; bp ^= 1; }
-        if (++acc == 2) { acc = 0; accp ^= 1; }
       }
+      __syncwarp();
+      u = end;
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ epilogue: a thread per row and half tile
     const int et = threadIdx.x - 128, wg = et >> 7, row = et & 127;
     const int sw = row & 7;
-    int ys = 0, acc = 0, row_tile = -1, d = 0, mine = -1, stored = 0;
+    int ys = 0, acc = 0, row_tile = -1, d = 0, mine = -1, stored = 0, turn = 0;
     uint32_t yp = 0, accp = 0;
     float scale = 0.f;
     bool ok = true;
-    uint32_t together = 0, done = 0;
+    uint32_t together = 0;
     auto sync = [&]() -> bool {                  // bounded: a warp that gave up elsewhere does not leave the others waiting
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&c->together));
@@ -354,59 +370,67 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     for (int u = u0; u < u1 && ok; ++u) {
       const int rt = u / q.col_tiles, col = (u - rt * q.col_tiles) * kExCols;
       if (rt != row_tile) {
-        // The MMAs of the previous row tile are done (their last sums have been read here): its v may go.  Everything of
-        // the new one is asked for at once: v, four numbers a thread and step with consecutive threads along a row, and ids.
+        // The MMAs of the previous row tile are done (their last sums have been read here): its v may go.  Eight threads to a
+        // row; ids and v are asked for together.
         row_tile = rt;
-        const int vecs = (p.rank + 15) / 16 * 4;
-        float4 x[KC * 8];
+        turn ^= 1;
+        const int r8 = et >> 3, l8 = et & 7, vecs = p.rank / 4;
+        int id[4];
+        float4 x[4][KC * 2];
 #pragma unroll
-        for (int s = 0; s < KC * 8; ++s) {
-          const int i = s * kExEpi + et, r = i / vecs, k4 = i - r * vecs;
-          x[s] = r < kTileRows && rt * kTileRows + r < p.rows && k4 * 4 < p.rank
-                     ? __ldg(reinterpret_cast<const float4*>(p.v + (long long)(rt * kTileRows + r) * p.rank + k4 * 4))
-                     : make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < 4; ++s) {
+          const int r = rt * kTileRows + s * 32 + r8;
+          id[s] = row_adapter(p.ids, r, p.rows, p.adapters);
+#pragma unroll
+          for (int h = 0; h < KC * 2; ++h) {
+            x[s][h] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < p.rows && h * 8 + l8 < vecs) x[s][h] = __ldg(reinterpret_cast<const float4*>(p.v) + (long long)r * vecs + h * 8 + l8);
+          }
         }
         mine = row_adapter(p.ids, rt * kTileRows + row, p.rows, p.adapters);
-        ok = sync();                             // all have left the previous list
-        if (!ok) break;
+        scale = mine >= 0 ? __ldg(p.scaling + mine) : 0.f;
         if (et < 32) {
-          d = find_adapters(rt, c->list[1]);
-          if (lane == 0) c->count = d;
+          const int n = find_adapters(rt, c->list[1 + turn]);
+          if (lane == 0) c->count[turn] = n;
         }
-        if (wg == 0) { c->id[row] = mine; c->row_max[row] = 0; }
-        ok = sync();
-        if (!ok) break;
-        d = c->count;
-        if (d >= 1 && d <= kTileAdapters) {
-          scale = mine >= 0 ? __ldg(p.scaling + mine) : 0.f;
-          if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
-            for (int s = 0; s < KC * 8; ++s) {
-              const int r = (s * kExEpi + et) / vecs;
-              const float m = fmaxf(fmaxf(finite_abs(x[s].x), finite_abs(x[s].y)), fmaxf(finite_abs(x[s].z), finite_abs(x[s].w)));
-              if (r < kTileRows) atomicMax(&c->row_max[r], __float_as_int(m));     // not negative: ordered like the numbers
-            }
-            ok = sync();
-            if (!ok) break;
-            scale *= exp2i(scale_exponent(__int_as_float(c->row_max[row])));
+        for (int s = 0; s < 4; ++s) {
+          const int r = s * 32 + r8;
+          float down = 1.f;
+          if (id[s] < 0) {                       // nothing has been summed up for it
+#pragma unroll
+            for (int h = 0; h < KC * 2; ++h) x[s][h] = make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+          if constexpr (std::is_same<T, __half>::value) {
+            float amax = 0.f;
+#pragma unroll
+            for (int h = 0; h < KC * 2; ++h)
+              amax = fmaxf(amax, fmaxf(fmaxf(finite_abs(x[s][h].x), finite_abs(x[s][h].y)),
+                                       fmaxf(finite_abs(x[s][h].z), finite_abs(x[s][h].w))));
+#pragma unroll
+            for (int off = 1; off < 8; off <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
+            const int e = scale_exponent(amax);
+            down = exp2i(-e);
+            if (l8 == 0) c->up[turn][r] = exp2i(e);
           }
 #pragma unroll
-          for (int s = 0; s < KC * 8; ++s) {
-            const int i = s * kExEpi + et, r = i / vecs, k4 = i - r * vecs;
-            if (r >= kTileRows) continue;
-            if (c->id[r] < 0) x[s] = make_float4(0.f, 0.f, 0.f, 0.f);      // nothing has been summed up for it
-            float down = 1.f;
-            if constexpr (std::is_same<T, __half>::value) down = exp2i(-scale_exponent(__int_as_float(c->row_max[r])));
+          for (int h = 0; h < KC * 2; ++h) {
+            const int k4 = h * 8 + l8;
+            if (k4 >= (p.rank + 15) / 16 * 4) continue;
             uint2 hi, lo;
-            split2<T>(x[s].x * down, x[s].y * down, hi.x, lo.x);
-            split2<T>(x[s].z * down, x[s].w * down, hi.y, lo.y);
+            split2<T>(x[s][h].x * down, x[s][h].y * down, hi.x, lo.x);
+            split2<T>(x[s][h].z * down, x[s][h].w * down, hi.y, lo.y);
             uint8_t* at = vtile + (k4 >> 4) * kChunkBytes + r * 128 + ((((k4 >> 1) & 7) ^ (r & 7)) * 16) + (k4 & 1) * 8;
             *reinterpret_cast<uint2*>(at) = hi;
             *reinterpret_cast<uint2*>(at + KC * kChunkBytes) = lo;
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          mbar_arrive(smem_u32(&c->row_ready));
         }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        ok = sync();                             // list and exponents, in this row tile's places, are written
+        if (!ok) break;
+        d = c->count[turn];
+        if constexpr (std::is_same<T, __half>::value) scale *= c->up[turn][row];
+        if (d >= 1 && d <= kTileAdapters) mbar_arrive(smem_u32(&c->row_ready));
       }
       if (d > kTileAdapters) continue;           // its rows are the other kernel's
       ok = warp_wait(smem_u32(&c->y_full[ys]), yp, abort_flag, q.status, 6);
@@ -420,7 +444,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
         ok = warp_wait(smem_u32(&c->acc_full[acc]), accp, abort_flag, q.status, 4);
         if (!ok) break;
         tcgen05_fence_after();
-        const bool hit = mine == c->list[1][i];
+        const bool hit = mine == c->list[1 + turn][i];
         if (__any_sync(0xffffffffu, hit)) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -447,17 +471,16 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
         tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&c->acc_empty[acc]));
-        if (++acc == 2) { acc = 0; accp ^= 1; }
+        if (++acc == kExAcc) { acc = 0; accp ^= 1; }
       }
       if (!ok) break;
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&c->tile_done));
+      if (lane == 0) mbar_arrive(smem_u32(&c->tile_done[ys]));
       if (et < 32) {
-        ok = warp_wait(smem_u32(&c->tile_done), done, abort_flag, q.status, 7);
+        ok = warp_wait(smem_u32(&c->tile_done[ys]), yp, abort_flag, q.status, 7);
         if (!ok) break;
       }
-      done ^= 1;
       if (et == 0) {
         const uint32_t src = smem_u32(smem + ys * 2 * kChunkBytes);
         tma_store_2d(&tmap_out, src, col * 2, rt * kTileRows);
@@ -475,7 +498,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   __syncthreads();
   if (warp == 1) {
     tcgen05_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(2 * kExCols)) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(kExAcc * kExCols)) : "memory");
   }
 }
 

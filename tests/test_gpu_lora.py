@@ -63,6 +63,7 @@ SIZES = [
     (1, 8, 8, 8, 1, "requests"), (1, 7168, 2112, 16, 4, "tokens"), (17, 264, 136, 24, 40, "tokens"),
     (64, 1024, 520, 16, 32, "tokens"), (33, 40, 1032, 128, 5, "tokens"), (130, 512, 256, 64, 3, "requests"),
     (1000, 328, 200, 32, 6, "requests"), (1500, 256, 264, 72, 2, "tokens"), (2100, 136, 72, 8, 1, "requests"), (700, 1096, 392, 48, 150, "tokens"), (512, 64, 72, 16, 1, "none"),
+    (640, 1288, 328, 128, 3, "requests"), (900, 72, 64, 8, 2, "requests"), (2600, 1032, 136, 56, 5, "requests"),
     (50, 64, 64, 40, 3, "none"), (600, 2048, 136, 104, 9, "tokens"),
 ]
 
@@ -105,6 +106,23 @@ def test_fp16_rows_far_from_one(size):
     check(gx, (dx, mx), 128 + 32, "dx")
     check(ga, (da, ma), 128 + 300, "da")
     check(gb, (db, mb), 512 + 300, "db")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_many_column_tiles_with_several_adapters_in_a_row_tile(dtype):
+    """Blocks walk through a dozen column tiles while some of their warps have no row of the adapter at hand."""
+    rows, k, n, rank, adapters = 2048, 256, 7168, 32, 4
+    p, dout = make(rows, k, n, rank, adapters, dtype, "requests", seed=4)
+    p["adapter_ids"] = ((torch.arange(rows, device="cuda") // 40) % (adapters + 1)).int()       # three or four of them in a tile
+    (out, mo), (dx, mx), (da, ma), (db, mb) = exact(p, dout)
+    q = {s: (t.clone().requires_grad_() if s in "xab" else t) for s, t in p.items()}
+    for _ in range(3):
+        res = lora_add(**q)
+        gx, ga, gb = torch.autograd.grad(res, (q["x"], q["a"], q["b"]), dout)
+        check(res.detach(), (out, mo), k + rank, "out")
+        check(gx, (dx, mx), n + rank, "dx")
+        check(ga, (da, ma), n + rows, "da")
+        check(gb, (db, mb), k + rows, "db")
 
 
 def test_no_rows():
