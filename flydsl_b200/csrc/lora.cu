@@ -61,24 +61,24 @@ struct Groups {
   int warp_sum[2][8], count, skip[kWindow / 128];
 };
 
-// skip_tiles: rows of 128-row tiles with at most kTileAdapters distinct adapters belong to the tcgen05 kernels.  keep_none:
+// skip_tiles: rows of 128-row tiles with at most that many distinct adapters belong to the tcgen05 kernels; 0: none do.  keep_none:
 // rows without an adapter form groups as well (adapter -1).
-__device__ __forceinline__ void build_groups(Groups* s, const int* ids, int row0, int rows, int adapters, bool skip_tiles,
+__device__ __forceinline__ void build_groups(Groups* s, const int* ids, int row0, int rows, int adapters, int skip_tiles,
                                              bool keep_none) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n = min(kWindow, rows - row0), chunks = (n + 31) / 32;
   const int mask = (n > 128 ? kTable : 256) - 1;               // at least twice as many entries as rows
   for (int i = tid; i <= mask; i += kGroupThreads) { s->key[i] = -2; s->first[i] = kWindow; }
   for (int i = tid; i < chunks * kWindow / 4; i += kGroupThreads) reinterpret_cast<int*>(s->in_chunk)[i] = 0;
-  if (skip_tiles && warp < kWindow / 128) {
+  if (skip_tiles > 0 && warp < kWindow / 128) {
     int q[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) q[i] = row_adapter(ids, row0 + warp * 128 + i * 32 + lane, rows, adapters);
-    const int d = tile_adapters(q, lane, nullptr);
-    if (lane == 0) s->skip[warp] = d <= kTileAdapters;
+    const int d = tile_adapters(q, lane, skip_tiles, nullptr);
+    if (lane == 0) s->skip[warp] = d <= skip_tiles;
   }
   __syncthreads();
-  if (skip_tiles && s->skip[0] && s->skip[1] && s->skip[2] && s->skip[3]) {      // nothing here (no rows: no adapters)
+  if (skip_tiles > 0 && s->skip[0] && s->skip[1] && s->skip[2] && s->skip[3]) {      // nothing here (no rows: no adapters)
     if (tid == 0) s->count = 0;
     __syncthreads();
     return;
@@ -91,7 +91,7 @@ __device__ __forceinline__ void build_groups(Groups* s, const int* ids, int row0
     if (i >= n) continue;
     const int id = row_adapter(ids, row0 + i, rows, adapters);
     s->id[i] = id;
-    if ((id < 0 && !keep_none) || (skip_tiles && s->skip[i / 128])) continue;
+    if ((id < 0 && !keep_none) || (skip_tiles > 0 && s->skip[i / 128])) continue;
     int h = int((uint32_t(id) * 0x9E3779B1u) >> 22) & mask;
     for (;; h = (h + 1) & mask) {
       const int old = atomicCAS(&s->key[h], -2, id);
@@ -159,7 +159,7 @@ constexpr int kShrinkWarps = kGroupThreads / 32;
 // a part of every group's product, and the parts meet in shared memory in a fixed order.
 template <typename T, int NT>
 __global__ void __launch_bounds__(kGroupThreads)
-lora_shrink_kernel(const ShrinkArgs p, const int slots, const bool skip_tiles) {
+lora_shrink_kernel(const ShrinkArgs p, const int slots, const int skip_tiles) {
   constexpr int RP = NT * 8;
   extern __shared__ __align__(16) float part[];        // [warps][16][RP]
   __shared__ __align__(16) Groups s;
@@ -243,7 +243,7 @@ lora_fold_kernel(const float4* __restrict__ planes, float4* __restrict__ v, long
 // consecutive ones: base and output move 16 bytes a lane.
 template <typename T, int KS>
 __global__ void __launch_bounds__(kGroupThreads)
-lora_expand_kernel(const ExpandArgs p, const int slots, const int per_warp, const bool skip_tiles) {
+lora_expand_kernel(const ExpandArgs p, const int slots, const int per_warp, const int skip_tiles) {
   __shared__ __align__(16) Groups s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int row0 = int(blockIdx.x) / slots * kWindow;
@@ -709,7 +709,7 @@ static int window_groups(int rows, int adapters) {
   return std::min(n, n / 16 + std::min(adapters + 1, n));
 }
 template <typename T, int NT>
-static int launch_shrink(const ShrinkArgs& p, bool skip_tiles, cudaStream_t stream) {
+static int launch_shrink(const ShrinkArgs& p, int skip_tiles, cudaStream_t stream) {
   auto* kernel = lora_shrink_kernel<T, NT>;
   constexpr int smem = kShrinkWarps * 16 * NT * 8 * 4;
   static SmemLimitSeen seen;
@@ -721,12 +721,12 @@ static int launch_shrink(const ShrinkArgs& p, bool skip_tiles, cudaStream_t stre
   return FLYMOE_OK;
 }
 template <typename T>
-static int launch_shrink_rank(const ShrinkArgs& p, bool skip, cudaStream_t s) {
+static int launch_shrink_rank(const ShrinkArgs& p, int skip, cudaStream_t s) {
   return p.rank <= 16 ? launch_shrink<T, 2>(p, skip, s) : p.rank <= 32 ? launch_shrink<T, 4>(p, skip, s)
        : p.rank <= 64 ? launch_shrink<T, 8>(p, skip, s) : launch_shrink<T, 16>(p, skip, s);
 }
 template <typename T, int KS>
-static int launch_expand(const ExpandArgs& p, bool skip_tiles, cudaStream_t stream) {
+static int launch_expand(const ExpandArgs& p, int skip_tiles, cudaStream_t stream) {
   const int windows = ceil_div(p.rows, kWindow), cols = ceil_div(p.n, 32), warps = kGroupThreads / 32;
   // Three blocks for every SM: row groups first, then columns.  A warp walks through up to eight column groups.
   const int want = 3 * sm_count();
@@ -740,7 +740,7 @@ static int launch_expand(const ExpandArgs& p, bool skip_tiles, cudaStream_t stre
   return FLYMOE_OK;
 }
 template <typename T>
-static int launch_expand_rank(const ExpandArgs& p, bool skip, cudaStream_t s) {
+static int launch_expand_rank(const ExpandArgs& p, int skip, cudaStream_t s) {
   return p.rank <= 16 ? launch_expand<T, 1>(p, skip, s) : p.rank <= 32 ? launch_expand<T, 2>(p, skip, s)
        : p.rank <= 64 ? launch_expand<T, 4>(p, skip, s) : launch_expand<T, 8>(p, skip, s);
 }
@@ -778,12 +778,13 @@ struct Chain {
   bool keep;
 };
 static int run_chain(const Chain& c, cudaStream_t s) {
-  const bool bf = c.dtype == FLYMOE_BF16, tiles = on_tiles(c.rows), others = !tiles || c.adapters > kTileAdapters;
+  const bool bf = c.dtype == FLYMOE_BF16, tiles = on_tiles(c.rows), others = !tiles || c.adapters > tile_limit(c.rank);
+  const int skip = tiles ? tile_limit(c.rank) : 0;
   const int splits = shrink_splits(c.rows, c.k);
   float* planes = splits > 1 ? c.v + (long long)c.rows * c.rank : c.v;
   ShrinkArgs sh = {c.x, c.a, c.ids, planes, c.rows, c.k, c.rank, c.adapters, splits, 0};
   int rc = FLYMOE_OK;
-  if (others) rc = bf ? launch_shrink_rank<__nv_bfloat16>(sh, tiles, s) : launch_shrink_rank<__half>(sh, tiles, s);
+  if (others) rc = bf ? launch_shrink_rank<__nv_bfloat16>(sh, skip, s) : launch_shrink_rank<__half>(sh, skip, s);
   if (rc == FLYMOE_OK && tiles) {
     if (c.a_t) { sh.a = c.a_t; sh.transposed = 1; }
     rc = launch_shrink_sm100(sh, bf, s);
@@ -799,7 +800,7 @@ static int run_chain(const Chain& c, cudaStream_t s) {
   if (!c.out) return FLYMOE_OK;
   ExpandArgs ex = {c.base, fold ? c.v : planes, c.b, c.ids, c.scaling, c.out, c.rows, c.n, c.rank, c.adapters,
                    fold ? 1 : splits, 0};
-  if (others) rc = bf ? launch_expand_rank<__nv_bfloat16>(ex, tiles, s) : launch_expand_rank<__half>(ex, tiles, s);
+  if (others) rc = bf ? launch_expand_rank<__nv_bfloat16>(ex, skip, s) : launch_expand_rank<__half>(ex, skip, s);
   if (rc == FLYMOE_OK && tiles) {
     if (c.b_t) { ex.b = c.b_t; ex.transposed = 1; }
     rc = launch_expand_sm100(ex, bf, s);
@@ -807,7 +808,7 @@ static int run_chain(const Chain& c, cudaStream_t s) {
   return rc;
 }
 // Whether a backward pass reads A and B through the kernels of this file, which want the contraction along a row.
-static bool needs_transposed(int rows, int adapters) { return !on_tiles(rows) || adapters > kTileAdapters; }
+static bool needs_transposed(int rows, int rank, int adapters) { return !on_tiles(rows) || adapters > tile_limit(rank); }
 
 // Pieces of the batch that the adapters' gradients are summed over: blocks for every place on the device (three an SM, two
 // from rank 33 on), at least 256 rows in a piece, and partial sums of 256 MB at most.
@@ -827,7 +828,7 @@ static BackwardScratch backward_scratch(int rows, int k, int n, int rank, int ad
   auto up4 = [](long long x) { return (x + 3) / 4 * 4; };
   w.dv_splits = shrink_splits(rows, n);
   w.splits = wgrad_splits(rows, k, n, rank, adapters);
-  const bool both = needs_transposed(rows, adapters);
+  const bool both = needs_transposed(rows, rank, adapters);
   const long long weights = (long long)adapters * rank;
   w.dv = 0;
   w.a_t = up4(v_elems(rows, w.dv_splits, rank));
@@ -891,7 +892,7 @@ extern "C" int flymoe_lora_backward(void* dx, void* da, void* db, const void* do
   float* dv = workspace + w.dv;
   if (dx || da) {
     const void *a_t = nullptr, *b_t = nullptr;   // dv contracts over B's columns, dx over A's rows: both the other way round
-    if (needs_transposed(rows, adapters)) {
+    if (needs_transposed(rows, rank, adapters)) {
       TransposeArgs t = {};
       uint16_t* at = reinterpret_cast<uint16_t*>(workspace + w.a_t);
       uint16_t* bt = reinterpret_cast<uint16_t*>(workspace + w.b_t);

@@ -75,15 +75,17 @@ inline cudaError_t launch_closely(void (*kernel)(Params...), dim3 grid, dim3 blo
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
-// Tiles of 128 rows on tcgen05 (lora_sm100.cu), of which these launches take those with at most kTileAdapters distinct
-// adapters among their rows; the kernels of lora.cu take the others, and batches of too few tiles.
-constexpr int kTileAdapters = 4;
+// Tiles of 128 rows on tcgen05 (lora_sm100.cu), of which these launches take those with at most tile_limit(rank) distinct
+// adapters among their rows; the kernels of lora.cu take the others, and batches of too few tiles.  As many as have room for
+// their sums in TMEM.
+constexpr int kTileAdapters = 8;
+__host__ __device__ inline int tile_limit(int rank) { return rank <= 64 ? kTileAdapters : kTileAdapters / 2; }
 int launch_shrink_sm100(const ShrinkArgs& p, int bf16, cudaStream_t stream);
 int launch_expand_sm100(const ExpandArgs& p, int bf16, cudaStream_t stream);
 
-// Distinct adapters among the 128 ids that a warp holds, four a lane (negative: none): their number, kTileAdapters + 1 if
-// there are more, and the first kTileAdapters of them in `list` (written by lane 0).
-__device__ __forceinline__ int tile_adapters(const int* id, int lane, int* list) {
+// Distinct adapters among the 128 ids that a warp holds, four a lane (negative: none): their number, most + 1 if there are
+// more, and the first `most` of them in `list` (written by lane 0).
+__device__ __forceinline__ int tile_adapters(const int* id, int lane, int most, int* list) {
   bool left[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) left[i] = id[i] >= 0;
@@ -91,7 +93,7 @@ __device__ __forceinline__ int tile_adapters(const int* id, int lane, int* list)
   while (true) {
     const bool any = left[0] || left[1] || left[2] || left[3];
     const uint32_t who = __ballot_sync(0xffffffffu, any);
-    if (who == 0 || count == kTileAdapters) return count + (who != 0);
+    if (who == 0 || count == most) return count + (who != 0);
     const int mine = left[0] ? id[0] : left[1] ? id[1] : left[2] ? id[2] : id[3];
     const int l = __shfl_sync(0xffffffffu, mine, __ffs(who) - 1);
     if (lane == 0 && list) list[count] = l;

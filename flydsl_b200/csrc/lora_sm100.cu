@@ -74,8 +74,8 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     int id[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, row0 + i * 32 + lane, p.rows, p.adapters);
-    const int n = tile_adapters(id, lane, c->list);
-    if (lane == 0) c->count = n <= kTileAdapters ? n : 0;        // the other tiles are not this kernel's
+    const int n = tile_adapters(id, lane, tile_limit(p.rank), c->list);
+    if (lane == 0) c->count = n <= tile_limit(p.rank) ? n : 0;        // the other tiles are not this kernel's
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -244,12 +244,13 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   const int steps = (p.rank + 15) / 16;          // of the contraction
   // an adapter's tile: 128 columns along the rank, or (transposed) two chunks of 64 columns with a row per rank
   const uint32_t b_bytes = p.transposed ? steps * 16 * 256 : KC * kChunkBytes;
+  const int most = tile_limit(p.rank);
   // adapters of a row tile: every role looks for itself, ahead of the others where it can
   auto find_adapters = [&](int rt, int* list) {
     int id[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, rt * kTileRows + i * 32 + lane, p.rows, p.adapters);
-    const int n = tile_adapters(id, lane, list);
+    const int n = tile_adapters(id, lane, most, list);
     __syncwarp();
     return n;
   };
@@ -259,13 +260,13 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   // Producers and issuer: a warp looks at the ids, one thread (the same every time) does the rest, waits included.
   if (warp == 0) {
     // ------------------------------------------------------------------ base tiles
-    const bool all_ours = p.adapters <= kTileAdapters;
+    const bool all_ours = p.adapters <= most;
     int ys = 0;
     uint32_t yp = 0;
     bool ok = true;
     for (int u = u0; u < u1;) {
       const int rt = u / q.col_tiles, end = min(u1, (rt + 1) * q.col_tiles);
-      const bool ours = all_ours || find_adapters(rt, nullptr) <= kTileAdapters;
+      const bool ours = all_ours || find_adapters(rt, nullptr) <= most;
       if (ours && elect_one()) {
         for (int t = u; t < end && ok; ++t) {
           const int col = (t - rt * q.col_tiles) * kExCols;
@@ -294,7 +295,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     for (int u = u0; u < u1;) {
       const int rt = u / q.col_tiles, end = min(u1, (rt + 1) * q.col_tiles);
       const int d = find_adapters(rt, list);
-      if (d <= kTileAdapters && elect_one()) {
+      if (d <= most && elect_one()) {
         for (int t = u; t < end && ok; ++t) {
           const int col = (t - rt * q.col_tiles) * kExCols;
           for (int i = 0; i < d && ok; ++i) {
@@ -326,7 +327,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     for (int u = u0; u < u1;) {
       const int rt = u / q.col_tiles, end = min(u1, (rt + 1) * q.col_tiles);
       const int d = find_adapters(rt, nullptr);
-      if (d >= 1 && d <= kTileAdapters && elect_one()) {         // otherwise nobody multiplies, and nobody signals
+      if (d >= 1 && d <= most && elect_one()) {         // otherwise nobody multiplies, and nobody signals
         ok = ok && mbar_wait(smem_u32(&c->row_ready), rp, abort_flag, q.status, 5);
         rp ^= 1;
         for (int t = (end - u) * d; t > 0 && ok; --t) {
@@ -430,9 +431,9 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
         if (!ok) break;
         d = c->count[turn];
         if constexpr (std::is_same<T, __half>::value) scale *= c->up[turn][row];
-        if (d >= 1 && d <= kTileAdapters) mbar_arrive(smem_u32(&c->row_ready));
+        if (d >= 1 && d <= most) mbar_arrive(smem_u32(&c->row_ready));
       }
-      if (d > kTileAdapters) continue;           // its rows are the other kernel's
+      if (d > most) continue;           // its rows are the other kernel's
       ok = warp_wait(smem_u32(&c->y_full[ys]), yp, abort_flag, q.status, 6);
       if (!ok) break;
       uint8_t* line = smem + (ys * 2 + wg) * kChunkBytes + row * 128;
@@ -515,9 +516,10 @@ int launch_shrink_sm100(const ShrinkArgs& p, int bf16, cudaStream_t stream) {
   if (q.status == nullptr) return FLYMOE_ERR_CUDA;
   q.a_bytes = p.transposed ? ceil_div(p.rank, 64) * 8192 : q.rank_pad * 128;
   q.slots = std::min(16, kShABytes / q.a_bytes);
-  // columns for kTileAdapters adapters; sums are read 32 columns at a time, so also for what the last read reaches
-  static_assert(kTileAdapters == 4, "TMEM columns below");
-  q.tmem_cols = q.rank_pad <= 64 ? 256 : 512;
+  // Columns for tile_limit() adapters; sums are read 32 columns at a time, so also for what the last read reaches past a rank
+  // of 16 modulo 32.
+  const int columns = (tile_limit(p.rank) - 1) * q.rank_pad + (q.rank_pad + 31) / 32 * 32;
+  q.tmem_cols = columns <= 256 ? 256 : 512;
   CUtensorMap mx, ma;
   int rc = matrix_map(&mx, p.x, p.k, p.rows, 0, kTileRows);
   if (rc == FLYMOE_OK)
