@@ -3,8 +3,10 @@
 from __future__ import annotations
 
 import contextlib
+import functools
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -23,6 +25,17 @@ def on(device: torch.device, stream=None):
     if device.index is None or device.index == torch.cuda.current_device():
         return _HERE
     return torch.cuda.device(device)
+
+
+def once(backward):
+    """``once_differentiable`` without its steps (2.5 us of host time a call) where no gradient of the gradient is asked for."""
+    checked = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        return (checked if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return wrapper
 
 
 def require_shape(name: str, t: torch.Tensor, shape: tuple) -> None:

@@ -21,10 +21,9 @@ unpadded form (its grouped GEMMs: kernels/moe_gemm_2stage.py:90-108, :1780-1796)
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._call import HALF, on, require_same_device, require_shape
+from ._call import HALF, on, once, require_same_device, require_shape
 
 
 def _check(rows_name, rows, mats_name, mats, offsets, out, out_shape):
@@ -71,6 +70,10 @@ def _check_rows_form(name, t, w, offsets, out, input_grad):
 def _rows_form(name, t, w, offsets, out, stream, input_grad):
     if not _fits(t, w, offsets, out, input_grad):
         _check_rows_form(name, t, w, offsets, out, input_grad)
+    return _run_rows_form(t, w, offsets, out, stream, input_grad)
+
+
+def _run_rows_form(t, w, offsets, out, stream, input_grad):
     (experts, n, k), rows = w.shape, t.shape[0]
     lib = _lib.load()
     with on(t.device, stream):
@@ -105,31 +108,41 @@ def grouped_gemm_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor,
     experts = offsets.shape[0] - 1
     _check_sizes(experts, n, k)
     _check("dy", dy, "x", x, offsets, out, (experts, n, k))
-    lib = _lib.load()
     with on(dy.device, stream):
-        res = dy.new_empty((experts, n, k)) if out is None else out
-        _lib.check(lib.flymoe_grouped_gemm_wgrad(res.data_ptr(), dy.data_ptr(), x.data_ptr(), offsets.data_ptr(), rows,
-                                                 experts, n, k, _lib.DTYPE_CODE[dy.dtype], _lib.stream_handle(None)),
-                   "grouped_gemm_wgrad")
-    return res
+        return _wgrad(dy, x, offsets, dy.new_empty((experts, n, k)) if out is None else out)
+
+
+def _wgrad(dy, x, offsets, out):
+    experts, n, k = out.shape
+    _lib.check(_lib.load().flymoe_grouped_gemm_wgrad(out.data_ptr(), dy.data_ptr(), x.data_ptr(), offsets.data_ptr(),
+                                                     x.shape[0], experts, n, k, _lib.DTYPE_CODE[dy.dtype],
+                                                     _lib.stream_handle(None)), "grouped_gemm_wgrad")
+    return out
 
 
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets):
         ctx.save_for_backward(x, w, offsets)
-        return grouped_gemm(x, w, offsets)
+        return _run_rows_form(x, w, offsets, None, None, False)
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
         dy = dy.contiguous()
-        dx = grouped_gemm_dgrad(dy, w, offsets) if ctx.needs_input_grad[0] else None
-        dw = grouped_gemm_wgrad(dy, x, offsets) if ctx.needs_input_grad[1] else None
+        dx = _run_rows_form(dy, w, offsets, None, None, True) if ctx.needs_input_grad[0] else None
+        dw = None
+        if ctx.needs_input_grad[1]:
+            with on(x.device):
+                dw = _wgrad(dy, x, offsets, torch.empty_like(w))
         return dx, dw, None
 
 
 def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     """``grouped_gemm`` in autograd: gradients reach ``x`` and ``w``.  Runs on the current stream."""
-    return _GroupedLinear.apply(x, w, offsets)
+    if not _fits(x, w, offsets, None, False):
+        _check_rows_form("x", x, w, offsets, None, False)
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+        return _GroupedLinear.apply(x, w, offsets)
+    return _run_rows_form(x, w, offsets, None, None, False)

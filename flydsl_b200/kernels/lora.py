@@ -18,10 +18,9 @@ and adapter only; nothing is atomic.  The reference has no counterpart.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._call import HALF, on, require_same_device, require_shape
+from ._call import HALF, on, once, require_same_device, require_shape
 
 MAX_RANK = 128
 
@@ -94,7 +93,7 @@ class _LoraAdd(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dout):
         x, a, b, ids, scaling, v = ctx.saved_tensors
         need_y, need_x, need_a, need_b = ctx.needs_input_grad[:4]
@@ -125,7 +124,10 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     With ``out`` or ``stream`` the call is for inference only (no input may require a gradient while gradients are on)."""
     if not _fits(y, x, a, b, adapter_ids, scaling, out):
         _check(y, x, a, b, adapter_ids, scaling, out)
-    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad):
+    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad
+                                    or scaling.requires_grad):
+        if scaling.requires_grad:
+            raise ValueError("scaling has no gradient here: detach it, or put it into b")
         if out is not None or stream is not None:
             raise ValueError("out= and stream= are for inference: an input requires a gradient")
         return _LoraAdd.apply(y, x, a, b, adapter_ids, scaling)

@@ -18,10 +18,9 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from ._call import on, require_same_device, require_shape
+from ._call import on, once, require_same_device, require_shape
 from .moe_sorting_kernel import moe_sorting_flydsl
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -73,16 +72,21 @@ def _require_rows(name: str, t: torch.Tensor) -> None:
 
 
 # ------------------------------------------------------------------------- gate
+def _gate(logits, topk, renormalize):
+    tokens, experts = logits.shape
+    with on(logits.device):
+        weights = logits.new_empty((tokens, topk), dtype=torch.float32)
+        ids = logits.new_empty((tokens, topk), dtype=torch.int32)
+        _lib.check(_lib.load().flymoe_topk_gating_softmax(
+            logits.data_ptr(), _lib.DTYPE_CODE[logits.dtype], weights.data_ptr(), ids.data_ptr(), None, tokens, experts,
+            topk, renormalize, _lib.stream_handle(None)), "topk_gating_softmax")
+    return weights, ids
+
+
 class _TopkGating(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, topk, renormalize):
-        tokens, experts = logits.shape
-        with on(logits.device):
-            weights = logits.new_empty((tokens, topk), dtype=torch.float32)
-            ids = logits.new_empty((tokens, topk), dtype=torch.int32)
-            _lib.check(_lib.load().flymoe_topk_gating_softmax(
-                logits.data_ptr(), _lib.DTYPE_CODE[logits.dtype], weights.data_ptr(), ids.data_ptr(), None, tokens, experts,
-                topk, renormalize, _lib.stream_handle(None)), "topk_gating_softmax")
+        weights, ids = _gate(logits, topk, renormalize)
         ctx.mark_non_differentiable(ids)
         ctx.set_materialize_grads(False)         # no zeros are made for the ids
         # weights that are a softmax over the picks are all that their gradient needs
@@ -91,7 +95,7 @@ class _TopkGating(torch.autograd.Function):
         return weights, ids
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dweights, _):
         if dweights is None:
             return None, None, None
@@ -118,7 +122,8 @@ def topk_gating(logits: torch.Tensor, topk: int, *, renormalize: bool = True) ->
         raise ValueError(f"logits must have 1 to 1024 experts, got {experts}")
     if not 1 <= int(topk) <= min(32, experts):
         raise ValueError(f"topk must be in [1, min(32, experts)], got {topk}")
-    return _TopkGating.apply(logits, int(topk), 1 if renormalize else 0)
+    run = _TopkGating.apply if logits.requires_grad and torch.is_grad_enabled() else _gate
+    return run(logits, int(topk), 1 if renormalize else 0)
 
 
 # ------------------------------------------------------------------------- plan
@@ -149,34 +154,56 @@ def route_rows(topk_ids: torch.Tensor, num_experts: int) -> RoutedRows:
 
 # ------------------------------------------------------------------------- rows
 def _combine(rows, weights, plan, tokens, topk):
-    out = rows.new_empty((tokens, rows.shape[1]))
-    _lib.check(_lib.load().flymoe_combine_rows(
-        rows.data_ptr(), _lib.ptr(weights), out.data_ptr(), plan[0].data_ptr(), plan[1].data_ptr(), plan[3].data_ptr(),
-        tokens, topk, rows.shape[0], rows.shape[1], _lib.DTYPE_CODE[rows.dtype], _lib.stream_handle(None)), "combine_rows")
+    (count, dim), (sorted_ids, num_valid_ids, _, row_index) = rows.shape, plan
+    out = rows.new_empty((tokens, dim))
+    rc = _lib.load().flymoe_combine_rows(
+        rows.data_ptr(), None if weights is None else weights.data_ptr(), out.data_ptr(), sorted_ids.data_ptr(),
+        num_valid_ids.data_ptr(), row_index.data_ptr(), tokens, topk, count, dim, _lib.DTYPE_CODE[rows.dtype],
+        _lib.stream_handle(None))
+    if rc:
+        _lib.check(rc, "combine_rows")
     return out
+
+
+def _permute(x, plan):
+    sorted_ids, num_valid_ids, _, row_index = plan
+    tokens, topk = row_index.shape
+    rows = tokens * topk
+    with on(x.device):
+        xs = x.new_empty((rows, x.shape[1]))
+        _lib.check(_lib.load().flymoe_permute_rows(
+            x.data_ptr(), xs.data_ptr(), sorted_ids.data_ptr(), num_valid_ids.data_ptr(), row_index.data_ptr(), tokens,
+            topk, rows, x.shape[1] * x.element_size(), _lib.stream_handle(None)), "permute_rows")
+    return xs
+
+
+# A plan goes into a graph as one object, which costs less than four inputs and saved tensors do; what autograd would look at
+# is looked at here: whether it was written between the passes.
+def _keep_plan(ctx, plan):
+    ctx.plan = plan
+    ctx.versions = plan[0]._version, plan[1]._version, plan[3]._version
+
+
+def _kept_plan(ctx):
+    plan = ctx.plan
+    if ctx.versions != (plan[0]._version, plan[1]._version, plan[3]._version):
+        raise RuntimeError("one of the plan's tensors was modified by an inplace operation after the forward pass")
+    return plan
 
 
 class _Permute(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, *plan):
-        sorted_ids, num_valid_ids, _, row_index = plan
-        tokens, topk = row_index.shape
-        rows = tokens * topk
-        with on(x.device):
-            xs = x.new_empty((rows, x.shape[1]))
-            _lib.check(_lib.load().flymoe_permute_rows(
-                x.data_ptr(), xs.data_ptr(), sorted_ids.data_ptr(), num_valid_ids.data_ptr(), row_index.data_ptr(), tokens,
-                topk, rows, x.shape[1] * x.element_size(), _lib.stream_handle(None)), "permute_rows")
-        ctx.save_for_backward(*plan)
-        return xs
+    def forward(ctx, x, plan):
+        _keep_plan(ctx, plan)
+        return _permute(x, plan)
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dxs):
-        plan = ctx.saved_tensors
+        plan = _kept_plan(ctx)
         dxs = dxs.contiguous()
         with on(dxs.device):
-            return (_combine(dxs, None, plan, *plan[3].shape), None, None, None, None)
+            return _combine(dxs, None, plan, *plan[3].shape), None
 
 
 def moe_permute(x: torch.Tensor, plan: RoutedRows) -> torch.Tensor:
@@ -185,30 +212,38 @@ def moe_permute(x: torch.Tensor, plan: RoutedRows) -> torch.Tensor:
     tokens, topk = _check_plan(plan, "x", x, 0)
     if x.shape[0] != tokens or plan[0].numel() < tokens * topk:
         raise ValueError(f"x has {x.shape[0]} rows, the plan is for {tokens} tokens of {topk} pairs")
-    return _Permute.apply(x, *plan)
+    return _Permute.apply(x, plan) if x.requires_grad and torch.is_grad_enabled() else _permute(x, plan)
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, weights, *plan):
-        ctx.save_for_backward(rows, weights, *plan)
+    def forward(ctx, rows, weights, plan):
+        ctx.save_for_backward(rows, weights)
+        _keep_plan(ctx, plan)
+        tokens, topk = weights.shape
         with on(rows.device):
-            return _combine(rows, weights, plan, *weights.shape)
+            return _combine(rows, weights, plan, tokens, topk)
 
     @staticmethod
-    @once_differentiable
+    @once
     def backward(ctx, dout):
-        rows, weights, *plan = ctx.saved_tensors
-        tokens, topk = weights.shape
-        dout = dout.contiguous()
+        rows, weights = ctx.saved_tensors
+        sorted_ids, num_valid_ids, _, row_index = _kept_plan(ctx)
+        (tokens, topk), (count, dim), drows, dw = weights.shape, rows.shape, None, None
+        need_rows, need_weights, _ = ctx.needs_input_grad
         with on(rows.device):
-            drows = torch.empty_like(rows) if ctx.needs_input_grad[0] else None
-            dw = torch.empty_like(weights) if ctx.needs_input_grad[1] else None
-            _lib.check(_lib.load().flymoe_combine_rows_backward(
-                dout.data_ptr(), rows.data_ptr(), weights.data_ptr(), _lib.ptr(drows), _lib.ptr(dw), plan[0].data_ptr(),
-                plan[1].data_ptr(), plan[3].data_ptr(), tokens, topk, rows.shape[0], rows.shape[1],
-                _lib.DTYPE_CODE[rows.dtype], _lib.stream_handle(None)), "combine_rows_backward")
-        return drows, dw, None, None, None, None
+            dout = dout.contiguous()
+            if need_rows:
+                drows = torch.empty_like(rows)
+            if need_weights:
+                dw = torch.empty_like(weights)
+            rc = _lib.load().flymoe_combine_rows_backward(
+                dout.data_ptr(), rows.data_ptr(), weights.data_ptr(), drows.data_ptr() if need_rows else None,
+                dw.data_ptr() if need_weights else None, sorted_ids.data_ptr(), num_valid_ids.data_ptr(),
+                row_index.data_ptr(), tokens, topk, count, dim, _lib.DTYPE_CODE[rows.dtype], _lib.stream_handle(None))
+        if rc:
+            _lib.check(rc, "combine_rows_backward")
+        return drows, dw, None
 
 
 def moe_combine(rows: torch.Tensor, weights: torch.Tensor, plan: RoutedRows) -> torch.Tensor:
@@ -219,4 +254,7 @@ def moe_combine(rows: torch.Tensor, weights: torch.Tensor, plan: RoutedRows) -> 
         _lib.require_cuda("weights", weights, (torch.float32,))
         require_shape("weights", weights, (tokens, topk))
         require_same_device("rows", rows.device, weights=weights)
-    return _Combine.apply(rows, weights, *plan)
+    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+        return _Combine.apply(rows, weights, plan)
+    with on(rows.device):
+        return _combine(rows, weights, plan, *weights.shape)

@@ -64,7 +64,8 @@ SIZES = [
     (64, 1024, 520, 16, 32, "tokens"), (33, 40, 1032, 128, 5, "tokens"), (130, 512, 256, 64, 3, "requests"),
     (1000, 328, 200, 32, 6, "requests"), (1500, 256, 264, 72, 2, "tokens"), (2100, 136, 72, 8, 1, "requests"), (700, 1096, 392, 48, 150, "tokens"), (512, 64, 72, 16, 1, "none"),
     (640, 1288, 328, 128, 3, "requests"), (900, 72, 64, 8, 2, "requests"), (2600, 1032, 136, 56, 5, "requests"),
-    (50, 64, 64, 40, 3, "none"), (600, 2048, 136, 104, 9, "tokens"),
+    (50, 64, 64, 40, 3, "none"), (600, 2048, 136, 104, 9, "tokens"), (900, 264, 584, 16, 8, "tokens"),
+    (777, 1032, 264, 64, 7, "tokens"), (1100, 520, 72, 56, 9, "tokens"), (640, 136, 264, 72, 4, "tokens"), (600, 72, 520, 88, 5, "tokens"),
 ]
 
 
@@ -168,6 +169,8 @@ def test_in_place_buffers_and_streams():
         lora_add(p["y"].clone().requires_grad_(), *(p[s] for s in ("x", "a", "b", "adapter_ids", "scaling")), out=buf)
     with pytest.raises(ValueError, match="dtype"):
         lora_add(p["y"].bfloat16(), *(p[s] for s in ("x", "a", "b", "adapter_ids", "scaling")))
+    with pytest.raises(ValueError, match="scaling has no gradient"):
+        lora_add(*(p[s] for s in ("y", "x", "a", "b", "adapter_ids")), p["scaling"].clone().requires_grad_())
 
 
 def test_rows_alone_equal_rows_in_a_batch_of_their_block():

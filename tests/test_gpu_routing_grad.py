@@ -136,6 +136,27 @@ def test_permute_and_combine(tokens, topk, experts, dim, dropped, dtype):
     assert torch.equal(only, drows)
 
 
+def test_what_autograd_refuses():
+    plan = route_rows(random_ids(40, 2, 8, 6), 8)
+    rows = torch.ones((80, 64), dtype=BF, device="cuda", requires_grad=True)
+    w = torch.ones((40, 2), device="cuda", requires_grad=True)
+    x = torch.ones((40, 64), device="cuda", requires_grad=True)
+    logits = torch.ones((40, 8), device="cuda", requires_grad=True)
+    for out, leaf in ((moe_combine(rows, w, plan), w), (moe_permute(x, plan), x), (topk_gating(logits, 2)[0], logits)):
+        (first,) = torch.autograd.grad(out.float().square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            first.sum().backward()
+    for out, leaf in ((moe_combine(rows, w, plan), w), (moe_permute(x, plan), x)):
+        plan.row_index.add_(0)                   # written after the forward pass
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out.sum(), leaf)
+    with torch.no_grad():
+        assert not moe_combine(rows, w, plan).requires_grad and not topk_gating(logits, 2)[0].requires_grad
+    with torch.inference_mode():
+        made = route_rows(random_ids(40, 2, 8, 6), 8)
+        assert torch.equal(moe_combine(moe_permute(x, made), w, made), x * 2)
+
+
 def test_tables_that_do_not_belong_together_lead_nowhere():
     plan = route_rows(random_ids(40, 2, 8, 6), 8)
     bad = plan.row_index.clone().reshape(-1)
