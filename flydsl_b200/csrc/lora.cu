@@ -355,7 +355,7 @@ struct AdapterGradArgs {
   int* present;                // [splits, adapters]: whether the split has rows of the adapter, when splits > 1
   int rows, rank, adapters, splits;
 };
-constexpr int kWgCols = 128, kWgRows = 32, kWgStages = 4, kWgList = 1024;
+constexpr int kWgThreads = 256, kWgCols = 256, kWgRows = 32, kWgList = 1024;
 constexpr int kWgRank = 64;                      // ranks a block sums up; more are shared out
 constexpr int kWgXStride = kWgCols * 2 + 16;     // 16 bytes of skew: a matrix's eight rows lie in different banks
 
@@ -366,27 +366,28 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+template <int NT> constexpr int wg_stages() { return NT <= 4 ? 4 : 3; }     // two blocks an SM
 template <int NT> constexpr int wg_v_stride() { return NT * 16 + 16; }
 template <int NT> constexpr size_t wg_smem() {
-  return size_t(kWgStages) * kWgRows * (kWgXStride + NT * 32) + 2 * 2 * kWgRows * size_t(wg_v_stride<NT>());
+  return size_t(wg_stages<NT>()) * kWgRows * (kWgXStride + NT * 32) + 2 * 2 * kWgRows * size_t(wg_v_stride<NT>());
 }
 
-// A block takes 128 columns (and up to 64 ranks) of a gradient and one split of the rows, and goes through the adapters with
-// rows in it: it lists an adapter's rows by scanning the ids, gathers them 32 at a time (cp.async, four chunks in flight)
+// A block takes 256 columns (and up to 64 ranks) of a gradient and one split of the rows, and goes through the adapters with
+// rows in it: it lists an adapter's rows by scanning the ids, gathers them 32 at a time (cp.async, three or two chunks in flight)
 // and contracts over them; both operands are read across their rows with transposing ldmatrix.  Splits are pieces of the
 // batch, so blocks have like amounts of rows however the adapters share them.  fp16: chunks of v share a running power of
 // two; when a chunk needs a larger one the sums are brought to it.
 template <typename T, int NT>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kWgThreads, 2)
 lora_wgrad_kernel(const AdapterGradArgs p) {
-  constexpr int RP = NT * 8, VS = wg_v_stride<NT>();
+  constexpr int RP = NT * 8, VS = wg_v_stride<NT>(), kStages = wg_stages<NT>();
   constexpr bool kHalf = std::is_same<T, __half>::value;
   extern __shared__ __align__(16) uint8_t sm[];
   uint8_t* xs = sm;                                                     // [stages][32][kWgXStride]
-  float* vf = reinterpret_cast<float*>(sm + kWgStages * kWgRows * kWgXStride);      // [stages][32][RP]
-  uint8_t* vh = sm + kWgStages * kWgRows * (kWgXStride + RP * 4);       // [2][hi, lo][32][VS]
-  __shared__ int list[kWgList + kWgRows], warp_n[4], next_adapter;
-  __shared__ float warp_max[4];
+  float* vf = reinterpret_cast<float*>(sm + kStages * kWgRows * kWgXStride);      // [stages][32][RP]
+  uint8_t* vh = sm + kStages * kWgRows * (kWgXStride + RP * 4);       // [2][hi, lo][32][VS]
+  __shared__ int list[kWgList + kWgRows], warp_n[8], next_adapter;
+  __shared__ float warp_max[8];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const bool second = int(blockIdx.x) >= p.g[0].tiles;
   const AdapterGrad q = second ? p.g[1] : p.g[0];
@@ -402,7 +403,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
     if (tid == 0) next_adapter = p.adapters;
     __syncthreads();
     int best = p.adapters;
-    for (int i = begin + tid; i < end; i += 128) {
+    for (int i = begin + tid; i < end; i += kWgThreads) {
       const int id = __ldg(p.ids + i);
       if (id > l && id < best) best = id;
     }
@@ -416,12 +417,12 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
   auto skip_adapters = [&](int from, int to) {
     if (p.splits > 1) {
       if (blockIdx.x == 0 && blockIdx.z == 0)
-        for (int l = from + tid; l < to; l += 128) p.present[(long long)blockIdx.y * p.adapters + l] = 0;
+        for (int l = from + tid; l < to; l += kWgThreads) p.present[(long long)blockIdx.y * p.adapters + l] = 0;
       return;
     }
     const int jn = min(kWgRank, p.rank - j0), cn = min(kWgCols, q.cols - col0);
     for (int l = from; l < to; ++l)
-      for (int i = tid; i < jn * cn; i += 128) {
+      for (int i = tid; i < jn * cn; i += kWgThreads) {
         const long long at = q.rank_major ? (long long)(j0 + i / cn) * q.cols + col0 + i % cn
                                           : (long long)(col0 + i / jn) * p.rank + j0 + i % jn;
         static_cast<T*>(q.out)[(long long)l * mat + at] = T(0.f);
@@ -447,11 +448,11 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
       taken = 0;
       while (have < kWgRows && next < end) {
         // 1024 ids, warp by warp 32 in a row
-        uint32_t mine[8];
+        uint32_t mine[4];
         int n = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int at = next + (warp * 8 + i) * 32 + lane;
+        for (int i = 0; i < 4; ++i) {
+          const int at = next + (warp * 4 + i) * 32 + lane;
           mine[i] = __ballot_sync(0xffffffffu, at < end && __ldg(p.ids + at) == l);
           n += __popc(mine[i]);
         }
@@ -459,13 +460,13 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
         __syncthreads();
         int pos = have, all = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
           if (i < warp) pos += warp_n[i];
           all += warp_n[i];
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if ((mine[i] >> lane) & 1) list[pos + __popc(mine[i] & ((1u << lane) - 1))] = next + (warp * 8 + i) * 32 + lane;
+        for (int i = 0; i < 4; ++i) {
+          if ((mine[i] >> lane) & 1) list[pos + __popc(mine[i] & ((1u << lane) - 1))] = next + (warp * 4 + i) * 32 + lane;
           pos += __popc(mine[i]);
         }
         have += all;
@@ -479,15 +480,16 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
       const int n = min(kWgRows, have - taken);
       if (n > 0) {
 #pragma unroll
-        for (int i0 = 0; i0 < kWgRows * (kWgCols / 8); i0 += 128) {
+        for (int i0 = 0; i0 < kWgRows * (kWgCols / 8); i0 += kWgThreads) {
           const int i = i0 + tid, r = i / (kWgCols / 8), c = i - r * (kWgCols / 8);
           const bool ok = r < n && col0 + c * 8 < q.cols;
           const T* src = X + (long long)list[taken + (r < n ? r : 0)] * q.cols + (ok ? col0 + c * 8 : 0);
           cp_async16(smem_u32(xs + (stage * kWgRows + r) * kWgXStride + c * 16), src, ok);
         }
 #pragma unroll
-        for (int i0 = 0; i0 < kWgRows * (RP / 4); i0 += 128) {
+        for (int i0 = 0; i0 < kWgRows * (RP / 4); i0 += kWgThreads) {
           const int i = i0 + tid, r = i / (RP / 4), c = i - r * (RP / 4);
+          if (i >= kWgRows * (RP / 4)) break;
           const bool ok = r < n && j0 + c * 4 < p.rank;
           const float* src = q.v + (long long)list[taken + (r < n ? r : 0)] * p.rank + (ok ? j0 + c * 4 : 0);
           cp_async16(smem_u32(vf + (stage * kWgRows + r) * RP + c * 4), src, ok);
@@ -508,12 +510,12 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
     // a chunk's v as high parts and remainders, into one of two buffers
     auto convert = [&](int i) {
       uint8_t* vb = vh + (i & 1) * 2 * kWgRows * VS;
-      const float* vc = vf + (i % kWgStages) * kWgRows * RP;
+      const float* vc = vf + (i % kStages) * kWgRows * RP;
       float down = 1.f;
       if constexpr (kHalf) {
         float amax = 0.f;
 #pragma unroll
-        for (int e = tid; e < kWgRows * RP / 4; e += 128) {
+        for (int e = tid; e < kWgRows * RP / 4; e += kWgThreads) {
           const float4 x = reinterpret_cast<const float4*>(vc)[e];
           amax = fmaxf(amax, fmaxf(fmaxf(finite_abs(x.x), finite_abs(x.y)), fmaxf(finite_abs(x.z), finite_abs(x.w))));
         }
@@ -521,13 +523,14 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
         for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, off));
         if (lane == 0) warp_max[warp] = amax;
         __syncthreads();
-        amax = fmaxf(fmaxf(warp_max[0], warp_max[1]), fmaxf(warp_max[2], warp_max[3]));
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, warp_max[i]);
         const int e = scale_exponent(amax);
         if (amax > 0.f && e > next_exponent) next_exponent = e;
         down = next_exponent < -110 ? 1.f : exp2i(-next_exponent);
       }
 #pragma unroll
-      for (int e = tid; e < kWgRows * RP / 4; e += 128) {
+      for (int e = tid; e < kWgRows * RP / 4; e += kWgThreads) {
         const int r = e / (RP / 4), j = e - r * (RP / 4);
         const float4 x = reinterpret_cast<const float4*>(vc)[e];
         uint2 h, w;
@@ -538,13 +541,13 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
       }
     };
 #pragma unroll
-    for (int s = 0; s < kWgStages - 1; ++s) filled |= load(s) > 0 ? 1u << s : 0u;
-    asm volatile("cp.async.wait_group %0;" ::"n"(kWgStages - 2) : "memory");
+    for (int s = 0; s < kStages - 1; ++s) filled |= load(s) > 0 ? 1u << s : 0u;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncthreads();
     convert(0);                                  // an adapter in the list has a row
-    // one barrier a chunk: chunk i is multiplied while chunk i + 1 is converted and chunk i + 3 asked for
-    for (int i = 0; (filled >> (i % kWgStages)) & 1; ++i) {
-      const int stage = i % kWgStages;
+    // one barrier a chunk: chunk i is multiplied while chunk i + 1 is converted and a later one asked for
+    for (int i = 0; (filled >> (i % kStages)) & 1; ++i) {
+      const int stage = i % kStages;
       if constexpr (kHalf) {
         if (next_exponent > exponent) {          // the scale that chunk i was converted with
           if (exponent >= -110) {
@@ -557,12 +560,12 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
           exponent = next_exponent;
         }
       }
-      asm volatile("cp.async.wait_group %0;" ::"n"(kWgStages - 3) : "memory");
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 3) : "memory");
       __syncthreads();                           // chunk i + 1 is here, chunk i converted, chunk i - 1 multiplied
-      const int into = (i + kWgStages - 1) % kWgStages;
+      const int into = (i + kStages - 1) % kStages;
       const bool got = load(into) > 0;
       filled = (filled & ~(1u << into)) | (got ? 1u << into : 0u);
-      if ((filled >> ((i + 1) % kWgStages)) & 1) convert(i + 1);
+      if ((filled >> ((i + 1) % kStages)) & 1) convert(i + 1);
       uint8_t* vb = vh + (i & 1) * 2 * kWgRows * VS;
       const uint32_t xa = smem_u32(xs + stage * kWgRows * kWgXStride) +
                           ((lane >> 4) * 8 + (lane & 7)) * kWgXStride + (warp * 32 + ((lane >> 3) & 1) * 8) * 2;
@@ -749,7 +752,7 @@ static int launch_wgrad(const AdapterGradArgs& p, cudaStream_t stream) {
   auto* kernel = lora_wgrad_kernel<T, NT>;
   static SmemLimitSeen seen;
   FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(wg_smem<NT>()), seen));
-  FLYMOE_CUDA_CHECK(launch_closely(kernel, dim3(p.g[0].tiles + p.g[1].tiles, p.splits, ceil_div(p.rank, kWgRank)), 128,
+  FLYMOE_CUDA_CHECK(launch_closely(kernel, dim3(p.g[0].tiles + p.g[1].tiles, p.splits, ceil_div(p.rank, kWgRank)), kWgThreads,
                                    wg_smem<NT>(), stream, p));
   if (p.splits == 1) return FLYMOE_OK;
   const long long most = (long long)std::max(p.g[0].cols, p.g[1].cols) * p.rank * p.adapters / 4;
@@ -814,7 +817,7 @@ static bool needs_transposed(int rows, int rank, int adapters) { return !on_tile
 // from rank 33 on), at least 256 rows in a piece, and partial sums of 256 MB at most.
 static int wgrad_splits(int rows, int k, int n, int rank, int adapters) {
   const long long blocks = (long long)(ceil_div(k, kWgCols) + ceil_div(n, kWgCols)) * ceil_div(rank, kWgRank);
-  const long long want = (rank <= 32 ? 3LL : 2LL) * sm_count() / blocks;
+  const long long want = 2LL * sm_count() / blocks;
   const long long fit = (256LL << 20) / ((long long)adapters * rank * ((long long)k + n) * 4);
   return int(std::max(1LL, std::min({(long long)kLoraMaxSplits, want, fit, (long long)rows / 256})));
 }
