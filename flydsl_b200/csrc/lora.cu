@@ -340,28 +340,9 @@ lora_expand_kernel(const ExpandArgs p, const int slots, const int per_warp, cons
 }
 
 // ---------------------------------------------------------------------------- gradients of the adapters
-struct AdapterGrad {
-  const void* x;               // [rows, cols]: x for dA, dout for dB
-  const float* v;              // [rows, rank]: dv for dA, v for dB
-  void* out;                   // dA [adapters, rank, cols], dB [adapters, cols, rank]
-  float* partial;              // [splits, adapters, cols, rank] in out's order, when splits > 1
-  int cols, tiles;
-  int rank_major;              // dA: columns are the inner axis
-};
-struct AdapterGradArgs {
-  AdapterGrad g[2];
-  const int* ids;
-  const float* scaling;
-  int* present;                // [splits, adapters]: whether the split has rows of the adapter, when splits > 1
-  int rows, rank, adapters, splits;
-};
-constexpr int kWgThreads = 256, kWgCols = 256, kWgRows = 32, kWgList = 1024;
-constexpr int kWgRank = 64;                      // ranks a block sums up; more are shared out
+constexpr int kWgThreads = 256, kWgRows = 32, kWgList = 1024;
 constexpr int kWgXStride = kWgCols * 2 + 16;     // 16 bytes of skew: a matrix's eight rows lie in different banks
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t* r, uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -377,11 +358,11 @@ template <int NT> constexpr size_t wg_smem() {
 // and contracts over them; both operands are read across their rows with transposing ldmatrix.  Splits are pieces of the
 // batch, so blocks have like amounts of rows however the adapters share them.  fp16: chunks of v share a running power of
 // two; when a chunk needs a larger one the sums are brought to it.
-template <typename T, int NT>
+template <int NT>
 __global__ void __launch_bounds__(kWgThreads, 2)
 lora_wgrad_kernel(const AdapterGradArgs p) {
   constexpr int RP = NT * 8, VS = wg_v_stride<NT>(), kStages = wg_stages<NT>();
-  constexpr bool kHalf = std::is_same<T, __half>::value;
+  using T = __half;
   extern __shared__ __align__(16) uint8_t sm[];
   uint8_t* xs = sm;                                                     // [stages][32][kWgXStride]
   float* vf = reinterpret_cast<float*>(sm + kStages * kWgRows * kWgXStride);      // [stages][32][RP]
@@ -512,7 +493,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
       uint8_t* vb = vh + (i & 1) * 2 * kWgRows * VS;
       const float* vc = vf + (i % kStages) * kWgRows * RP;
       float down = 1.f;
-      if constexpr (kHalf) {
+      {
         float amax = 0.f;
 #pragma unroll
         for (int e = tid; e < kWgRows * RP / 4; e += kWgThreads) {
@@ -548,7 +529,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
     // one barrier a chunk: chunk i is multiplied while chunk i + 1 is converted and a later one asked for
     for (int i = 0; (filled >> (i % kStages)) & 1; ++i) {
       const int stage = i % kStages;
-      if constexpr (kHalf) {
+      {
         if (next_exponent > exponent) {          // the scale that chunk i was converted with
           if (exponent >= -110) {
             const float f = exp2i(max(-126, exponent - next_exponent));
@@ -596,7 +577,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
     const float s = (p.splits == 1 ? __ldg(p.scaling + l) : 1.f);
-    const float up = kHalf && exponent >= -110 ? exp2i(exponent) : 1.f;
+    const float up = exponent >= -110 ? exp2i(exponent) : 1.f;
 #pragma unroll
     for (int f = 0; f < 2; ++f)
 #pragma unroll
@@ -747,22 +728,23 @@ static int launch_expand_rank(const ExpandArgs& p, int skip, cudaStream_t s) {
   return p.rank <= 16 ? launch_expand<T, 1>(p, skip, s) : p.rank <= 32 ? launch_expand<T, 2>(p, skip, s)
        : p.rank <= 64 ? launch_expand<T, 4>(p, skip, s) : launch_expand<T, 8>(p, skip, s);
 }
-template <typename T, int NT>
-static int launch_wgrad(const AdapterGradArgs& p, cudaStream_t stream) {
-  auto* kernel = lora_wgrad_kernel<T, NT>;
+template <int NT>
+static int launch_wgrad_f16(const AdapterGradArgs& p, cudaStream_t stream) {
+  auto* kernel = lora_wgrad_kernel<NT>;
   static SmemLimitSeen seen;
   FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(wg_smem<NT>()), seen));
   FLYMOE_CUDA_CHECK(launch_closely(kernel, dim3(p.g[0].tiles + p.g[1].tiles, p.splits, ceil_div(p.rank, kWgRank)), kWgThreads,
                                    wg_smem<NT>(), stream, p));
-  if (p.splits == 1) return FLYMOE_OK;
-  const long long most = (long long)std::max(p.g[0].cols, p.g[1].cols) * p.rank * p.adapters / 4;
-  FLYMOE_CUDA_CHECK(launch_closely(lora_wgrad_finish_kernel<T>, dim3(unsigned(std::min<long long>((most + 255) / 256, 8LL * sm_count())), 2),
-                                   256, 0, stream, p));
   return FLYMOE_OK;
 }
-template <typename T>
-static int launch_wgrad_rank(const AdapterGradArgs& p, cudaStream_t s) {
-  return p.rank <= 16 ? launch_wgrad<T, 2>(p, s) : p.rank <= 32 ? launch_wgrad<T, 4>(p, s) : launch_wgrad<T, 8>(p, s);
+static int launch_wgrad(const AdapterGradArgs& p, bool bf, cudaStream_t s) {
+  const int rc = bf ? launch_wgrad_sm100(p, s) : p.rank <= 16 ? launch_wgrad_f16<2>(p, s)
+               : p.rank <= 32 ? launch_wgrad_f16<4>(p, s) : launch_wgrad_f16<8>(p, s);
+  if (rc != FLYMOE_OK || p.splits == 1) return rc;
+  const long long most = (long long)std::max(p.g[0].cols, p.g[1].cols) * p.rank * p.adapters / 4;
+  FLYMOE_CUDA_CHECK(launch_closely(bf ? lora_wgrad_finish_kernel<__nv_bfloat16> : lora_wgrad_finish_kernel<__half>,
+                                   dim3(unsigned(std::min<long long>((most + 255) / 256, 8LL * sm_count())), 2), 256, 0, s, p));
+  return FLYMOE_OK;
 }
 
 // Floats of v: the sum and, where there are several, the splits behind it.
@@ -925,5 +907,5 @@ extern "C" int flymoe_lora_backward(void* dx, void* da, void* db, const void* do
   p.rank = rank;
   p.adapters = adapters;
   p.splits = w.splits;
-  return dtype == FLYMOE_BF16 ? launch_wgrad_rank<__nv_bfloat16>(p, s) : launch_wgrad_rank<__half>(p, s);
+  return launch_wgrad(p, dtype == FLYMOE_BF16, s);
 }

@@ -53,6 +53,28 @@ struct ExpandArgs {
   int rows, n, rank, adapters, splits, transposed;
 };
 
+struct AdapterGrad {
+  const void* x;               // [rows, cols]: x for dA, dout for dB
+  const float* v;              // [rows, rank]: dv for dA, v for dB
+  void* out;                   // dA [adapters, rank, cols], dB [adapters, cols, rank]
+  float* partial;              // [splits, adapters, cols, rank] in out's order, when splits > 1
+  int cols, tiles;
+  int rank_major;              // dA: columns are the inner axis
+};
+struct AdapterGradArgs {
+  AdapterGrad g[2];
+  const int* ids;
+  const float* scaling;
+  int* present;                // [splits, adapters]: whether the split has rows of the adapter, when splits > 1
+  int rows, rank, adapters, splits;
+};
+constexpr int kWgCols = 256;                     // columns of a gradient a block sums up
+constexpr int kWgRank = 64;                      // and its ranks; more are shared out
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+
 // The launches of one operator follow each other closely (programmatic stream serialisation): the next one's blocks start,
 // and set up what touches no global memory, while the last blocks of this one run.  Every kernel launched this way waits
 // here before its first access to global memory; the wait ends when all launches before it are done.
@@ -82,6 +104,7 @@ constexpr int kTileAdapters = 8;
 __host__ __device__ inline int tile_limit(int rank) { return rank <= 64 ? kTileAdapters : kTileAdapters / 2; }
 int launch_shrink_sm100(const ShrinkArgs& p, int bf16, cudaStream_t stream);
 int launch_expand_sm100(const ExpandArgs& p, int bf16, cudaStream_t stream);
+int launch_wgrad_sm100(const AdapterGradArgs& p, cudaStream_t stream);           // bf16 (lora_grad_sm100.cu)
 
 // Distinct adapters among the 128 ids that a warp holds, four a lane (negative: none): their number, most + 1 if there are
 // more, and the first `most` of them in `list` (written by lane 0).
