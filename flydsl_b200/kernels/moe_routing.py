@@ -36,18 +36,23 @@ class RoutedRows(NamedTuple):
     row_index: torch.Tensor
 
 
-def _combine_fits(rows, weights, plan):
-    """Whether the arguments are right, in as few steps as it takes; ``_check_plan`` and the rest say what is not."""
+def _combine_sizes(rows, weights, plan):
+    """(tokens, topk, rows, dim) if the arguments are right, in as few steps as it takes; ``_check_plan`` and the rest say
+    what is not."""
     try:
-        (sorted_ids, nv, _, row_index), dev, i32 = plan, rows.device, torch.int32
-        return (rows.is_cuda and rows.dtype in _FLOATS and rows.dim() == 2 and rows.shape[1] >= 8 and not rows.shape[1] % 8
-                and weights.shape == row_index.shape and weights.dim() == 2 and weights.dtype is torch.float32
-                and sorted_ids.numel() >= rows.shape[0] and nv.numel() >= 1 and sorted_ids.dtype is i32 and nv.dtype is i32
-                and row_index.dtype is i32 and weights.device == dev and sorted_ids.device == dev and nv.device == dev
-                and row_index.device == dev and rows.is_contiguous() and weights.is_contiguous()
-                and sorted_ids.is_contiguous() and nv.is_contiguous() and row_index.is_contiguous())
+        (sorted_ids, nv, _, row_index), dev, i32 = plan, rows.get_device(), torch.int32
+        (count, dim), pairs = rows.shape, weights.shape
+        tokens, topk = pairs
+        if (rows.is_cuda and rows.dtype in _FLOATS and dim >= 8 and not dim % 8 and row_index.shape == pairs
+                and weights.dtype is torch.float32 and sorted_ids.numel() >= count and nv.numel() >= 1
+                and sorted_ids.dtype is i32 and nv.dtype is i32 and row_index.dtype is i32
+                and dev == weights.get_device() == sorted_ids.get_device() == nv.get_device() == row_index.get_device()
+                and rows.is_contiguous() and weights.is_contiguous() and sorted_ids.is_contiguous() and nv.is_contiguous()
+                and row_index.is_contiguous()):
+            return tokens, topk, count, dim
     except (AttributeError, TypeError, ValueError):
-        return False
+        pass
+    return None
 
 
 def _check_plan(plan: RoutedRows, name: str, t: torch.Tensor, rows: int) -> tuple[int, int]:
@@ -153,13 +158,13 @@ def route_rows(topk_ids: torch.Tensor, num_experts: int) -> RoutedRows:
 
 
 # ------------------------------------------------------------------------- rows
-def _combine(rows, weights, plan, tokens, topk):
-    (count, dim), (sorted_ids, num_valid_ids, _, row_index) = rows.shape, plan
-    out = rows.new_empty((tokens, dim))
-    rc = _lib.load().flymoe_combine_rows(
-        rows.data_ptr(), None if weights is None else weights.data_ptr(), out.data_ptr(), sorted_ids.data_ptr(),
-        num_valid_ids.data_ptr(), row_index.data_ptr(), tokens, topk, count, dim, _lib.DTYPE_CODE[rows.dtype],
-        _lib.stream_handle(None))
+def _combine(rows, weights, plan, sizes):
+    sorted_ids, num_valid_ids, _, row_index = plan
+    with on(rows.device):
+        out = rows.new_empty((sizes[0], sizes[3]))
+        rc = _lib.load().flymoe_combine_rows(
+            rows.data_ptr(), None if weights is None else weights.data_ptr(), out.data_ptr(), sorted_ids.data_ptr(),
+            num_valid_ids.data_ptr(), row_index.data_ptr(), *sizes, _lib.DTYPE_CODE[rows.dtype], _lib.stream_handle(None))
     if rc:
         _lib.check(rc, "combine_rows")
     return out
@@ -201,9 +206,9 @@ class _Permute(torch.autograd.Function):
     @once
     def backward(ctx, dxs):
         plan = _kept_plan(ctx)
-        dxs = dxs.contiguous()
         with on(dxs.device):
-            return _combine(dxs, None, plan, *plan[3].shape), None
+            dxs = dxs.contiguous()
+        return _combine(dxs, None, plan, (*plan[3].shape, *dxs.shape)), None
 
 
 def moe_permute(x: torch.Tensor, plan: RoutedRows) -> torch.Tensor:
@@ -217,20 +222,19 @@ def moe_permute(x: torch.Tensor, plan: RoutedRows) -> torch.Tensor:
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, weights, plan):
+    def forward(ctx, rows, weights, plan, sizes):
         ctx.save_for_backward(rows, weights)
         _keep_plan(ctx, plan)
-        tokens, topk = weights.shape
-        with on(rows.device):
-            return _combine(rows, weights, plan, tokens, topk)
+        ctx.sizes = sizes
+        return _combine(rows, weights, plan, sizes)
 
     @staticmethod
     @once
     def backward(ctx, dout):
         rows, weights = ctx.saved_tensors
         sorted_ids, num_valid_ids, _, row_index = _kept_plan(ctx)
-        (tokens, topk), (count, dim), drows, dw = weights.shape, rows.shape, None, None
-        need_rows, need_weights, _ = ctx.needs_input_grad
+        need_rows, need_weights, _, _ = ctx.needs_input_grad
+        drows = dw = None
         with on(rows.device):
             dout = dout.contiguous()
             if need_rows:
@@ -240,21 +244,22 @@ class _Combine(torch.autograd.Function):
             rc = _lib.load().flymoe_combine_rows_backward(
                 dout.data_ptr(), rows.data_ptr(), weights.data_ptr(), drows.data_ptr() if need_rows else None,
                 dw.data_ptr() if need_weights else None, sorted_ids.data_ptr(), num_valid_ids.data_ptr(),
-                row_index.data_ptr(), tokens, topk, count, dim, _lib.DTYPE_CODE[rows.dtype], _lib.stream_handle(None))
+                row_index.data_ptr(), *ctx.sizes, _lib.DTYPE_CODE[rows.dtype], _lib.stream_handle(None))
         if rc:
             _lib.check(rc, "combine_rows_backward")
-        return drows, dw, None
+        return drows, dw, None, None
 
 
 def moe_combine(rows: torch.Tensor, weights: torch.Tensor, plan: RoutedRows) -> torch.Tensor:
     """rows [any, dim] in expert order, weights f32 [tokens, topk] -> [tokens, dim]; gradients reach rows and weights."""
-    if not _combine_fits(rows, weights, plan):
+    sizes = _combine_sizes(rows, weights, plan)
+    if sizes is None:
         _require_rows("rows", rows)
         tokens, topk = _check_plan(plan, "rows", rows, rows.shape[0])
         _lib.require_cuda("weights", weights, (torch.float32,))
         require_shape("weights", weights, (tokens, topk))
         require_same_device("rows", rows.device, weights=weights)
+        sizes = tokens, topk, *rows.shape
     if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
-        return _Combine.apply(rows, weights, plan)
-    with on(rows.device):
-        return _combine(rows, weights, plan, *weights.shape)
+        return _Combine.apply(rows, weights, plan, sizes)
+    return _combine(rows, weights, plan, sizes)
