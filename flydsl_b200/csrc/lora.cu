@@ -374,16 +374,18 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
   const AdapterGrad q = second ? p.g[1] : p.g[0];
   const int col0 = (second ? int(blockIdx.x) - p.g[0].tiles : int(blockIdx.x)) * kWgCols;
   const int j0 = int(blockIdx.z) * kWgRank;      // first of this block's ranks
-  const int begin = int((long long)p.rows * blockIdx.y / p.splits), end = int((long long)p.rows * (blockIdx.y + 1) / p.splits);
+  const int split = int(blockIdx.y) / p.groups, group = int(blockIdx.y) - split * p.groups;
+  const int group_begin = int((long long)p.adapters * group / p.groups), group_end = int((long long)p.adapters * (group + 1) / p.groups);
+  const int begin = int((long long)p.rows * split / p.splits), end = int((long long)p.rows * (split + 1) / p.splits);
   const T* X = static_cast<const T*>(q.x);
   const long long mat = (long long)q.cols * p.rank;
   after_previous_launch();
 
-  // the smallest adapter above `l` with rows here, or p.adapters
+  // the smallest adapter above `l` with rows here, or the end of the group
   auto find_next = [&](int l) -> int {
-    if (tid == 0) next_adapter = p.adapters;
+    if (tid == 0) next_adapter = group_end;
     __syncthreads();
-    int best = p.adapters;
+    int best = group_end;
     for (int i = begin + tid; i < end; i += kWgThreads) {
       const int id = __ldg(p.ids + i);
       if (id > l && id < best) best = id;
@@ -398,7 +400,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
   auto skip_adapters = [&](int from, int to) {
     if (p.splits > 1) {
       if (blockIdx.x == 0 && blockIdx.z == 0)
-        for (int l = from + tid; l < to; l += kWgThreads) p.present[(long long)blockIdx.y * p.adapters + l] = 0;
+        for (int l = from + tid; l < to; l += kWgThreads) p.present[(long long)split * p.adapters + l] = 0;
       return;
     }
     const int jn = min(kWgRank, p.rank - j0), cn = min(kWgCols, q.cols - col0);
@@ -410,11 +412,11 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
       }
   };
 
-  int done = 0;                                  // adapters below this one are dealt with
-  for (int l = find_next(-1); l < p.adapters; l = find_next(l)) {
+  int done = group_begin;                        // adapters below this one are dealt with
+  for (int l = find_next(group_begin - 1); l < group_end; l = find_next(l)) {
     skip_adapters(done, l);
     done = l + 1;
-    if (p.splits > 1 && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) p.present[(long long)blockIdx.y * p.adapters + l] = 1;
+    if (p.splits > 1 && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) p.present[(long long)split * p.adapters + l] = 1;
 
     int next = begin, taken = 0, have = 0;       // ids scanned, entries of the list used and in it (same in all threads)
     // appends rows of this adapter until the list holds a chunk or the rows are through
@@ -590,7 +592,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
           const long long at = q.rank_major ? (long long)j * q.cols + col : (long long)col * p.rank + j;
           const long long step = q.rank_major ? q.cols : 1;
           if (p.splits > 1) {
-            float* o = q.partial + ((long long)blockIdx.y * p.adapters + l) * mat + at;
+            float* o = q.partial + ((long long)split * p.adapters + l) * mat + at;
             o[0] = v0;
             o[step] = v1;
           } else {
@@ -602,7 +604,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
         }
     __syncthreads();                             // the list and the stages are free for the next adapter
   }
-  skip_adapters(done, p.adapters);
+  skip_adapters(done, group_end);
 }
 
 // out = s_l * sum of the splits' partials that hold rows of the adapter, in split order.
@@ -733,7 +735,7 @@ static int launch_wgrad_f16(const AdapterGradArgs& p, cudaStream_t stream) {
   auto* kernel = lora_wgrad_kernel<NT>;
   static SmemLimitSeen seen;
   FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(wg_smem<NT>()), seen));
-  FLYMOE_CUDA_CHECK(launch_closely(kernel, dim3(p.g[0].tiles + p.g[1].tiles, p.splits, ceil_div(p.rank, kWgRank)), kWgThreads,
+  FLYMOE_CUDA_CHECK(launch_closely(kernel, dim3(p.g[0].tiles + p.g[1].tiles, p.splits * p.groups, ceil_div(p.rank, kWgRank)), kWgThreads,
                                    wg_smem<NT>(), stream, p));
   return FLYMOE_OK;
 }
@@ -795,13 +797,19 @@ static int run_chain(const Chain& c, cudaStream_t s) {
 // Whether a backward pass reads A and B through the kernels of this file, which want the contraction along a row.
 static bool needs_transposed(int rows, int rank, int adapters) { return !on_tiles(rows) || adapters > tile_limit(rank); }
 
-// Pieces of the batch that the adapters' gradients are summed over: blocks for every place on the device (three an SM, two
-// from rank 33 on), at least 256 rows in a piece, and partial sums of 256 MB at most.
+// Blocks for every place on the device (two an SM) that the adapters' gradients are shared out to, besides their columns:
+// pieces of the batch, whose blocks have like amounts of rows however the adapters share them, and groups of adapters, which
+// need no partial sums.  Pieces as long as their sums, written and read again, move half the bytes of the rows at most, with
+// at least 256 rows in a piece; then groups.
+static int wgrad_places(int k, int n, int rank) {
+  return 2 * sm_count() / ((ceil_div(k, kWgCols) + ceil_div(n, kWgCols)) * ceil_div(rank, kWgRank));
+}
 static int wgrad_splits(int rows, int k, int n, int rank, int adapters) {
-  const long long blocks = (long long)(ceil_div(k, kWgCols) + ceil_div(n, kWgCols)) * ceil_div(rank, kWgRank);
-  const long long want = 2LL * sm_count() / blocks;
-  const long long fit = (256LL << 20) / ((long long)adapters * rank * ((long long)k + n) * 4);
-  return int(std::max(1LL, std::min({(long long)kLoraMaxSplits, want, fit, (long long)rows / 256})));
+  const long long fit = rows / (8LL * adapters * rank);
+  return int(std::max(1LL, std::min({(long long)kLoraMaxSplits, (long long)wgrad_places(k, n, rank), fit, rows / 256LL})));
+}
+static int wgrad_groups(int splits, int k, int n, int rank, int adapters) {
+  return std::max(1, std::min(wgrad_places(k, n, rank) / splits, adapters));
 }
 // The backward pass's scratch, in floats: dv | A transposed | B transposed | partial sums, 16-byte aligned each.
 struct BackwardScratch {
@@ -907,5 +915,6 @@ extern "C" int flymoe_lora_backward(void* dx, void* da, void* db, const void* do
   p.rank = rank;
   p.adapters = adapters;
   p.splits = w.splits;
+  p.groups = wgrad_groups(w.splits, k, n, rank, adapters);
   return launch_wgrad(p, dtype == FLYMOE_BF16, s);
 }

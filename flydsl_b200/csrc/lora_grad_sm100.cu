@@ -44,8 +44,8 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t* v) {
         "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(taddr));
 }
 
-// A block takes 256 columns (and up to RP ranks) of a gradient and one split of the rows, and goes through the adapters with
-// rows in it.  Warps 0..7 gather, warp 8 multiplies, warps 9..12 write the sums.  RP: its ranks, rounded up.
+// A block takes 256 columns (and up to RP ranks) of a gradient, one split of the rows and one group of adapters, and goes
+// through those that have rows in it.  Warps 0..7 gather, warp 8 multiplies, warps 9..12 write the sums.  RP: its ranks, rounded up.
 template <int RP>
 __global__ void __launch_bounds__(kGradThreads, 2)
 lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
@@ -64,6 +64,7 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
   const int j0 = int(blockIdx.z) * kWgRank;      // first of this block's ranks
   const int ranks = min(kWgRank, p.rank - j0);
   const long long mat = (long long)q.cols * p.rank;
+  const int split = int(blockIdx.y) / p.groups, group = int(blockIdx.y) - split * p.groups;
 
   if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
@@ -83,7 +84,9 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
 
   if (warp < kGradFill / 32) {
     // ------------------------------------------------------------------ gather
-    const int begin = int((long long)p.rows * blockIdx.y / p.splits), end = int((long long)p.rows * (blockIdx.y + 1) / p.splits);
+    const int begin = int((long long)p.rows * split / p.splits), end = int((long long)p.rows * (split + 1) / p.splits);
+    const int group_begin = int((long long)p.adapters * group / p.groups);
+    const int group_end = int((long long)p.adapters * (group + 1) / p.groups);
     const uint8_t* X = static_cast<const uint8_t*>(q.x);
     auto together = [] { asm volatile("bar.sync 1, %0;" ::"n"(kGradFill) : "memory"); };
     // The warps meet at a barrier without a limit, so a wait that gave up makes nobody leave: the walk through the rows goes on
@@ -92,11 +95,11 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
     int asked = 0, handed = 0;                   // chunks asked for, chunks handed over to the MMAs
     int older = 0, newer = 0;                    // adapters of up to two chunks between
 
-    // the smallest adapter above `l` with rows here, or p.adapters
+    // the smallest adapter above `l` with rows here, or the end of the group
     auto find_next = [&](int l) -> int {
-      if (tid == 0) c->next_adapter = p.adapters;
+      if (tid == 0) c->next_adapter = group_end;
       together();
-      int best = p.adapters;
+      int best = group_end;
       for (int i = begin + tid; i < end; i += kGradFill) {
         const int id = __ldg(p.ids + i);
         if (id > l && id < best) best = id;
@@ -111,7 +114,7 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
     auto skip_adapters = [&](int from, int to) {
       if (p.splits > 1) {
         if (blockIdx.x == 0 && blockIdx.z == 0)
-          for (int l = from + tid; l < to; l += kGradFill) p.present[(long long)blockIdx.y * p.adapters + l] = 0;
+          for (int l = from + tid; l < to; l += kGradFill) p.present[(long long)split * p.adapters + l] = 0;
         return;
       }
       const int cn = min(kWgCols, q.cols - col0);
@@ -153,11 +156,11 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
     const uint8_t* xsrc = X + (inside ? (long long)(col0 + piece * 8) * 2 : 0);
     const long long row_bytes = (long long)q.cols * 2;
 
-    int done = 0;                                // adapters below this one are dealt with
-    for (int l = find_next(-1); l < p.adapters; l = find_next(l)) {
+    int done = group_begin;                      // adapters below this one are dealt with
+    for (int l = find_next(group_begin - 1); l < group_end; l = find_next(l)) {
       skip_adapters(done, l);
       done = l + 1;
-      if (p.splits > 1 && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) p.present[(long long)blockIdx.y * p.adapters + l] = 1;
+      if (p.splits > 1 && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) p.present[(long long)split * p.adapters + l] = 1;
       int next = begin, taken = 0, have = 0;     // ids scanned, entries of the list used and in it (same in all threads)
       while (true) {
         if (have - taken < kGradRows && next < end) {
@@ -227,7 +230,7 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
         ++asked;
       }
     }
-    skip_adapters(done, p.adapters);
+    skip_adapters(done, group_end);
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (asked - handed == 2) hand_over(older | (newer != older ? kGradLast : 0));
     if (asked > handed) hand_over(newer | kGradLast);
@@ -285,7 +288,7 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
       if (l < 0) break;
       tcgen05_fence_after();
       const float scale = p.splits == 1 ? __ldg(p.scaling + l) : 1.f;
-      float* partial = q.partial + ((long long)blockIdx.y * p.adapters + l) * mat;
+      float* partial = q.partial + ((long long)split * p.adapters + l) * mat;
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(q.out) + (long long)l * mat;
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
@@ -345,7 +348,7 @@ static int launch(const AdapterGradArgs& p, cudaStream_t stream) {
   if (status == nullptr) return FLYMOE_ERR_CUDA;
   static SmemLimitSeen seen;
   FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(grad_smem<RP>()), seen));
-  FLYMOE_CUDA_CHECK(launch_closely(kernel, dim3(p.g[0].tiles + p.g[1].tiles, p.splits, ceil_div(p.rank, kWgRank)), kGradThreads,
+  FLYMOE_CUDA_CHECK(launch_closely(kernel, dim3(p.g[0].tiles + p.g[1].tiles, p.splits * p.groups, ceil_div(p.rank, kWgRank)), kGradThreads,
                                    grad_smem<RP>(), stream, p, status));
   return FLYMOE_OK;
 }
