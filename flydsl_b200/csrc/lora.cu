@@ -633,7 +633,8 @@ lora_wgrad_finish_kernel(const AdapterGradArgs p) {
   }
 }
 
-// dst[m][c][r] = src[m][r][c] for two sets of matrices (blockIdx.z: of the first, then of the second), 32 x 32 tiles.
+// dst[m][c][r] = src[m][r][c] for two sets of matrices (blockIdx.y: of the first, then of the second), 64 x 64 tiles, 16 bytes
+// in and out of global memory (both sizes are multiples of 8).
 struct TransposeArgs {
   const uint16_t* src[2];
   uint16_t* dst[2];
@@ -641,20 +642,31 @@ struct TransposeArgs {
 };
 __global__ void __launch_bounds__(256)
 lora_transpose_kernel(const TransposeArgs p) {
-  __shared__ uint16_t tile[32][34];
+  __shared__ uint16_t tile[64][66];
   const int which = int(blockIdx.y) >= p.mats;
-  const int rows = p.rows[which], cols = p.cols[which], across = (cols + 31) / 32;
+  const int rows = p.rows[which], cols = p.cols[which], across = (cols + 63) / 64;
   const long long mat = (long long)(int(blockIdx.y) - which * p.mats) * rows * cols;
   const uint16_t* src = p.src[which] + mat;
   uint16_t* dst = p.dst[which] + mat;
   after_previous_launch();
-  for (int t = blockIdx.x; t < across * ((rows + 31) / 32); t += gridDim.x) {
-    const int c0 = t % across * 32, r0 = t / across * 32, x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    for (int i = y; i < 32; i += 8)
-      if (r0 + i < rows && c0 + x < cols) tile[i][x] = src[(long long)(r0 + i) * cols + c0 + x];
+  for (int t = blockIdx.x; t < across * ((rows + 63) / 64); t += gridDim.x) {
+    const int c0 = t % across * 64, r0 = t / across * 64, x = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;
+#pragma unroll
+    for (int i = y; i < 64; i += 32)
+      if (r0 + i < rows && c0 + x < cols) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + (long long)(r0 + i) * cols + c0 + x));
+        uint32_t* to = reinterpret_cast<uint32_t*>(&tile[i][x]);
+        to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+      }
     __syncthreads();
-    for (int i = y; i < 32; i += 8)
-      if (c0 + i < cols && r0 + x < rows) dst[(long long)(c0 + i) * rows + r0 + x] = tile[x][i];
+#pragma unroll
+    for (int i = y; i < 64; i += 32)
+      if (c0 + i < cols && r0 + x < rows) {
+        uint32_t v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = uint32_t(tile[x + u * 2][i]) | uint32_t(tile[x + u * 2 + 1][i]) << 16;
+        *reinterpret_cast<uint4*>(dst + (long long)(c0 + i) * rows + r0 + x) = make_uint4(v[0], v[1], v[2], v[3]);
+      }
     __syncthreads();
   }
 }
@@ -892,7 +904,7 @@ extern "C" int flymoe_lora_backward(void* dx, void* da, void* db, const void* do
       t.src[0] = static_cast<const uint16_t*>(b); t.dst[0] = bt; t.rows[0] = n; t.cols[0] = rank;
       t.src[1] = static_cast<const uint16_t*>(a); t.dst[1] = at; t.rows[1] = rank; t.cols[1] = k;
       t.mats = adapters;
-      const int tiles = ceil_div(std::max(k, n), 32) * ceil_div(rank, 32);
+      const int tiles = ceil_div(std::max(k, n), 64) * ceil_div(rank, 64);
       FLYMOE_CUDA_CHECK(launch_closely(lora_transpose_kernel,
                                        dim3(std::max(1, std::min(tiles, 16 * sm_count() / adapters)), dx ? 2 * adapters : adapters),
                                        256, 0, s, t));

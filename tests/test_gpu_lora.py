@@ -17,6 +17,8 @@ def make(rows, k, n, rank, adapters, dtype, mix, seed=0, size=1.0):
 
     if mix == "tokens":
         ids = torch.randint(-1, adapters + 1, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    elif mix == "one":
+        ids = torch.full((rows,), adapters // 2, dtype=torch.int32, device="cuda")
     elif mix == "none":
         ids = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
     else:                                        # runs of uneven length, one adapter skipped
@@ -66,6 +68,7 @@ SIZES = [
     (640, 1288, 328, 128, 3, "requests"), (900, 72, 64, 8, 2, "requests"), (2600, 1032, 136, 56, 5, "requests"),
     (50, 64, 64, 40, 3, "none"), (600, 2048, 136, 104, 9, "tokens"), (900, 264, 584, 16, 8, "tokens"),
     (777, 1032, 264, 64, 7, "tokens"), (1100, 520, 72, 56, 9, "tokens"), (640, 136, 264, 72, 4, "tokens"), (600, 72, 520, 88, 5, "tokens"),
+    (1200, 256, 264, 16, 40, "one"), (300, 200, 1096, 120, 33, "tokens"),
 ]
 
 
