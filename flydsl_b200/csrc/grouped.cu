@@ -10,11 +10,12 @@
 // transposed in memory.
 //
 // This file: forms 0 and 1 on one CTA per tile, of 128 rows x 256 or 128 columns or, where most experts have few rows, of 32
-// rows x 128 or 32 (form 1: 64) columns; all of form 2 and experts with many rows run on CTA pairs (grouped_pair.cu).  A tile may read rows
-// of the next expert; they only reach accumulator rows that are not stored.  A 32-row tile loads 32 rows per K block; the MMAs
+// rows x 128 or 32 (form 1: 64) columns; all of form 2 and experts with many rows run on CTA pairs (grouped_pair.cu).  A tile
+// may read rows of the next expert; they only reach accumulator rows that are not stored.  A 32-row tile loads 32 rows per K block; the MMAs
 // have 128 and read on into whatever follows in shared memory, which reaches no stored row either.  What small launches need
 // is bytes in flight (a K block takes about 2 us from its request to its release when the weights come from HBM), so their
-// tiles are narrow and the ring is deep: one expert of 4096 x 4096 with one row takes 33 us on 128-row tiles.
+// tiles are narrow and the ring is deep: one expert of 4096 x 4096 with one row takes 13 us, on 128-row tiles 33.  64 rows on 32
+// experts of 4096 x 7168: 1.63 GB of weights in 249 to 276 us, 5.9 to 6.5 TB/s.
 #include <cuda.h>
 #include <stdio.h>
 

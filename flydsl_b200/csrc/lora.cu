@@ -2,23 +2,27 @@
 //
 //   out[m] = base[m] + s_l B_l (A_l x[m]),   l = ids[m];  a row whose id names no adapter passes through
 //
-// in two launches: shrink, v = x A_l^T (fp32 [rows, rank], summed over K), and expand, which adds s_l v B_l^T to the base.
-// Rows may come in any order of adapters: a warp works on a fragment of 16 or 32 rows and goes through the distinct
-// adapters among them, and of each product only that adapter's rows are kept (so nothing of one request, not even an
-// infinity, reaches another).  The rank is the only small extent; both launches are bound by the bytes of x, the adapters
-// in use, the base and the output.
+// in two steps: shrink, v = x A_l^T (fp32 [rows, rank]), and expand, which adds s_l v B_l^T to the base.  The rank is the only
+// small extent: both are bound by the bytes of x, the adapters in use, the base and the output, or by launches where rows
+// are few.  Of every product only the adapter's own rows are kept, so nothing of one request, not even an infinity, reaches
+// another.
 //
-// v enters the second product as the sum of two 16-bit numbers (high part and remainder, two MMAs), which keeps 16 (bf16)
-// or 22 (fp16) bits of it: one rounding of the output is all that shows.  fp16 has few exponent bits, so there a row of v
-// is brought to the same power of two first.
+// Two forms.  From 512 rows on, tiles of 128 rows with few adapters go through tcgen05 (lora_sm100.cu).  This file has the
+// other: few rows, and tiles of many adapters.  Its blocks sort the rows of a window into groups of 16 that share an adapter
+// and put each through mma.sync, whose smallest tile is 16 rows where tcgen05's is 128: with an adapter for every row or two the
+// rows of a tile are what the work goes by.  Operand fragments are read from global memory 16 or 8 bytes a lane: the
+// contraction index may be permuted as long as both operands agree, so a lane takes consecutive elements where the
+// instruction's layout has pairs.
+//
+// v enters the second product as the sum of two 16-bit numbers (high part and remainder), which keeps 16 (bf16) or 22 (fp16)
+// bits of it: one rounding of the output is all that shows.  fp16 has few exponent bits, so there a row of v is brought to
+// the same power of two first.
 //
 // Gradients use the same kernels: dv = dout B_l is a shrink with B transposed, dx = s_l dv A_l an expand with A transposed
-// (the adapters are small next to the rows); dA_l = s_l sum dv^T x and dB_l = s_l sum dout^T v contract over an adapter's
-// rows, found by scanning ids.  No atomics anywhere: results do not depend on the order of execution.
-//
-// All products run on mma.sync: the shapes are thin (rank 8 to 128), the bound is memory.  Operand fragments are read from
-// global memory 16 or 8 bytes a lane: the contraction index may be permuted as long as both operands agree, so a lane takes
-// consecutive elements where the instruction's layout has pairs.
+// (the tiles read them across, this file's kernels want copies).  dA_l = s_l sum dv^T x and dB_l = s_l sum dout^T v contract
+// over an adapter's rows, found by scanning ids: bf16 on tcgen05 (lora_grad_sm100.cu), fp16 here, since a common power of two
+// that may still grow needs the sums in registers (8192 rows, 4096 + 4096 columns, rank 32: 44 us and 49).  No sum depends on the
+// order of execution.
 #include <algorithm>
 #include <stdio.h>
 #include <type_traits>
@@ -354,10 +358,9 @@ template <int NT> constexpr size_t wg_smem() {
 }
 
 // A block takes 256 columns (and up to 64 ranks) of a gradient and one split of the rows, and goes through the adapters with
-// rows in it: it lists an adapter's rows by scanning the ids, gathers them 32 at a time (cp.async, three or two chunks in flight)
-// and contracts over them; both operands are read across their rows with transposing ldmatrix.  Splits are pieces of the
-// batch, so blocks have like amounts of rows however the adapters share them.  fp16: chunks of v share a running power of
-// two; when a chunk needs a larger one the sums are brought to it.
+// rows in it (of its group): it lists an adapter's rows by scanning the ids, gathers them 32 at a time (cp.async, three or two
+// chunks in flight) and contracts over them; both operands are read across their rows with transposing ldmatrix.  Chunks of
+// v share a running power of two; when a chunk needs a larger one the sums are brought to it.
 template <int NT>
 __global__ void __launch_bounds__(kWgThreads, 2)
 lora_wgrad_kernel(const AdapterGradArgs p) {
@@ -672,7 +675,7 @@ lora_transpose_kernel(const TransposeArgs p) {
 }
 
 // ---------------------------------------------------------------------------- host
-// Tiles of 128 rows from 512 rows on.  Both ways, whole calls, 4096 -> 4096, bf16, us on one B200 (tiles / groups of 16 rows):
+// Tiles of 128 rows from 512 rows on.  Both ways (tiles of up to four adapters), whole calls, 4096 -> 4096, bf16, us on one B200 (tiles / groups of 16 rows):
 // 4 adapters in runs: 256 rows, rank 16 13.8 / 13.4, rank 128 20.8 / 43.5; 512 rows 13.6 / 16.8 and 24.5 / 50.6; 1024 rows
 // 15.9 / 26.2 and 27.0 / 95.3.  16 adapters in any order (tiles then only add launches that find nothing to do): 256 rows,
 // rank 16 21.2 / 12.7; 512 rows 29.1 / 20.5, rank 128 88.6 / 74.6; 8192 rows 134 / 82 and 484 / 388.
@@ -811,7 +814,8 @@ static bool needs_transposed(int rows, int rank, int adapters) { return !on_tile
 
 // Blocks for every place on the device (two an SM) that the adapters' gradients are shared out to, besides their columns:
 // pieces of the batch, whose blocks have like amounts of rows however the adapters share them, and groups of adapters, which
-// need no partial sums.  Pieces as long as their sums, written and read again, move half the bytes of the rows at most, with
+// need no partial sums.  Pieces only: 4096 rows in any order of 64 adapters of rank 64 took 404 us instead of 71, 8192 rows of 16
+// adapters of rank 16 87 instead of 66.  Groups only would leave a batch of one adapter to a few blocks.  Pieces as long as their sums, written and read again, move half the bytes of the rows at most, with
 // at least 256 rows in a piece; then groups.
 static int wgrad_places(int k, int n, int rank) {
   return 2 * sm_count() / ((ceil_div(k, kWgCols) + ceil_div(n, kWgCols)) * ceil_div(rank, kWgRank));

@@ -1,7 +1,9 @@
 // Adapters on tcgen05: shrink and expand for batches that fill tiles of 128 rows (see lora.cu for the operator).
 //
 // Both kernels stream their large operand through TMA and leave the thin products to the tensor cores, so what is left is
-// the traffic: x once for the shrink, base and output once each for the expand.  A tile goes through the distinct adapters
+// the traffic: x once for the shrink, base and output once each for the expand (from 8192 to 32768 rows of 4096 columns
+// each further 8192 rows cost 10 and 20 us, 6.7 TB/s, and an expand without a base, which only writes, 15.6 us, 4.3 TB/s;
+// start and end of a launch cost 6 to 9 us more).  A tile goes through the distinct adapters
 // among its rows; of each product only that adapter's rows are kept.
 //
 // Shrink: 128 rows x one split of K.  Every adapter of the tile has its own columns of TMEM (rank each); a K block of x is
@@ -10,7 +12,8 @@
 // read a row tile's v, took 15000 cycles to add up nine splits where one takes 2000.
 //
 // Expand: the base tile (128 x 128) is loaded into shared memory, gets the adapters' products added row by row where it
-// lies, and is stored from there; rows without an adapter are simply not touched.  The rows' v stands in shared memory as
+// lies, and is stored from there; rows without an adapter are simply not touched.  A warp of its own issues the stores: while
+// an epilogue warp also waited for the store before to be read out, the launch without a base took 24.8 us instead of 22.  The rows' v stands in shared memory as
 // high parts and remainders, [128, rank] each, for all column tiles of the row tile.
 #include <cuda.h>
 
@@ -245,6 +248,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   // an adapter's tile: 128 columns along the rank, or (transposed) two chunks of 64 columns with a row per rank
   const uint32_t b_bytes = p.transposed ? steps * 16 * 256 : KC * kChunkBytes;
   const int most = tile_limit(p.rank);
+  const bool all_ours = p.adapters <= most;
   // adapters of a row tile: every role looks for itself, ahead of the others where it can
   auto find_adapters = [&](int rt, int* list) {
     int id[4];
@@ -260,7 +264,6 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   // Producers and issuer: a warp looks at the ids, one thread (the same every time) does the rest, waits included.
   if (warp == 0) {
     // ------------------------------------------------------------------ base tiles
-    const bool all_ours = p.adapters <= most;
     int ys = 0;
     uint32_t yp = 0;
     bool ok = true;
@@ -352,11 +355,39 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
       __syncwarp();
       u = end;
     }
+  } else if (warp == 3) {
+    // ------------------------------------------------------------------ output tiles
+    int ys = 0, stored = 0;
+    uint32_t yp = 0;
+    bool ok = true;
+    for (int u = u0; u < u1;) {
+      const int rt = u / q.col_tiles, end = min(u1, (rt + 1) * q.col_tiles);
+      const bool ours = all_ours || find_adapters(rt, nullptr) <= most;
+      if (ours && lane == 0) {                   // the same thread every time: the groups of stores are its own
+        for (int t = u; t < end && ok; ++t) {
+          const int col = (t - rt * q.col_tiles) * kExCols;
+          ok = mbar_wait(smem_u32(&c->tile_done[ys]), yp, abort_flag, q.status, 7);
+          if (!ok) break;
+          const uint32_t src = smem_u32(smem + ys * 2 * kChunkBytes);
+          tma_store_2d(&tmap_out, src, col * 2, rt * kTileRows);
+          if (col + 64 < p.n) tma_store_2d(&tmap_out, src + kChunkBytes, col * 2 + 128, rt * kTileRows);
+          bulk_commit();
+          // the store before this one has been read out of its tile: that tile is free
+          asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          if (stored++ > 0) mbar_arrive(smem_u32(&c->y_empty[ys == 0 ? kExY - 1 : ys - 1]));
+          if (++ys == kExY) { ys = 0; yp ^= 1; }
+        }
+      }
+      __syncwarp();
+      u = end;
+    }
+    if (lane == 0) bulk_wait_all();
+    __syncwarp();
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ epilogue: a thread per row and half tile
     const int et = threadIdx.x - 128, wg = et >> 7, row = et & 127;
     const int sw = row & 7;
-    int ys = 0, acc = 0, row_tile = -1, d = 0, mine = -1, stored = 0, turn = 0;
+    int ys = 0, acc = 0, row_tile = -1, d = 0, mine = -1, turn = 0;
     uint32_t yp = 0, accp = 0;
     float scale = 0.f;
     bool ok = true;
@@ -437,9 +468,17 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
       ok = warp_wait(smem_u32(&c->y_full[ys]), yp, abort_flag, q.status, 6);
       if (!ok) break;
       uint8_t* line = smem + (ys * 2 + wg) * kChunkBytes + row * 128;
-      if (p.base == nullptr) {
+      uint4 y[8];                                // the base, on its way while the MMAs are waited for
 #pragma unroll
-        for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(line + ((j ^ sw) * 16)) = make_uint4(0, 0, 0, 0);
+      for (int j = 0; j < 8; ++j) y[j] = make_uint4(0, 0, 0, 0);
+      if (p.base == nullptr) {
+        if (mine < 0) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(line + ((j ^ sw) * 16)) = y[j];
+        }
+      } else if (mine >= 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = *reinterpret_cast<const uint4*>(line + ((j ^ sw) * 16));
       }
       for (int i = 0; i < d && ok; ++i) {
         ok = warp_wait(smem_u32(&c->acc_full[acc]), accp, abort_flag, q.status, 4);
@@ -447,25 +486,22 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
         tcgen05_fence_after();
         const bool hit = mine == c->list[1 + turn][i];
         if (__any_sync(0xffffffffu, hit)) {
+          float v[64];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float v[32];
+          for (int h = 0; h < 2; ++h)
             tmem_ld_x32(tmem + (uint32_t((warp & 3) * 32) << 16) + acc * kExCols + wg * 64 + h * 32,
-                        reinterpret_cast<uint32_t*>(v));
-            tmem_ld_wait();
-            if (hit) {
+                        reinterpret_cast<uint32_t*>(v + h * 32));
+          tmem_ld_wait();
+          if (hit) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                uint4* at = reinterpret_cast<uint4*>(line + (((h * 4 + j) ^ sw) * 16));
-                uint4 y = *at;
-                uint32_t* w = reinterpret_cast<uint32_t*>(&y);
+            for (int j = 0; j < 8; ++j) {
+              uint32_t* w = reinterpret_cast<uint32_t*>(&y[j]);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const float2 f = unpack2<T>(w[k]);
-                  w[k] = pack2<T>(fmaf(scale, v[j * 8 + k * 2], f.x), fmaf(scale, v[j * 8 + k * 2 + 1], f.y));
-                }
-                *at = y;
+              for (int k = 0; k < 4; ++k) {
+                const float2 f = unpack2<T>(w[k]);
+                w[k] = pack2<T>(fmaf(scale, v[j * 8 + k * 2], f.x), fmaf(scale, v[j * 8 + k * 2 + 1], f.y));
               }
+              *reinterpret_cast<uint4*>(line + ((j ^ sw) * 16)) = y[j];
             }
           }
         }
@@ -478,22 +514,8 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&c->tile_done[ys]));
-      if (et < 32) {
-        ok = warp_wait(smem_u32(&c->tile_done[ys]), yp, abort_flag, q.status, 7);
-        if (!ok) break;
-      }
-      if (et == 0) {
-        const uint32_t src = smem_u32(smem + ys * 2 * kChunkBytes);
-        tma_store_2d(&tmap_out, src, col * 2, rt * kTileRows);
-        if (col + 64 < p.n) tma_store_2d(&tmap_out, src + kChunkBytes, col * 2 + 128, rt * kTileRows);
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        // the store before this one has been read out of its tile: that tile is free
-        asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-        if (stored++ > 0) mbar_arrive(smem_u32(&c->y_empty[ys == 0 ? kExY - 1 : ys - 1]));
-      }
       if (++ys == kExY) { ys = 0; yp ^= 1; }
     }
-    if (et == 0) bulk_wait_all();
   }
   tcgen05_fence_before();
   __syncthreads();

@@ -87,7 +87,7 @@ permute_rows_kernel(const uint4* __restrict__ src, uint4* __restrict__ dst, cons
 
 // out[t] = sum_s weights[t, s] * rows[row of (t, s)], fp32 in slot order, rounded once; weights null: ones.
 // A block per token: its rows are looked up once, then every thread has eight of their 16-byte pieces in flight.  4096
-// tokens x 8 rows of 7168, bf16 (one B200): with the look-up in every thread 159 us.
+// tokens x 8 rows of 7168, bf16 (one B200): 86 us, with the look-up in every thread 159.
 constexpr int kCombineSlots = 256;
 template <typename T>
 __global__ void __launch_bounds__(256)
