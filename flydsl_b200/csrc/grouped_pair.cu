@@ -28,21 +28,26 @@
 namespace flymoe {
 
 constexpr int kRpTile = 256;
-constexpr int kRpStages = 5;
 constexpr int kRpHalf = 128 * kRagK * 2;                         // 16 KB: one operand of one CTA and K block
 constexpr int kRpStageBytes = 2 * kRpHalf;
 constexpr int kRpThreads = 384;
 constexpr int kRpStaging = 128 * 128;                            // 128 rows x 64 columns of output per warpgroup
+// Staging areas of a warpgroup, and operand stages.  AREAS == 2: the weight gradient of experts with few rows, whose tiles
+// take more time to write than to sum up.  bf16, one area and five stages / two and four: 64 experts of 64 rows, 2048 x 2048,
+// 145 / 131 us; 16 of 192, 2112 x 1088, 26.6 / 24.6; 8 of 500, 4096 x 4096, 150 / 146; 32 of 1024, 7168 x 4096, 1282 / 1370.
+constexpr int rp_stages(int areas) { return areas == 2 ? 4 : 5; }
 
 struct __align__(16) RagPairCtrl {
-  unsigned long long full[kRpStages], empty[kRpStages];
+  unsigned long long full[5], empty[5];
   unsigned long long acc_full[2], acc_empty[2];
   uint32_t tmem_base;
   int abort_flag;
   RaggedTables tab;
 };
-constexpr size_t kRpSmem = size_t(kRpStages) * kRpStageBytes + 2 * kRpStaging + sizeof(RagPairCtrl) + 1024;
-static_assert(kRpSmem <= 232448, "shared memory budget of one SM exceeded");
+constexpr size_t rp_smem(int areas) {
+  return size_t(rp_stages(areas)) * kRpStageBytes + 2 * areas * kRpStaging + sizeof(RagPairCtrl) + 1024;
+}
+static_assert(rp_smem(1) <= 232448 && rp_smem(2) <= 232448, "shared memory budget of one SM exceeded");
 
 // Boxes of 64 columns and 16, 8, 4, 2, 1 rows of both operands: the weight gradient's last K blocks.
 constexpr int kTailBoxes = 5;
@@ -59,14 +64,15 @@ __device__ __forceinline__ void load_tail(uint32_t dst, const CUtensorMap* maps,
   }
 }
 
-template <int FORM>
+template <int FORM, int AREAS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kRpThreads, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                     const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ TailMaps tails, const RaggedArgs a) {
   extern __shared__ uint8_t smem_dyn[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
+  constexpr int kRpStages = rp_stages(AREAS);
   uint8_t* staging = smem + size_t(kRpStages) * kRpStageBytes;
-  RagPairCtrl* ctrl = reinterpret_cast<RagPairCtrl*>(staging + 2 * kRpStaging);
+  RagPairCtrl* ctrl = reinterpret_cast<RagPairCtrl*>(staging + 2 * AREAS * kRpStaging);
   volatile int* abort_flag = &ctrl->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = int(cluster_rank());
@@ -202,8 +208,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     const int row = (warp & 3) * 32 + lane;
     const uint32_t tcol = tmem_base + (uint32_t((warp & 3) * 32) << 16) + uint32_t(wg * 128);
     const uint32_t empty_bar = map_to_rank(smem_u32(&ctrl->acc_empty[0]), 0);
-    uint8_t* stg = staging + wg * kRpStaging;
-    uint8_t* line = stg + row * 128;
+    uint8_t* stg = staging + wg * AREAS * kRpStaging;
+    int area = 0;
     const int sw = row & 7;
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -236,7 +242,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
           if (lane == 0) mbar_arrive_relaxed_cluster(empty_bar + uint32_t(acc) * 8u);
         }
         if (!wanted) continue;
-        if (tid == 0) bulk_wait_read_all();      // the staging area's last store has been read out
+        if (AREAS == 2) {
+          area ^= kRpStaging;
+          stg = staging + wg * AREAS * kRpStaging + area;
+        }
+        uint8_t* line = stg + row * 128;
+        // the staging area's last store has been read out
+        if (tid == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(AREAS - 1) : "memory");
         asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -276,14 +288,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
 }
 
 // ------------------------------------------------------------------------------ host
-template <int FORM>
+template <int FORM, int AREAS>
 static int launch_pair_form(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const TailMaps& tails,
                             const RaggedArgs& a, long long max_tiles, cudaStream_t stream) {
-  auto* kernel = grouped_pair_kernel<FORM>;
+  auto* kernel = grouped_pair_kernel<FORM, AREAS>;
   static SmemLimitSeen seen;
-  FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(kRpSmem), seen));
+  FLYMOE_CUDA_CHECK(allow_smem(reinterpret_cast<const void*>(kernel), int(rp_smem(AREAS)), seen));
   const unsigned pairs = unsigned(std::min<long long>(max_tiles, sm_count() / 2));
-  kernel<<<2 * pairs, kRpThreads, kRpSmem, stream>>>(ma, mb, mo, tails, a);
+  kernel<<<2 * pairs, kRpThreads, rp_smem(AREAS), stream>>>(ma, mb, mo, tails, a);
   FLYMOE_CUDA_CHECK(cudaGetLastError());
   return FLYMOE_OK;
 }
@@ -304,15 +316,17 @@ int launch_ragged_pair(int form, const void* p, const void* q, const RaggedArgs&
       if (rc == FLYMOE_OK) rc = ragged_map(&tails.b[i], q, k, a.rows, 0, 16 >> i);
     }
     const long long tiles = (long long)a.experts * a.m_tiles * a.n_tiles;
-    return rc != FLYMOE_OK ? rc : launch_pair_form<2>(ma, mb, mo, tails, a, tiles, stream);
+    if (rc != FLYMOE_OK) return rc;
+    return a.rows / a.experts <= 512 ? launch_pair_form<2, 2>(ma, mb, mo, tails, a, tiles, stream)
+                                     : launch_pair_form<2, 1>(ma, mb, mo, tails, a, tiles, stream);
   }
   rc = ragged_map(&ma, p, a.k_dim, a.rows, 0, 128);
   if (rc == FLYMOE_OK) rc = ragged_map(&mb, q, k, n, a.experts, form == 1 ? kRagK : 128);
   if (rc == FLYMOE_OK) rc = ragged_map(&mo, a.out, a.n_dim, a.rows, 0, 128);
   if (rc != FLYMOE_OK) return rc;
   const long long tiles = ((long long)a.rows / kRpTile + a.experts) * a.n_tiles;
-  return form == 1 ? launch_pair_form<1>(ma, mb, mo, tails, a, tiles, stream)
-                   : launch_pair_form<0>(ma, mb, mo, tails, a, tiles, stream);
+  return form == 1 ? launch_pair_form<1, 1>(ma, mb, mo, tails, a, tiles, stream)
+                   : launch_pair_form<0, 1>(ma, mb, mo, tails, a, tiles, stream);
 }
 
 }  // namespace flymoe
