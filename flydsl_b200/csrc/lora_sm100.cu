@@ -45,7 +45,7 @@ constexpr size_t kShSmem = size_t(kShX) * kChunkBytes + kShABytes + sizeof(Shrin
 
 struct ShrinkTcArgs {
   ShrinkArgs p;
-  int bf16, rank_pad, slots, tmem_cols;
+  int bf16, rank_pad, slots;
   int a_bytes;                 // an adapter's block in shared memory
   int* status;
 };
@@ -63,23 +63,30 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
   const int row0 = blockIdx.x * kTileRows;
   const int a_bytes = q.a_bytes;
 
+  // Columns of TMEM for the adapters that are there: with room for as many as there may be, ranks from 33 on would leave one
+  // block on an SM.  Sums are read 32 columns at a time, so also what the last read reaches past a rank of 16 modulo 32.
+  uint32_t tmem_cols = 0;
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                 ::"r"(smem_u32(&c->tmem_base)), "r"(uint32_t(q.tmem_cols)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    after_previous_launch();
+    int id[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, row0 + i * 32 + lane, p.rows, p.adapters);
+    int n = tile_adapters(id, lane, tile_limit(p.rank), c->list);
+    if (n > tile_limit(p.rank)) n = 0;           // the other tiles are not this kernel's
+    if (lane == 0) c->count = n;
+    if (n > 0) {
+      tmem_cols = 32;
+      while (int(tmem_cols) < (n - 1) * q.rank_pad + (q.rank_pad + 31) / 32 * 32) tmem_cols *= 2;
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                   ::"r"(smem_u32(&c->tmem_base)), "r"(tmem_cols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   } else if (threadIdx.x == 0) {
     for (int i = 0; i < kShX; ++i) { mbar_init(smem_u32(&c->x_full[i]), 1); mbar_init(smem_u32(&c->x_empty[i]), 1); }
     for (int i = 0; i < 16; ++i) { mbar_init(smem_u32(&c->a_full[i]), 1); mbar_init(smem_u32(&c->a_empty[i]), 1); }
     mbar_init(smem_u32(&c->acc_full), 1);
     c->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  } else if (warp == 2) {
-    after_previous_launch();
-    int id[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, row0 + i * 32 + lane, p.rows, p.adapters);
-    const int n = tile_adapters(id, lane, tile_limit(p.rank), c->list);
-    if (lane == 0) c->count = n <= tile_limit(p.rank) ? n : 0;        // the other tiles are not this kernel's
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -177,9 +184,9 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
   }
   tcgen05_fence_before();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == 1 && tmem_cols > 0) {
     tcgen05_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(q.tmem_cols)) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(tmem_cols) : "memory");
   }
 }
 
@@ -535,14 +542,10 @@ static int matrix_map(CUtensorMap* map, const void* base, long long cols, long l
 }
 
 int launch_shrink_sm100(const ShrinkArgs& p, int bf16, cudaStream_t stream) {
-  ShrinkTcArgs q = {p, bf16, (p.rank + 15) / 16 * 16, 0, 0, 0, device_status_ptr()};
+  ShrinkTcArgs q = {p, bf16, (p.rank + 15) / 16 * 16, 0, 0, device_status_ptr()};
   if (q.status == nullptr) return FLYMOE_ERR_CUDA;
   q.a_bytes = p.transposed ? ceil_div(p.rank, 64) * 8192 : q.rank_pad * 128;
   q.slots = std::min(16, kShABytes / q.a_bytes);
-  // Columns for tile_limit() adapters; sums are read 32 columns at a time, so also for what the last read reaches past a rank
-  // of 16 modulo 32.
-  const int columns = (tile_limit(p.rank) - 1) * q.rank_pad + (q.rank_pad + 31) / 32 * 32;
-  q.tmem_cols = columns <= 256 ? 256 : 512;
   CUtensorMap mx, ma;
   int rc = matrix_map(&mx, p.x, p.k, p.rows, 0, kTileRows);
   if (rc == FLYMOE_OK)
