@@ -21,6 +21,8 @@ def on(device: torch.device, stream=None):
     if stream is not None:
         if isinstance(stream, int) or not isinstance(stream, torch.cuda.Stream):
             stream = torch.cuda.ExternalStream(_lib.stream_handle(stream), device=device)
+        if device.index is not None and stream.device != device:
+            raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
         return torch.cuda.stream(stream)
     if device.index is None or device.index == torch.cuda.current_device():
         return _HERE
@@ -43,6 +45,14 @@ def require_shape(name: str, t: torch.Tensor, shape: tuple) -> None:
     if t.dim() != len(shape) or any(s is not None and s != d for s, d in zip(shape, t.shape)):
         want = ", ".join("*" if s is None else str(s) for s in shape)
         raise ValueError(f"{name} must have shape [{want}], got {list(t.shape)}")
+
+
+def require_apart(out: torch.Tensor, **inputs) -> None:
+    """``out`` shares no memory with the inputs, which are read while it is written."""
+    at, end = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    for name, t in inputs.items():
+        if at < t.data_ptr() + t.numel() * t.element_size() and t.data_ptr() < end:
+            raise ValueError(f"out must not share memory with {name}")
 
 
 def require_same_device(first: str, device: torch.device, **others) -> None:

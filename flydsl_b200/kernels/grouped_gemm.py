@@ -23,7 +23,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._call import HALF, on, once, require_same_device, require_shape
+from ._call import HALF, on, once, require_apart, require_same_device, require_shape
 
 
 def _check(rows_name, rows, mats_name, mats, offsets, out, out_shape):
@@ -33,6 +33,7 @@ def _check(rows_name, rows, mats_name, mats, offsets, out, out_shape):
     if out is not None:
         _lib.require_cuda("out", out, (rows.dtype,))
         require_shape("out", out, out_shape)
+        require_apart(out, **{rows_name: rows, mats_name: mats})
     require_same_device(rows_name, rows.device, **{mats_name: mats, "offsets": offsets, "out": out})
 
 

@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._call import HALF, on, once, require_same_device, require_shape
+from ._call import HALF, on, once, require_apart, require_same_device, require_shape
 
 MAX_RANK = 128
 
@@ -65,8 +65,9 @@ def _check(y, x, a, b, adapter_ids, scaling, out):
             _lib.require_cuda(name, t, (x.dtype,))
     if out is not None:
         require_shape("out", out, (rows, n))
-        if x.data_ptr() == out.data_ptr() and rows:
-            raise ValueError("out must not be x")
+        require_apart(out, x=x, a=a, b=b)
+        if out.data_ptr() != y.data_ptr():
+            require_apart(out, y=y)
     _lib.require_cuda("adapter_ids", adapter_ids, (torch.int32,))
     _lib.require_cuda("scaling", scaling, (torch.float32,))
     require_same_device("x", x.device, y=y, a=a, b=b, adapter_ids=adapter_ids, scaling=scaling, out=out)

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from flydsl_b200.kernels._call import on
 from flydsl_b200.kernels.grouped_gemm import grouped_gemm, grouped_gemm_dgrad, grouped_gemm_wgrad, grouped_linear
 
 pytestmark = pytest.mark.gpu
@@ -183,3 +184,17 @@ def test_another_stream_and_a_captured_step():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(res, eager[i]))
+
+
+def test_results_apart_from_inputs_and_streams_of_their_device():
+    x, w = torch.ones((12, 64), dtype=BF, device="cuda"), torch.ones((2, 64, 64), dtype=BF, device="cuda")
+    off = torch.tensor([0, 4, 12], dtype=torch.int32, device="cuda")
+    for out in (x, w.view(-1, 64)[10:22]):
+        with pytest.raises(ValueError, match="share memory"):
+            grouped_gemm(x, w, off, out=out)
+        with pytest.raises(ValueError, match="share memory"):
+            grouped_gemm_dgrad(x, w, off, out=out)
+    with pytest.raises(ValueError, match="share memory"):
+        grouped_gemm_wgrad(w.view(-1, 64)[:12], x, off, out=w)
+    with pytest.raises(ValueError, match="stream is on"):
+        on(torch.device("cuda", torch.cuda.current_device() + 1), torch.cuda.Stream())

@@ -172,6 +172,12 @@ def test_in_place_buffers_and_streams():
         lora_add(p["y"].clone().requires_grad_(), *(p[s] for s in ("x", "a", "b", "adapter_ids", "scaling")), out=buf)
     with pytest.raises(ValueError, match="dtype"):
         lora_add(p["y"].bfloat16(), *(p[s] for s in ("x", "a", "b", "adapter_ids", "scaling")))
+    rest = [p[s] for s in ("a", "b", "adapter_ids", "scaling")]
+    store = torch.zeros(71 * 520, dtype=HF, device="cuda")
+    whole, shifted = store[: 70 * 520].view(70, 520), store[520:].view(70, 520)
+    for y, x, out in ((whole, p["x"], shifted), (p["y"], store[: 70 * 256].view(70, 256), whole)):
+        with pytest.raises(ValueError, match="share memory"):
+            lora_add(y, x, *rest, out=out)
     with pytest.raises(ValueError, match="scaling has no gradient"):
         lora_add(*(p[s] for s in ("y", "x", "a", "b", "adapter_ids")), p["scaling"].clone().requires_grad_())
 
