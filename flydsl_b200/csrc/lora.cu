@@ -764,8 +764,11 @@ static int launch_wgrad(const AdapterGradArgs& p, bool bf, cudaStream_t s) {
   return FLYMOE_OK;
 }
 
-// Floats of v: the sum and, where there are several, the splits behind it.
-static long long v_elems(int rows, int splits, int rank) { return (splits > 1 ? splits + 1LL : 1LL) * rows * rank; }
+// Floats of v: the sum, where there are several the splits behind it, and on tiles a number for each.
+static long long v_planes(int rows, int splits, int rank) { return (splits > 1 ? splits + 1LL : 1LL) * rows * rank; }
+static long long v_elems(int rows, int splits, int rank) {
+  return v_planes(rows, splits, rank) + (on_tiles(rows) ? ceil_div(rows, 128) : 0);
+}
 
 // One product with the adapters and back: out = base + scaling * (x A^T) B^T, or with a_t / b_t (then `a` and `b` are only
 // read where needs_transposed) for A and B given the other way round.  v: v_elems() floats; `keep`: its first rows * rank
@@ -784,7 +787,8 @@ static int run_chain(const Chain& c, cudaStream_t s) {
   const int skip = tiles ? tile_limit(c.rank) : 0;
   const int splits = shrink_splits(c.rows, c.k);
   float* planes = splits > 1 ? c.v + (long long)c.rows * c.rank : c.v;
-  ShrinkArgs sh = {c.x, c.a, c.ids, planes, c.rows, c.k, c.rank, c.adapters, splits, 0};
+  int* counts = reinterpret_cast<int*>(c.v + v_planes(c.rows, splits, c.rank));
+  ShrinkArgs sh = {c.x, c.a, c.ids, planes, counts, c.rows, c.k, c.rank, c.adapters, splits, 0};
   int rc = FLYMOE_OK;
   if (others) rc = bf ? launch_shrink_rank<__nv_bfloat16>(sh, skip, s) : launch_shrink_rank<__half>(sh, skip, s);
   if (rc == FLYMOE_OK && tiles) {
@@ -800,7 +804,7 @@ static int run_chain(const Chain& c, cudaStream_t s) {
                                      reinterpret_cast<const float4*>(planes), reinterpret_cast<float4*>(c.v), vecs, splits));
   }
   if (!c.out) return FLYMOE_OK;
-  ExpandArgs ex = {c.base, fold ? c.v : planes, c.b, c.ids, c.scaling, c.out, c.rows, c.n, c.rank, c.adapters,
+  ExpandArgs ex = {c.base, fold ? c.v : planes, c.b, c.ids, c.scaling, c.out, counts, c.rows, c.n, c.rank, c.adapters,
                    fold ? 1 : splits, 0};
   if (others) rc = bf ? launch_expand_rank<__nv_bfloat16>(ex, skip, s) : launch_expand_rank<__half>(ex, skip, s);
   if (rc == FLYMOE_OK && tiles) {

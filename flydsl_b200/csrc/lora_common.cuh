@@ -41,6 +41,7 @@ struct ShrinkArgs {
   const void* a;               // [adapters, rank, k], or transposed [adapters, k, rank] (on tiles only)
   const int* ids;              // [rows]
   float* v;                    // [splits, rows, rank]
+  int* counts;                 // on tiles: [tiles of 128 rows], distinct adapters of a tile, tile_limit() + 1 for more
   int rows, k, rank, adapters, splits, transposed;
 };
 struct ExpandArgs {
@@ -50,6 +51,7 @@ struct ExpandArgs {
   const int* ids;
   const float* scaling;        // [adapters]
   void* out;                   // [rows, n]
+  const int* counts;           // on tiles: the shrink's
   int rows, n, rank, adapters, splits, transposed;
 };
 

@@ -72,6 +72,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
 #pragma unroll
     for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, row0 + i * 32 + lane, p.rows, p.adapters);
     int n = tile_adapters(id, lane, tile_limit(p.rank), c->list);
+    if (blockIdx.y == 0 && lane == 0) p.counts[blockIdx.x] = n;
     if (n > tile_limit(p.rank)) n = 0;           // the other tiles are not this kernel's
     if (lane == 0) c->count = n;
     if (n > 0) {
@@ -202,7 +203,9 @@ struct __align__(16) ExpandCtrl {
   // through with a tile early, and may be with the next one before another warp is with this.
   unsigned long long tile_done[4];
   uint32_t tmem_base;
-  int abort_flag, count[2], list[3][kTileAdapters];            // the producer's, and the epilogue's for two row tiles
+  int abort_flag, list[3][kTileAdapters];        // the adapter tiles' producer's, and the epilogue's for two row tiles
+  int first[2];                                  // of this block's units, and of the next one's
+  long long warp_cost[kExThreads / 32];
   float up[2][kTileRows];
 };
 constexpr int kExAcc = 4;                        // accumulators
@@ -256,8 +259,11 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   // an adapter's tile: 128 columns along the rank, or (transposed) two chunks of 64 columns with a row per rank
   const uint32_t b_bytes = p.transposed ? steps * 16 * 256 : KC * kChunkBytes;
   const int most = tile_limit(p.rank);
-  const bool all_ours = p.adapters <= most;
-  // adapters of a row tile: every role looks for itself, ahead of the others where it can
+  // adapters of a row tile; more than `most`: nothing to do here (the other kernel's, or no adapter and the base in place)
+  auto adapters_of = [&](int rt) {
+    const int d = __ldg(p.counts + rt);
+    return d == 0 && p.base == p.out ? most + 1 : d;
+  };
   auto find_adapters = [&](int rt, int* list) {
     int id[4];
 #pragma unroll
@@ -266,8 +272,48 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     __syncwarp();
     return n;
   };
-  // consecutive column tiles of a row tile, so that the rows' v is set up once or twice per block
-  const int u0 = int((long long)q.units * blockIdx.x / gridDim.x), u1 = int((long long)q.units * (blockIdx.x + 1) / gridDim.x);
+  // Blocks take consecutive column tiles of a row tile, so that the rows' v is set up once or twice per block, and as much
+  // work each: a tile's time is that of its bytes up to two adapters, from there on each costs a third of that more.  In equal
+  // numbers of tiles the blocks with the most adapters held the launch up (4096 rows, 16 runs of 8 adapters of rank 64, 7168
+  // columns: 36 us against 30).
+  auto cost_of = [&](int rt) {
+    const int d = adapters_of(rt);
+    return d > most ? 0 : max(35, 19 + 11 * d);
+  };
+  {
+    const int tiles = (p.rows + kTileRows - 1) / kTileRows, per = (tiles + kExThreads - 1) / kExThreads;
+    const int t0 = min(tiles, int(threadIdx.x) * per), t1 = min(tiles, t0 + per);
+    long long mine = 0;
+    for (int t = t0; t < t1; ++t) mine += (long long)cost_of(t) * q.col_tiles;
+    long long upto = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long o = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += o;
+    }
+    if (lane == 31) c->warp_cost[warp] = upto;
+    if (threadIdx.x < 2) c->first[threadIdx.x] = q.units;        // where nothing is left
+    __syncthreads();
+    long long all = 0;
+#pragma unroll
+    for (int i = 0; i < kExThreads / 32; ++i) {
+      const long long w = c->warp_cost[i];
+      if (i < warp) upto += w;
+      all += w;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const long long want = all * (blockIdx.x + i) / gridDim.x;
+      long long at = upto - mine;
+      if (want < at || want >= upto) continue;
+      int t = t0;
+      for (; want >= at + (long long)cost_of(t) * q.col_tiles; ++t) at += (long long)cost_of(t) * q.col_tiles;
+      const int cost = cost_of(t);
+      c->first[i] = t * q.col_tiles + int((want - at + cost - 1) / cost);
+    }
+    __syncthreads();
+  }
+  const int u0 = c->first[0], u1 = c->first[1];
 
   // Producers and issuer: a warp looks at the ids, one thread (the same every time) does the rest, waits included.
   if (warp == 0) {
@@ -277,7 +323,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     bool ok = true;
     for (int u = u0; u < u1;) {
       const int rt = u / q.col_tiles, end = min(u1, (rt + 1) * q.col_tiles);
-      const bool ours = all_ours || find_adapters(rt, nullptr) <= most;
+      const bool ours = adapters_of(rt) <= most;
       if (ours && elect_one()) {
         for (int t = u; t < end && ok; ++t) {
           const int col = (t - rt * q.col_tiles) * kExCols;
@@ -337,7 +383,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     bool ok = true;
     for (int u = u0; u < u1;) {
       const int rt = u / q.col_tiles, end = min(u1, (rt + 1) * q.col_tiles);
-      const int d = find_adapters(rt, nullptr);
+      const int d = adapters_of(rt);
       if (d >= 1 && d <= most && elect_one()) {         // otherwise nobody multiplies, and nobody signals
         ok = ok && mbar_wait(smem_u32(&c->row_ready), rp, abort_flag, q.status, 5);
         rp ^= 1;
@@ -370,7 +416,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
     bool ok = true;
     for (int u = u0; u < u1;) {
       const int rt = u / q.col_tiles, end = min(u1, (rt + 1) * q.col_tiles);
-      const bool ours = all_ours || find_adapters(rt, nullptr) <= most;
+      const bool ours = adapters_of(rt) <= most;
       if (ours && lane == 0) {                   // the same thread every time: the groups of stores are its own
         for (int t = u; t < end && ok; ++t) {
           const int col = (t - rt * q.col_tiles) * kExCols;
@@ -413,6 +459,8 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
         // The MMAs of the previous row tile are done (their last sums have been read here): its v may go.  Eight threads to a
         // row; ids and v are asked for together.
         row_tile = rt;
+        d = adapters_of(rt);
+        if (d > most) continue;                  // its rows are the other kernel's
         turn ^= 1;
         const int r8 = et >> 3, l8 = et & 7, vecs = p.rank / 4;
         int id[4];
@@ -429,10 +477,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
         }
         mine = row_adapter(p.ids, rt * kTileRows + row, p.rows, p.adapters);
         scale = mine >= 0 ? __ldg(p.scaling + mine) : 0.f;
-        if (et < 32) {
-          const int n = find_adapters(rt, c->list[1 + turn]);
-          if (lane == 0) c->count[turn] = n;
-        }
+        if (et < 32) find_adapters(rt, c->list[1 + turn]);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           const int r = s * 32 + r8;
@@ -468,11 +513,10 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         ok = sync();                             // list and exponents, in this row tile's places, are written
         if (!ok) break;
-        d = c->count[turn];
         if constexpr (std::is_same<T, __half>::value) scale *= c->up[turn][row];
-        if (d >= 1 && d <= most) mbar_arrive(smem_u32(&c->row_ready));
+        if (d >= 1) mbar_arrive(smem_u32(&c->row_ready));
       }
-      if (d > most) continue;           // its rows are the other kernel's
+      if (d > most) continue;
       ok = warp_wait(smem_u32(&c->y_full[ys]), yp, abort_flag, q.status, 6);
       if (!ok) break;
       uint8_t* line = smem + (ys * 2 + wg) * kChunkBytes + row * 128;
