@@ -275,7 +275,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   // Blocks take consecutive column tiles of a row tile, so that the rows' v is set up once or twice per block, and as much
   // work each: a tile's time is that of its bytes up to two adapters, from there on each costs a third of that more.  In equal
   // numbers of tiles the blocks with the most adapters held the launch up (4096 rows, 16 runs of 8 adapters of rank 64, 7168
-  // columns: 36 us against 30).
+  // columns: 36 us against 33).
   auto cost_of = [&](int rt) {
     const int d = adapters_of(rt);
     return d > most ? 0 : max(35, 19 + 11 * d);
