@@ -24,7 +24,7 @@ def on(device: torch.device, stream=None):
         if device.index is not None and stream.device != device:
             raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
         return torch.cuda.stream(stream)
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == torch._C._cuda_getDevice():     # current_device() without its wrapper
         return _HERE
     return torch.cuda.device(device)
 

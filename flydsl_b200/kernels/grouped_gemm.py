@@ -44,17 +44,18 @@ def _check_sizes(experts, n, k):
         raise ValueError(f"n ({n}) and k ({k}) must be positive multiples of 8")
 
 
-def _fits(t, w, offsets, out, input_grad):
-    """Whether the arguments are right, in as few steps as it takes; ``_check_rows_form`` says what is not."""
+def _sizes(t, w, offsets, out, input_grad):
+    """(rows, experts, n, k) if the arguments are right, in as few steps as it takes; ``_check_rows_form`` says what is not."""
     try:
-        experts, n, k = w.shape
-        dt, dev = t.dtype, t.device
-        return (t.is_cuda and dt in HALF and t.dim() == 2 and t.shape[1] == (n if input_grad else k)
-                and offsets.shape == (experts + 1,) and w.dtype is dt and offsets.dtype is torch.int32 and w.device == dev
-                and offsets.device == dev and t.is_contiguous() and w.is_contiguous() and offsets.is_contiguous()
-                and n >= 8 and not n % 8 and k >= 8 and not k % 8 and 1 <= experts <= 1024 and out is None)
+        (experts, n, k), (rows, inner), (bounds,), dt = w.shape, t.shape, offsets.shape, t.dtype
+        if (t.is_cuda and dt in HALF and inner == (n if input_grad else k) and bounds == experts + 1 and w.dtype is dt
+                and offsets.dtype is torch.int32 and t.get_device() == w.get_device() == offsets.get_device()
+                and t.is_contiguous() and w.is_contiguous() and offsets.is_contiguous() and n >= 8 and not n % 8 and k >= 8
+                and not k % 8 and 1 <= experts <= 1024 and out is None):
+            return rows, experts, n, k
     except (AttributeError, ValueError):
-        return False
+        pass
+    return None
 
 
 def _check_rows_form(name, t, w, offsets, out, input_grad):
@@ -66,22 +67,22 @@ def _check_rows_form(name, t, w, offsets, out, input_grad):
     require_shape(name, t, (None, n if input_grad else k))
     require_shape("offsets", offsets, (experts + 1,))
     _check(name, t, "w", w, offsets, out, (t.shape[0], k if input_grad else n))
+    return t.shape[0], experts, n, k
 
 
 def _rows_form(name, t, w, offsets, out, stream, input_grad):
-    if not _fits(t, w, offsets, out, input_grad):
-        _check_rows_form(name, t, w, offsets, out, input_grad)
-    return _run_rows_form(t, w, offsets, out, stream, input_grad)
+    sizes = _sizes(t, w, offsets, out, input_grad) or _check_rows_form(name, t, w, offsets, out, input_grad)
+    return _run_rows_form(t, w, offsets, out, stream, input_grad, sizes)
 
 
-def _run_rows_form(t, w, offsets, out, stream, input_grad):
-    (experts, n, k), rows = w.shape, t.shape[0]
-    lib = _lib.load()
+def _run_rows_form(t, w, offsets, out, stream, input_grad, sizes):
     with on(t.device, stream):
-        res = t.new_empty((rows, k if input_grad else n)) if out is None else out
-        _lib.check(lib.flymoe_grouped_gemm(res.data_ptr(), t.data_ptr(), w.data_ptr(), offsets.data_ptr(), rows, experts, n,
-                                           k, _lib.DTYPE_CODE[t.dtype], 1 if input_grad else 0, 1 if out is None else 0,
-                                           _lib.stream_handle(None)), "grouped_gemm")
+        res = t.new_empty((sizes[0], sizes[3 if input_grad else 2])) if out is None else out
+        rc = _lib.load().flymoe_grouped_gemm(
+            res.data_ptr(), t.data_ptr(), w.data_ptr(), offsets.data_ptr(), *sizes, _lib.DTYPE_CODE[t.dtype],
+            1 if input_grad else 0, 1 if out is None else 0, _lib.stream_handle(None))
+    if rc:
+        _lib.check(rc, "grouped_gemm")
     return res
 
 
@@ -123,27 +124,27 @@ def _wgrad(dy, x, offsets, out):
 
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, offsets):
+    def forward(ctx, x, w, offsets, sizes):
         ctx.save_for_backward(x, w, offsets)
-        return _run_rows_form(x, w, offsets, None, None, False)
+        ctx.sizes = sizes
+        return _run_rows_form(x, w, offsets, None, None, False, sizes)
 
     @staticmethod
     @once
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
         dy = dy.contiguous()
-        dx = _run_rows_form(dy, w, offsets, None, None, True) if ctx.needs_input_grad[0] else None
+        dx = _run_rows_form(dy, w, offsets, None, None, True, ctx.sizes) if ctx.needs_input_grad[0] else None
         dw = None
         if ctx.needs_input_grad[1]:
             with on(x.device):
                 dw = _wgrad(dy, x, offsets, torch.empty_like(w))
-        return dx, dw, None
+        return dx, dw, None, None
 
 
 def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     """``grouped_gemm`` in autograd: gradients reach ``x`` and ``w``.  Runs on the current stream."""
-    if not _fits(x, w, offsets, None, False):
-        _check_rows_form("x", x, w, offsets, None, False)
+    sizes = _sizes(x, w, offsets, None, False) or _check_rows_form("x", x, w, offsets, None, False)
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
-        return _GroupedLinear.apply(x, w, offsets)
-    return _run_rows_form(x, w, offsets, None, None, False)
+        return _GroupedLinear.apply(x, w, offsets, sizes)
+    return _run_rows_form(x, w, offsets, None, None, False, sizes)

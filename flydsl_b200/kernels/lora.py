@@ -28,11 +28,11 @@ MAX_RANK = 128
 def _fits(y, x, a, b, ids, scaling, out):
     """Whether the arguments are right, in as few steps as it takes; ``_check`` says what is not."""
     try:
-        (rows, k), (adapters, rank, ka), n, dt, dev = x.shape, a.shape, y.shape[1], x.dtype, x.device
+        (rows, k), (adapters, rank, ka), n, dt = x.shape, a.shape, y.shape[1], x.dtype
         return (x.is_cuda and dt in HALF and ka == k and y.shape == (rows, n) and b.shape == (adapters, n, rank)
                 and ids.shape == (rows,) and scaling.shape == (adapters,) and y.dtype is dt and a.dtype is dt and b.dtype is dt
-                and ids.dtype is torch.int32 and scaling.dtype is torch.float32 and y.device == dev and a.device == dev
-                and b.device == dev and ids.device == dev and scaling.device == dev and x.is_contiguous()
+                and ids.dtype is torch.int32 and scaling.dtype is torch.float32 and x.get_device() == y.get_device()
+                == a.get_device() == b.get_device() == ids.get_device() == scaling.get_device() and x.is_contiguous()
                 and y.is_contiguous() and a.is_contiguous() and b.is_contiguous() and ids.is_contiguous()
                 and scaling.is_contiguous() and 8 <= rank <= MAX_RANK and not rank % 8 and k >= 8 and not k % 8 and n >= 8
                 and not n % 8 and 1 <= adapters <= 32767 and out is None)
