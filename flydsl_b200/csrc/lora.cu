@@ -21,7 +21,7 @@
 // Gradients use the same kernels: dv = dout B_l is a shrink with B transposed, dx = s_l dv A_l an expand with A transposed
 // (the tiles read them across, this file's kernels want copies).  dA_l = s_l sum dv^T x and dB_l = s_l sum dout^T v contract
 // over an adapter's rows, found by scanning ids: bf16 on tcgen05 (lora_grad_sm100.cu), fp16 here, since a common power of two
-// that may still grow needs the sums in registers (8192 rows, 4096 + 4096 columns, rank 32: 44 us and 49).  No sum depends on the
+// that may still grow needs the sums in registers (8192 rows, 4096 + 4096 columns, 4 adapters of rank 32: 43 us and 49).  No sum depends on the
 // order of execution.
 #include <algorithm>
 #include <stdio.h>
@@ -378,20 +378,20 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
   const int col0 = (second ? int(blockIdx.x) - p.g[0].tiles : int(blockIdx.x)) * kWgCols;
   const int j0 = int(blockIdx.z) * kWgRank;      // first of this block's ranks
   const int split = int(blockIdx.y) / p.groups, group = int(blockIdx.y) - split * p.groups;
-  const int group_begin = int((long long)p.adapters * group / p.groups), group_end = int((long long)p.adapters * (group + 1) / p.groups);
+  const int others = p.groups - 1;               // an adapter's group is its number modulo `groups`, a power of two
   const int begin = int((long long)p.rows * split / p.splits), end = int((long long)p.rows * (split + 1) / p.splits);
   const T* X = static_cast<const T*>(q.x);
   const long long mat = (long long)q.cols * p.rank;
   after_previous_launch();
 
-  // the smallest adapter above `l` with rows here, or the end of the group
+  // the smallest adapter of the group above `l` with rows here, or p.adapters
   auto find_next = [&](int l) -> int {
-    if (tid == 0) next_adapter = group_end;
+    if (tid == 0) next_adapter = p.adapters;
     __syncthreads();
-    int best = group_end;
+    int best = p.adapters;
     for (int i = begin + tid; i < end; i += kWgThreads) {
       const int id = __ldg(p.ids + i);
-      if (id > l && id < best) best = id;
+      if (id > l && id < best && (id & others) == group) best = id;
     }
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, off));
@@ -403,11 +403,11 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
   auto skip_adapters = [&](int from, int to) {
     if (p.splits > 1) {
       if (blockIdx.x == 0 && blockIdx.z == 0)
-        for (int l = from + tid; l < to; l += kWgThreads) p.present[(long long)split * p.adapters + l] = 0;
+        for (int l = from + tid * p.groups; l < to; l += kWgThreads * p.groups) p.present[(long long)split * p.adapters + l] = 0;
       return;
     }
     const int jn = min(kWgRank, p.rank - j0), cn = min(kWgCols, q.cols - col0);
-    for (int l = from; l < to; ++l)
+    for (int l = from; l < to; l += p.groups)
       for (int i = tid; i < jn * cn; i += kWgThreads) {
         const long long at = q.rank_major ? (long long)(j0 + i / cn) * q.cols + col0 + i % cn
                                           : (long long)(col0 + i / jn) * p.rank + j0 + i % jn;
@@ -415,10 +415,10 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
       }
   };
 
-  int done = group_begin;                        // adapters below this one are dealt with
-  for (int l = find_next(group_begin - 1); l < group_end; l = find_next(l)) {
+  int done = group;                               // adapters of the group below this one are dealt with
+  for (int l = find_next(-1); l < p.adapters; l = find_next(l)) {
     skip_adapters(done, l);
-    done = l + 1;
+    done = l + p.groups;
     if (p.splits > 1 && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) p.present[(long long)split * p.adapters + l] = 1;
 
     int next = begin, taken = 0, have = 0;       // ids scanned, entries of the list used and in it (same in all threads)
@@ -607,7 +607,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
         }
     __syncthreads();                             // the list and the stages are free for the next adapter
   }
-  skip_adapters(done, group_end);
+  skip_adapters(done, p.adapters);
 }
 
 // out = s_l * sum of the splits' partials that hold rows of the adapter, in split order.
@@ -824,18 +824,23 @@ static bool needs_transposed(int rows, int rank, int adapters) { return !on_tile
 
 // Blocks for every place on the device (two an SM) that the adapters' gradients are shared out to, besides their columns:
 // pieces of the batch, whose blocks have like amounts of rows however the adapters share them, and groups of adapters, which
-// need no partial sums.  Pieces only: 4096 rows in any order of 64 adapters of rank 64 took 404 us instead of 71, 8192 rows of 16
-// adapters of rank 16 87 instead of 66.  Groups only would leave a batch of one adapter to a few blocks.  Pieces as long as their sums, written and read again, move half the bytes of the rows at most, with
-// at least 256 rows in a piece; then groups.
+// need no partial sums but have like amounts only where the adapters have.  Pieces as long as their sums, written and read
+// again, move at most the bytes of the rows where every piece has every adapter, with at least 256 rows in a piece;
+// then groups.  Pieces only: 4096 rows in any order of 64 adapters of rank 64 took 404 us instead of 77.  Groups from half the
+// bytes of the rows on: 8192 rows in runs of 4 adapters of rank 64 took 91 us instead of 52, in any order of 16 adapters of
+// rank 16 66 instead of 87.
 static int wgrad_places(int k, int n, int rank) {
   return 2 * sm_count() / ((ceil_div(k, kWgCols) + ceil_div(n, kWgCols)) * ceil_div(rank, kWgRank));
 }
 static int wgrad_splits(int rows, int k, int n, int rank, int adapters) {
-  const long long fit = rows / (8LL * adapters * rank);
+  const long long fit = rows / (4LL * adapters * rank);
   return int(std::max(1LL, std::min({(long long)kLoraMaxSplits, (long long)wgrad_places(k, n, rank), fit, rows / 256LL})));
 }
 static int wgrad_groups(int splits, int k, int n, int rank, int adapters) {
-  return std::max(1, std::min(wgrad_places(k, n, rank) / splits, adapters));
+  const int most = std::min(wgrad_places(k, n, rank) / splits, adapters);
+  int groups = 1;
+  while (groups * 2 <= most) groups *= 2;
+  return groups;
 }
 // The backward pass's scratch, in floats: dv | A transposed | B transposed | partial sums, 16-byte aligned each.
 struct BackwardScratch {

@@ -69,7 +69,7 @@ struct AdapterGradArgs {
   const float* scaling;
   int* present;                // [splits, adapters]: whether the split has rows of the adapter, when splits > 1
   int rows, rank, adapters, splits;
-  int groups;                  // of adapters: blockIdx.y = split * groups + group
+  int groups;                  // of adapters, a power of two: blockIdx.y = split * groups + group
 };
 constexpr int kWgCols = 256;                     // columns of a gradient a block sums up
 constexpr int kWgRank = 64;                      // and its ranks; more are shared out

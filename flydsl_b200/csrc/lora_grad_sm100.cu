@@ -85,8 +85,7 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
   if (warp < kGradFill / 32) {
     // ------------------------------------------------------------------ gather
     const int begin = int((long long)p.rows * split / p.splits), end = int((long long)p.rows * (split + 1) / p.splits);
-    const int group_begin = int((long long)p.adapters * group / p.groups);
-    const int group_end = int((long long)p.adapters * (group + 1) / p.groups);
+    const int others = p.groups - 1;             // an adapter's group is its number modulo `groups`, a power of two
     const uint8_t* X = static_cast<const uint8_t*>(q.x);
     auto together = [] { asm volatile("bar.sync 1, %0;" ::"n"(kGradFill) : "memory"); };
     // The warps meet at a barrier without a limit, so a wait that gave up makes nobody leave: the walk through the rows goes on
@@ -95,14 +94,14 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
     int asked = 0, handed = 0;                   // chunks asked for, chunks handed over to the MMAs
     int older = 0, newer = 0;                    // adapters of up to two chunks between
 
-    // the smallest adapter above `l` with rows here, or the end of the group
+    // the smallest adapter of the group above `l` with rows here, or p.adapters
     auto find_next = [&](int l) -> int {
-      if (tid == 0) c->next_adapter = group_end;
+      if (tid == 0) c->next_adapter = p.adapters;
       together();
-      int best = group_end;
+      int best = p.adapters;
       for (int i = begin + tid; i < end; i += kGradFill) {
         const int id = __ldg(p.ids + i);
-        if (id > l && id < best) best = id;
+        if (id > l && id < best && (id & others) == group) best = id;
       }
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) best = min(best, __shfl_xor_sync(0xffffffffu, best, off));
@@ -114,11 +113,11 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
     auto skip_adapters = [&](int from, int to) {
       if (p.splits > 1) {
         if (blockIdx.x == 0 && blockIdx.z == 0)
-          for (int l = from + tid; l < to; l += kGradFill) p.present[(long long)split * p.adapters + l] = 0;
+          for (int l = from + tid * p.groups; l < to; l += kGradFill * p.groups) p.present[(long long)split * p.adapters + l] = 0;
         return;
       }
       const int cn = min(kWgCols, q.cols - col0);
-      for (int l = from; l < to; ++l)
+      for (int l = from; l < to; l += p.groups)
         for (int i = tid; i < ranks * cn; i += kGradFill) {
           const long long at = q.rank_major ? (long long)(j0 + i / cn) * q.cols + col0 + i % cn
                                             : (long long)(col0 + i / ranks) * p.rank + j0 + i % ranks;
@@ -154,12 +153,12 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
     const bool inside = col0 + piece * 8 < q.cols;
     const uint32_t xdst = smem_u32(xs) + (piece >> 3) * kGradChunk + warp * 128 + (((piece & 7) ^ (warp & 7)) * 16);
     const uint8_t* xsrc = X + (inside ? (long long)(col0 + piece * 8) * 2 : 0);
-    const long long row_bytes = (long long)q.cols * 2;
+    const uint32_t row_bytes = uint32_t(q.cols) * 2;             // below 2^31
 
-    int done = group_begin;                      // adapters below this one are dealt with
-    for (int l = find_next(group_begin - 1); l < group_end; l = find_next(l)) {
+    int done = group;                             // adapters of the group below this one are dealt with
+    for (int l = find_next(-1); l < p.adapters; l = find_next(l)) {
       skip_adapters(done, l);
-      done = l + 1;
+      done = l + p.groups;
       if (p.splits > 1 && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) p.present[(long long)split * p.adapters + l] = 1;
       int next = begin, taken = 0, have = 0;     // ids scanned, entries of the list used and in it (same in all threads)
       while (true) {
@@ -209,14 +208,16 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
           for (int k = 0; k < kGradRows / 8; ++k) {
             const int r = warp + k * 8;
             const bool here = r < n;
-            cp_async16(xdst + stage * kGradXBytes + k * 1024, xsrc + (here ? c->list[taken + r] : 0) * row_bytes, here && inside);
+            const uint32_t row = here ? uint32_t(c->list[taken + r]) : 0u;
+            cp_async16(xdst + stage * kGradXBytes + k * 1024, xsrc + uint64_t(row) * row_bytes, here && inside);
           }
 #pragma unroll
           for (int i = tid; i < kGradRows * (RP / 4); i += kGradFill) {
             const int r = i / (RP / 4), j = i - r * (RP / 4);
             const bool here = r < n && j * 4 < ranks;
+            const uint32_t row = here ? uint32_t(c->list[taken + r]) : 0u;
             cp_async16(smem_u32(vf + stage * kGradRows * RP * 4 + i * 16),
-                       q.v + (here ? (long long)c->list[taken + r] * p.rank + j0 + j * 4 : 0), here);
+                       q.v + (uint64_t(row) * uint32_t(p.rank) + uint32_t(here ? j0 + j * 4 : 0)), here);
           }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -230,7 +231,7 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
         ++asked;
       }
     }
-    skip_adapters(done, group_end);
+    skip_adapters(done, p.adapters);
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (asked - handed == 2) hand_over(older | (newer != older ? kGradLast : 0));
     if (asked > handed) hand_over(newer | kGradLast);
