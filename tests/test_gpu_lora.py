@@ -68,7 +68,7 @@ SIZES = [
     (640, 1288, 328, 128, 3, "requests"), (900, 72, 64, 8, 2, "requests"), (2600, 1032, 136, 56, 5, "requests"),
     (50, 64, 64, 40, 3, "none"), (600, 2048, 136, 104, 9, "tokens"), (900, 264, 584, 16, 8, "tokens"),
     (777, 1032, 264, 64, 7, "tokens"), (1100, 520, 72, 56, 9, "tokens"), (640, 136, 264, 72, 4, "tokens"), (600, 72, 520, 88, 5, "tokens"),
-    (1200, 256, 264, 16, 40, "one"), (300, 200, 1096, 120, 33, "tokens"),
+    (1200, 256, 264, 16, 40, "one"), (300, 200, 1096, 120, 33, "tokens"), (40, 64, 72, 8, 3000, "tokens"), (5000, 64, 72, 8, 300, "tokens"),
 ]
 
 
