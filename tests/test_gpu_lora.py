@@ -253,3 +253,24 @@ def test_beside_the_shared_projection_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(c, eager[j])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("adapters", [3, 40])
+def test_in_place_where_tiles_have_no_adapter(adapters, dtype):
+    """Runs of rows without an adapter longer than a tile, beside tiles of few adapters and of many."""
+    p, _ = make(1700, 136, 392, 24, adapters, dtype, "tokens", seed=12)
+    ids = p["adapter_ids"]
+    ids[:300] = -1
+    ids[300:700] = 1
+    ids[1100:1450] = adapters                    # names no adapter either
+    want = lora_add(**p)
+    (out, mag), *_ = exact(p, want)
+    check(want, (out, mag), 136 + 24, "out")
+    none = (ids < 0) | (ids >= adapters)
+    assert torch.equal(want[none], p["y"][none])
+    y = p["y"].clone()
+    rest = [p[s] for s in ("x", "a", "b", "adapter_ids", "scaling")]
+    assert lora_add(y, *rest, out=y) is y and torch.equal(y, want)
+    ids.fill_(-1)
+    assert torch.equal(lora_add(y, *rest, out=y), want) and torch.equal(lora_add(want, *rest), want)
