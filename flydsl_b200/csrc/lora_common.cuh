@@ -81,9 +81,15 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool o
 // The launches of one operator follow each other closely (programmatic stream serialisation): the next one's blocks start,
 // and set up what touches no global memory, while the last blocks of this one run.  Every kernel launched this way waits
 // here before its first access to global memory; the wait ends when all launches before it are done.
-__device__ __forceinline__ void after_previous_launch() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+//
+// TMEM is taken between the two, never before the wait and never after the signal.  A block that held some while it waited
+// could share an SM with a block of the launch that it waits for, which needs more than is left: neither
+// tcgen05.alloc nor this wait has a limit.  The first thread of a block that signals does so for all of it.
+__device__ __forceinline__ void wait_for_previous_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_launch_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void after_previous_launch() {        // for kernels without TMEM
+  wait_for_previous_launch();
+  let_next_launch_start();
 }
 template <typename... Params, typename... Args>
 inline cudaError_t launch_closely(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {

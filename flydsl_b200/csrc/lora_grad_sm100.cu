@@ -67,6 +67,7 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
   const int split = int(blockIdx.y) / p.groups, group = int(blockIdx.y) - split * p.groups;
 
   if (warp == 8) {
+    wait_for_previous_launch();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(&c->tmem_base)), "r"(uint32_t(kGradTmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -79,7 +80,8 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  after_previous_launch();
+  wait_for_previous_launch();
+  let_next_launch_start();
   const uint32_t tmem = c->tmem_base;
 
   if (warp < kGradFill / 32) {

@@ -67,7 +67,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
   // block on an SM.  Sums are read 32 columns at a time, so also what the last read reaches past a rank of 16 modulo 32.
   uint32_t tmem_cols = 0;
   if (warp == 1) {
-    after_previous_launch();
+    wait_for_previous_launch();
     int id[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, row0 + i * 32 + lane, p.rows, p.adapters);
@@ -92,7 +92,8 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  after_previous_launch();
+  wait_for_previous_launch();
+  let_next_launch_start();
   const uint32_t tmem = c->tmem_base;
   const int d = c->count;
   const int blocks = (p.k + 63) / 64;
@@ -238,6 +239,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (warp == 1) {
+    wait_for_previous_launch();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(smem_u32(&c->tmem_base)), "r"(uint32_t(kExAcc * kExCols)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -253,7 +255,8 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   tcgen05_fence_before();
   __syncthreads();
   tcgen05_fence_after();
-  after_previous_launch();
+  wait_for_previous_launch();
+  let_next_launch_start();
   const uint32_t tmem = c->tmem_base;
   const int steps = (p.rank + 15) / 16;          // of the contraction
   // an adapter's tile: 128 columns along the rank, or (transposed) two chunks of 64 columns with a row per rank

@@ -274,3 +274,31 @@ def test_in_place_where_tiles_have_no_adapter(adapters, dtype):
     assert lora_add(y, *rest, out=y) is y and torch.equal(y, want)
     ids.fill_(-1)
     assert torch.equal(lora_add(y, *rest, out=y), want) and torch.equal(lora_add(want, *rest), want)
+
+
+@pytest.mark.parametrize("rank", [64, 128])
+def test_gradient_of_a_alone_behind_other_launches(rank):
+    """Without dx the kernel of the adapters' gradients follows the shrink of dv directly, and tiles of up to eight adapters want
+    all of TMEM: steps queued one behind the other, then captured."""
+    rows, k, n, adapters = 20000, 136, 264, 8
+    p, dout = make(rows, k, n, rank, adapters, BF, "requests", seed=13)
+    p["adapter_ids"] = ((torch.arange(rows, device="cuda") // 30) % adapters).int()
+    *_, (da, ma), _ = exact(p, dout)
+    a = p["a"].clone().requires_grad_()
+
+    def step():
+        out = lora_add(p["y"], p["x"], a, p["b"], p["adapter_ids"], p["scaling"])
+        return torch.autograd.grad(out, (a,), dout)[0]
+
+    torch.cuda.synchronize()
+    grads = [step() for _ in range(20)]
+    check(grads[0], (da, ma), n + rows, "da")
+    assert all(torch.equal(g, grads[0]) for g in grads)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(5):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, grads[0])
