@@ -47,7 +47,7 @@ __device__ __forceinline__ void mma16816<__half>(float* c, const uint32_t* a, ui
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint4 ldg16(const void* p) { return __ldg(static_cast<const uint4*>(p)); }
+__device__ __forceinline__ uint4 load16(const void* p) { return fetch(static_cast<const uint4*>(p)); }
 
 // ---------------------------------------------------------------------------- groups of rows
 // The rows of a window (512) in groups of up to 16 that share an adapter, whatever order they come in.  Every block builds
@@ -170,7 +170,7 @@ lora_shrink_kernel(const ShrinkArgs p, const int slots, const int skip_tiles) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int row0 = int(blockIdx.x) / slots * kWindow;
   after_previous_launch();
-  build_groups(&s, p.ids, row0, p.rows, p.adapters, skip_tiles, false);
+  build_groups(&s, written_before(p.ids), row0, p.rows, p.adapters, skip_tiles, false);
   const int steps = (p.k + 31) / 32;
   const int s0 = int((long long)steps * blockIdx.y / p.splits), s1 = int((long long)steps * (blockIdx.y + 1) / p.splits);
   const int from = s0 + (s1 - s0) * warp / kShrinkWarps, to = s0 + (s1 - s0) * (warp + 1) / kShrinkWarps;
@@ -193,10 +193,10 @@ lora_shrink_kernel(const ShrinkArgs p, const int slots, const int skip_tiles) {
         const int k = (st + u) * 32 + t * 8;
         const bool ok = st + u < to && k < p.k;
         const uint4 zero = make_uint4(0, 0, 0, 0);
-        x0[u] = ok ? ldg16(xr0 + k) : zero;
-        x1[u] = ok ? ldg16(xr1 + k) : zero;
+        x0[u] = ok ? load16(xr0 + k) : zero;
+        x1[u] = ok ? load16(xr1 + k) : zero;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) b[u][i] = ok && i * 8 + g < p.rank ? ldg16(al + (long long)(i * 8 + g) * p.k + k) : zero;
+        for (int i = 0; i < NT; ++i) b[u][i] = ok && i * 8 + g < p.rank ? load16(al + (long long)(i * 8 + g) * p.k + k) : zero;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -229,12 +229,13 @@ lora_shrink_kernel(const ShrinkArgs p, const int slots, const int skip_tiles) {
 
 // The splits' sums added up, in their order.
 __global__ void __launch_bounds__(256)
-lora_fold_kernel(const float4* __restrict__ planes, float4* __restrict__ v, long long vecs, int splits) {
+lora_fold_kernel(const float4* sums, float4* v, long long vecs, int splits) {
   after_previous_launch();
+  const float4* planes = written_before(sums);
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < vecs; i += (long long)gridDim.x * 256) {
-    float4 sum = __ldg(planes + i);
+    float4 sum = fetch(planes + i);
     for (int s = 1; s < splits; ++s) {
-      const float4 x = __ldg(planes + s * vecs + i);
+      const float4 x = fetch(planes + s * vecs + i);
       sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
     }
     v[i] = sum;
@@ -253,7 +254,7 @@ lora_expand_kernel(const ExpandArgs p, const int slots, const int per_warp, cons
   const int row0 = int(blockIdx.x) / slots * kWindow;
   after_previous_launch();
   // rows without an adapter have to be written unless they are there already
-  build_groups(&s, p.ids, row0, p.rows, p.adapters, skip_tiles, p.out != p.base);
+  build_groups(&s, written_before(p.ids), row0, p.rows, p.adapters, skip_tiles, p.out != p.base);
   const int c0 = (int(blockIdx.y) * (kGroupThreads / 32) + warp) * per_warp * 32;
   if (c0 >= p.n) return;
   for (int grp = int(blockIdx.x) % slots; grp < s.count; grp += slots) {
@@ -265,17 +266,21 @@ lora_expand_kernel(const ExpandArgs p, const int slots, const int per_warp, cons
     uint32_t hi[KS][4], lo[KS][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      scale[h] = l >= 0 ? __ldg(p.scaling + l) : 0.f;
+      scale[h] = l >= 0 ? fetch(p.scaling + l) : 0.f;
       float4 x[KS];
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        x[ks] = make_float4(0.f, 0.f, 0.f, 0.f);
-        const int k = ks * 16 + t * 4;
-        if (l >= 0 && live[h] && k < p.rank)
-          for (int q = 0; q < p.splits; ++q) {
-            const float4 v = __ldg(reinterpret_cast<const float4*>(p.v + ((long long)q * p.rows + row[h]) * p.rank + k));
-            x[ks].x += v.x; x[ks].y += v.y; x[ks].z += v.z; x[ks].w += v.w;
-          }
+      for (int ks = 0; ks < KS; ++ks) x[ks] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (l >= 0 && live[h]) {
+        const float* from = p.v + row[h] * p.rank + t * 4;
+#pragma unroll 4
+        for (int q = 0; q < p.splits; ++q, from += (long long)p.rows * p.rank) {
+          float4 v[KS];                          // all in flight together
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+            v[ks] = ks * 16 + t * 4 < p.rank ? fetch(reinterpret_cast<const float4*>(from + ks * 16)) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) { x[ks].x += v[ks].x; x[ks].y += v[ks].y; x[ks].z += v[ks].z; x[ks].w += v[ks].w; }
+        }
       }
       if constexpr (std::is_same<T, __half>::value) {
         float amax = 0.f;
@@ -314,7 +319,7 @@ lora_expand_kernel(const ExpandArgs p, const int slots, const int per_warp, cons
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int k = ks * 16 + t * 4, bc = c0 + cg * 32 + 8 * (g >> 1) + 2 * j + (g & 1);
-            b[ks][j] = bc < p.n && k < p.rank ? __ldg(reinterpret_cast<const uint2*>(bl + (long long)bc * p.rank + k))
+            b[ks][j] = bc < p.n && k < p.rank ? fetch(reinterpret_cast<const uint2*>(bl + (long long)bc * p.rank + k))
                                               : make_uint2(0, 0);
           }
 #pragma unroll
@@ -383,6 +388,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
   const T* X = static_cast<const T*>(q.x);
   const long long mat = (long long)q.cols * p.rank;
   after_previous_launch();
+  const int* ids = written_before(p.ids);
 
   // the smallest adapter of the group above `l` with rows here, or p.adapters
   auto find_next = [&](int l) -> int {
@@ -390,7 +396,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
     __syncthreads();
     int best = p.adapters;
     for (int i = begin + tid; i < end; i += kWgThreads) {
-      const int id = __ldg(p.ids + i);
+      const int id = fetch(ids + i);
       if (id > l && id < best && (id & others) == group) best = id;
     }
 #pragma unroll
@@ -439,7 +445,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int at = next + (warp * 4 + i) * 32 + lane;
-          mine[i] = __ballot_sync(0xffffffffu, at < end && __ldg(p.ids + at) == l);
+          mine[i] = __ballot_sync(0xffffffffu, at < end && fetch(ids + at) == l);
           n += __popc(mine[i]);
         }
         if (lane == 0) warp_n[warp] = n;
@@ -581,7 +587,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 
-    const float s = (p.splits == 1 ? __ldg(p.scaling + l) : 1.f);
+    const float s = (p.splits == 1 ? fetch(p.scaling + l) : 1.f);
     const float up = exponent >= -110 ? exp2i(exponent) : 1.f;
 #pragma unroll
     for (int f = 0; f < 2; ++f)
@@ -618,17 +624,20 @@ lora_wgrad_finish_kernel(const AdapterGradArgs p) {
   if (q.out == nullptr) return;
   const long long mat = (long long)q.cols * p.rank, all = mat * p.adapters;
   after_previous_launch();
+  const float* partial = written_before(q.partial);
+  const int* present = written_before(p.present);
+  const float* scaling = written_before(p.scaling);
   for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < all; i += (long long)gridDim.x * 1024) {
     const int l = int(i / mat);
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     bool any = false;
     for (int s = 0; s < p.splits; ++s) {
-      if (__ldg(p.present + (long long)s * p.adapters + l) == 0) continue;
-      const float4 v = __ldg(reinterpret_cast<const float4*>(q.partial + s * all + i));
+      if (fetch(present + (long long)s * p.adapters + l) == 0) continue;
+      const float4 v = fetch(reinterpret_cast<const float4*>(partial + s * all + i));
       sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
       any = true;
     }
-    const float f = any ? __ldg(p.scaling + l) : 0.f;
+    const float f = any ? fetch(scaling + l) : 0.f;
     uint2 o;
     o.x = pack2<T>(sum.x * f, sum.y * f);
     o.y = pack2<T>(sum.z * f, sum.w * f);
@@ -652,12 +661,13 @@ lora_transpose_kernel(const TransposeArgs p) {
   const uint16_t* src = p.src[which] + mat;
   uint16_t* dst = p.dst[which] + mat;
   after_previous_launch();
+  src = written_before(src);
   for (int t = blockIdx.x; t < across * ((rows + 63) / 64); t += gridDim.x) {
     const int c0 = t % across * 64, r0 = t / across * 64, x = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;
 #pragma unroll
     for (int i = y; i < 64; i += 32)
       if (r0 + i < rows && c0 + x < cols) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + (long long)(r0 + i) * cols + c0 + x));
+        const uint4 v = fetch(reinterpret_cast<const uint4*>(src + (long long)(r0 + i) * cols + c0 + x));
         uint32_t* to = reinterpret_cast<uint32_t*>(&tile[i][x]);
         to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
       }

@@ -89,6 +89,7 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
     const int begin = int((long long)p.rows * split / p.splits), end = int((long long)p.rows * (split + 1) / p.splits);
     const int others = p.groups - 1;             // an adapter's group is its number modulo `groups`, a power of two
     const uint8_t* X = static_cast<const uint8_t*>(q.x);
+    const int* ids = written_before(p.ids);
     auto together = [] { asm volatile("bar.sync 1, %0;" ::"n"(kGradFill) : "memory"); };
     // The warps meet at a barrier without a limit, so a wait that gave up makes nobody leave: the walk through the rows goes on
     // and touches nothing any more.
@@ -102,7 +103,7 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
       together();
       int best = p.adapters;
       for (int i = begin + tid; i < end; i += kGradFill) {
-        const int id = __ldg(p.ids + i);
+        const int id = fetch(ids + i);
         if (id > l && id < best && (id & others) == group) best = id;
       }
 #pragma unroll
@@ -179,7 +180,7 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int at = next + (warp * 4 + i) * 32 + lane;
-              mine[i] = __ballot_sync(0xffffffffu, at < end && __ldg(p.ids + at) == l);
+              mine[i] = __ballot_sync(0xffffffffu, at < end && fetch(ids + at) == l);
               n += __popc(mine[i]);
             }
             if (lane == 0) c->warp_n[warp] = n;
@@ -290,7 +291,7 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
       const int l = *const_cast<volatile int*>(&c->sum_adapter[sum]);
       if (l < 0) break;
       tcgen05_fence_after();
-      const float scale = p.splits == 1 ? __ldg(p.scaling + l) : 1.f;
+      const float scale = p.splits == 1 ? fetch(p.scaling + l) : 1.f;
       float* partial = q.partial + ((long long)split * p.adapters + l) * mat;
       __nv_bfloat16* out = static_cast<__nv_bfloat16*>(q.out) + (long long)l * mat;
 #pragma unroll 1

@@ -70,7 +70,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     wait_for_previous_launch();
     int id[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, row0 + i * 32 + lane, p.rows, p.adapters);
+    for (int i = 0; i < 4; ++i) id[i] = row_adapter(written_before(p.ids), row0 + i * 32 + lane, p.rows, p.adapters);
     int n = tile_adapters(id, lane, tile_limit(p.rank), c->list);
     if (blockIdx.y == 0 && lane == 0) p.counts[blockIdx.x] = n;
     if (n > tile_limit(p.rank)) n = 0;           // the other tiles are not this kernel's
@@ -159,7 +159,7 @@ lora_shrink_tc_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_c
     __syncwarp();
   } else if (warp >= 4 && d > 0) {
     // ------------------------------------------------------------------ epilogue: a thread per row
-    const int i = threadIdx.x - 128, mine = row_adapter(p.ids, row0 + i, p.rows, p.adapters);
+    const int i = threadIdx.x - 128, mine = row_adapter(written_before(p.ids), row0 + i, p.rows, p.adapters);
     float* out = p.v + ((long long)blockIdx.y * p.rows + row0 + i) * p.rank;
     const bool summed = kb1 > kb0;               // more splits than K blocks: some have nothing to add
     if (!summed || warp_wait(smem_u32(&c->acc_full), 0, abort_flag, q.status, 4)) {
@@ -258,19 +258,20 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
   wait_for_previous_launch();
   let_next_launch_start();
   const uint32_t tmem = c->tmem_base;
+  const int *ids = written_before(p.ids), *counts = written_before(p.counts);
   const int steps = (p.rank + 15) / 16;          // of the contraction
   // an adapter's tile: 128 columns along the rank, or (transposed) two chunks of 64 columns with a row per rank
   const uint32_t b_bytes = p.transposed ? steps * 16 * 256 : KC * kChunkBytes;
   const int most = tile_limit(p.rank);
   // adapters of a row tile; more than `most`: nothing to do here (the other kernel's, or no adapter and the base in place)
   auto adapters_of = [&](int rt) {
-    const int d = __ldg(p.counts + rt);
+    const int d = fetch(counts + rt);
     return d == 0 && p.base == p.out ? most + 1 : d;
   };
   auto find_adapters = [&](int rt, int* list) {
     int id[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) id[i] = row_adapter(p.ids, rt * kTileRows + i * 32 + lane, p.rows, p.adapters);
+    for (int i = 0; i < 4; ++i) id[i] = row_adapter(ids, rt * kTileRows + i * 32 + lane, p.rows, p.adapters);
     const int n = tile_adapters(id, lane, most, list);
     __syncwarp();
     return n;
@@ -471,15 +472,15 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
           const int r = rt * kTileRows + s * 32 + r8;
-          id[s] = row_adapter(p.ids, r, p.rows, p.adapters);
+          id[s] = row_adapter(ids, r, p.rows, p.adapters);
 #pragma unroll
           for (int h = 0; h < KC * 2; ++h) {
             x[s][h] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (r < p.rows && h * 8 + l8 < vecs) x[s][h] = __ldg(reinterpret_cast<const float4*>(p.v) + (long long)r * vecs + h * 8 + l8);
+            if (r < p.rows && h * 8 + l8 < vecs) x[s][h] = fetch(reinterpret_cast<const float4*>(p.v) + (long long)r * vecs + h * 8 + l8);
           }
         }
-        mine = row_adapter(p.ids, rt * kTileRows + row, p.rows, p.adapters);
-        scale = mine >= 0 ? __ldg(p.scaling + mine) : 0.f;
+        mine = row_adapter(ids, rt * kTileRows + row, p.rows, p.adapters);
+        scale = mine >= 0 ? fetch(p.scaling + mine) : 0.f;
         if (et < 32) find_adapters(rt, c->list[1 + turn]);
 #pragma unroll
         for (int s = 0; s < 4; ++s) {

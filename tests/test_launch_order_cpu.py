@@ -44,3 +44,11 @@ def test_tmem_is_taken_between_the_wait_and_the_signal(body):
     # everyone else waits as well before the first access to global memory
     met = body.index("__syncthreads();", taken[-1])
     assert body[met:signal].count(WAIT) == 1
+
+
+@pytest.mark.parametrize("name", sorted(p.name for p in CSRC.glob("lora*")))
+def test_nothing_is_read_through_the_read_only_path(name):
+    """Their inputs may have been written by a launch that was still running when they started."""
+    text = re.sub(r"//.*", "", (CSRC / name).read_text())
+    assert not re.findall(r"__ldg|__restrict__|ld\.global\.nc", text)
+    assert "vec8.cuh" not in text                # its loads are read-only ones
