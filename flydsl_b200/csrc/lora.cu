@@ -16,7 +16,9 @@
 //
 // v enters the second product as the sum of two 16-bit numbers (high part and remainder), which keeps 16 (bf16) or 22 (fp16)
 // bits of it: one rounding of the output is all that shows.  fp16 has few exponent bits, so there a row of v is brought to
-// the same power of two first.
+// the same power of two first.  A remainder that is zero or of the other sign makes no number of an infinity (0 * inf, inf - inf):
+// where the product with the high part is not finite it is the result.  (In fp16 a number below 2^-38 of the largest beside
+// it has no high part and counts as zero.)
 //
 // Gradients use the same kernels: dv = dout B_l is a shrink with B transposed, dx = s_l dv A_l an expand with A transposed
 // (the tiles read them across, this file's kernels want copies).  dA_l = s_l sum dv^T x and dB_l = s_l sum dout^T v contract
@@ -309,9 +311,11 @@ lora_expand_kernel(const ExpandArgs p, const int slots, const int per_warp, cons
       for (int h = 0; h < 2; ++h)
         y[h] = p.base && live[h] && col < p.n ? *reinterpret_cast<const uint4*>(static_cast<const T*>(p.base) + row[h] * p.n + col)
                                               : make_uint4(0, 0, 0, 0);
-      float c[4][4];
+      float c[4][4], d[4][4];                    // products with the high parts, with the remainders
 #pragma unroll
-      for (int j = 0; j < 4; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[j][i] = d[j][i] = 0.f;
       if (l >= 0) {
         uint2 b[KS][4];
 #pragma unroll
@@ -327,8 +331,12 @@ lora_expand_kernel(const ExpandArgs p, const int slots, const int per_warp, cons
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             mma16816<T>(c[j], hi[ks], b[ks][j].x, b[ks][j].y);
-            mma16816<T>(c[j], lo[ks], b[ks][j].x, b[ks][j].y);
+            mma16816<T>(d[j], lo[ks], b[ks][j].x, b[ks][j].y);
           }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) c[j][i] = of_two_parts(c[j][i], d[j][i]);
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -421,12 +429,10 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
       }
   };
 
-  int done = group;                               // adapters of the group below this one are dealt with
-  for (int l = find_next(-1); l < p.adapters; l = find_next(l)) {
-    skip_adapters(done, l);
-    done = l + p.groups;
-    if (p.splits > 1 && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) p.present[(long long)split * p.adapters + l] = 1;
-
+  // The sums of adapter l.  High parts and remainders share them; an adapter whose sums have a NaN is gone through once more
+  // (`first` false) with the high parts alone, for the sums that are then not finite: against an infinity the remainder would
+  // turn them into NaN.  Returns whether this thread has one.
+  auto sum_up = [&](int l, auto first) -> bool {
     int next = begin, taken = 0, have = 0;       // ids scanned, entries of the list used and in it (same in all threads)
     // appends rows of this adapter until the list holds a chunk or the rows are through
     auto refill = [&]() {
@@ -579,6 +585,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
           }
 #pragma unroll
           for (int f = 0; f < 2; ++f) {
+            if (!first) break;
             mma16816<T>(c[f][2 * j], a[f], w[0], w[1]);
             mma16816<T>(c[f][2 * j + 1], a[f], w[2], w[3]);
           }
@@ -589,6 +596,7 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
 
     const float s = (p.splits == 1 ? fetch(p.scaling + l) : 1.f);
     const float up = exponent >= -110 ? exp2i(exponent) : 1.f;
+    uint64_t sums = 0;                           // looks for NaNs
 #pragma unroll
     for (int f = 0; f < 2; ++f)
 #pragma unroll
@@ -598,20 +606,35 @@ lora_wgrad_kernel(const AdapterGradArgs p) {
           const int col = col0 + warp * 32 + f * 16 + h * 8 + g, j = j0 + i * 8 + t * 2;
           if (col >= q.cols || j >= p.rank) continue;
           const float v0 = c[f][i][h * 2] * up * s, v1 = c[f][i][h * 2 + 1] * up * s;
+          add_pair(sums, c[f][i][h * 2], c[f][i][h * 2 + 1]);
+          const bool put0 = first || !isfinite(c[f][i][h * 2]), put1 = first || !isfinite(c[f][i][h * 2 + 1]);
           const long long at = q.rank_major ? (long long)j * q.cols + col : (long long)col * p.rank + j;
           const long long step = q.rank_major ? q.cols : 1;
           if (p.splits > 1) {
             float* o = q.partial + ((long long)split * p.adapters + l) * mat + at;
-            o[0] = v0;
-            o[step] = v1;
+            if (put0) o[0] = v0;
+            if (put1) o[step] = v1;
           } else {
             const uint32_t pk = pack2<T>(v0, v1);
             T* o = static_cast<T*>(q.out) + (long long)l * mat + at;
-            o[0] = reinterpret_cast<const T*>(&pk)[0];
-            o[step] = reinterpret_cast<const T*>(&pk)[1];
+            if (put0) o[0] = reinterpret_cast<const T*>(&pk)[0];
+            if (put1) o[step] = reinterpret_cast<const T*>(&pk)[1];
           }
         }
-    __syncthreads();                             // the list and the stages are free for the next adapter
+    return either_nan(sums);
+  };
+
+  int done = group;                               // adapters of the group below this one are dealt with
+  for (int l = find_next(-1); l < p.adapters; l = find_next(l)) {
+    skip_adapters(done, l);
+    done = l + p.groups;
+    if (p.splits > 1 && blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) p.present[(long long)split * p.adapters + l] = 1;
+    const bool undefined = sum_up(l, std::true_type());
+    // from here on the list and the stages are free for the next adapter
+    if (__syncthreads_or(undefined)) {
+      sum_up(l, std::false_type());
+      __syncthreads();
+    }
   }
   skip_adapters(done, p.adapters);
 }

@@ -26,6 +26,15 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   const float2 h = unpack2<T>(hi);
   lo = pack2<T>(isfinite(h.x) ? a - h.x : 0.f, isfinite(h.y) ? b - h.y : 0.f);
 }
+// Sum of products with the high parts and with the remainders.
+__device__ __forceinline__ float of_two_parts(float hi, float lo) { return isfinite(hi) ? hi + lo : hi; }
+// Sums of many numbers, two at a time, that are NaN where one of the numbers is (or two infinities of either sign are there).
+__device__ __forceinline__ void add_pair(uint64_t& sums, float a, float b) {
+  asm("{\n\t.reg .b64 p;\n\tmov.b64 p, {%1, %2};\n\tadd.rn.f32x2 %0, %0, p;\n\t}" : "+l"(sums) : "f"(a), "f"(b));
+}
+__device__ __forceinline__ bool either_nan(uint64_t sums) {
+  return isnan(__uint_as_float(uint32_t(sums))) || isnan(__uint_as_float(uint32_t(sums >> 32)));
+}
 // 2^e and 2^-e with the largest of `amax`'s numbers at 2^13 .. 2^14 afterwards (fp16 overflows at 2^16).
 __device__ __forceinline__ int scale_exponent(float amax) {
   if (!(amax > 0.f)) return 0;

@@ -306,7 +306,7 @@ lora_wgrad_tc_kernel(const AdapterGradArgs p, int* status) {
           tmem_ld_wait();
           float v[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = (__uint_as_float(hi[i]) + __uint_as_float(lo[i])) * scale;
+          for (int i = 0; i < 16; ++i) v[i] = of_two_parts(__uint_as_float(hi[i]), __uint_as_float(lo[i])) * scale;
           if (col >= q.cols) continue;
 #pragma unroll
           for (int i = 0; i < 16; i += 8) {

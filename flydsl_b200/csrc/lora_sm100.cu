@@ -223,11 +223,30 @@ struct ExpandTcArgs {
   int* status;
 };
 
+// Products that came out as NaN, once more from the definition: high part and remainder share an accumulator, where against an
+// infinity the remainder turns infinite products into NaN (see lora.cu).  64 columns of a row's output in shared memory.
+template <typename T>
+__device__ __noinline__ void expand_again(const ExpandArgs& p, uint8_t* line, int sw, int adapter, int row, int col) {
+  const T* b = static_cast<const T*>(p.b) + (long long)adapter * p.n * p.rank;
+  const T* base = static_cast<const T*>(p.base);
+  const float* v = p.v + (long long)row * p.rank;
+  for (int i = 0; i < min(64, p.n - col); ++i) {
+    T* out = reinterpret_cast<T*>(line + ((i >> 3) ^ sw) * 16) + (i & 7);
+    if (!isnan(float(*out))) continue;
+    float sum = 0.f;
+    for (int j = 0; j < p.rank; ++j)
+      sum = fmaf(v[j], float(b[p.transposed ? (long long)j * p.n + col + i : (long long)(col + i) * p.rank + j]), sum);
+    const float y = base ? float(base[(long long)row * p.n + col + i]) : 0.f;       // the tile is not stored yet
+    const uint32_t pk = pack2<T>(fmaf(p.scaling[adapter], sum, y), 0.f);
+    *out = reinterpret_cast<const T*>(&pk)[0];
+  }
+}
+
 // KC: chunks of 64 in the rank.
 template <typename T, int KC>
 __global__ void __launch_bounds__(kExThreads, 1)
 lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_constant__ CUtensorMap tmap_out,
-                      const __grid_constant__ CUtensorMap tmap_b, const ExpandTcArgs q) {
+                      const __grid_constant__ CUtensorMap tmap_b, const __grid_constant__ ExpandTcArgs q) {
   constexpr int kExY = ex_y_stages<KC>(), kExB = ex_b_stages<KC>();
   extern __shared__ uint8_t smem_dyn[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~uintptr_t(1023));
@@ -549,16 +568,19 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
                         reinterpret_cast<uint32_t*>(v + h * 32));
           tmem_ld_wait();
           if (hit) {
+            uint64_t sums = 0;                   // looks for NaNs
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               uint32_t* w = reinterpret_cast<uint32_t*>(&y[j]);
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
+                add_pair(sums, v[j * 8 + k * 2], v[j * 8 + k * 2 + 1]);
                 const float2 f = unpack2<T>(w[k]);
                 w[k] = pack2<T>(fmaf(scale, v[j * 8 + k * 2], f.x), fmaf(scale, v[j * 8 + k * 2 + 1], f.y));
               }
               *reinterpret_cast<uint4*>(line + ((j ^ sw) * 16)) = y[j];
             }
+            if (either_nan(sums)) expand_again<T>(p, line, sw, mine, rt * kTileRows + row, col + wg * 64);
           }
         }
         tcgen05_fence_before();

@@ -302,3 +302,25 @@ def test_gradient_of_a_alone_behind_other_launches(rank):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, grads[0])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("rows,rank,adapters,mix", [(100, 24, 4, "requests"), (700, 24, 4, "requests"), (1500, 128, 3, "requests"),
+                                                    (700, 16, 40, "tokens"), (900, 72, 3, "requests")])
+def test_infinities_stay_infinities(rows, rank, adapters, mix, dtype):
+    """One entry of a tensor is infinite: what the formulas make infinite, NaN or finite comes out as that."""
+    k, n, inf = 136, 200, float("inf")
+    for place, sign in (("x", 1), ("a", -1), ("b", 1), ("dout", -1), ("b", -1), ("x", -1)):
+        p, dout = make(rows, k, n, rank, adapters, dtype, mix, seed=14)
+        row = int((p["adapter_ids"] == 1).nonzero()[-1])
+        {"x": p["x"][row], "a": p["a"][1, rank - 1], "b": p["b"][1, n - 1], "dout": dout[row]}[place][3] = sign * inf
+        want = exact(p, dout)
+        q = {s: (t.clone().requires_grad_() if s in "xab" else t) for s, t in p.items()}
+        res = lora_add(**q)
+        got = (res.detach(), *torch.autograd.grad(res, (q["x"], q["a"], q["b"]), dout))
+        for name, out, (ref, mag), terms in zip(("out", "dx", "da", "db"), got, want, (k + rank, n + rank, n + rows, k + rows)):
+            what = f"{name}, {place} {sign * inf}"
+            assert torch.equal(out.isnan(), ref.isnan()), what
+            odd = ~ref.isfinite()
+            assert torch.equal(out[ref.isinf()].double(), ref[ref.isinf()]), what
+            check(out[~odd], (ref[~odd], mag[~odd]), terms, what)
