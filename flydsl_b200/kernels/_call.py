@@ -6,6 +6,7 @@ import contextlib
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
@@ -27,6 +28,16 @@ def on(device: torch.device, stream=None):
     if device.index is None or device.index == torch._C._cuda_getDevice():     # current_device() without its wrapper
         return _HERE
     return torch.cuda.device(device)
+
+
+def tracked(*tensors) -> bool:
+    """Whether autograd has to see a call: one of its inputs requires a gradient, or carries a tangent of forward mode (which
+    the functions here have not, and then say so)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                return True
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def once(backward):

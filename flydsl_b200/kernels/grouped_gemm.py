@@ -23,7 +23,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._call import HALF, on, once, require_apart, require_same_device, require_shape
+from ._call import HALF, on, once, require_apart, require_same_device, require_shape, tracked
 
 
 def _check(rows_name, rows, mats_name, mats, offsets, out, out_shape):
@@ -145,6 +145,6 @@ class _GroupedLinear(torch.autograd.Function):
 def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     """``grouped_gemm`` in autograd: gradients reach ``x`` and ``w``.  Runs on the current stream."""
     sizes = _sizes(x, w, offsets, None, False) or _check_rows_form("x", x, w, offsets, None, False)
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+    if tracked(x, w):
         return _GroupedLinear.apply(x, w, offsets, sizes)
     return _run_rows_form(x, w, offsets, None, None, False, sizes)

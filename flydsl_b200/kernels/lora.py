@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._call import HALF, on, once, require_apart, require_same_device, require_shape
+from ._call import HALF, on, once, require_apart, require_same_device, require_shape, tracked
 
 MAX_RANK = 128
 
@@ -125,12 +125,11 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     With ``out`` or ``stream`` the call is for inference only (no input may require a gradient while gradients are on)."""
     if not _fits(y, x, a, b, adapter_ids, scaling, out):
         _check(y, x, a, b, adapter_ids, scaling, out)
-    if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad
-                                    or scaling.requires_grad):
+    if tracked(y, x, a, b, scaling):
         if scaling.requires_grad:
             raise ValueError("scaling has no gradient here: detach it, or put it into b")
         if out is not None or stream is not None:
-            raise ValueError("out= and stream= are for inference: an input requires a gradient")
+            raise ValueError("out= and stream= are for inference: an input requires a gradient or has a tangent")
         return _LoraAdd.apply(y, x, a, b, adapter_ids, scaling)
     with on(x.device, stream):
         if out is None:

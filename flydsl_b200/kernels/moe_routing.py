@@ -20,7 +20,7 @@ from typing import NamedTuple
 import torch
 
 from .. import _lib
-from ._call import on, once, require_same_device, require_shape
+from ._call import on, once, require_same_device, require_shape, tracked
 from .moe_sorting_kernel import moe_sorting_flydsl
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -127,7 +127,7 @@ def topk_gating(logits: torch.Tensor, topk: int, *, renormalize: bool = True) ->
         raise ValueError(f"logits must have 1 to 1024 experts, got {experts}")
     if not 1 <= int(topk) <= min(32, experts):
         raise ValueError(f"topk must be in [1, min(32, experts)], got {topk}")
-    run = _TopkGating.apply if logits.requires_grad and torch.is_grad_enabled() else _gate
+    run = _TopkGating.apply if tracked(logits) else _gate
     return run(logits, int(topk), 1 if renormalize else 0)
 
 
@@ -217,7 +217,7 @@ def moe_permute(x: torch.Tensor, plan: RoutedRows) -> torch.Tensor:
     tokens, topk = _check_plan(plan, "x", x, 0)
     if x.shape[0] != tokens or plan[0].numel() < tokens * topk:
         raise ValueError(f"x has {x.shape[0]} rows, the plan is for {tokens} tokens of {topk} pairs")
-    return _Permute.apply(x, plan) if x.requires_grad and torch.is_grad_enabled() else _permute(x, plan)
+    return _Permute.apply(x, plan) if tracked(x) else _permute(x, plan)
 
 
 class _Combine(torch.autograd.Function):
@@ -260,6 +260,6 @@ def moe_combine(rows: torch.Tensor, weights: torch.Tensor, plan: RoutedRows) -> 
         require_shape("weights", weights, (tokens, topk))
         require_same_device("rows", rows.device, weights=weights)
         sizes = tokens, topk, *rows.shape
-    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+    if tracked(rows, weights):
         return _Combine.apply(rows, weights, plan, sizes)
     return _combine(rows, weights, plan, sizes)
