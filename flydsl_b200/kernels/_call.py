@@ -40,6 +40,13 @@ def tracked(*tensors) -> bool:
     return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
+def in_order(grad: torch.Tensor) -> torch.Tensor:
+    """A gradient as autograd hands it over (any strides, any place in memory) as the kernels want it: contiguous, 16-byte
+    aligned."""
+    grad = grad.contiguous()
+    return grad.clone() if grad.data_ptr() % 16 else grad
+
+
 def once(backward):
     """``once_differentiable`` without its steps (2.5 us of host time a call) where no gradient of the gradient is asked for."""
     checked = once_differentiable(backward)

@@ -23,7 +23,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._call import HALF, on, once, require_apart, require_same_device, require_shape, tracked
+from ._call import HALF, in_order, on, once, require_apart, require_same_device, require_shape, tracked
 
 
 def _check(rows_name, rows, mats_name, mats, offsets, out, out_shape):
@@ -133,7 +133,7 @@ class _GroupedLinear(torch.autograd.Function):
     @once
     def backward(ctx, dy):
         x, w, offsets = ctx.saved_tensors
-        dy = dy.contiguous()
+        dy = in_order(dy)
         dx = _run_rows_form(dy, w, offsets, None, None, True, ctx.sizes) if ctx.needs_input_grad[0] else None
         dw = None
         if ctx.needs_input_grad[1]:

@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._call import HALF, on, once, require_apart, require_same_device, require_shape, tracked
+from ._call import HALF, in_order, on, once, require_apart, require_same_device, require_shape, tracked
 
 MAX_RANK = 128
 
@@ -102,7 +102,7 @@ class _LoraAdd(torch.autograd.Function):
         if need_x or need_a or need_b:
             lib, (rows, k), (adapters, n, rank) = _lib.load(), x.shape, b.shape
             with on(x.device):
-                dout = dout.contiguous()
+                dout = in_order(dout)
                 elems = lib.flymoe_lora_backward_workspace_elems(rows, k, n, rank, adapters)
                 work = x.new_empty(elems, dtype=torch.float32)
                 if need_x:

@@ -20,7 +20,7 @@ from typing import NamedTuple
 import torch
 
 from .. import _lib
-from ._call import on, once, require_same_device, require_shape, tracked
+from ._call import in_order, on, once, require_same_device, require_shape, tracked
 from .moe_sorting_kernel import moe_sorting_flydsl
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -106,7 +106,7 @@ class _TopkGating(torch.autograd.Function):
             return None, None, None
         weights, ids, *logits = ctx.saved_tensors
         (tokens, experts), dtype, renormalize = ctx.logits
-        dweights = dweights.contiguous()
+        dweights = in_order(dweights)
         with on(weights.device):
             d = weights.new_empty((tokens, experts), dtype=dtype)
             _lib.check(_lib.load().flymoe_topk_gating_softmax_backward(
@@ -207,7 +207,7 @@ class _Permute(torch.autograd.Function):
     def backward(ctx, dxs):
         plan = _kept_plan(ctx)
         with on(dxs.device):
-            dxs = dxs.contiguous()
+            dxs = in_order(dxs)
         return _combine(dxs, None, plan, (*plan[3].shape, *dxs.shape)), None
 
 
@@ -236,7 +236,7 @@ class _Combine(torch.autograd.Function):
         need_rows, need_weights, _, _ = ctx.needs_input_grad
         drows = dw = None
         with on(rows.device):
-            dout = dout.contiguous()
+            dout = in_order(dout)
             if need_rows:
                 drows = torch.empty_like(rows)
             if need_weights:

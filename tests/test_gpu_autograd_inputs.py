@@ -1,4 +1,4 @@
-"""What autograd may hand to the operators: forward-mode tangents."""
+"""What autograd may hand to the operators: forward-mode tangents, gradients in any order and place."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -49,3 +49,29 @@ def test_tangents_are_not_dropped(name):
     with forward_ad.dual_level(), pytest.raises(ValueError, match="tangent"):
         y, x, a, b, s = calls()["lora_add"][1]
         lora_add(forward_ad.make_dual(y, y), x, a, b, calls()["lora_add"][2][0], s, out=torch.empty_like(y))
+
+
+@pytest.mark.parametrize("rows", [40, 600])
+@pytest.mark.parametrize("name", NAMES)
+def test_gradients_of_any_strides_and_alignment(name, rows):
+    f, inputs, rest = calls(rows)[name]
+    leaves = [t.clone().requires_grad_(i < 4) for i, t in enumerate(inputs)]       # the adapters' scaling has no gradient
+    out = f(*leaves, *rest)
+    leaves = leaves[:4]
+    dout = torch.randn(out.shape, generator=torch.Generator(device="cuda").manual_seed(22), device="cuda").to(out.dtype)
+    want = torch.autograd.grad(out, leaves, dout, retain_graph=True)
+    shifted = torch.empty(out.numel() + 1, dtype=out.dtype, device="cuda")[1:].view(out.shape).copy_(dout)
+    flipped = dout.t().contiguous().t()
+    joined = torch.cat([dout, dout], 1)[:, : out.shape[1]]
+    assert shifted.is_contiguous() and shifted.data_ptr() % 16 and not flipped.is_contiguous()
+    for given in (shifted, flipped, joined):
+        for a, b in zip(torch.autograd.grad(out, leaves, given, retain_graph=True), want):
+            assert torch.equal(a, b)
+    # as a loss makes them: behind a single number in one tensor, and one value for all of it
+    both = torch.cat([torch.ones(1, dtype=out.dtype, device="cuda", requires_grad=True), out.reshape(-1)])
+    pieces = torch.cat([torch.zeros(1, dtype=out.dtype, device="cuda"), dout.reshape(-1)])
+    for a, b in zip(torch.autograd.grad(both, leaves, pieces, retain_graph=True), want):
+        assert torch.equal(a, b)
+    ones = torch.autograd.grad(out, leaves, torch.ones_like(out), retain_graph=True)
+    for a, b in zip(torch.autograd.grad(out.sum(), leaves), ones):
+        assert torch.equal(a, b)
