@@ -44,7 +44,8 @@ def _combine_sizes(rows, weights, plan):
         (count, dim), pairs = rows.shape, weights.shape
         tokens, topk = pairs
         if (rows.is_cuda and rows.dtype in _FLOATS and dim >= 8 and not dim % 8 and row_index.shape == pairs
-                and weights.dtype is torch.float32 and sorted_ids.numel() >= count and nv.numel() >= 1
+                and weights.dtype is torch.float32 and min(sorted_ids.numel(), tokens * topk) <= count <= sorted_ids.numel()
+                and nv.numel() >= 1
                 and sorted_ids.dtype is i32 and nv.dtype is i32 and row_index.dtype is i32
                 and dev == weights.get_device() == sorted_ids.get_device() == nv.get_device() == row_index.get_device()
                 and rows.is_contiguous() and weights.is_contiguous() and sorted_ids.is_contiguous() and nv.is_contiguous()
@@ -251,13 +252,17 @@ class _Combine(torch.autograd.Function):
 
 
 def moe_combine(rows: torch.Tensor, weights: torch.Tensor, plan: RoutedRows) -> torch.Tensor:
-    """rows [any, dim] in expert order, weights f32 [tokens, topk] -> [tokens, dim]; gradients reach rows and weights."""
+    """rows [tokens * topk, dim] in expert order, weights f32 [tokens, topk] -> [tokens, dim]; gradients reach rows and
+    weights.  A plan whose ``sorted_ids`` are cut off behind its last pair takes as many rows as it then names, a longer one up to
+    as many as it has."""
     sizes = _combine_sizes(rows, weights, plan)
     if sizes is None:
         _require_rows("rows", rows)
         tokens, topk = _check_plan(plan, "rows", rows, rows.shape[0])
         _lib.require_cuda("weights", weights, (torch.float32,))
         require_shape("weights", weights, (tokens, topk))
+        if rows.shape[0] < min(plan[0].numel(), tokens * topk):
+            raise ValueError(f"rows has {rows.shape[0]} rows, the plan is for {min(plan[0].numel(), tokens * topk)}")
         require_same_device("rows", rows.device, weights=weights)
         sizes = tokens, topk, *rows.shape
     if tracked(rows, weights):

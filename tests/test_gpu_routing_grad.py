@@ -250,3 +250,19 @@ def test_a_captured_training_step_beside_an_eager_one():
         torch.cuda.synchronize()
         for a, b in zip(res, eager[i]):
             assert torch.equal(a, b)
+
+
+def test_rows_that_do_not_fit_the_plan_are_refused():
+    plan = route_rows(random_ids(40, 2, 8, 6, 0.3), 8)
+    used = int(plan.num_valid_ids[0])
+    rows, w = torch.ones((81, 64), dtype=BF, device="cuda"), torch.ones((40, 2), device="cuda")
+    want = moe_combine(rows[:80], w, plan)
+    for count in (0, 40, used, 79, 81):
+        with pytest.raises(ValueError, match="rows"):
+            moe_combine(rows[:count], w, plan)
+    # a plan cut off behind the pairs that have rows, and one with room behind its last row
+    cut = RoutedRows(plan.sorted_ids[:used], *plan[1:])
+    long = RoutedRows(torch.cat([plan.sorted_ids, plan.sorted_ids[:6]]), *plan[1:])
+    assert used < 80 and torch.equal(moe_combine(rows[:used], w, cut), want) and torch.equal(moe_combine(rows, w, long), want)
+    with pytest.raises(ValueError, match="rows"):
+        moe_combine(rows[: used - 1], w, cut)
