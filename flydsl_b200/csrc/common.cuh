@@ -36,6 +36,8 @@ void set_last_error_msg(const char* msg);
   } while (0)
 
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+// Rows of a batch: kernels look up to 1024 rows past the last in 32 bits.
+constexpr int kMostRows = 0x7fffffff - 1024;
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Raises a kernel's limit of dynamic shared memory, once per kernel (`seen` belongs to it) and device: the runtime call

@@ -295,6 +295,7 @@ static int ragged_common(RaggedArgs* a, const char* what, const void* out, const
     return FLYMOE_ERR_INVALID_ARGUMENT;
   };
   if (rows < 0) return fail("rows < 0");
+  if (rows > kMostRows) return fail("rows must not exceed 2^31 - 1025");
   if (experts < 1 || experts > kRagMaxExperts) return fail("experts must be in [1, 1024]");
   if (n < 8 || n % 8 || k < 8 || k % 8) return fail("n and k must be positive multiples of 8");
   // the tensor maps count bytes and the kernels columns in 32 bits

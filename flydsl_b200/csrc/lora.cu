@@ -718,6 +718,7 @@ static int lora_check(const char* what, int rows, int k, int n, int rank, int ad
   char msg[160];
   const char* why = nullptr;
   if (rows < 0) why = "rows < 0";
+  else if (rows > kMostRows) why = "rows must not exceed 2^31 - 1025";
   else if (k < 8 || k % 8 || n < 8 || n % 8) why = "k and n must be positive multiples of 8";
   else if (k > (1 << 29) || n > (1 << 29)) why = "k and n must not exceed 2^29";       // the tiles count bytes in 32 bits
   else if (rank < 8 || rank % 8 || rank > kLoraMaxRank) why = "rank must be a multiple of 8 in [8, 128]";

@@ -270,7 +270,7 @@ static int launch_gating_backward(const void* logits, const float* w, const int*
 
 static int check_routed(const char* null_msg, const char* size_msg, const void* sorted_ids, const void* num_valid_ids,
                         const void* row_index, int tokens, int topk, int rows) {
-  FLYMOE_REQUIRE(tokens >= 0 && tokens < (1 << 24) && topk >= 1 && topk <= 255 && rows >= 0, size_msg);
+  FLYMOE_REQUIRE(tokens >= 0 && tokens < (1 << 24) && topk >= 1 && topk <= 255 && rows >= 0 && rows <= kMostRows, size_msg);
   FLYMOE_REQUIRE(num_valid_ids && (rows == 0 || sorted_ids) && (tokens == 0 || row_index), null_msg);
   return FLYMOE_OK;
 }

@@ -12,6 +12,9 @@ from torch.autograd.function import once_differentiable
 from .. import _lib
 
 HALF = (torch.bfloat16, torch.float16)
+# The library takes sizes as 32-bit numbers, a larger one would arrive as another; the kernels look up to 1024 rows past the last.
+MOST_ROWS = 2 ** 31 - 1 - 1024
+MOST_COLUMNS = 2 ** 29
 _HERE = contextlib.nullcontext()
 
 
@@ -63,6 +66,11 @@ def require_shape(name: str, t: torch.Tensor, shape: tuple) -> None:
     if t.dim() != len(shape) or any(s is not None and s != d for s, d in zip(shape, t.shape)):
         want = ", ".join("*" if s is None else str(s) for s in shape)
         raise ValueError(f"{name} must have shape [{want}], got {list(t.shape)}")
+
+
+def require_count(what: str, count: int, most: int = MOST_ROWS) -> None:
+    if count > most:
+        raise ValueError(f"{what} must not exceed {most}, got {count}")
 
 
 def require_apart(out: torch.Tensor, **inputs) -> None:

@@ -23,7 +23,8 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._call import HALF, in_order, on, once, require_apart, require_same_device, require_shape, tracked
+from ._call import HALF, MOST_COLUMNS, MOST_ROWS, in_order, on, once, require_apart, require_count, require_same_device, \
+    require_shape, tracked
 
 
 def _check(rows_name, rows, mats_name, mats, offsets, out, out_shape):
@@ -37,11 +38,13 @@ def _check(rows_name, rows, mats_name, mats, offsets, out, out_shape):
     require_same_device(rows_name, rows.device, **{mats_name: mats, "offsets": offsets, "out": out})
 
 
-def _check_sizes(experts, n, k):
+def _check_sizes(rows, experts, n, k):
     if not 1 <= experts <= 1024:
         raise ValueError(f"experts must be in [1, 1024], got {experts}")
     if n < 8 or n % 8 or k < 8 or k % 8:
         raise ValueError(f"n ({n}) and k ({k}) must be positive multiples of 8")
+    require_count("rows", rows)
+    require_count("n and k", max(n, k), MOST_COLUMNS)
 
 
 def _sizes(t, w, offsets, out, input_grad):
@@ -51,7 +54,8 @@ def _sizes(t, w, offsets, out, input_grad):
         if (t.is_cuda and dt in HALF and inner == (n if input_grad else k) and bounds == experts + 1 and w.dtype is dt
                 and offsets.dtype is torch.int32 and t.get_device() == w.get_device() == offsets.get_device()
                 and t.is_contiguous() and w.is_contiguous() and offsets.is_contiguous() and n >= 8 and not n % 8 and k >= 8
-                and not k % 8 and 1 <= experts <= 1024 and out is None):
+                and not k % 8 and 1 <= experts <= 1024 and rows <= MOST_ROWS and n <= MOST_COLUMNS and k <= MOST_COLUMNS
+                and out is None):
             return rows, experts, n, k
     except (AttributeError, ValueError):
         pass
@@ -63,7 +67,7 @@ def _check_rows_form(name, t, w, offsets, out, input_grad):
         raise TypeError(f"{name}, w and offsets must be torch.Tensors")
     require_shape("w", w, (None, None, None))
     experts, n, k = w.shape
-    _check_sizes(experts, n, k)
+    _check_sizes(len(t), experts, n, k)
     require_shape(name, t, (None, n if input_grad else k))
     require_shape("offsets", offsets, (experts + 1,))
     _check(name, t, "w", w, offsets, out, (t.shape[0], k if input_grad else n))
@@ -108,7 +112,7 @@ def grouped_gemm_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor,
     k = x.shape[1]
     require_shape("offsets", offsets, (None,))
     experts = offsets.shape[0] - 1
-    _check_sizes(experts, n, k)
+    _check_sizes(rows, experts, n, k)
     _check("dy", dy, "x", x, offsets, out, (experts, n, k))
     with on(dy.device, stream):
         return _wgrad(dy, x, offsets, dy.new_empty((experts, n, k)) if out is None else out)

@@ -20,7 +20,8 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from ._call import HALF, in_order, on, once, require_apart, require_same_device, require_shape, tracked
+from ._call import HALF, MOST_COLUMNS, MOST_ROWS, in_order, on, once, require_apart, require_count, require_same_device, \
+    require_shape, tracked
 
 MAX_RANK = 128
 
@@ -35,7 +36,8 @@ def _fits(y, x, a, b, ids, scaling, out):
                 == a.get_device() == b.get_device() == ids.get_device() == scaling.get_device() and x.is_contiguous()
                 and y.is_contiguous() and a.is_contiguous() and b.is_contiguous() and ids.is_contiguous()
                 and scaling.is_contiguous() and 8 <= rank <= MAX_RANK and not rank % 8 and k >= 8 and not k % 8 and n >= 8
-                and not n % 8 and 1 <= adapters <= 32767 and out is None)
+                and not n % 8 and 1 <= adapters <= 32767 and rows <= MOST_ROWS and k <= MOST_COLUMNS and n <= MOST_COLUMNS
+                and out is None)
     except (AttributeError, ValueError, IndexError):
         return False
 
@@ -59,6 +61,8 @@ def _check(y, x, a, b, adapter_ids, scaling, out):
         raise ValueError(f"k ({k}) and n ({n}) must be positive multiples of 8")
     if not 1 <= adapters <= 32767:
         raise ValueError(f"adapters must be in [1, 32767], got {adapters}")
+    require_count("rows", rows)
+    require_count("k and n", max(k, n), MOST_COLUMNS)
     _lib.require_cuda("x", x, HALF)
     for name, t in (("y", y), ("a", a), ("b", b), ("out", out)):
         if t is not None:

@@ -20,7 +20,7 @@ from typing import NamedTuple
 import torch
 
 from .. import _lib
-from ._call import in_order, on, once, require_same_device, require_shape, tracked
+from ._call import MOST_COLUMNS, MOST_ROWS, in_order, on, once, require_count, require_same_device, require_shape, tracked
 from .moe_sorting_kernel import moe_sorting_flydsl
 
 _FLOATS = (torch.bfloat16, torch.float16, torch.float32)
@@ -45,7 +45,7 @@ def _combine_sizes(rows, weights, plan):
         tokens, topk = pairs
         if (rows.is_cuda and rows.dtype in _FLOATS and dim >= 8 and not dim % 8 and row_index.shape == pairs
                 and weights.dtype is torch.float32 and min(sorted_ids.numel(), tokens * topk) <= count <= sorted_ids.numel()
-                and nv.numel() >= 1
+                and count <= MOST_ROWS and dim <= MOST_COLUMNS and nv.numel() >= 1
                 and sorted_ids.dtype is i32 and nv.dtype is i32 and row_index.dtype is i32
                 and dev == weights.get_device() == sorted_ids.get_device() == nv.get_device() == row_index.get_device()
                 and rows.is_contiguous() and weights.is_contiguous() and sorted_ids.is_contiguous() and nv.is_contiguous()
@@ -75,6 +75,8 @@ def _require_rows(name: str, t: torch.Tensor) -> None:
     require_shape(name, t, (None, None))
     if t.shape[1] < 8 or t.shape[1] % 8:
         raise ValueError(f"{name} must have a positive multiple of 8 columns, got {t.shape[1]}")
+    require_count(f"rows of {name}", t.shape[0])
+    require_count(f"columns of {name}", t.shape[1], MOST_COLUMNS)
 
 
 # ------------------------------------------------------------------------- gate
@@ -128,6 +130,7 @@ def topk_gating(logits: torch.Tensor, topk: int, *, renormalize: bool = True) ->
         raise ValueError(f"logits must have 1 to 1024 experts, got {experts}")
     if not 1 <= int(topk) <= min(32, experts):
         raise ValueError(f"topk must be in [1, min(32, experts)], got {topk}")
+    require_count("tokens", logits.shape[0])
     run = _TopkGating.apply if tracked(logits) else _gate
     return run(logits, int(topk), 1 if renormalize else 0)
 
@@ -142,6 +145,8 @@ def route_rows(topk_ids: torch.Tensor, num_experts: int) -> RoutedRows:
         raise ValueError(f"num_experts must be in [1, 1024], got {num_experts}")
     if not 1 <= topk <= min(255, num_experts):
         raise ValueError(f"topk must be in [1, min(255, num_experts)], got {topk}")
+    require_count("tokens", tokens, 2 ** 24 - 1)
+    require_count("tokens * topk + num_experts", tokens * topk + num_experts)
     dev, i32 = topk_ids.device, torch.int32
     with on(dev):
         capacity = tokens * topk + num_experts - topk
