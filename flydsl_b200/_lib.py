@@ -89,6 +89,7 @@ _SIGNATURES = {
     "flymoe_combine_rows": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
     "flymoe_combine_rows_backward": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
     "flymoe_lora_v_elems": (c_int64, [c_int, c_int, c_int]),
+    "flymoe_lora_forward": (c_int, [_P] * 9 + [c_int64] + [c_int] * 6 + [_P]),
     "flymoe_lora_add": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int, _P]),
     "flymoe_lora_backward_workspace_elems": (c_int64, [c_int, c_int, c_int, c_int, c_int]),
     "flymoe_lora_backward": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64,

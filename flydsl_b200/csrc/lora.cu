@@ -811,8 +811,8 @@ static long long v_elems(int rows, int splits, int rank) {
 }
 
 // One product with the adapters and back: out = base + scaling * (x A^T) B^T, or with a_t / b_t (then `a` and `b` are only
-// read where needs_transposed) for A and B given the other way round.  v: v_elems() floats; `keep`: its first rows * rank
-// hold x A^T afterwards.
+// read where needs_transposed) for A and B given the other way round.  v: v_elems() floats; `kept`: null, or rows * rank
+// floats (the first of v, or of their own) that hold x A^T afterwards.
 struct Chain {
   const void *x, *a, *a_t, *base, *b, *b_t;
   void* out;                   // null: only x A^T
@@ -820,13 +820,14 @@ struct Chain {
   const int* ids;
   const float* scaling;
   int rows, k, n, rank, adapters, dtype;
-  bool keep;
+  float* kept;
 };
 static int run_chain(const Chain& c, cudaStream_t s) {
   const bool bf = c.dtype == FLYMOE_BF16, tiles = on_tiles(c.rows), others = !tiles || c.adapters > tile_limit(c.rank);
   const int skip = tiles ? tile_limit(c.rank) : 0;
   const int splits = shrink_splits(c.rows, c.k);
-  float* planes = splits > 1 ? c.v + (long long)c.rows * c.rank : c.v;
+  float* sum = c.kept ? c.kept : c.v;
+  float* planes = splits > 1 ? c.v + (long long)c.rows * c.rank : sum;
   int* counts = reinterpret_cast<int*>(c.v + v_planes(c.rows, splits, c.rank));
   ShrinkArgs sh = {c.x, c.a, c.ids, planes, counts, c.rows, c.k, c.rank, c.adapters, splits, 0};
   int rc = FLYMOE_OK;
@@ -837,14 +838,14 @@ static int run_chain(const Chain& c, cudaStream_t s) {
   }
   if (rc != FLYMOE_OK) return rc;
   // tiles read a row's v once for every block that works on it, and the gradient wants it whole: one sum, not several
-  const bool fold = splits > 1 && (tiles || c.keep);
+  const bool fold = splits > 1 && (tiles || c.kept);
   if (fold) {
     const long long vecs = (long long)c.rows * c.rank / 4;
     FLYMOE_CUDA_CHECK(launch_closely(lora_fold_kernel, unsigned(std::min<long long>((vecs + 255) / 256, 4LL * sm_count())), 256, 0, s,
-                                     reinterpret_cast<const float4*>(planes), reinterpret_cast<float4*>(c.v), vecs, splits));
+                                     reinterpret_cast<const float4*>(planes), reinterpret_cast<float4*>(sum), vecs, splits));
   }
   if (!c.out) return FLYMOE_OK;
-  ExpandArgs ex = {c.base, fold ? c.v : planes, c.b, c.ids, c.scaling, c.out, counts, c.rows, c.n, c.rank, c.adapters,
+  ExpandArgs ex = {c.base, fold ? sum : planes, c.b, c.ids, c.scaling, c.out, counts, c.rows, c.n, c.rank, c.adapters,
                    fold ? 1 : splits, 0};
   if (others) rc = bf ? launch_expand_rank<__nv_bfloat16>(ex, skip, s) : launch_expand_rank<__half>(ex, skip, s);
   if (rc == FLYMOE_OK && tiles) {
@@ -906,17 +907,25 @@ extern "C" int64_t flymoe_lora_v_elems(int rows, int k, int rank) {
 extern "C" int flymoe_lora_add(void* out, const void* base, const void* x, const void* a, const void* b, const int32_t* ids,
                                const float* scaling, float* v, int64_t v_floats, int rows, int k, int n, int rank, int adapters,
                                int keep_v, int dtype, void* stream) {
+  return flymoe_lora_forward(out, base, x, a, b, ids, scaling, keep_v ? v : nullptr, v, v_floats, rows, k, n, rank, adapters, dtype,
+                             stream);
+}
+
+extern "C" int flymoe_lora_forward(void* out, const void* base, const void* x, const void* a, const void* b, const int32_t* ids,
+                                   const float* scaling, float* kept, float* v, int64_t v_floats, int rows, int k, int n,
+                                   int rank, int adapters, int dtype, void* stream) {
   using namespace flymoe;
   int rc = lora_check("lora_add", rows, k, n, rank, adapters, dtype);
   if (rc != FLYMOE_OK || rows == 0) return rc;
   FLYMOE_REQUIRE(out && base && x && a && b && ids && scaling && v, "lora_add: null pointer");
-  FLYMOE_REQUIRE(aligned16(out) && aligned16(base) && aligned16(x) && aligned16(a) && aligned16(b) && aligned16(v),
+  FLYMOE_REQUIRE(aligned16(out) && aligned16(base) && aligned16(x) && aligned16(a) && aligned16(b) && aligned16(v) &&
+                     aligned16(kept),
                  "lora_add: pointers must be 16-byte aligned");
   if (v_floats < v_elems(rows, shrink_splits(rows, k), rank)) {
     set_last_error_msg("lora_add: v is smaller than flymoe_lora_v_elems()");
     return FLYMOE_ERR_WORKSPACE;
   }
-  return run_chain({x, a, nullptr, base, b, nullptr, out, v, ids, scaling, rows, k, n, rank, adapters, dtype, keep_v != 0},
+  return run_chain({x, a, nullptr, base, b, nullptr, out, v, ids, scaling, rows, k, n, rank, adapters, dtype, kept},
                    static_cast<cudaStream_t>(stream));
 }
 
@@ -939,7 +948,7 @@ extern "C" int flymoe_lora_backward(void* dx, void* da, void* db, const void* do
     if (db) FLYMOE_CUDA_CHECK(cudaMemsetAsync(db, 0, b_bytes, s));
     return FLYMOE_OK;
   }
-  FLYMOE_REQUIRE(dout && x && a && b && ids && scaling && v && workspace, "lora_backward: null pointer");
+  FLYMOE_REQUIRE(dout && x && a && b && ids && scaling && (v || !db) && workspace, "lora_backward: null pointer");
   FLYMOE_REQUIRE(aligned16(dx) && aligned16(da) && aligned16(db) && aligned16(dout) && aligned16(x) && aligned16(a) &&
                      aligned16(b) && aligned16(v) && aligned16(workspace), "lora_backward: pointers must be 16-byte aligned");
   const BackwardScratch w = backward_scratch(rows, k, n, rank, adapters);
@@ -964,7 +973,7 @@ extern "C" int flymoe_lora_backward(void* dx, void* da, void* db, const void* do
       a_t = at;
       b_t = bt;
     }
-    rc = run_chain({dout, b_t, b, nullptr, a_t, a, dx, dv, ids, scaling, rows, n, k, rank, adapters, dtype, da != nullptr}, s);
+    rc = run_chain({dout, b_t, b, nullptr, a_t, a, dx, dv, ids, scaling, rows, n, k, rank, adapters, dtype, da ? dv : nullptr}, s);
     if (rc != FLYMOE_OK) return rc;
   }
   if (!da && !db) return FLYMOE_OK;

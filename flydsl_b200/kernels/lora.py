@@ -78,14 +78,17 @@ def _check(y, x, a, b, adapter_ids, scaling, out):
 
 
 def _add(out, y, x, a, b, ids, scaling, keep_v):
-    """Enqueues the forward pass; returns its scratch, which begins with v if ``keep_v``."""
+    """Enqueues the forward pass; returns v (in the first numbers of a tensor) if ``keep_v``."""
     lib, (rows, k), (adapters, rank, _) = _lib.load(), x.shape, a.shape
     elems = lib.flymoe_lora_v_elems(rows, k, rank)
     v = x.new_empty(elems, dtype=torch.float32)
-    _lib.check(lib.flymoe_lora_add(out.data_ptr(), y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(),
-                                   scaling.data_ptr(), v.data_ptr(), elems, rows, k, y.shape[1], rank, adapters, keep_v,
-                                   _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(None)), "lora_add")
-    return v
+    kept = None
+    if keep_v:                                   # sums in several pieces are scratch, which is not kept alive for one
+        kept = v if elems < 2 * rows * rank else x.new_empty(rows * rank, dtype=torch.float32)
+    _lib.check(lib.flymoe_lora_forward(out.data_ptr(), y.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(), ids.data_ptr(),
+                                       scaling.data_ptr(), _lib.ptr(kept), v.data_ptr(), elems, rows, k, y.shape[1], rank,
+                                       adapters, _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(None)), "lora_add")
+    return kept
 
 
 class _LoraAdd(torch.autograd.Function):
@@ -93,7 +96,7 @@ class _LoraAdd(torch.autograd.Function):
     def forward(ctx, y, x, a, b, ids, scaling):
         with on(x.device):
             out = torch.empty_like(y)
-            v = _add(out, y, x, a, b, ids, scaling, 1)
+            v = _add(out, y, x, a, b, ids, scaling, ctx.needs_input_grad[3])       # only the gradient of b wants it
         ctx.save_for_backward(x, a, b, ids, scaling, v)
         return out
 
@@ -117,7 +120,7 @@ class _LoraAdd(torch.autograd.Function):
                     db = torch.empty_like(b)
                 _lib.check(lib.flymoe_lora_backward(
                     _lib.ptr(dx), _lib.ptr(da), _lib.ptr(db), dout.data_ptr(), x.data_ptr(), a.data_ptr(), b.data_ptr(),
-                    ids.data_ptr(), scaling.data_ptr(), v.data_ptr(), work.data_ptr(), elems, rows, k, n, rank, adapters,
+                    ids.data_ptr(), scaling.data_ptr(), _lib.ptr(v), work.data_ptr(), elems, rows, k, n, rank, adapters,
                     _lib.DTYPE_CODE[x.dtype], _lib.stream_handle(None)), "lora_backward")
         return dout if need_y else None, dx, da, db, None, None
 
@@ -138,5 +141,5 @@ def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
     with on(x.device, stream):
         if out is None:
             out = torch.empty_like(y)
-        _add(out, y, x, a, b, adapter_ids, scaling, 0)
+        _add(out, y, x, a, b, adapter_ids, scaling, False)
     return out

@@ -371,15 +371,19 @@ int flymoe_combine_rows_backward(const void* dout, const void* rows_in, const fl
  * order, scaling f32 [adapters].  rank a multiple of 8 up to 128, k and n multiples of 8, at most 32767 adapters, pointers
  * 16-byte aligned.  Sums in fp32, the output rounded once; no atomics decide a result.
  * v: f32 scratch of flymoe_lora_v_elems(); with keep_v its first rows * rank floats hold A_l x[m] afterwards, as the gradient
- * wants it (rows without an adapter: unspecified).
+ * wants it (rows without an adapter: unspecified).  flymoe_lora_forward is the same with that in memory of its own: kept, NULL
+ * or rows * rank floats, so that the scratch need not live until the backward pass.
  * flymoe_lora_backward: from dout [rows, n], dx [rows, k] = scaling (dout B_l) A_l (zeros without an adapter), da[l] =
  * scaling[l] sum over l's rows of (dout B_l)^T x, db[l] = scaling[l] sum of dout^T v (zeros for an adapter without rows);
- * each of the three may be NULL.  workspace: f32 of flymoe_lora_backward_workspace_elems().  No counterpart in the
+ * each of the three may be NULL, and v where db is.  workspace: f32 of flymoe_lora_backward_workspace_elems().  No counterpart in the
  * reference. */
 int64_t flymoe_lora_v_elems(int rows, int k, int rank);
 int flymoe_lora_add(void* out, const void* base, const void* x, const void* a, const void* b, const int32_t* ids,
                     const float* scaling, float* v, int64_t v_elems, int rows, int k, int n, int rank, int adapters,
                     int keep_v, int dtype, void* stream);
+int flymoe_lora_forward(void* out, const void* base, const void* x, const void* a, const void* b, const int32_t* ids,
+                        const float* scaling, float* kept, float* v, int64_t v_elems, int rows, int k, int n, int rank,
+                        int adapters, int dtype, void* stream);
 int64_t flymoe_lora_backward_workspace_elems(int rows, int k, int n, int rank, int adapters);
 int flymoe_lora_backward(void* dx, void* da, void* db, const void* dout, const void* x, const void* a, const void* b,
                          const int32_t* ids, const float* scaling, const float* v, float* workspace, int64_t workspace_elems,

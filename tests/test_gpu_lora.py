@@ -324,3 +324,24 @@ def test_infinities_stay_infinities(rows, rank, adapters, mix, dtype):
             odd = ~ref.isfinite()
             assert torch.equal(out[ref.isinf()].double(), ref[ref.isinf()]), what
             check(out[~odd], (ref[~odd], mag[~odd]), terms, what)
+
+
+@pytest.mark.parametrize("rows", [40, 600, 20000])
+def test_what_a_graph_keeps(rows):
+    """The middle factor once, where the gradient of b wants it, and nothing else that the call made."""
+    p, dout = make(rows, 2048, 136, 24, 5, BF, "requests", seed=15)
+    want = lora_add(**p)
+    given = {t.untyped_storage().data_ptr() for t in p.values()}
+    for names, floats in (("yxab", rows * 24), ("b", rows * 24), ("y", 0), ("xa", 0)):
+        q = {s: (t.detach().requires_grad_() if s in names else t) for s, t in p.items()}
+        out = lora_add(**q)
+        kept = [t for t in out.grad_fn.saved_tensors if t is not None and t.untyped_storage().data_ptr() not in given]
+        assert sum(t.untyped_storage().nbytes() for t in kept) <= floats * 4 + (rows + 127) // 128 * 4
+        grads = torch.autograd.grad(out, [q[s] for s in names], dout)
+        if names == "yxab":
+            full = dict(zip(names, grads))
+            (ref, mag), (dx, mx), (da, ma), (db, mb) = exact(p, dout)
+            check(full["b"], (db, mb), 2048 + rows, "db")
+        assert all(torch.equal(g, full[s]) for s, g in zip(names, grads))
+        check(out.detach(), (ref, mag), 2048 + 24, "out")
+        check(want, (ref, mag), 2048 + 24, "out")
