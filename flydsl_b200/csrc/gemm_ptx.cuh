@@ -436,6 +436,13 @@ __device__ __forceinline__ int build_tile_table(const GemmArgs& a, int valid_row
 // Tensor map over bytes with the 128-byte swizzle (dims and box of the innermost axis in bytes, out of bounds reads zero).
 int make_map(CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
              const cuuint32_t* box);
+// Row-major 16-bit matrix [rows, cols] (mats > 0: that many of them, rank 3), boxes of 64 columns x box_rows rows.
+inline int matrix_map(CUtensorMap* map, const void* base, long long cols, long long rows, int mats, int box_rows) {
+  const cuuint64_t dims[3] = {cuuint64_t(cols) * 2, cuuint64_t(rows), cuuint64_t(mats)};
+  const cuuint64_t strides[2] = {cuuint64_t(cols) * 2, cuuint64_t(cols) * 2 * cuuint64_t(rows)};
+  const cuuint32_t box[3] = {128, cuuint32_t(box_rows), 1};
+  return make_map(map, base, mats > 0 ? 3 : 2, dims, strides, box);
+}
 // Tensor maps of both operands: boxes of `a_box_rows` rows of A and of `b_box_rows` weight rows, 128 bytes of K wide.
 int make_gemm_maps(int stage, const GemmArgs& a, int a_box_rows, int b_box_rows, CUtensorMap* map_a, CUtensorMap* map_b);
 // Cluster sizes 1, 2, 4, 8: how many CTAs share a tile's K range, given how many clusters of each size run at once

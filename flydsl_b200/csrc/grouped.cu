@@ -223,19 +223,12 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
 }
 
 // ------------------------------------------------------------------------------ host
-int ragged_map(CUtensorMap* map, const void* base, long long cols, long long rows, int mats, int box_rows) {
-  cuuint64_t dims[3] = {cuuint64_t(cols) * 2, cuuint64_t(rows), cuuint64_t(mats)};
-  cuuint64_t strides[2] = {cuuint64_t(cols) * 2, cuuint64_t(cols) * 2 * cuuint64_t(rows)};
-  cuuint32_t box[3] = {128, cuuint32_t(box_rows), 1};
-  return make_map(map, base, mats > 0 ? 3 : 2, dims, strides, box);
-}
-
 template <int FORM, int TM, int BN>
 static int launch_ragged(const void* x, const void* w, RaggedArgs a, int n, int k, cudaStream_t stream) {
   a.n_tiles = ceil_div(a.n_dim, BN);
   CUtensorMap ma, mb;
-  int rc = ragged_map(&ma, x, a.k_dim, a.rows, 0, TM);
-  if (rc == FLYMOE_OK) rc = ragged_map(&mb, w, k, n, a.experts, FORM == 1 ? kRagK * rag_sub<TM>() : BN);
+  int rc = matrix_map(&ma, x, a.k_dim, a.rows, 0, TM);
+  if (rc == FLYMOE_OK) rc = matrix_map(&mb, w, k, n, a.experts, FORM == 1 ? kRagK * rag_sub<TM>() : BN);
   if (rc != FLYMOE_OK) return rc;
   auto* kernel = grouped_gemm_kernel<FORM, TM, BN>;
   constexpr size_t smem = rag_ring<TM, BN>() + sizeof(RaggedCtrl) + 1024;

@@ -88,16 +88,6 @@ __device__ __forceinline__ uint4 pack8(const float* v, int bf16) {
   }
   return pk;
 }
-// Zeros in the rows [from, from + n) of an operand block of `chunks` 64-column chunks: behind the end of an expert there may
-// be anything.  The swizzle stays inside a row.  One warp.
-__device__ __forceinline__ void zero_block_rows(uint8_t* block, int chunks, int from, int n, int lane) {
-  for (int i = lane; i < n * chunks * 8; i += 32) {
-    const int chunk = i / (n * 8), rem = i - chunk * n * 8;
-    *reinterpret_cast<uint4*>(block + chunk * kRagK * 128 + (from + rem / 8) * 128 + (rem & 7) * 16) = make_uint4(0, 0, 0, 0);
-  }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-  __syncwarp();
-}
 // Rows that belong to no expert, in front of the first segment and behind the last, zeroed by `threads` threads of each CTA.
 __device__ __forceinline__ void zero_uncovered_rows(const RaggedArgs& a, const RaggedTables* c, int thread, int threads) {
   const int lo = c->start[0], hi = c->start[a.experts];
@@ -106,9 +96,6 @@ __device__ __forceinline__ void zero_uncovered_rows(const RaggedArgs& a, const R
   for (long long i = (long long)blockIdx.x * threads + thread; i < all; i += (long long)gridDim.x * threads)
     out[i < head ? i : (long long)hi * vec + i - head] = make_uint4(0, 0, 0, 0);
 }
-
-// Row-major 16-bit matrix [rows, cols] (or `mats` of them), boxes of 64 columns x box_rows rows.
-int ragged_map(CUtensorMap* map, const void* base, long long cols, long long rows, int mats, int box_rows);
 
 // CTA pairs (grouped_pair.cu).  form 0, 1: forward, input gradient; 2: weight gradient.
 int launch_ragged_pair(int form, const void* p, const void* q, const RaggedArgs& a, int n, int k, cudaStream_t stream);

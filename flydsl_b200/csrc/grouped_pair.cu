@@ -308,21 +308,21 @@ int launch_ragged_pair(int form, const void* p, const void* q, const RaggedArgs&
   TailMaps tails = {};
   int rc;
   if (form == 2) {
-    rc = ragged_map(&ma, p, n, a.rows, 0, kRagK);
-    if (rc == FLYMOE_OK) rc = ragged_map(&mb, q, k, a.rows, 0, kRagK);
-    if (rc == FLYMOE_OK) rc = ragged_map(&mo, a.out, a.n_dim, a.m_dim, a.experts, 128);
+    rc = matrix_map(&ma, p, n, a.rows, 0, kRagK);
+    if (rc == FLYMOE_OK) rc = matrix_map(&mb, q, k, a.rows, 0, kRagK);
+    if (rc == FLYMOE_OK) rc = matrix_map(&mo, a.out, a.n_dim, a.m_dim, a.experts, 128);
     for (int i = 0; i < kTailBoxes && rc == FLYMOE_OK; ++i) {
-      rc = ragged_map(&tails.a[i], p, n, a.rows, 0, 16 >> i);
-      if (rc == FLYMOE_OK) rc = ragged_map(&tails.b[i], q, k, a.rows, 0, 16 >> i);
+      rc = matrix_map(&tails.a[i], p, n, a.rows, 0, 16 >> i);
+      if (rc == FLYMOE_OK) rc = matrix_map(&tails.b[i], q, k, a.rows, 0, 16 >> i);
     }
     const long long tiles = (long long)a.experts * a.m_tiles * a.n_tiles;
     if (rc != FLYMOE_OK) return rc;
     return a.rows / a.experts <= 512 ? launch_pair_form<2, 2>(ma, mb, mo, tails, a, tiles, stream)
                                      : launch_pair_form<2, 1>(ma, mb, mo, tails, a, tiles, stream);
   }
-  rc = ragged_map(&ma, p, a.k_dim, a.rows, 0, 128);
-  if (rc == FLYMOE_OK) rc = ragged_map(&mb, q, k, n, a.experts, form == 1 ? kRagK : 128);
-  if (rc == FLYMOE_OK) rc = ragged_map(&mo, a.out, a.n_dim, a.rows, 0, 128);
+  rc = matrix_map(&ma, p, a.k_dim, a.rows, 0, 128);
+  if (rc == FLYMOE_OK) rc = matrix_map(&mb, q, k, n, a.experts, form == 1 ? kRagK : 128);
+  if (rc == FLYMOE_OK) rc = matrix_map(&mo, a.out, a.n_dim, a.rows, 0, 128);
   if (rc != FLYMOE_OK) return rc;
   const long long tiles = ((long long)a.rows / kRpTile + a.experts) * a.n_tiles;
   return form == 1 ? launch_pair_form<1, 1>(ma, mb, mo, tails, a, tiles, stream)

@@ -604,13 +604,6 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
 }
 
 // ---------------------------------------------------------------------------- host
-static int matrix_map(CUtensorMap* map, const void* base, long long cols, long long rows, int mats, int box_rows) {
-  cuuint64_t dims[3] = {cuuint64_t(cols) * 2, cuuint64_t(rows), cuuint64_t(mats)};
-  cuuint64_t strides[2] = {cuuint64_t(cols) * 2, cuuint64_t(cols) * 2 * cuuint64_t(rows)};
-  cuuint32_t box[3] = {128, cuuint32_t(box_rows), 1};
-  return make_map(map, base, mats > 0 ? 3 : 2, dims, strides, box);
-}
-
 int launch_shrink_sm100(const ShrinkArgs& p, int bf16, cudaStream_t stream) {
   ShrinkTcArgs q = {p, bf16, (p.rank + 15) / 16 * 16, 0, 0, device_status_ptr()};
   if (q.status == nullptr) return FLYMOE_ERR_CUDA;
