@@ -345,3 +345,48 @@ def test_what_a_graph_keeps(rows):
         assert all(torch.equal(g, full[s]) for s, g in zip(names, grads))
         check(out.detach(), (ref, mag), 2048 + 24, "out")
         check(want, (ref, mag), 2048 + 24, "out")
+
+
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), "lowest"])
+@pytest.mark.parametrize("rows,rank,adapters,mix,dtype", [(100, 16, 4, "tokens", HF), (700, 24, 4, "tokens", BF), (700, 24, 4, "tokens", HF),
+                                                          (1500, 128, 4, "requests", BF), (1500, 128, 4, "requests", HF),
+                                                          (900, 64, 40, "tokens", BF), (900, 64, 40, "tokens", HF)])
+def test_one_request_does_not_reach_another_on_tiles(rows, rank, adapters, mix, dtype, poison):
+    if poison == "lowest":
+        poison = torch.finfo(dtype).min
+    p, dout = make(rows, 136, 200, rank, adapters, dtype, mix, seed=16)
+    mine = p["adapter_ids"] == 2
+    def run():
+        q = {s: (t.clone().requires_grad_() if s in "xab" else t) for s, t in p.items()}
+        out = lora_add(**q)
+        return (out.detach(), *torch.autograd.grad(out, (q["x"], q["a"], q["b"]), dout))
+    clean = run()
+    for t in (p["y"], p["x"], dout):
+        t[~mine] = poison
+    for t in (p["a"], p["b"], p["scaling"]):
+        t[:2], t[3:] = poison, poison
+    dirty = run()
+    assert torch.equal(dirty[0][mine], clean[0][mine]) and torch.equal(dirty[1][mine], clean[1][mine])
+    assert torch.equal(dirty[2][2], clean[2][2]) and torch.equal(dirty[3][2], clean[3][2])
+
+
+@pytest.mark.parametrize("rows,n,rank", [(700, 200, 24), (1500, 72, 128), (30000, 136, 16), (30000, 136, 88)])
+def test_fp16_rows_of_every_size_beside_each_other(rows, n, rank):
+    """Each row of a tile, and each tile that a block goes through, has a power of two of its own."""
+    k = 72
+    p, dout = make(rows, k, n, rank, 4, HF, "requests", seed=17)
+    p["x"] *= (2.0 ** (torch.arange(rows, device="cuda") * 7 % 21 - 11))[:, None].half()
+    dout = dout * (2.0 ** (torch.arange(rows, device="cuda") * 5 % 19 - 10))[:, None].half()
+    p["b"] /= 64
+    p["y"].zero_()
+    (out, mo), (dx, mx), (da, ma), (db, mb) = exact(p, dout)
+    q = {s: (t.clone().requires_grad_() if s in "xab" else t) for s, t in p.items()}
+    res = lora_add(**q)
+    gx, ga, gb = torch.autograd.grad(res, (q["x"], q["a"], q["b"]), dout)
+    fits = [bool((t.abs() < 6e4).all()) for t in (out, dx, da, db)]
+    assert fits[0] and fits[1]                   # sums over thousands of rows may pass what fp16 holds
+    check(res.detach(), (out, mo), k + rank, "out")
+    check(gx, (dx, mx), n + rank, "dx")
+    for got, ref, mag, terms, what in ((ga, da, ma, n + rows, "da"), (gb, db, mb, k + rows, "db")):
+        held = ref.abs() < 6e4
+        check(got[held], (ref[held], mag[held]), terms, what)
