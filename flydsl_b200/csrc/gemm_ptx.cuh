@@ -86,8 +86,8 @@ __device__ __forceinline__ bool elect_one() {
 }
 // All lanes of a warp wait together.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code,
-                                          unsigned backoff_ns = 0) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code, backoff_ns));
+                                          unsigned backoff_ns = 0, unsigned long long limit_ns = kWaitLimitNs) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code, backoff_ns, limit_ns));
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
   asm volatile(

@@ -223,7 +223,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
       const long long row0 = FORM == 2 ? (long long)e * a.m_dim + m0 : (long long)tab->start[e] + m0;
       const bool none = FORM == 2 && seg == 0;
       if (!none) {
-        ok = ok && warp_wait(smem_u32(&ctrl->acc_full[acc]), acc_phase, abort_flag, a.status, 4);
+        // a sum takes as long as its K blocks do, 0.29 us each (2^27 rows of 8 + 8 columns): the limit of a wait grows with them
+        const unsigned long long limit = kWaitLimitNs + (FORM == 2 ? seg / kRagK * 4000ull : 0ull);
+        ok = ok && warp_wait(smem_u32(&ctrl->acc_full[acc]), acc_phase, abort_flag, a.status, 4, 0, limit);
         tcgen05_fence_after();
       }
 #pragma unroll

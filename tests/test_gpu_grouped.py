@@ -198,3 +198,11 @@ def test_results_apart_from_inputs_and_streams_of_their_device():
         grouped_gemm_wgrad(w.view(-1, 64)[:12], x, off, out=w)
     with pytest.raises(ValueError, match="stream is on"):
         on(torch.device("cuda", torch.cuda.current_device() + 1), torch.cuda.Stream())
+
+
+def test_weight_gradient_over_millions_of_rows():
+    rows = 2 ** 24 + 37
+    x, dy = torch.zeros((rows, 8), dtype=BF, device="cuda"), torch.ones((rows, 8), dtype=BF, device="cuda")
+    x[0], x[rows // 2], x[rows - 1] = 1, 4, 2
+    offsets = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    assert bool((grouped_gemm_wgrad(dy, x, offsets) == 7).all())
