@@ -390,3 +390,31 @@ def test_fp16_rows_of_every_size_beside_each_other(rows, n, rank):
     for got, ref, mag, terms, what in ((ga, da, ma, n + rows, "da"), (gb, db, mb, k + rows, "db")):
         held = ref.abs() < 6e4
         check(got[held], (ref[held], mag[held]), terms, what)
+
+
+@pytest.mark.parametrize("rows,adapters", [(64, 30), (2048, 4), (700, 30)])
+def test_calls_that_read_what_the_call_before_wrote(rows, adapters):
+    """Thirty in a row, each of whose launches start while the one before still runs."""
+    p, _ = make(rows, 264, 264, 16, adapters, BF, "tokens", seed=18)
+    rest = (p["a"], p["b"], p["adapter_ids"], p["scaling"] / 16)
+
+    def chain(wait):
+        h = p["x"]
+        for _ in range(30):
+            h = lora_add(h, h, *rest)
+            if wait:
+                torch.cuda.synchronize()
+        return h
+
+    want = chain(True)
+    assert bool(want.isfinite().all())
+    for _ in range(10):
+        assert torch.equal(chain(False), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain(False)
+    for _ in range(10):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
