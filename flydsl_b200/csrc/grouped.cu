@@ -14,8 +14,8 @@
 // may read rows of the next expert; they only reach accumulator rows that are not stored.  A 32-row tile loads 32 rows per K block; the MMAs
 // have 128 and read on into whatever follows in shared memory, which reaches no stored row either.  What small launches need
 // is bytes in flight (a K block takes about 2 us from its request to its release when the weights come from HBM), so their
-// tiles are narrow and the ring is deep: one expert of 4096 x 4096 with one row takes 13 us, on 128-row tiles 33.  64 rows on 32
-// experts of 4096 x 7168: 1.63 GB of weights in 249 to 276 us, 5.9 to 6.5 TB/s.
+// tiles are narrow and the ring is deep: one expert of 4096 x 4096 with one row takes 14 us, on 128-row tiles 23 to 28.  64 rows on 32
+// experts of 4096 x 7168: 1.63 GB of weights in 249 to 306 us by box, 5.3 to 6.5 TB/s.
 #include <cuda.h>
 #include <stdio.h>
 
@@ -255,10 +255,10 @@ static double expected_tiles(double mean, int tm) {
 }
 // Tile of forms 0 and 1, by estimated cycles.  A K block costs what is longest of its MMAs (with the issuing thread's work)
 // and its bytes at 70 to 77 a cycle; that and the time on HBM hide each other only in part (root of the sum of squares).
-// Over 154 sizes (1 to 64 experts, 1 to 700 rows each, even and skewed) both forms took 1.014 of the time of the best kind
-// on geometric mean, 1.35 at worst (16 experts of 1048 x 2104, whose rows are not aligned to 128 bytes).  A fixed kind costs
-// more: pairs for one row on one expert of 4096 x 4096 23 us against 13, 128 x 256 tiles for 8 experts of 2048 x 2048 with 40
-// rows 16 against 11, 32-row tiles for 32 experts of 4096 x 7168 with 160 rows 1343 against 382.
+// Over 154 sizes (1 to 64 experts, 1 to 700 rows each, even and skewed) the two forms took 1.014 and 1.011 of the time of the
+// best kind on geometric mean, 1.38 at worst (16 experts of 1048 x 2104, whose rows are not aligned to 128 bytes).  A fixed kind
+// takes 1.12 to 2.12 on geometric mean: pairs for one row on one expert of 4096 x 4096 25 us against 14, 128 x 256 tiles for 8
+// experts of 2048 x 2048 with 40 rows 20 against 16, 32 x 128 tiles for 32 experts of 4096 x 7168 with 160 rows 953 against 438.
 static RaggedTileKind choose_tile(bool input_grad, int rows, int experts, int n_dim, int k_dim) {
   const int narrow = input_grad ? 64 : 32;       // columns across the contraction come 64 at a time
   struct Kind { int tm, tn, per_sm_x2, block, launch; double hbm; };

@@ -23,7 +23,7 @@
 // Gradients use the same kernels: dv = dout B_l is a shrink with B transposed, dx = s_l dv A_l an expand with A transposed
 // (the tiles read them across, this file's kernels want copies).  dA_l = s_l sum dv^T x and dB_l = s_l sum dout^T v contract
 // over an adapter's rows, found by scanning ids: bf16 on tcgen05 (lora_grad_sm100.cu), fp16 here, since a common power of two
-// that may still grow needs the sums in registers (8192 rows, 4096 + 4096 columns, 4 adapters of rank 32: 43 us and 49).  No sum depends on the
+// that may still grow needs the sums in registers (8192 rows, 4096 + 4096 columns, 4 adapters of rank 32: 45 us and 60).  No sum depends on the
 // order of execution.
 #include <algorithm>
 #include <stdio.h>
@@ -708,10 +708,11 @@ lora_transpose_kernel(const TransposeArgs p) {
 }
 
 // ---------------------------------------------------------------------------- host
-// Tiles of 128 rows from 512 rows on.  Both ways (tiles of up to four adapters), whole calls, 4096 -> 4096, bf16, us on one B200 (tiles / groups of 16 rows):
-// 4 adapters in runs: 256 rows, rank 16 13.8 / 13.4, rank 128 20.8 / 43.5; 512 rows 13.6 / 16.8 and 24.5 / 50.6; 1024 rows
-// 15.9 / 26.2 and 27.0 / 95.3.  16 adapters in any order (tiles then only add launches that find nothing to do): 256 rows,
-// rank 16 21.2 / 12.7; 512 rows 29.1 / 20.5, rank 128 88.6 / 74.6; 8192 rows 134 / 82 and 484 / 388.
+// Tiles of 128 rows from 512 rows on.  Both ways, whole calls, 4096 -> 4096, bf16, us on one B200 (tiles / groups of 16 rows):
+// 4 adapters in runs: 256 rows, rank 16 14.4 / 13.3, rank 128 21.4 / 37.3; 512 rows 14.4 / 16.9 and 20.2 / 43.5; 8192 rows
+// 48.1 / 86.3 and 66.1 / 284.  8 adapters in runs, 512 rows: 15.8 / 24.0 and 30.3 / 49.2.  16 adapters in any order (tiles then
+// only add launches that find nothing to do): 256 rows 21.7 / 13.1 and 48.8 / 41.3; 512 rows 28.4 / 20.7 and 69.9 / 64.3;
+// 8192 rows 132 / 87.6 and 411 / 323.
 static bool on_tiles(int rows) { return rows >= 512; }
 
 static int lora_check(const char* what, int rows, int k, int n, int rank, int adapters, int dtype) {

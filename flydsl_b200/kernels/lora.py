@@ -9,10 +9,10 @@ share (``compile_blockscale_preshuffle_gemm`` or any other):
     adapter_ids int32 [rows]   any order, one request a row or runs of rows; an id outside [0, adapters) means no adapter
     scaling     f32 [adapters]
 
-The product with ``a`` is kept in fp32 between the two steps and the result is rounded once.  ``out=`` takes the caller's
-buffer and may be ``y`` itself (serving: in place).  Gradients reach y, x, a and b; adapters of smaller rank are padded with
-zeros by the caller.  rank is a multiple of 8 up to 128, k and n multiples of 8.  A row's result depends on its own inputs
-and adapter only; nothing is atomic.  The reference has no counterpart.
+The product with ``a`` is summed in fp32 and enters the second one with 16 (bf16) or 22 (fp16) significant bits; the result
+is rounded once.  ``out=`` takes the caller's buffer and may be ``y`` itself (serving: in place).  Gradients reach y, x, a
+and b; adapters of smaller rank are padded with zeros by the caller.  rank is a multiple of 8 up to 128, k and n multiples of
+8.  A row's result depends on its own inputs and adapter only; nothing is atomic.  The reference has no counterpart.
 """
 
 from __future__ import annotations
