@@ -224,22 +224,35 @@ struct ExpandTcArgs {
 };
 
 // Products that came out as NaN, once more from the definition: high part and remainder share an accumulator, where against an
-// infinity the remainder turns infinite products into NaN (see lora.cu).  64 columns of a row's output in shared memory.
+// infinity the remainder turns infinite products into NaN (see lora.cu).  A warp goes through the rows of its lanes with `mine`,
+// two of their 64 columns of output (in shared memory, from `tile` on) a lane; where a row's v has a NaN its outputs stay.
+// A call and its synchronisation at 8192 rows, 4096 -> 4096, rank 128: 0.11 ms, with an infinity in one row 0.35, with NaNs
+// everywhere 0.29 (16 with every lane on its own row alone).
 template <typename T>
-__device__ __noinline__ void expand_again(const ExpandArgs& p, uint8_t* line, int sw, int adapter, int row, int col) {
-  const T* b = static_cast<const T*>(p.b) + (long long)adapter * p.n * p.rank;
+__device__ __noinline__ void expand_again(const ExpandArgs& p, bool mine, uint8_t* tile, int adapter, int row0, int col) {
+  const int lane = threadIdx.x & 31, first = int(threadIdx.x & 96);          // of the warp's rows in the tile
   const T* base = static_cast<const T*>(p.base);
-  const float* v = p.v + (long long)row * p.rank;
-  for (int i = 0; i < min(64, p.n - col); ++i) {
-    T* out = reinterpret_cast<T*>(line + ((i >> 3) ^ sw) * 16) + (i & 7);
-    if (!isnan(float(*out))) continue;
-    float sum = 0.f;
-    for (int j = 0; j < p.rank; ++j)
-      sum = fmaf(v[j], float(b[p.transposed ? (long long)j * p.n + col + i : (long long)(col + i) * p.rank + j]), sum);
-    const float y = base ? float(base[(long long)row * p.n + col + i]) : 0.f;       // the tile is not stored yet
-    const uint32_t pk = pack2<T>(fmaf(p.scaling[adapter], sum, y), 0.f);
-    *out = reinterpret_cast<const T*>(&pk)[0];
+  __syncwarp();                                  // the rows are written
+  for (uint32_t who = __ballot_sync(0xffffffffu, mine); who; who &= who - 1) {
+    const int from = __ffs(who) - 1, l = __shfl_sync(0xffffffffu, adapter, from);
+    const long long row = row0 + first + from;
+    const T* b = static_cast<const T*>(p.b) + (long long)l * p.n * p.rank;
+    const float* v = p.v + row * p.rank;
+    bool nan = false;
+    for (int j = lane; j < p.rank; j += 32) nan |= isnan(v[j]);
+    if (__any_sync(0xffffffffu, nan)) continue;
+    for (int i = lane; i < min(64, p.n - col); i += 32) {
+      T* out = reinterpret_cast<T*>(tile + (first + from) * 128 + ((i >> 3) ^ (from & 7)) * 16) + (i & 7);
+      if (!isnan(float(*out))) continue;
+      float sum = 0.f;
+      for (int j = 0; j < p.rank; ++j)
+        sum = fmaf(v[j], float(b[p.transposed ? (long long)j * p.n + col + i : (long long)(col + i) * p.rank + j]), sum);
+      const float y = base ? float(base[row * p.n + col + i]) : 0.f;         // the tile is not stored yet
+      const uint32_t pk = pack2<T>(fmaf(p.scaling[l], sum, y), 0.f);
+      *out = reinterpret_cast<const T*>(&pk)[0];
+    }
   }
+  __syncwarp();
 }
 
 // KC: chunks of 64 in the rank.
@@ -567,6 +580,7 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
             tmem_ld_x32(tmem + (uint32_t((warp & 3) * 32) << 16) + acc * kExCols + wg * 64 + h * 32,
                         reinterpret_cast<uint32_t*>(v + h * 32));
           tmem_ld_wait();
+          bool undefined = false;
           if (hit) {
             uint64_t sums = 0;                   // looks for NaNs
 #pragma unroll
@@ -580,8 +594,10 @@ lora_expand_tc_kernel(const __grid_constant__ CUtensorMap tmap_y, const __grid_c
               }
               *reinterpret_cast<uint4*>(line + ((j ^ sw) * 16)) = y[j];
             }
-            if (either_nan(sums)) expand_again<T>(p, line, sw, mine, rt * kTileRows + row, col + wg * 64);
+            undefined = either_nan(sums);
           }
+          if (__any_sync(0xffffffffu, undefined))
+            expand_again<T>(p, undefined, smem + (ys * 2 + wg) * kChunkBytes, mine, rt * kTileRows, col + wg * 64);
         }
         tcgen05_fence_before();
         __syncwarp();
