@@ -67,7 +67,7 @@ def _check_rows_form(name, t, w, offsets, out, input_grad):
         raise TypeError(f"{name}, w and offsets must be torch.Tensors")
     require_shape("w", w, (None, None, None))
     experts, n, k = w.shape
-    _check_sizes(len(t), experts, n, k)
+    _check_sizes(t.shape[0] if t.dim() else 0, experts, n, k)
     require_shape(name, t, (None, n if input_grad else k))
     require_shape("offsets", offsets, (experts + 1,))
     _check(name, t, "w", w, offsets, out, (t.shape[0], k if input_grad else n))

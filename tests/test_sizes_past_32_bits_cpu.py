@@ -67,6 +67,13 @@ def test_columns():
         moe_permute(empty(4, 2 ** 30 + 8, dtype=F32), plan())        # 2^32 + 32 bytes
 
 
+def test_a_single_number_is_no_matrix():
+    with FakeTensorMode(), pytest.raises(ValueError, match="x must have shape"):
+        grouped_gemm(empty(), empty(2, 8, 8), empty(3, dtype=I32))
+    with FakeTensorMode(), pytest.raises(ValueError, match="dy must have shape"):
+        grouped_gemm_wgrad(empty(), empty(4, 8), empty(3, dtype=I32))
+
+
 def test_c_entries(lib):
     most = 2 ** 31 - 1 - 1024
     assert lib.flymoe_grouped_gemm(None, None, None, None, most + 1, 2, 8, 16, 2, 0, 0, None) == -1
